@@ -1,0 +1,429 @@
+// Attention over the paged KV cache (C-ABI in iekv_ops.h, work items in attention_plan.h).
+//
+// For a query row q at position p and the keys j it sees (j <= p, and j > p - window or
+// j < sinks): o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), s_j = scale q.k_j, m = max s_j.
+// Powers are taken to base 2: scores are scaled by scale * log2(e).
+#include "ops_common.h"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "attention_plan.h"
+
+namespace iekv_ops {
+
+thread_local std::string g_error;
+
+int set_error(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_error = buf;
+  return code;
+}
+
+}  // namespace iekv_ops
+
+using namespace iekv_ops;
+using iekv_attention::Item;
+using iekv_attention::Launch;
+
+struct iekv_attention_plan {
+  iekv_attention_shape shape;
+  Launch narrow, wide;
+  int32_t joined;                // tokens with several parts
+  int64_t tokens, slots;
+  int64_t positions_at, join_tokens_at, join_starts_at, join_parts_at, tables_at;  // words
+  std::vector<int32_t> words;
+};
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWave = 64;
+
+struct Args {
+  const int32_t* words;       // the plan's words: its items first
+  const void* k;
+  const void* v;
+  const void* q;
+  void* out;
+  float* part_o;              // [slots][kv_heads][head_dim]: sums of e^(s - m) v
+  float2* part_ml;            // [slots][kv_heads]: m (base 2) and the sum of e^(s - m)
+  int64_t positions_at, tables_at;
+  int64_t q_token_stride, q_head_stride;
+  int64_t window, sinks;      // window: INT32_MAX for all keys
+  int32_t kv_heads, group, head_dim, block_size;
+  float scale;                // times log2(e)
+};
+
+__device__ __forceinline__ Item item_of(const Args& a, int32_t i) {
+  return reinterpret_cast<const Item*>(a.words)[i];
+}
+
+// Key number `v` of the item's ranges laid end to end.
+__device__ __forceinline__ int32_t key_at(const Item& it, int32_t v) {
+  const int32_t na = it.a1 - it.a0;
+  return v < na ? it.a0 + v : it.b0 + (v - na);
+}
+
+__device__ __forceinline__ bool sees(const Args& a, int32_t position, int32_t key) {
+  return key <= position && (key > position - a.window || key < a.sinks);
+}
+
+// The cache row of key `j`, of every KV head.
+__device__ __forceinline__ int64_t row_of(const Args& a, const Item& it, int32_t j) {
+  const int32_t block = a.words[a.tables_at + it.table + j / a.block_size];
+  return static_cast<int64_t>(block) * a.block_size + j % a.block_size;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
+  return x;
+}
+
+// One query row key by key, by one wave: a lane scores a key of each 64, then holds two
+// dimensions of the output. Keys the row does not see are not read for it at all, so that
+// whatever they hold (infinities, NaN) stays out.
+template <typename T, typename C>
+__device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32_t row, int lane) {
+  const int32_t token = it.token0 + row / a.group, in_group = row % a.group;
+  const int32_t position = a.words[a.positions_at + token];
+  const int32_t d = a.head_dim;
+  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
+  const T* q = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
+  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
+  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
+  const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0);
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int32_t v0 = 0; v0 < n; v0 += kWave) {
+    const bool in = v0 + lane < n;
+    const int32_t j = key_at(it, in ? v0 + lane : n - 1);
+    const int64_t at = row_of(a, it, j) * width;
+    const bool seen = in && sees(a, position, j);
+    float s = -INFINITY;
+    if (seen) {
+      float dot = 0.f;
+      for (int32_t i = 0; i < d; ++i) dot = fmaf(to_float(q[i]), to_float(kc[at + i]), dot);
+      s = dot * a.scale;
+    }
+    // A score that is NaN stays in the sum, and the row is NaN as it has to be.
+    const float top = fmaxf(m, wave_max(s));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float fade = exp2f(m - base);
+    const float p = seen ? exp2f(s - base) : 0.f;
+    m = top;
+    l = l * fade + wave_sum(p);
+    o0 *= fade;
+    o1 *= fade;
+    uint64_t left = __ballot(seen);
+    while (left) {
+      const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
+      left &= left - 1;
+      const float pi = __shfl(p, i);
+      const int64_t ai = __shfl(at, i);
+      if (lane < d) o0 = fmaf(pi, to_float(vc[ai + lane]), o0);
+      if (lane + kWave < d) o1 = fmaf(pi, to_float(vc[ai + lane + kWave]), o1);
+    }
+  }
+  if (it.slot >= 0) {
+    const int64_t slot = static_cast<int64_t>(it.slot + row) * a.kv_heads + kv_head;
+    if (lane < d) a.part_o[slot * d + lane] = o0;
+    if (lane + kWave < d) a.part_o[slot * d + lane + kWave] = o1;
+    if (lane == 0) a.part_ml[slot] = {m, l};
+    return;
+  }
+  T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
+  if (lane < d) out[lane] = from_float<T>(o0 / l);
+  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
+}
+
+template <typename T, typename C>
+__global__ __launch_bounds__(kThreads) void attend_rows(Args a, int32_t first) {
+  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
+  const int32_t kv_head = blockIdx.x % a.kv_heads;
+  const int32_t rows = it.tokens * a.group;
+  for (int32_t r = threadIdx.x / kWave; r < rows; r += kThreads / kWave)
+    attend_row<T, C>(a, it, kv_head, r, threadIdx.x % kWave);
+}
+
+// Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, in
+// the order of the parts. One wave a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* tokens,
+                                                       const int32_t* starts,
+                                                       const int32_t* parts, int32_t n) {
+  const int lane = threadIdx.x % kWave;
+  const int32_t heads = a.kv_heads * a.group, d = a.head_dim;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
+  if (row >= static_cast<int64_t>(n) * heads) return;
+  const int32_t entry = static_cast<int32_t>(row / heads), head = static_cast<int32_t>(row % heads);
+  const int32_t kv_head = head / a.group, in_group = head % a.group;
+  const int32_t p0 = starts[entry], p1 = starts[entry + 1];
+  float m = -INFINITY;
+  for (int32_t p = p0; p < p1; ++p)
+    m = fmaxf(m, a.part_ml[static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int32_t p = p0; p < p1; ++p) {
+    const int64_t slot = static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
+    const float2 ml = a.part_ml[slot];
+    const float w = exp2f(ml.x - base);
+    l = fmaf(w, ml.y, l);
+    if (lane < d) o0 = fmaf(w, a.part_o[slot * d + lane], o0);
+    if (lane + kWave < d) o1 = fmaf(w, a.part_o[slot * d + lane + kWave], o1);
+  }
+  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(tokens[entry]) * heads + head) * d;
+  if (lane < d) out[lane] = from_float<T>(o0 / l);
+  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
+}
+
+template <typename T, typename C>
+int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
+  for (const Launch& part : {plan.narrow, plan.wide}) {
+    if (!part.n) continue;
+    hipLaunchKernelGGL((attend_rows<T, C>), dim3(part.n * a.kv_heads), dim3(kThreads), 0, stream, a,
+                       part.first);
+    IEKV_OPS_HIP(hipGetLastError());
+  }
+  if (plan.joined) {
+    const int64_t rows = int64_t(plan.joined) * a.kv_heads * a.group;
+    const int32_t* w = a.words;
+    hipLaunchKernelGGL((join_parts<T>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, a,
+                       w + plan.join_tokens_at, w + plan.join_starts_at, w + plan.join_parts_at,
+                       plan.joined);
+    IEKV_OPS_HIP(hipGetLastError());
+  }
+  return IEKV_OK;
+}
+
+int64_t workspace_bytes_of(const iekv_attention_plan& p) {
+  return p.slots * p.shape.num_kv_heads * (p.shape.head_dim + 2) * int64_t(sizeof(float));
+}
+
+bool known_types(int32_t query, int32_t cache) {
+  if (query == IEKV_TYPE_F32) return cache >= IEKV_TYPE_F32 && cache <= IEKV_TYPE_E4M3;
+  return (query == IEKV_TYPE_F16 || query == IEKV_TYPE_BF16) &&
+         (cache == query || cache == IEKV_TYPE_E4M3);
+}
+
+int check_shape(const iekv_attention_shape& s) {
+  const auto bad = [](const char* what, int64_t v) {
+    return set_error(IEKV_ERR_INVALID, "%s %lld out of range", what, static_cast<long long>(v));
+  };
+  if (s.num_kv_heads < 1 || s.num_kv_heads > 4096) return bad("num_kv_heads", s.num_kv_heads);
+  if (s.num_heads < 1 || s.num_heads % s.num_kv_heads)
+    return set_error(IEKV_ERR_INVALID, "%d query heads for %d KV heads", s.num_heads,
+                     s.num_kv_heads);
+  if (s.num_heads / s.num_kv_heads > IEKV_ATTENTION_MAX_GROUP)
+    return set_error(IEKV_ERR_INVALID, "%d query heads per KV head, at most %d are taken",
+                     s.num_heads / s.num_kv_heads, IEKV_ATTENTION_MAX_GROUP);
+  if (s.head_dim < 8 || s.head_dim > IEKV_ATTENTION_MAX_DIM || s.head_dim % 8)
+    return set_error(IEKV_ERR_INVALID, "head_dim %d is not a multiple of 8 up to %d", s.head_dim,
+                     IEKV_ATTENTION_MAX_DIM);
+  if (s.block_size < 1 || s.block_size > (1 << 20)) return bad("block_size", s.block_size);
+  if (s.num_blocks < 1 || s.num_blocks > INT32_MAX) return bad("num_blocks", s.num_blocks);
+  if (!known_types(s.query_type, s.cache_type))
+    return set_error(IEKV_ERR_INVALID, "queries of type %d on a cache of type %d", s.query_type,
+                     s.cache_type);
+  if (s.window < 0) return bad("window", s.window);
+  if (s.sinks < 0) return bad("sinks", s.sinks);
+  if (s.shared_blocks < 0 || s.shared_blocks > IEKV_ATTENTION_MAX_CONTEXT / s.block_size)
+    return bad("shared_blocks", s.shared_blocks);
+  return IEKV_OK;
+}
+
+int compute_units() {
+  static const int units = [] {
+    int device = 0, n = 0;
+    if (hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+        n <= 0) {
+      (void)hipGetLastError();
+      return 256;   // no GPU in sight: a plan made to be looked at
+    }
+    return n;
+  }();
+  return units;
+}
+
+int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* context_lens,
+         const int32_t* query_lens, const int32_t* tables, const int64_t* starts,
+         iekv_attention_plan** out) {
+  const int64_t bs = shape.block_size;
+  std::vector<iekv_attention::Sequence> seqs(n_seqs);
+  std::vector<int32_t> entries;
+  int64_t tokens = 0;
+  const int32_t* leading = nullptr;
+  for (int32_t s = 0; s < n_seqs; ++s) {
+    const int64_t context = context_lens[s], queries = query_lens[s];
+    if (context < 0 || context > IEKV_ATTENTION_MAX_CONTEXT || queries < 0 || queries > context)
+      return set_error(IEKV_ERR_INVALID, "sequence %d: %lld queries in a context of %lld", s,
+                       static_cast<long long>(queries), static_cast<long long>(context));
+    const int64_t used = (context + bs - 1) / bs, held = starts[s + 1] - starts[s];
+    if (starts[s] < 0 || held < used)
+      return set_error(IEKV_ERR_RANGE, "sequence %d: context of %lld needs %lld blocks, table has %lld",
+                       s, static_cast<long long>(context), static_cast<long long>(used),
+                       static_cast<long long>(held));
+    const int32_t* table = tables + starts[s];
+    for (int64_t b = 0; b < used; ++b)
+      if (table[b] < 0 || table[b] >= shape.num_blocks)
+        return set_error(IEKV_ERR_RANGE, "sequence %d: block id %d out of range for a pool of %lld blocks",
+                         s, table[b], static_cast<long long>(shape.num_blocks));
+    if (shape.shared_blocks && queries) {
+      if (context < shape.shared_blocks * bs)
+        return set_error(IEKV_ERR_IDS, "sequence %d: a context of %lld does not fill %lld shared blocks",
+                         s, static_cast<long long>(context),
+                         static_cast<long long>(shape.shared_blocks));
+      if (!leading) leading = table;
+      if (!std::equal(leading, leading + shape.shared_blocks, table))
+        return set_error(IEKV_ERR_IDS, "sequence %d does not begin with the %lld shared blocks", s,
+                         static_cast<long long>(shape.shared_blocks));
+    }
+    if (tokens + queries > INT32_MAX / 2 / shape.num_heads ||
+        static_cast<int64_t>(entries.size()) + used > INT32_MAX)
+      return set_error(IEKV_ERR_INVALID, "too many query rows or blocks in one step");
+    seqs[s] = {static_cast<int32_t>(context), static_cast<int32_t>(queries),
+               static_cast<int32_t>(tokens), static_cast<int32_t>(entries.size())};
+    if (queries) entries.insert(entries.end(), table, table + used);
+    tokens += queries;
+  }
+  iekv_attention::Shape sh{shape.num_heads / shape.num_kv_heads, shape.num_kv_heads,
+                           shape.block_size, shape.window, shape.sinks,
+                           static_cast<int32_t>(shape.shared_blocks * bs), 128};
+  iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units());
+  if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||
+      made.slots > INT32_MAX)
+    return set_error(IEKV_ERR_INVALID, "too many work items in one step");
+  auto plan = new iekv_attention_plan{};
+  plan->shape = shape;
+  plan->narrow = made.narrow;
+  plan->wide = made.wide;
+  plan->joined = static_cast<int32_t>(made.join_tokens.size());
+  plan->tokens = tokens;
+  plan->slots = made.slots;
+  std::vector<int32_t>& w = plan->words;
+  const auto* items = reinterpret_cast<const int32_t*>(made.items.data());
+  w.assign(items, items + made.items.size() * iekv_attention::kItemWords);
+  const auto append = [&w](const std::vector<int32_t>& x) {
+    const int64_t at = static_cast<int64_t>(w.size());
+    w.insert(w.end(), x.begin(), x.end());
+    return at;
+  };
+  plan->positions_at = append(made.positions);
+  plan->join_tokens_at = append(made.join_tokens);
+  plan->join_starts_at = append(made.join_starts);
+  plan->join_parts_at = append(made.join_parts);
+  plan->tables_at = append(entries);
+  *out = plan;
+  return IEKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int iekv_ops_abi_version(void) { return IEKV_OPS_ABI_VERSION; }
+
+const char* iekv_ops_last_error(void) { return g_error.c_str(); }
+
+int iekv_attention_plan_create(const iekv_attention_shape* shape, int32_t n_seqs,
+                               const int32_t* context_lens, const int32_t* query_lens,
+                               const int32_t* tables, const int64_t* table_starts,
+                               iekv_attention_plan** out) {
+  if (!out) return set_error(IEKV_ERR_INVALID, "out is null");
+  *out = nullptr;
+  if (!shape) return set_error(IEKV_ERR_INVALID, "shape is null");
+  if (n_seqs < 0) return set_error(IEKV_ERR_INVALID, "n_seqs %d is negative", n_seqs);
+  if (n_seqs && (!context_lens || !query_lens || !table_starts))
+    return set_error(IEKV_ERR_INVALID, "context_lens, query_lens or table_starts is null");
+  if (n_seqs && !tables && table_starts[n_seqs] > 0)
+    return set_error(IEKV_ERR_INVALID, "tables is null");
+  if (const int rc = check_shape(*shape)) return rc;
+  try {
+    return make(*shape, n_seqs, context_lens, query_lens, tables, table_starts, out);
+  } catch (const std::bad_alloc&) {
+    return set_error(IEKV_ERR_CAPACITY, "out of host memory for a plan of %d sequences", n_seqs);
+  }
+}
+
+int iekv_attention_plan_destroy(iekv_attention_plan* plan) {
+  delete plan;
+  return IEKV_OK;
+}
+
+int iekv_attention_plan_info(const iekv_attention_plan* plan, const int32_t** words,
+                             int64_t* n_words, int64_t* tokens, int64_t* workspace_bytes) {
+  if (!plan || !words || !n_words || !tokens || !workspace_bytes)
+    return set_error(IEKV_ERR_INVALID, "null argument");
+  *words = plan->words.data();
+  *n_words = static_cast<int64_t>(plan->words.size());
+  *tokens = plan->tokens;
+  *workspace_bytes = workspace_bytes_of(*plan);
+  return IEKV_OK;
+}
+
+int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const void* k,
+                const void* v, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                float scale, void* out, void* workspace, int64_t workspace_bytes,
+                hipStream_t stream) {
+  if (!plan) return set_error(IEKV_ERR_INVALID, "plan is null");
+  if (!plan->tokens) return IEKV_OK;
+  if (!words || !k || !v || !q || !out)
+    return set_error(IEKV_ERR_INVALID, "words, k, v, q or out is null");
+  if (reinterpret_cast<uintptr_t>(words) % 16)
+    return set_error(IEKV_ERR_INVALID, "words is not aligned to 16 bytes");
+  if (!std::isfinite(scale)) return set_error(IEKV_ERR_INVALID, "scale is not finite");
+  const int64_t need = workspace_bytes_of(*plan);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(IEKV_ERR_CAPACITY, "workspace of %lld bytes, %lld are needed",
+                     static_cast<long long>(workspace ? workspace_bytes : 0),
+                     static_cast<long long>(need));
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return set_error(IEKV_ERR_INVALID, "workspace is not aligned to 16 bytes");
+  const iekv_attention_shape& s = plan->shape;
+  Args a{};
+  a.words = words;
+  a.k = k;
+  a.v = v;
+  a.q = q;
+  a.out = out;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + plan->slots * s.num_kv_heads * s.head_dim);
+  a.positions_at = plan->positions_at;
+  a.tables_at = plan->tables_at;
+  a.q_token_stride = q_token_stride;
+  a.q_head_stride = q_head_stride;
+  a.window = s.window ? s.window : INT32_MAX;
+  a.sinks = s.sinks;
+  a.kv_heads = s.num_kv_heads;
+  a.group = s.num_heads / s.num_kv_heads;
+  a.head_dim = s.head_dim;
+  a.block_size = s.block_size;
+  a.scale = scale * 1.4426950408889634f;
+  switch (s.query_type * 8 + s.cache_type) {
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F32: return launch<float, float>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F16: return launch<float, _Float16>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_BF16: return launch<float, Bf16>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_E4M3: return launch<float, E4m3>(*plan, a, stream);
+    case IEKV_TYPE_F16 * 8 + IEKV_TYPE_F16: return launch<_Float16, _Float16>(*plan, a, stream);
+    case IEKV_TYPE_F16 * 8 + IEKV_TYPE_E4M3: return launch<_Float16, E4m3>(*plan, a, stream);
+    case IEKV_TYPE_BF16 * 8 + IEKV_TYPE_BF16: return launch<Bf16, Bf16>(*plan, a, stream);
+    default: return launch<Bf16, E4m3>(*plan, a, stream);
+  }
+}
+
+}  // extern "C"

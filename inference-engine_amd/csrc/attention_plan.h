@@ -1,0 +1,185 @@
+// How a step's attention is cut into work items: host code, no GPU (checked on the CPU by
+// tests/attention_plan_check.cpp).
+//
+// A query row is (token, head). The rows of one KV head that read the same keys go
+// together: an item is a run of tokens, all `group` heads of each, over a set of keys of
+// one block table. The keys are two ranges: [a0, a1), of the sink tokens, then [b0, b1).
+// An item whose rows see other keys in other items leaves partial results (the sum of
+// e^(s - m) v, m and the sum of e^(s - m)) for a second launch that joins them.
+#ifndef IEKV_ATTENTION_PLAN_H_
+#define IEKV_ATTENTION_PLAN_H_
+
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+namespace iekv_attention {
+
+struct Item {
+  int32_t token0, tokens;  // rows: tokens token0 .. token0 + tokens - 1, every head of the group
+  int32_t table;           // first entry of the block table among the plan's tables
+  int32_t a0, a1, b0, b1;  // keys
+  int32_t slot;            // first partial slot, or -1: the item alone makes its rows
+  int32_t low, high;       // smallest and largest position of its tokens
+  int32_t pad[2];
+};
+static_assert(sizeof(Item) == 48, "items are read as 12 words");
+constexpr int kItemWords = 12;
+
+struct Shape {
+  int32_t group, kv_heads, block_size;
+  int64_t window, sinks;  // window 0: every key up to the query's own
+  int32_t shared;         // keys of the shared blocks (0: none)
+  int32_t wide_rows;      // rows an item of the wide kernel holds at most (0: there is none)
+};
+
+struct Sequence {
+  int32_t context, queries, token0, table;
+};
+
+// What one launch runs: `n` items from item `first` on.
+struct Launch {
+  int32_t first = 0, n = 0;
+};
+
+struct Plan {
+  std::vector<Item> items;
+  Launch narrow, wide;
+  std::vector<int32_t> positions;      // per token
+  std::vector<int32_t> join_tokens;    // tokens with several parts
+  std::vector<int32_t> join_starts;    // n + 1: where each one's parts begin
+  std::vector<int32_t> join_parts;     // first slot of the token in each part
+  int64_t slots = 0;                   // partial slots per KV head
+};
+
+constexpr int kNarrowRows = 16;
+
+// Keys of [lo, hi) that any of positions low..high sees.
+inline void visible(const Shape& sh, int64_t low, int64_t high, int64_t lo, int64_t hi, Item* it) {
+  hi = std::min(hi, high + 1);
+  const int64_t window = sh.window > 0 ? sh.window : int64_t(1) << 40;
+  const int64_t a1 = std::max(lo, std::min(sh.sinks, hi));
+  const int64_t b0 = std::max(a1, low - window + 1);
+  it->a0 = static_cast<int32_t>(lo);
+  it->a1 = static_cast<int32_t>(a1);
+  it->b0 = static_cast<int32_t>(std::min(b0, std::max(hi, a1)));
+  it->b1 = static_cast<int32_t>(std::max<int64_t>(hi, it->b0));
+  if (it->b0 == it->a1) {  // one range
+    it->b0 = it->a0;
+    it->a1 = it->a0;
+  }
+}
+
+inline int32_t keys_of(const Item& it) { return (it.a1 - it.a0) + (it.b1 - it.b0); }
+
+// Keys v0 .. v1 - 1 of the item's ranges laid end to end.
+inline Item cut(const Item& it, int32_t v0, int32_t v1) {
+  const int32_t na = it.a1 - it.a0;
+  Item out = it;
+  out.a0 = it.a0 + std::min(v0, na);
+  out.a1 = it.a0 + std::min(v1, na);
+  out.b0 = it.b0 + std::max(v0 - na, 0);
+  out.b1 = it.b0 + std::max(v1 - na, 0);
+  return out;
+}
+
+// Items of a run of tokens over keys [lo, hi) of a table, at most `rows` rows each.
+inline void add_tiles(const Shape& sh, const std::vector<int32_t>& positions, int32_t token0,
+                      int32_t tokens, int32_t table, int64_t lo, int64_t hi, int32_t rows,
+                      std::vector<Item>* out) {
+  const int32_t per = std::max(1, rows / sh.group);
+  for (int32_t t = 0; t < tokens; t += per) {
+    Item it{};
+    it.token0 = token0 + t;
+    it.tokens = std::min(per, tokens - t);
+    it.table = table;
+    const auto first = positions.begin() + it.token0;
+    it.low = *std::min_element(first, first + it.tokens);
+    it.high = *std::max_element(first, first + it.tokens);
+    visible(sh, it.low, it.high, lo, hi, &it);
+    if (keys_of(it)) out->push_back(it);
+  }
+}
+
+// Splits long items so that a launch has enough workgroups.
+inline std::vector<Item> split(const std::vector<Item>& in, int32_t kv_heads, int64_t want,
+                               int32_t least, int32_t step) {
+  int64_t keys = 0;
+  for (const Item& it : in) keys += keys_of(it);
+  const int64_t items = std::max<int64_t>(1, (want + kv_heads - 1) / kv_heads);
+  const int64_t each = std::max<int64_t>(least, (keys + items - 1) / items);
+  std::vector<Item> out;
+  for (const Item& it : in) {
+    const int64_t n = keys_of(it);
+    const int64_t parts = std::max<int64_t>(1, (n + each / 2) / each);
+    const int64_t size = ((n + parts - 1) / parts + step - 1) / step * step;
+    for (int64_t v = 0; v < n; v += size)
+      out.push_back(cut(it, static_cast<int32_t>(v), static_cast<int32_t>(std::min(n, v + size))));
+  }
+  return out;
+}
+
+inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_t compute_units) {
+  Plan plan;
+  int32_t tokens = 0;
+  for (const Sequence& s : seqs)
+    for (int32_t i = 0; i < s.queries; ++i, ++tokens)
+      plan.positions.push_back(s.context - s.queries + i);
+  std::vector<Item> narrow, wide;
+  auto add = [&](int32_t token0, int32_t n, int32_t table, int64_t lo, int64_t hi) {
+    const bool is_wide = sh.wide_rows > 0 && int64_t(n) * sh.group > kNarrowRows;
+    add_tiles(sh, plan.positions, token0, n, table, lo, hi,
+              is_wide ? sh.wide_rows : kNarrowRows, is_wide ? &wide : &narrow);
+  };
+  if (sh.shared && tokens) {
+    const auto first = std::find_if(seqs.begin(), seqs.end(),
+                                    [](const Sequence& s) { return s.queries > 0; });
+    add(0, tokens, first->table, 0, sh.shared);
+  }
+  for (const Sequence& s : seqs)
+    if (s.queries) add(s.token0, s.queries, s.table, sh.shared, s.context);
+  narrow = split(narrow, sh.kv_heads, 4 * compute_units, 256, 64);
+  wide = split(wide, sh.kv_heads, 2 * compute_units, 512, 64);
+  // The longest first: the last workgroups to start are short ones.
+  auto longer = [](const Item& x, const Item& y) { return keys_of(x) > keys_of(y); };
+  std::stable_sort(narrow.begin(), narrow.end(), longer);
+  std::stable_sort(wide.begin(), wide.end(), longer);
+  plan.narrow = {0, static_cast<int32_t>(narrow.size())};
+  plan.wide = {plan.narrow.n, static_cast<int32_t>(wide.size())};
+  plan.items = std::move(narrow);
+  plan.items.insert(plan.items.end(), wide.begin(), wide.end());
+
+  // A token is joined unless one item makes its rows, and those of the item's other tokens,
+  // alone.
+  std::vector<int32_t> parts(tokens, 0);
+  std::vector<char> joined(tokens, 0);
+  for (const Item& it : plan.items)
+    for (int32_t t = 0; t < it.tokens; ++t) ++parts[it.token0 + t];
+  for (Item& it : plan.items) {
+    bool alone = true;
+    for (int32_t t = 0; t < it.tokens; ++t) alone = alone && parts[it.token0 + t] == 1;
+    it.slot = alone ? -1 : 0;
+    for (int32_t t = 0; t < it.tokens && !alone; ++t) joined[it.token0 + t] = 1;
+  }
+  std::vector<int32_t> at(tokens, -1);
+  plan.join_starts.push_back(0);
+  for (int32_t t = 0; t < tokens; ++t) {
+    if (!joined[t]) continue;
+    at[t] = plan.join_starts.back();
+    plan.join_tokens.push_back(t);
+    plan.join_starts.push_back(plan.join_starts.back() + parts[t]);
+  }
+  plan.join_parts.resize(plan.join_starts.back());
+  for (Item& it : plan.items) {
+    if (it.slot < 0) continue;
+    it.slot = static_cast<int32_t>(plan.slots);
+    for (int32_t t = 0; t < it.tokens; ++t)
+      plan.join_parts[at[it.token0 + t]++] = it.slot + t * sh.group;
+    plan.slots += int64_t(it.tokens) * sh.group;
+  }
+  return plan;
+}
+
+}  // namespace iekv_attention
+
+#endif  // IEKV_ATTENTION_PLAN_H_
