@@ -6,6 +6,7 @@
 #include "ops_common.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdarg>
@@ -14,7 +15,7 @@
 #include <string>
 #include <vector>
 
-#include "attention_plan.h"
+#include "attention_kernels.h"
 
 namespace iekv_ops {
 
@@ -33,7 +34,6 @@ int set_error(int code, const char* fmt, ...) {
 }  // namespace iekv_ops
 
 using namespace iekv_ops;
-using iekv_attention::Item;
 using iekv_attention::Launch;
 
 struct iekv_attention_plan {
@@ -47,156 +47,31 @@ struct iekv_attention_plan {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWave = 64;
+constexpr int kWideRows = 128;  // rows an item of the wide kernel holds at most
 
-struct Args {
-  const int32_t* words;       // the plan's words: its items first
-  const void* k;
-  const void* v;
-  const void* q;
-  void* out;
-  float* part_o;              // [slots][kv_heads][head_dim]: sums of e^(s - m) v
-  float2* part_ml;            // [slots][kv_heads]: m (base 2) and the sum of e^(s - m)
-  int64_t positions_at, tables_at;
-  int64_t q_token_stride, q_head_stride;
-  int64_t window, sinks;      // window: INT32_MAX for all keys
-  int32_t kv_heads, group, head_dim, block_size;
-  float scale;                // times log2(e)
-};
-
-__device__ __forceinline__ Item item_of(const Args& a, int32_t i) {
-  return reinterpret_cast<const Item*>(a.words)[i];
+// Its LDS passes what a kernel may have without asking.
+template <typename K>
+int allow_lds(K kernel, int bytes) {
+  static const hipError_t status = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  IEKV_OPS_HIP(status);
+  return IEKV_OK;
 }
 
-// Key number `v` of the item's ranges laid end to end.
-__device__ __forceinline__ int32_t key_at(const Item& it, int32_t v) {
-  const int32_t na = it.a1 - it.a0;
-  return v < na ? it.a0 + v : it.b0 + (v - na);
-}
-
-__device__ __forceinline__ bool sees(const Args& a, int32_t position, int32_t key) {
-  return key <= position && (key > position - a.window || key < a.sinks);
-}
-
-// The cache row of key `j`, of every KV head.
-__device__ __forceinline__ int64_t row_of(const Args& a, const Item& it, int32_t j) {
-  const int32_t block = a.words[a.tables_at + it.table + j / a.block_size];
-  return static_cast<int64_t>(block) * a.block_size + j % a.block_size;
-}
-
-__device__ __forceinline__ float wave_max(float x) {
-  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
-  return x;
-}
-
-// One query row key by key, by one wave: a lane scores a key of each 64, then holds two
-// dimensions of the output. Keys the row does not see are not read for it at all, so that
-// whatever they hold (infinities, NaN) stays out.
-template <typename T, typename C>
-__device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32_t row, int lane) {
-  const int32_t token = it.token0 + row / a.group, in_group = row % a.group;
-  const int32_t position = a.words[a.positions_at + token];
-  const int32_t d = a.head_dim;
-  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
-  const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
-  const T* q = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
-  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
-  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
-  const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0);
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int32_t v0 = 0; v0 < n; v0 += kWave) {
-    const bool in = v0 + lane < n;
-    const int32_t j = key_at(it, in ? v0 + lane : n - 1);
-    const int64_t at = row_of(a, it, j) * width;
-    const bool seen = in && sees(a, position, j);
-    float s = -INFINITY;
-    if (seen) {
-      float dot = 0.f;
-      for (int32_t i = 0; i < d; ++i) dot = fmaf(to_float(q[i]), to_float(kc[at + i]), dot);
-      s = dot * a.scale;
-    }
-    // A score that is NaN stays in the sum, and the row is NaN as it has to be.
-    const float top = fmaxf(m, wave_max(s));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float fade = exp2f(m - base);
-    const float p = seen ? exp2f(s - base) : 0.f;
-    m = top;
-    l = l * fade + wave_sum(p);
-    o0 *= fade;
-    o1 *= fade;
-    uint64_t left = __ballot(seen);
-    while (left) {
-      const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
-      left &= left - 1;
-      const float pi = __shfl(p, i);
-      const int64_t ai = __shfl(at, i);
-      if (lane < d) o0 = fmaf(pi, to_float(vc[ai + lane]), o0);
-      if (lane + kWave < d) o1 = fmaf(pi, to_float(vc[ai + lane + kWave]), o1);
+template <typename T, typename C, int DP>
+int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
+  if (plan.wide.n) {
+    if constexpr (sizeof(T) == 2) {
+      constexpr int R = kWideRows / 128, bytes = sizeof(typename Wide<T, DP>::Lds);
+      if (const int rc = allow_lds(attend_wide<T, C, DP, R>, bytes)) return rc;
+      hipLaunchKernelGGL((attend_wide<T, C, DP, R>), dim3(plan.wide.n * a.kv_heads),
+                         dim3(kThreads), bytes, stream, a, plan.wide.first);
+      IEKV_OPS_HIP(hipGetLastError());
     }
   }
-  if (it.slot >= 0) {
-    const int64_t slot = static_cast<int64_t>(it.slot + row) * a.kv_heads + kv_head;
-    if (lane < d) a.part_o[slot * d + lane] = o0;
-    if (lane + kWave < d) a.part_o[slot * d + lane + kWave] = o1;
-    if (lane == 0) a.part_ml[slot] = {m, l};
-    return;
-  }
-  T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
-  if (lane < d) out[lane] = from_float<T>(o0 / l);
-  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
-}
-
-template <typename T, typename C>
-__global__ __launch_bounds__(kThreads) void attend_rows(Args a, int32_t first) {
-  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
-  const int32_t kv_head = blockIdx.x % a.kv_heads;
-  const int32_t rows = it.tokens * a.group;
-  for (int32_t r = threadIdx.x / kWave; r < rows; r += kThreads / kWave)
-    attend_row<T, C>(a, it, kv_head, r, threadIdx.x % kWave);
-}
-
-// Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, in
-// the order of the parts. One wave a row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* tokens,
-                                                       const int32_t* starts,
-                                                       const int32_t* parts, int32_t n) {
-  const int lane = threadIdx.x % kWave;
-  const int32_t heads = a.kv_heads * a.group, d = a.head_dim;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
-  if (row >= static_cast<int64_t>(n) * heads) return;
-  const int32_t entry = static_cast<int32_t>(row / heads), head = static_cast<int32_t>(row % heads);
-  const int32_t kv_head = head / a.group, in_group = head % a.group;
-  const int32_t p0 = starts[entry], p1 = starts[entry + 1];
-  float m = -INFINITY;
-  for (int32_t p = p0; p < p1; ++p)
-    m = fmaxf(m, a.part_ml[static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head].x);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int32_t p = p0; p < p1; ++p) {
-    const int64_t slot = static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
-    const float2 ml = a.part_ml[slot];
-    const float w = exp2f(ml.x - base);
-    l = fmaf(w, ml.y, l);
-    if (lane < d) o0 = fmaf(w, a.part_o[slot * d + lane], o0);
-    if (lane + kWave < d) o1 = fmaf(w, a.part_o[slot * d + lane + kWave], o1);
-  }
-  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(tokens[entry]) * heads + head) * d;
-  if (lane < d) out[lane] = from_float<T>(o0 / l);
-  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
-}
-
-template <typename T, typename C>
-int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
-  for (const Launch& part : {plan.narrow, plan.wide}) {
-    if (!part.n) continue;
-    hipLaunchKernelGGL((attend_rows<T, C>), dim3(part.n * a.kv_heads), dim3(kThreads), 0, stream, a,
-                       part.first);
+  if (plan.narrow.n) {
+    hipLaunchKernelGGL((attend_narrow<T, C, DP>),
+                       dim3(plan.narrow.n * a.kv_heads, (a.group + 15) / 16), dim3(kThreads), 0, stream, a, plan.narrow.first);
     IEKV_OPS_HIP(hipGetLastError());
   }
   if (plan.joined) {
@@ -208,6 +83,16 @@ int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
     IEKV_OPS_HIP(hipGetLastError());
   }
   return IEKV_OK;
+}
+
+template <typename T, typename C>
+int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
+  switch ((a.head_dim + 31) / 32) {
+    case 1: return launch_dim<T, C, 32>(plan, a, stream);
+    case 2: return launch_dim<T, C, 64>(plan, a, stream);
+    case 3: return launch_dim<T, C, 96>(plan, a, stream);
+    default: return launch_dim<T, C, 128>(plan, a, stream);
+  }
 }
 
 int64_t workspace_bytes_of(const iekv_attention_plan& p) {
@@ -236,6 +121,9 @@ int check_shape(const iekv_attention_shape& s) {
                      IEKV_ATTENTION_MAX_DIM);
   if (s.block_size < 1 || s.block_size > (1 << 20)) return bad("block_size", s.block_size);
   if (s.num_blocks < 1 || s.num_blocks > INT32_MAX) return bad("num_blocks", s.num_blocks);
+  if (s.num_blocks * s.block_size > UINT32_MAX)
+    return set_error(IEKV_ERR_INVALID, "%lld blocks of %d rows: more than 2^32 rows",
+                     static_cast<long long>(s.num_blocks), s.block_size);
   if (!known_types(s.query_type, s.cache_type))
     return set_error(IEKV_ERR_INVALID, "queries of type %d on a cache of type %d", s.query_type,
                      s.cache_type);
@@ -303,7 +191,8 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
   }
   iekv_attention::Shape sh{shape.num_heads / shape.num_kv_heads, shape.num_kv_heads,
                            shape.block_size, shape.window, shape.sinks,
-                           static_cast<int32_t>(shape.shared_blocks * bs), 128};
+                           static_cast<int32_t>(shape.shared_blocks * bs),
+                           shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows};
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units());
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||
       made.slots > INT32_MAX)
@@ -407,13 +296,20 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
   a.tables_at = plan->tables_at;
   a.q_token_stride = q_token_stride;
   a.q_head_stride = q_head_stride;
-  a.window = s.window ? s.window : INT32_MAX;
-  a.sinks = s.sinks;
+  a.window = static_cast<int32_t>(std::min<int64_t>(s.window ? s.window : INT32_MAX, INT32_MAX));
+  a.sinks = static_cast<int32_t>(std::min<int64_t>(s.sinks, INT32_MAX));
   a.kv_heads = s.num_kv_heads;
   a.group = s.num_heads / s.num_kv_heads;
   a.head_dim = s.head_dim;
   a.block_size = s.block_size;
-  a.scale = scale * 1.4426950408889634f;
+  // Division by a constant as a product (Granlund and Montgomery), for numerators below 2^31.
+  while ((uint64_t(1) << a.block_shift) < static_cast<uint64_t>(s.block_size)) ++a.block_shift;
+  a.block_magic = static_cast<uint32_t>(
+      ((uint64_t(1) << 32) * ((uint64_t(1) << a.block_shift) - s.block_size)) / s.block_size + 1);
+  // The kernels take the maximum before they scale, so the sign goes to q; a scale of zero
+  // is held above it, so that it leaves the -inf of a hidden key alone.
+  a.q_sign = !std::signbit(scale) ? 0 : s.query_type == IEKV_TYPE_F32 ? 0x80000000u : 0x80008000u;
+  a.scale = std::max(std::fabs(scale) * 1.4426950408889634f, FLT_MIN);
   switch (s.query_type * 8 + s.cache_type) {
     case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F32: return launch<float, float>(*plan, a, stream);
     case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F16: return launch<float, _Float16>(*plan, a, stream);

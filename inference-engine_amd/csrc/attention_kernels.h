@@ -1,0 +1,813 @@
+// Device code of attention over the paged cache: the rows of a work item (attention_plan.h)
+// against its keys. `narrow` holds up to 16 rows and streams the cache, a wave to itself;
+// `wide` holds many rows, whose waves share tiles of keys; `join` puts parts together.
+//
+// Both compute S^T = K Q^T and then O^T = V^T P^T. A matrix instruction returns a column of
+// S^T per lane, four (or eight) of its keys at a time, which is also how it takes a column of
+// P^T: the weights go from one product into the other without leaving their lane, and a
+// row's maximum, sum and rescaling are that lane's own. Which key sits at which place of the
+// contraction is free as long as V^T is given in the same order; the key orders below make
+// the two fit.
+#ifndef IEKV_ATTENTION_KERNELS_H_
+#define IEKV_ATTENTION_KERNELS_H_
+
+#include "attention_plan.h"
+#include "ops_common.h"
+
+namespace iekv_ops {
+
+using iekv_attention::Item;
+
+constexpr int kThreads = 256;
+constexpr int kWave = 64;
+constexpr int kWaves = kThreads / kWave;
+
+struct Args {
+  const int32_t* words;       // the plan's words: its items first
+  const void* k;
+  const void* v;
+  const void* q;
+  void* out;
+  float* part_o;              // [slots][kv_heads][head_dim]: sums of e^(s - m) v
+  float2* part_ml;            // [slots][kv_heads]: m (base 2) and the sum of e^(s - m)
+  int64_t positions_at, tables_at;
+  int64_t q_token_stride, q_head_stride;
+  int32_t window, sinks;      // window: INT32_MAX for all keys
+  int32_t kv_heads, group, head_dim, block_size;
+  uint32_t block_magic, block_shift;  // j / block_size = (mulhi(j, magic) + j) >> shift
+  uint32_t q_sign;            // flips the sign of q (in each half for 16 bits): scale >= 0
+  float scale;                // |scale| log2(e)
+};
+
+// --- elements ----------------------------------------------------------------------------
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+// BYTES from any address (caches and queries may begin at any element).
+template <int BYTES>
+__device__ __forceinline__ Words<(BYTES + 3) / 4> load_bytes(const void* p) {
+  Words<(BYTES + 3) / 4> r;
+  r.w[(BYTES - 1) / 4] = 0;
+  __builtin_memcpy(&r, p, BYTES);
+  return r;
+}
+
+// Two elements of the compute type in a word, rounded to nearest even.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<Bf16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<_Float16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
+
+// N elements of type C as elements of the compute type T (exact: T holds every value of C).
+template <typename T, typename C, int N>
+struct Convert {                                 // T == C
+  static __device__ __forceinline__ Words<N * sizeof(T) / 4> of(
+      const Words<(N * sizeof(C) + 3) / 4>& x) {
+    return x;
+  }
+};
+template <int N>
+struct Convert<Bf16, E4m3, N> {
+  static __device__ __forceinline__ Words<N / 2> of(const Words<(N + 3) / 4>& x) {
+    Words<N / 2> r;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      r.w[i] = __builtin_bit_cast(
+          uint32_t, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w[i / 2], 1.f, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w[i / 2], 1.f, false));
+    return r;
+  }
+};
+template <int N>
+struct Convert<_Float16, E4m3, N> {
+  static __device__ __forceinline__ Words<N / 2> of(const Words<(N + 3) / 4>& x) {
+    Words<N / 2> r;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+      r.w[i] = __builtin_bit_cast(
+          uint32_t, i % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.w[i / 2], 1.f, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.w[i / 2], 1.f, false));
+    return r;
+  }
+};
+template <int N>
+struct Convert<float, E4m3, N> {
+  static __device__ __forceinline__ Words<N> of(const Words<(N + 3) / 4>& x) {
+    Words<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      r.w[i] = __builtin_bit_cast(
+          uint32_t, to_float(E4m3{static_cast<uint8_t>(x.w[i / 4] >> (i % 4 * 8))}));
+    return r;
+  }
+};
+template <int N>
+struct Convert<float, Bf16, N> {
+  static __device__ __forceinline__ Words<N> of(const Words<N / 2>& x) {
+    Words<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      r.w[i] = i % 2 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16;
+    return r;
+  }
+};
+template <int N>
+struct Convert<float, _Float16, N> {
+  static __device__ __forceinline__ Words<N> of(const Words<N / 2>& x) {
+    Words<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint16_t h = static_cast<uint16_t>(x.w[i / 2] >> (i % 2 * 16));
+      r.w[i] = __builtin_bit_cast(uint32_t, static_cast<float>(__builtin_bit_cast(_Float16, h)));
+    }
+    return r;
+  }
+};
+
+// c += A B with 16 rows and columns over the lane's elements of A and B: eight of 16 bits
+// (32 in all), or four of 32 bits (16 in all).
+__device__ __forceinline__ f32x4 mma16(const Words<4>& a, const Words<4>& b, f32x4 c, Bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Words<4>& a, const Words<4>& b, f32x4 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Words<4>& a, const Words<4>& b, f32x4 c, float) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, a.w[e]),
+                                             __builtin_bit_cast(float, b.w[e]), c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f32x16 mma32(const Words<4>& a, const Words<4>& b, f32x16 c, Bf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(const Words<4>& a, const Words<4>& b, f32x16 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// --- keys --------------------------------------------------------------------------------
+
+__device__ __forceinline__ Item item_of(const Args& a, int32_t i) {
+  return reinterpret_cast<const Item*>(a.words)[i];
+}
+
+// Key number `v` of the item's ranges laid end to end.
+__device__ __forceinline__ int32_t key_at(const Item& it, int32_t v) {
+  const int32_t na = it.a1 - it.a0;
+  return v < na ? it.a0 + v : it.b0 + (v - na);
+}
+
+__device__ __forceinline__ bool sees(const Args& a, int32_t position, int32_t key) {
+  return key <= position && (key > position - a.window || key < a.sinks);
+}
+
+// Every position of the item sees every one of its keys v0 .. v1 - 1.
+__device__ __forceinline__ bool all_see(const Args& a, const Item& it, int32_t v0, int32_t v1) {
+  if (it.low == it.high) return true;            // its ranges are what the position sees
+  const int32_t first = key_at(it, v0), last = key_at(it, v1 - 1);
+  return last - first == v1 - 1 - v0 && last <= it.low &&
+         (first > it.high - a.window || last < a.sinks);
+}
+
+// A key's place in the pool: its block's entry in the tables, and its row there.
+struct Place {
+  int32_t block, within;
+};
+__device__ __forceinline__ Place place_of(const Args& a, const Item& it, int32_t j) {
+  const uint32_t b = (__umulhi(j, a.block_magic) + j) >> a.block_shift;
+  return {a.words[a.tables_at + it.table + b],
+          static_cast<int32_t>(j - b * static_cast<uint32_t>(a.block_size))};
+}
+__device__ __forceinline__ uint32_t row_of(const Args& a, Place p) {
+  return static_cast<uint32_t>(p.block) * static_cast<uint32_t>(a.block_size) + p.within;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
+  return x;
+}
+
+__device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// --- one row key by key ------------------------------------------------------------------
+
+// One query row by one wave: a lane scores a key of each 64, then holds two dimensions of
+// the output. A key the row does not see is not read for it at all, so that whatever the
+// cache holds there (infinities, NaN) stays out. The matrix kernels multiply such a V by a
+// weight of zero; where that, or anything else, leaves a NaN in their output they come here
+// for the item's rows, at a hundredth of their speed.
+template <typename T, typename C>
+__device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32_t row, int lane) {
+  const int32_t token = it.token0 + row / a.group, in_group = row % a.group;
+  const int32_t position = a.words[a.positions_at + token];
+  const int32_t d = a.head_dim;
+  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
+  const T* q = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
+  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
+  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
+  const float scale = a.q_sign ? -a.scale : a.scale;
+  const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0);
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int32_t v0 = 0; v0 < n; v0 += kWave) {
+    const bool in = v0 + lane < n;
+    const int32_t j = key_at(it, in ? v0 + lane : n - 1);
+    const int64_t at = row_of(a, place_of(a, it, j)) * width;
+    const bool seen = in && sees(a, position, j);
+    float s = -INFINITY;
+    if (seen) {
+      float dot = 0.f;
+      for (int32_t i = 0; i < d; ++i) dot = fmaf(to_float(q[i]), to_float(kc[at + i]), dot);
+      s = dot * scale;
+    }
+    // A score that is NaN stays in the sum, and the row is NaN as it has to be.
+    const float top = fmaxf(m, wave_max(s));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float fade = exp2f(m - base);
+    const float p = seen ? exp2f(s - base) : 0.f;
+    m = top;
+    l = l * fade + wave_sum(p);
+    o0 *= fade;
+    o1 *= fade;
+    uint64_t left = __ballot(seen);
+    while (left) {
+      const int i = __ffsll(static_cast<unsigned long long>(left)) - 1;
+      left &= left - 1;
+      const float pi = __shfl(p, i);
+      const int64_t ai = __shfl(at, i);
+      if (lane < d) o0 = fmaf(pi, to_float(vc[ai + lane]), o0);
+      if (lane + kWave < d) o1 = fmaf(pi, to_float(vc[ai + lane + kWave]), o1);
+    }
+  }
+  if (it.slot >= 0) {
+    const int64_t slot = static_cast<int64_t>(it.slot + row) * a.kv_heads + kv_head;
+    if (lane < d) a.part_o[slot * d + lane] = o0;
+    if (lane + kWave < d) a.part_o[slot * d + lane + kWave] = o1;
+    if (lane == 0) a.part_ml[slot] = {m, l};
+    return;
+  }
+  T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
+  if (lane < d) out[lane] = from_float<T>(o0 / l);
+  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
+}
+
+// --- narrow: up to 16 rows ---------------------------------------------------------------
+
+// N floats of a row's output, as T.
+template <typename T, int N>
+__device__ __forceinline__ void store_out(T* out, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    __builtin_memcpy(out, x, N * 4);
+  } else {
+    Words<N / 2> w;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w.w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+    __builtin_memcpy(out, &w, N * 2);
+  }
+}
+
+// What bounds it is the cache's stream: each wave has a step's K or V (64 keys; 32 of 32-bit
+// caches) in flight at any time, straight into the registers the products read, and nothing
+// but block ids passes through LDS. A wave takes every fourth step, and the four join at the
+// end. Of a pair of key tiles (32 keys), lane group g = lane / 16 holds the weights of keys
+// 8 g .. 8 g + 7: a lane loads those keys' V, EV dimensions each, and turns them in its own
+// registers into the EV operands of V^T (dimension c EV + t at place c of tile t).
+template <typename T, typename C, int DP>
+struct Narrow {
+  static constexpr int EK = sizeof(T) == 4 ? 4 : 8;       // K elements a lane feeds at a time
+  static constexpr int NK = DP / (4 * EK);                // and how many times
+  static constexpr int EV = DP <= 32 ? 2 : DP <= 64 ? 4 : 8;
+  static constexpr int KT = sizeof(C) == 4 ? 2 : 4;       // key tiles of 16 in a step
+  static constexpr int KS = 16 * KT;
+  using RawK = Words<EK * int(sizeof(C)) / 4>;
+  using RawV = Words<(EV * int(sizeof(C)) + 3) / 4>;
+  static constexpr int LDO = DP + 4;                      // floats of a row of o in LDS
+  struct Lds {
+    alignas(16) uint32_t rows[kWaves][2][KS];
+    float2 ml[kWaves][16];
+    alignas(16) float o[kWaves][16][LDO];
+    int32_t redo;
+  };
+};
+
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_narrow(
+    Args a, int32_t first) {
+  using N = Narrow<T, C, DP>;
+  constexpr int EK = N::EK, NK = N::NK, EV = N::EV, KT = N::KT, KS = N::KS;
+  __shared__ typename N::Lds lds;
+  // A group of more than 16 heads takes several workgroups for each of its tokens.
+  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
+  const int32_t kv_head = blockIdx.x % a.kv_heads;
+  const int32_t head0 = blockIdx.y * 16, heads = a.group - head0 < 16 ? a.group - head0 : 16;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
+  const int32_t d = a.head_dim, rows = it.tokens * heads;
+  const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
+  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  if (threadIdx.x == 0) lds.redo = 0;
+
+  // Q^T: row c, zeros past the rows and past the dimensions.
+  Words<4> q[NK];
+  int32_t position;
+  {
+    const int32_t row = c < rows ? c : 0, token = it.token0 + row / heads;
+    const int64_t head = static_cast<int64_t>(kv_head) * a.group + head0 + row % heads;
+    position = a.words[a.positions_at + token];
+    const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int32_t d0 = (4 * i + g) * EK;
+      const bool in = c < rows && d0 < d;
+      q[i] = load_bytes<EK * sizeof(T)>(at + (d0 < d ? d0 : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[i].w[e] = in ? q[i].w[e] ^ a.q_sign : 0;
+    }
+  }
+  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
+  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d +
+                (c * EV < d ? c * EV : 0);
+
+  const auto place = [&](int32_t s) {
+    const int32_t v = s * KS + lane % KS;
+    return place_of(a, it, key_at(it, v < n ? v : n - 1));
+  };
+  const auto keep = [&](int half, Place p) {
+    if (lane < KS) lds.rows[wave][half][lane] = row_of(a, p);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  typename N::RawK k[KT][NK];
+  const auto load_k = [&](int half) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      const uint32_t row =
+          lds.rows[wave][half][t / 2 * 32 + (c >> 2) * 8 + t % 2 * 4 + (c & 3)];
+      const C* at = kc + row * width;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const int32_t d0 = (4 * i + g) * EK;
+        k[t][i] = load_bytes<EK * sizeof(C)>(at + (d0 < d ? d0 : 0));
+        if (i == NK - 1 || sizeof(T) == 4)
+          for (uint32_t& w : k[t][i].w) w = d0 < d ? w : 0;
+      }
+    }
+  };
+
+  f32x4 o[EV];
+#pragma unroll
+  for (int t = 0; t < EV; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;                 // l: of the lane's own keys
+
+  int half = 0;
+  Place next{0, 0};
+  if (wave < steps) {
+    keep(0, place(wave));
+    load_k(0);
+    next = place(wave + kWaves);
+  }
+  for (int32_t s = wave; s < steps; s += kWaves, half ^= 1) {
+    keep(half ^ 1, next);
+    typename N::RawV v[KT / 2][8];
+#pragma unroll
+    for (int p = 0; p < KT / 2; ++p)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t row = lds.rows[wave][half][p * 32 + g * 8 + e];
+        v[p][e] = load_bytes<EV * sizeof(C)>(vc + row * width);
+      }
+    f32x4 sc[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        sc[t] = mma16(Convert<T, C, EK>::of(k[t][i]), q[i], sc[t], T{});
+    }
+    if (s + kWaves < steps) load_k(half ^ 1);
+    next = place(s + 2 * kWaves);
+
+    const int32_t v0 = s * KS;
+    if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int32_t at = v0 + t / 2 * 32 + g * 8 + t % 2 * 4 + r;
+          if (at >= n || !sees(a, position, key_at(it, at))) sc[t][r] = -INFINITY;
+        }
+    }
+    float top = m;
+    {
+      float x = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][r]);
+      x = fmaxf(x, __shfl_xor(x, 16));
+      x = fmaxf(x, __shfl_xor(x, 32));
+      top = fmaxf(m, x * a.scale);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    if (__any(top > m)) {
+      const float fade = power2(m - base);
+      l *= fade;
+#pragma unroll
+      for (int t = 0; t < EV; ++t) o[t] *= fade;
+      m = top;
+    }
+    float p[KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[t][r] = power2(fmaf(sc[t][r], a.scale, -base));
+        l += p[t][r];
+      }
+#pragma unroll
+    for (int pr = 0; pr < KT / 2; ++pr) {
+      if constexpr (sizeof(T) == 4) {
+        Words<EV> x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = Convert<T, C, EV>::of(v[pr][e]);
+#pragma unroll
+        for (int t = 0; t < EV; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x[e].w[t]),
+                                                        p[2 * pr + e / 4][e % 4], o[t], 0, 0, 0);
+      } else {
+        Words<EV / 2> x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = Convert<T, C, EV>::of(v[pr][e]);
+        Words<4> w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w.w[i] = pack2<T>(p[2 * pr + i / 2][i % 2 * 2], p[2 * pr + i / 2][i % 2 * 2 + 1]);
+#pragma unroll
+        for (int t = 0; t < EV; ++t) {
+          Words<4> vt;                          // dimension c EV + t of keys 8 g ..
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            vt.w[i] = __builtin_amdgcn_perm(x[2 * i + 1].w[t / 2], x[2 * i].w[t / 2],
+                                            t % 2 ? 0x07060302u : 0x05040100u);
+          o[t] = mma16(vt, w, o[t], T{});
+        }
+      }
+    }
+  }
+
+  // The waves' parts.
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (lane < 16) lds.ml[wave][lane] = {m, l};
+  __syncthreads();
+  float all = -INFINITY;
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, lds.ml[w][c].x);
+  const float fade = power2(m - (all == -INFINITY ? 0.f : all));
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int t = 0; t < EV; ++t)
+      if ((g * 4 + r) * EV + t < DP) lds.o[wave][c][(g * 4 + r) * EV + t] = o[t][r] * fade;
+  __syncthreads();
+  // Eight dimensions a thread.
+  const int32_t row = threadIdx.x / 16, d0 = threadIdx.x % 16 * 8;
+  const bool mine = row < rows && d0 < d;
+  float x[8], total = 0.f, most = -INFINITY;
+  if (mine) {
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, lds.ml[w][row].x);
+    const float from = most == -INFINITY ? 0.f : most;
+    for (int w = 0; w < kWaves; ++w)
+      total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
+    bool odd = total != total;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = lds.o[0][row][d0 + i];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) x[i] += lds.o[w][row][d0 + i];
+      odd = odd || x[i] != x[i];
+    }
+    if (odd) lds.redo = 1;
+  }
+  __syncthreads();
+  if (lds.redo) {
+    for (int32_t r = wave; r < rows; r += kWaves)
+      attend_row<T, C>(a, it, kv_head, r / heads * a.group + head0 + r % heads, lane);
+    return;
+  }
+  if (!mine) return;
+  const int32_t in_group = head0 + row % heads;
+  if (it.slot >= 0) {
+    const int64_t slot =
+        static_cast<int64_t>(it.slot + row / heads * a.group + in_group) * a.kv_heads + kv_head;
+    __builtin_memcpy(a.part_o + slot * d + d0, x, 32);
+    if (d0 == 0) a.part_ml[slot] = {most, total};
+    return;
+  }
+  const int64_t token = it.token0 + row / heads;
+  const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] /= total;
+  store_out<T, 8>(static_cast<T*>(a.out) +
+                      (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d + d0, x);
+}
+
+// --- wide: many rows ---------------------------------------------------------------------
+
+// Four waves, 32 R rows each, share tiles of 64 keys in LDS, two tiles in turn: a tile's
+// loads are issued before the products of the one before it and stored to LDS after them.
+// V^T is read from V's rows by the transposing LDS load (a group of 16 lanes reads 4 keys of
+// 16 dimensions, and each lane gets one dimension of the four). Row strides in LDS put what
+// the lanes read at a time into different banks: 16 bytes past a multiple of 128 for K's
+// 16-byte reads, 32 bytes past for V's four rows of 32 bytes.
+template <typename T, int DP>
+struct Wide {
+  static constexpr int KS = 64;
+  static constexpr int KW = DP * 2 + 16, VW = DP * 2 + 32;   // bytes of a row in LDS
+  static constexpr int CHUNKS = DP / 8;                      // of eight elements, a row's
+  static constexpr int LOADS = KS * CHUNKS / kThreads;       // chunks a thread brings
+  struct Lds {
+    alignas(16) char k[2][KS * KW];
+    alignas(16) char v[2][KS * VW];
+    uint32_t rows[2][KS];
+    int32_t redo;
+  };
+};
+
+__device__ __forceinline__ Words<2> transposed(const char* lds) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(
+      Words<2>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)const_cast<char*>(lds)));
+}
+
+template <typename T, typename C, int DP, int R>
+__global__ __launch_bounds__(kThreads, R == 1 ? 2 : 1) void attend_wide(Args a, int32_t first) {
+  using W = Wide<T, DP>;
+  constexpr int KS = W::KS, KW = W::KW, VW = W::VW, CHUNKS = W::CHUNKS, LOADS = W::LOADS;
+  constexpr int NQ = DP / 16, ND = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char shared[];
+  auto& lds = *reinterpret_cast<typename W::Lds*>(shared);
+  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
+  const int32_t kv_head = blockIdx.x % a.kv_heads;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, h = lane / 32, c = lane % 32;
+  const int32_t d = a.head_dim, rows = it.tokens * a.group;
+  const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
+  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  if (threadIdx.x == 0) lds.redo = 0;
+
+  Words<4> q[R][NQ];
+  int32_t position[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int32_t r = (wave * R + u) * 32 + c, row = r < rows ? r : 0;
+    const int32_t token = it.token0 + row / a.group;
+    const int64_t head = static_cast<int64_t>(kv_head) * a.group + row % a.group;
+    position[u] = a.words[a.positions_at + token];
+    const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int32_t d0 = i * 16 + h * 8;
+      const bool in = r < rows && d0 < d;
+      q[u][i] = load_bytes<16>(at + (d0 < d ? d0 : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[u][i].w[e] = in ? q[u][i].w[e] ^ a.q_sign : 0;
+    }
+  }
+
+  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
+  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
+  const auto place = [&](int32_t s) {
+    const int32_t v = s * KS + lane;
+    return place_of(a, it, key_at(it, v < n ? v : n - 1));
+  };
+  using Raw = Words<8 * int(sizeof(C)) / 4>;
+  Raw kr[LOADS], vr[LOADS];
+  const auto load = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int32_t at = threadIdx.x + i * kThreads, d0 = at % CHUNKS * 8;
+      const int64_t from = lds.rows[half][at / CHUNKS] * width + (d0 < d ? d0 : 0);
+      kr[i] = load_bytes<8 * sizeof(C)>(kc + from);
+      vr[i] = load_bytes<8 * sizeof(C)>(vc + from);
+    }
+  };
+  const auto store = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int32_t at = threadIdx.x + i * kThreads, key = at / CHUNKS, ch = at % CHUNKS;
+      Words<4> k = Convert<T, C, 8>::of(kr[i]), v = Convert<T, C, 8>::of(vr[i]);
+      if (ch * 8 >= d) k = v = Words<4>{};
+      *reinterpret_cast<u32x4*>(lds.k[half] + key * KW + ch * 16) = __builtin_bit_cast(u32x4, k);
+      *reinterpret_cast<u32x4*>(lds.v[half] + key * VW + ch * 16) = __builtin_bit_cast(u32x4, v);
+    }
+  };
+
+  f32x16 o[R][ND];
+  float m[R], l[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[u][t][r] = 0.f;
+  }
+
+  if (wave == 0) {
+    lds.rows[0][lane] = row_of(a, place(0));
+    lds.rows[1][lane] = row_of(a, place(1));
+  }
+  __syncthreads();
+  load(0);
+  store(0);
+  __syncthreads();
+  for (int32_t s = 0; s < steps; ++s) {
+    const int half = s & 1;
+    const bool more = s + 1 < steps;
+    if (more) load(half ^ 1);
+    Place next{0, 0};
+    if (wave == 0 && more) next = place(s + 2);
+
+    f32x16 sc[R][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[u][t][r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const Words<4> k = __builtin_bit_cast(
+            Words<4>,
+            *reinterpret_cast<const u32x4*>(lds.k[half] + (t * 32 + c) * KW + i * 32 + h * 16));
+#pragma unroll
+        for (int u = 0; u < R; ++u) sc[u][t] = mma32(k, q[u][i], sc[u][t], T{});
+      }
+    }
+
+    const int32_t v0 = s * KS;
+    if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t at = v0 + t * 32 + r / 4 * 8 + h * 4 + r % 4;
+          const int32_t j = key_at(it, at);
+#pragma unroll
+          for (int u = 0; u < R; ++u)
+            if (at >= n || !sees(a, position[u], j)) sc[u][t][r] = -INFINITY;
+        }
+    }
+    Words<4> p[R][4];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      float x = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x = fmaxf(x, sc[u][t][r]);
+      x = fmaxf(x, __shfl_xor(x, 32));
+      const float top = fmaxf(m[u], x * a.scale), base = top == -INFINITY ? 0.f : top;
+      if (__any(top > m[u])) {
+        const float fade = power2(m[u] - base);
+        l[u] *= fade;
+#pragma unroll
+        for (int t = 0; t < ND; ++t) o[u][t] *= fade;
+        m[u] = top;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float p0 = power2(fmaf(sc[u][t][r], a.scale, -base));
+          const float p1 = power2(fmaf(sc[u][t][r + 1], a.scale, -base));
+          l[u] += p0 + p1;
+          p[u][t * 2 + r / 8].w[r % 8 / 2] = pack2<T>(p0, p1);
+        }
+    }
+    // Of 16 keys, half h holds the weights of 4 h .. 4 h + 3 and 8 + 4 h ..
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const char* at = lds.v[half] + (i * 16 + h * 4 + c % 16 / 4) * VW + t * 64 +
+                         c / 16 * 32 + c % 4 * 8;
+        const Words<2> lo = transposed(at), hi = transposed(at + 8 * VW);
+        const Words<4> v{{lo.w[0], lo.w[1], hi.w[0], hi.w[1]}};
+#pragma unroll
+        for (int u = 0; u < R; ++u) o[u][t] = mma32(v, p[u][i], o[u][t], T{});
+      }
+    if (more) store(half ^ 1);
+    if (wave == 0 && more) lds.rows[half][lane] = row_of(a, next);
+    __syncthreads();
+  }
+
+  bool odd = false;
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    l[u] += __shfl_xor(l[u], 32);
+    if ((wave * R + u) * 32 + c >= rows) continue;
+    odd = odd || l[u] != l[u];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        odd = odd || (t * 32 + r / 4 * 8 < d && o[u][t][r] != o[u][t][r]);
+  }
+  if (odd) lds.redo = 1;
+  __syncthreads();
+  if (lds.redo) {
+    for (int32_t r = wave; r < rows; r += kWaves) attend_row<T, C>(a, it, kv_head, r, lane);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < R; ++u) {
+    const int32_t row = (wave * R + u) * 32 + c;
+    if (row >= rows) continue;
+    const int64_t token = it.token0 + row / a.group;
+    const int64_t head = static_cast<int64_t>(kv_head) * a.group + row % a.group;
+    const int64_t slot = static_cast<int64_t>(it.slot + row) * a.kv_heads + kv_head;
+    T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
+    const float inverse = 1.f / l[u];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int32_t d0 = t * 32 + r * 2 + h * 4;
+        if (d0 >= d) continue;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = it.slot >= 0 ? o[u][t][r + e] : o[u][t][r + e] * inverse;
+        if (it.slot >= 0)
+          __builtin_memcpy(a.part_o + slot * d + d0, x, 16);
+        else
+          store_out<T, 4>(out + d0, x);
+      }
+    if (it.slot >= 0 && h == 0) a.part_ml[slot] = {m[u], l[u]};
+  }
+}
+
+// --- join --------------------------------------------------------------------------------
+
+// Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, in
+// the order of the parts. One wave a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* tokens,
+                                                       const int32_t* starts,
+                                                       const int32_t* parts, int32_t n) {
+  const int lane = threadIdx.x % kWave;
+  const int32_t heads = a.kv_heads * a.group, d = a.head_dim;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
+  if (row >= static_cast<int64_t>(n) * heads) return;
+  const int32_t entry = static_cast<int32_t>(row / heads), head = static_cast<int32_t>(row % heads);
+  const int32_t kv_head = head / a.group, in_group = head % a.group;
+  const int32_t p0 = starts[entry], p1 = starts[entry + 1];
+  float m = -INFINITY;
+  for (int32_t p = p0; p < p1; ++p)
+    m = fmaxf(m, a.part_ml[static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int32_t p = p0; p < p1; ++p) {
+    const int64_t slot = static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
+    const float2 ml = a.part_ml[slot];
+    const float w = exp2f(ml.x - base);
+    l = fmaf(w, ml.y, l);
+    if (lane < d) o0 = fmaf(w, a.part_o[slot * d + lane], o0);
+    if (lane + kWave < d) o1 = fmaf(w, a.part_o[slot * d + lane + kWave], o1);
+  }
+  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(tokens[entry]) * heads + head) * d;
+  if (lane < d) out[lane] = from_float<T>(o0 / l);
+  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
+}
+
+}  // namespace iekv_ops
+
+#endif  // IEKV_ATTENTION_KERNELS_H_
