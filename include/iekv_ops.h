@@ -88,7 +88,7 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
  * top_ids [n_rows][top]. Logits of -inf have probability zero. A row of nothing but -inf
  * has log probabilities of -inf and entropy 0; a row with a NaN or +inf has NaN log
  * probabilities and entropy (its alternatives put NaN first); a token outside 0..vocab-1
- * has log probability NaN. The workspace (iekv_logprobs_workspace bytes) is used until the
+ * has log probability NaN. The workspace (iekv_logprobs_workspace bytes, aligned to 16) is used until the
  * call's kernels end. */
 int64_t iekv_logprobs_workspace(int32_t type, int64_t n_rows, int64_t vocab, int32_t top);
 int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,

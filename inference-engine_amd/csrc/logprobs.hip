@@ -6,6 +6,12 @@
 // (x_t - (m + ln s) would lose ln s next to a type's lowest value, a usual mask.)
 // The alternatives are ordered by a 64-bit key: the logit as a whole number that orders as
 // the values do (NaN above all), then the index, smaller first, so that no two are alike.
+//
+// The logits are read once: a row is cut into parts of at most 8,192, each held whole in the
+// registers of a workgroup, which leaves m, s, w and its part's alternatives to a second
+// launch that joins a row's parts in their order. Rows of one part are done in one launch.
+// How a row is cut depends on the vocabulary alone, so a row's result does not depend on the
+// rows beside it.
 #include "ops_common.h"
 
 #include <cmath>
@@ -16,6 +22,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWave = 64;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kCandidates = 512;   // of a part, or of a row's parts, that are ranked at once
+constexpr int kSmall = 8, kLarge = 32;  // logits a thread holds
 
 // A logit as an unsigned number of the same order; NaN is the largest. Zeros of both signs
 // are equal.
@@ -25,16 +34,50 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// Keys of logits are above 0.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
   return static_cast<uint64_t>(ordered(x)) << 32 | (0xffffffffu - index);
 }
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t o = static_cast<uint32_t>(key >> 32);
+  return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) {
+  return 0xffffffffu - static_cast<uint32_t>(key);
+}
 
+__device__ __forceinline__ uint64_t shuffled(uint64_t k, int mask) {
+  return __shfl_xor(static_cast<unsigned long long>(k), mask);
+}
 __device__ __forceinline__ uint64_t wave_top(uint64_t k) {
   for (int s = 32; s; s >>= 1) {
-    const uint64_t other = __shfl_xor(static_cast<unsigned long long>(k), s);
+    const uint64_t other = shuffled(k, s);
     k = other > k ? other : k;
   }
   return k;
+}
+__device__ __forceinline__ float wave_max(float x) {
+  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
+  return x;
+}
+
+// The lanes' values in falling order (Batcher's bitonic network).
+template <typename V>
+__device__ __forceinline__ V wave_sorted(V x, int lane) {
+#pragma unroll
+  for (int size = 2; size <= kWave; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step; step /= 2) {
+      const V other = __shfl_xor(x, step);
+      const bool first = !(lane & step), falling = !(lane & size);
+      const bool larger = other > x;
+      x = (first == falling) == larger ? other : x;
+    }
+  return x;
 }
 
 // Sums of a part of a row: m, s and w above.
@@ -42,74 +85,289 @@ struct Sums {
   float m, s, w;
 };
 
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-  const float m = a.m > b.m || a.m != a.m ? a.m : b.m;      // a NaN stays
-  const float base = m == -INFINITY ? 0.f : m;
-  const float da = a.m - base, db = b.m - base;
-  const float ea = expf(da), eb = expf(db);
-  // e^(x - m) (x - m) = e^(m_a - m) (e^(x - m_a) (x - m_a) + e^(x - m_a) (m_a - m))
-  const float wa = ea > 0.f ? ea * fmaf(a.s, da, a.w) : 0.f;
-  const float wb = eb > 0.f ? eb * fmaf(b.s, db, b.w) : 0.f;
-  return {m, fmaf(a.s, ea, b.s * eb), wa + wb};
+// e^d for d <= 0, flushed to zero where e^d is no normal number.
+__device__ __forceinline__ float exponential(float d) {
+  return __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+}
+
+// The part's sums as they count next to a maximum m of all parts.
+__device__ __forceinline__ Sums moved(Sums a, float m) {
+  const float d = a.m == -INFINITY ? 0.f : a.m - m;
+  const float e = exponential(d);
+  // e^(x - m) (x - m) = e^(a.m - m) (e^(x - a.m) (x - a.m) + e^(x - a.m) (a.m - m))
+  return {m, a.s * e, e > 0.f ? e * fmaf(a.s, d, a.w) : 0.f};
+}
+
+// What a row's results are written from.
+struct Scores {
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_ids;
+  int32_t vocab, top;
+};
+
+// A row of nothing but -inf has no sum.
+__device__ __forceinline__ float logprob_of(float x, const Sums& a, float log_s) {
+  return a.s == 0.f ? -INFINITY : (x - a.m) - log_s;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void score_rows(const T* logits, int64_t stride,
-                                                       int32_t vocab, const int64_t* tokens,
-                                                       int32_t top, float* logprobs,
-                                                       float* entropy, float* top_logprobs,
-                                                       int64_t* top_ids) {
-  const int64_t row = blockIdx.x;
+__device__ __forceinline__ void write_row(const Scores& out, const T* x, int64_t row,
+                                          const Sums& a, float log_s) {
+  const int64_t t = out.tokens[row];
+  out.logprobs[row] = t < 0 || t >= out.vocab ? NAN : logprob_of(to_float(x[t]), a, log_s);
+  out.entropy[row] = a.s == 0.f ? 0.f : log_s - a.w / a.s;
+}
+
+__device__ __forceinline__ void write_top(const Scores& out, int64_t row, int32_t rank,
+                                          uint64_t key, const Sums& a, float log_s) {
+  out.top_logprobs[row * out.top + rank] = logprob_of(logit_of(key), a, log_s);
+  out.top_ids[row * out.top + rank] = index_of(key);
+}
+
+// Parts of rows in the workspace: their sums, then the keys of their alternatives.
+struct Parts {
+  Sums* sums;        // [rows][parts]
+  uint64_t* keys;    // [rows][parts][top], falling; 0 past the part's logits
+  int32_t parts, size;
+};
+
+// One part of a row by one workgroup.
+//
+// The alternatives: a lower bound of the part's k-th largest logit is found from the lanes'
+// own largest ones. Each wave sorts its 64: if every wave has ceil(k / 4) lanes of at least
+// b, or one wave has k, there are k logits of at least b. What reaches the bound, a few more
+// than k as a rule, is put on a list in LDS and ranked by counting the larger keys. Where
+// more reach it than the list holds (rows of equal logits, all but barred rows) or the part
+// holds a NaN, the largest key is taken k times instead.
+template <typename T, int HELD>
+__global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t stride, Scores out,
+                                                       Parts parts) {
+  constexpr int VEC = 16 / sizeof(T), LOADS = HELD / VEC;
+  const int64_t row = blockIdx.x / parts.parts;
+  const int32_t part = blockIdx.x % parts.parts, tid = threadIdx.x;
+  const int wave = tid / kWave, lane = tid % kWave;
+  const int32_t first = part * parts.size;
+  const int32_t n = parts.size < out.vocab - first ? parts.size : out.vocab - first;
   const T* x = logits + row * stride;
-  __shared__ Sums sums[kThreads];
-  __shared__ uint64_t best[kThreads / kWave];
-  Sums mine{-INFINITY, 0.f, 0.f};
-  for (int32_t i = threadIdx.x; i < vocab; i += kThreads)
-    mine = join(mine, {to_float(x[i]), 1.f, 0.f});
-  sums[threadIdx.x] = mine;
-  __syncthreads();
-  for (int n = kThreads / 2; n; n >>= 1) {
-    if (threadIdx.x < n) sums[threadIdx.x] = join(sums[threadIdx.x], sums[threadIdx.x + n]);
-    __syncthreads();
+  __shared__ float most[kWaves];
+  __shared__ float2 sums[kWaves], bounds[kWaves];
+  __shared__ uint64_t list[kCandidates];
+  __shared__ int32_t listed;
+
+  // Logit v (of this thread's `HELD`) is number (v / VEC * kThreads + tid) * VEC + v % VEC.
+  float held[HELD];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int32_t at = (i * kThreads + tid) * VEC;
+    T e[VEC];
+    if (at + VEC <= n) {
+      __builtin_memcpy(e, x + first + at, sizeof(e));
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) held[i * VEC + j] = to_float(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        held[i * VEC + j] = at + j < n ? to_float(x[first + at + j]) : -INFINITY;
+    }
   }
-  const Sums all = sums[0];
+  const auto index = [&](int v) { return (v / VEC * kThreads + tid) * VEC + v % VEC; };
+
+  float mine = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < HELD; ++v) mine = fmaxf(mine, held[v]);
+  const float of_wave = wave_max(mine);
+  if (lane == 0) most[wave] = of_wave;
+  if (tid == 0) listed = 0;
+  __syncthreads();
+  Sums all;
+  all.m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+  const float base = all.m == -INFINITY ? 0.f : all.m;
+  float s = 0.f, w = 0.f;
+#pragma unroll
+  for (int v = 0; v < HELD; ++v) {
+    const float d = held[v] - base, e = exponential(d);
+    s += e;
+    w = fmaf(e, fmaxf(d, -200.f), w);     // e is 0 from -104 on; 0 * -inf would be NaN
+  }
+  s = wave_sum(s);
+  w = wave_sum(w);
+  if (lane == 0) sums[wave] = {s, w};
+  const int32_t top = out.top;
+  if (top) {
+    float each = of_wave, alone = of_wave;  // the wave's ceil(k / 4)-th and k-th largest lane
+    if (top > 1) {
+      const float sorted = wave_sorted(mine, lane);
+      each = __shfl(sorted, (top + kWaves - 1) / kWaves - 1);
+      alone = __shfl(sorted, top - 1);
+    }
+    if (lane == 0) bounds[wave] = {each, alone};
+  }
+  __syncthreads();
+  all.s = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
+  all.w = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
   const float log_s = logf(all.s);
-  if (threadIdx.x == 0) {
-    const int64_t t = tokens[row];
-    const bool none = all.m == -INFINITY;
-    logprobs[row] = t < 0 || t >= vocab ? NAN : none ? -INFINITY : (to_float(x[t]) - all.m) - log_s;
-    entropy[row] = none ? 0.f : log_s - all.w / all.s;
+  const bool whole = parts.parts == 1;
+  if (tid == 0) {
+    if (whole)
+      write_row(out, x, row, all, log_s);
+    else
+      parts.sums[blockIdx.x] = all;
+  }
+  if (!top) return;
+
+  const auto put = [&](int32_t rank, uint64_t key) {
+    if (whole)
+      write_top(out, row, rank, key, all, log_s);
+    else
+      parts.keys[static_cast<int64_t>(blockIdx.x) * top + rank] = key;
+  };
+  const float bound =
+      fmaxf(fminf(fminf(bounds[0].x, bounds[1].x), fminf(bounds[2].x, bounds[3].x)),
+            fmaxf(fmaxf(bounds[0].y, bounds[1].y), fmaxf(bounds[2].y, bounds[3].y)));
+  if (mine >= bound) {
+#pragma unroll
+    for (int v = 0; v < HELD; ++v)
+      if (held[v] >= bound && index(v) < n) {
+        const int at = atomicAdd(&listed, 1);
+        if (at < kCandidates) list[at] = key_of(held[v], first + index(v));
+      }
+  }
+  __syncthreads();
+  const int32_t count = listed;
+  if (count <= kCandidates && all.s == all.s) {
+    for (int32_t i = tid; i < count; i += kThreads) {
+      const uint64_t key = list[i];
+      int32_t rank = 0;
+      for (int32_t j = 0; j < count; ++j) rank += list[j] > key;
+      if (rank < top) put(rank, key);
+    }
+    // A part of fewer logits than alternatives (of a row of several parts).
+    for (int32_t rank = count + tid; rank < top; rank += kThreads) put(rank, 0);
+    return;
   }
   uint64_t below = ~uint64_t(0);
-  for (int32_t k = 0; k < top; ++k) {
+  for (int32_t rank = 0; rank < top; ++rank) {
     uint64_t key = 0;
-    for (int32_t i = threadIdx.x; i < vocab; i += kThreads) {
-      const uint64_t c = key_of(to_float(x[i]), i);
-      key = c < below && c > key ? c : key;
+#pragma unroll
+    for (int v = 0; v < HELD; ++v) {
+      const uint64_t k = index(v) < n ? key_of(held[v], first + index(v)) : 0;
+      key = k < below && k > key ? k : key;
     }
     key = wave_top(key);
-    if (threadIdx.x % kWave == 0) best[threadIdx.x / kWave] = key;
     __syncthreads();
-    for (int w = 0; w < kThreads / kWave; ++w) key = best[w] > key ? best[w] : key;
+    if (lane == 0) list[wave] = key;
+    __syncthreads();
+    for (int i = 0; i < kWaves; ++i) key = list[i] > key ? list[i] : key;
     below = key;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint32_t id = 0xffffffffu - static_cast<uint32_t>(key);
-      const float v = to_float(x[id]);
-      top_logprobs[row * top + k] = all.m == -INFINITY ? -INFINITY : (v - all.m) - log_s;
-      top_ids[row * top + k] = id;
-    }
+    if (tid == 0) put(rank, key);
   }
 }
 
+// A row's parts, by one wave. Bounds of the row's k-th largest key, as above: any part's
+// k-th, and the least of the parts' ceil(k / parts)-th.
 template <typename T>
-int launch(const void* logits, int64_t stride, int64_t n_rows, int64_t vocab,
-           const int64_t* tokens, int32_t top, float* logprobs, float* entropy,
-           float* top_logprobs, int64_t* top_ids, hipStream_t stream) {
-  hipLaunchKernelGGL((score_rows<T>), dim3(n_rows), dim3(kThreads), 0, stream,
-                     static_cast<const T*>(logits), stride, static_cast<int32_t>(vocab), tokens,
-                     top, logprobs, entropy, top_logprobs, top_ids);
+__global__ __launch_bounds__(kThreads) void join_rows(const T* logits, int64_t stride,
+                                                      int64_t n_rows, Scores out, Parts parts) {
+  __shared__ uint64_t lists[kWaves][kCandidates];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
+  if (row >= n_rows) return;
+  const Sums* sums = parts.sums + row * parts.parts;
+  const int32_t n = parts.parts, top = out.top;
+  const uint64_t* keys = parts.keys + row * n * top;
+  uint64_t any = 0, least = ~uint64_t(0);
+  const int32_t each = (top + n - 1) / n;
+  float m = -INFINITY;
+  for (int32_t p = lane; p < n; p += kWave) {
+    m = fmaxf(m, sums[p].m);
+    if (top) {
+      const uint64_t last = keys[static_cast<int64_t>(p) * top + top - 1];
+      const uint64_t share = keys[static_cast<int64_t>(p) * top + each - 1];
+      any = last > any ? last : any;
+      least = share < least ? share : least;
+    }
+  }
+  Sums all{wave_max(m), 0.f, 0.f};
+  for (int32_t p = lane; p < n; p += kWave) {
+    const Sums a = moved(sums[p], all.m);
+    all.s += a.s;
+    all.w += a.w;
+  }
+  all.s = wave_sum(all.s);
+  all.w = wave_sum(all.w);
+  const float log_s = logf(all.s);
+  if (lane == 0) write_row(out, logits + row * stride, row, all, log_s);
+  if (!top) return;
+
+  any = wave_top(any);
+  least = ~wave_top(~least);
+  const uint64_t bound = any > least ? any : least;
+  uint64_t* list = lists[wave];
+  int32_t count = 0;
+  const int32_t total = n * top;
+  for (int32_t i = 0; i < total && count <= kCandidates; i += kWave) {
+    const uint64_t key = i + lane < total ? keys[i + lane] : 0;
+    const uint64_t in = __ballot(key && key >= bound);
+    const int32_t at = count + __popcll(in & ((uint64_t(1) << lane) - 1));
+    if (key && key >= bound && at < kCandidates) list[at] = key;
+    count += __popcll(in);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (count <= kCandidates) {
+    for (int32_t i = lane; i < count; i += kWave) {
+      const uint64_t key = list[i];
+      int32_t rank = 0;
+      for (int32_t j = 0; j < count; ++j) rank += list[j] > key;
+      if (rank < top) write_top(out, row, rank, key, all, log_s);
+    }
+    return;
+  }
+  uint64_t below = ~uint64_t(0);
+  for (int32_t rank = 0; rank < top; ++rank) {
+    uint64_t key = 0;
+    for (int32_t i = lane; i < total; i += kWave)
+      key = keys[i] < below && keys[i] > key ? keys[i] : key;
+    below = wave_top(key);
+    if (lane == 0) write_top(out, row, rank, below, all, log_s);
+  }
+}
+
+// How rows are cut: parts of equal size (a multiple of 8) that a workgroup can hold.
+struct Cut {
+  int32_t held, parts, size;
+};
+
+Cut cut_of(int64_t vocab) {
+  const int held = vocab <= kSmall * kThreads ? kSmall : kLarge;
+  const int64_t most = int64_t(held) * kThreads, parts = (vocab + most - 1) / most;
+  return {held, static_cast<int32_t>(parts),
+          static_cast<int32_t>(((vocab + parts - 1) / parts + 7) / 8 * 8)};
+}
+
+template <typename T>
+int launch(const Cut& cut, const T* logits, int64_t stride, int64_t n_rows, const Scores& out,
+           void* workspace, hipStream_t stream) {
+  // Parts of the rounded size may be one fewer.
+  const int32_t count = (out.vocab + cut.size - 1) / cut.size;
+  auto* keys = static_cast<uint64_t*>(workspace);
+  Parts parts{reinterpret_cast<Sums*>(keys + n_rows * count * out.top), keys, count, cut.size};
+  const dim3 grid(static_cast<uint32_t>(n_rows * count));
+  if (cut.held == kSmall)
+    hipLaunchKernelGGL((score_part<T, kSmall>), grid, dim3(kThreads), 0, stream, logits, stride, out,
+                       parts);
+  else
+    hipLaunchKernelGGL((score_part<T, kLarge>), grid, dim3(kThreads), 0, stream, logits, stride, out,
+                       parts);
   IEKV_OPS_HIP(hipGetLastError());
+  if (count > 1) {
+    hipLaunchKernelGGL((join_rows<T>), dim3(static_cast<uint32_t>((n_rows + kWaves - 1) / kWaves)),
+                       dim3(kThreads), 0, stream, logits, stride, n_rows, out, parts);
+    IEKV_OPS_HIP(hipGetLastError());
+  }
   return IEKV_OK;
 }
 
@@ -117,7 +375,11 @@ int launch(const void* logits, int64_t stride, int64_t n_rows, int64_t vocab,
 
 extern "C" {
 
-int64_t iekv_logprobs_workspace(int32_t, int64_t, int64_t, int32_t) { return 0; }
+int64_t iekv_logprobs_workspace(int32_t, int64_t n_rows, int64_t vocab, int32_t top) {
+  if (n_rows < 1 || vocab < 1 || vocab > INT32_MAX || top < 0) return 0;
+  const Cut cut = cut_of(vocab);
+  return cut.parts == 1 ? 0 : n_rows * cut.parts * int64_t(sizeof(Sums) + top * sizeof(uint64_t));
+}
 
 int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,
                   int64_t vocab, const int64_t* tokens, int32_t top, float* logprobs,
@@ -125,7 +387,7 @@ int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t 
                   int64_t workspace_bytes, hipStream_t stream) {
   if (n_rows < 0 || n_rows > INT32_MAX)
     return set_error(IEKV_ERR_INVALID, "n_rows %lld out of range", static_cast<long long>(n_rows));
-  if (vocab < 1 || vocab > INT32_MAX)
+  if (vocab < 1 || vocab > INT32_MAX - 8 * kThreads * kLarge)
     return set_error(IEKV_ERR_INVALID, "vocab %lld out of range", static_cast<long long>(vocab));
   if (top < 0 || top > IEKV_LOGPROBS_MAX_TOP || top > vocab)
     return set_error(IEKV_ERR_INVALID, "top %d out of range for a vocabulary of %lld (at most %d)",
@@ -138,21 +400,29 @@ int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t 
   if (!n_rows) return IEKV_OK;
   if (!logits || !tokens || !logprobs || !entropy || (top && (!top_logprobs || !top_ids)))
     return set_error(IEKV_ERR_INVALID, "null argument");
+  const Cut cut = cut_of(vocab);
+  if (n_rows * cut.parts > INT32_MAX)
+    return set_error(IEKV_ERR_INVALID, "%lld rows of %lld logits: too many in one call",
+                     static_cast<long long>(n_rows), static_cast<long long>(vocab));
   const int64_t need = iekv_logprobs_workspace(type, n_rows, vocab, top);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(IEKV_ERR_CAPACITY, "workspace of %lld bytes, %lld are needed",
                      static_cast<long long>(workspace ? workspace_bytes : 0),
                      static_cast<long long>(need));
+  if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
+    return set_error(IEKV_ERR_INVALID, "workspace is not aligned to 16 bytes");
+  const Scores out{tokens,       logprobs, entropy, top_logprobs, top_ids,
+                   static_cast<int32_t>(vocab), top};
   switch (type) {
     case IEKV_TYPE_F32:
-      return launch<float>(logits, row_stride, n_rows, vocab, tokens, top, logprobs, entropy,
-                           top_logprobs, top_ids, stream);
+      return launch(cut, static_cast<const float*>(logits), row_stride, n_rows, out, workspace,
+                    stream);
     case IEKV_TYPE_F16:
-      return launch<_Float16>(logits, row_stride, n_rows, vocab, tokens, top, logprobs, entropy,
-                              top_logprobs, top_ids, stream);
+      return launch(cut, static_cast<const _Float16*>(logits), row_stride, n_rows, out, workspace,
+                    stream);
     default:
-      return launch<Bf16>(logits, row_stride, n_rows, vocab, tokens, top, logprobs, entropy,
-                          top_logprobs, top_ids, stream);
+      return launch(cut, static_cast<const Bf16*>(logits), row_stride, n_rows, out, workspace,
+                    stream);
   }
 }
 
