@@ -39,6 +39,7 @@ using iekv_attention::Launch;
 struct iekv_attention_plan {
   iekv_attention_shape shape;
   Launch narrow, wide;
+  int32_t together;              // KV heads a workgroup of the narrow kernel takes
   int32_t joined;                // tokens with several parts
   int64_t tokens, slots;
   int64_t positions_at, join_tokens_at, join_starts_at, join_parts_at, tables_at;  // words
@@ -47,37 +48,66 @@ struct iekv_attention_plan {
 
 namespace {
 
-constexpr int kWideRows = 128;  // rows an item of the wide kernel holds at most
+constexpr int64_t kJoinFew = 2048;  // rows that are joined by four waves each
 
-// Its LDS passes what a kernel may have without asking.
+int compute_units() {
+  static const int units = [] {
+    int device = 0, n = 0;
+    if (hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+        n <= 0) {
+      (void)hipGetLastError();
+      return 256;   // no GPU in sight: a plan made to be looked at
+    }
+    return n;
+  }();
+  return units;
+}
+
+// More LDS than a kernel may have without asking.
 template <typename K>
-int allow_lds(K kernel, int bytes) {
-  static const hipError_t status = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  IEKV_OPS_HIP(status);
-  return IEKV_OK;
+hipError_t allow_lds(K kernel, int bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
-  if (plan.wide.n) {
-    if constexpr (sizeof(T) == 2) {
-      constexpr int R = kWideRows / 128, bytes = sizeof(typename Wide<T, DP>::Lds);
-      if (const int rc = allow_lds(attend_wide<T, C, DP, R>, bytes)) return rc;
-      hipLaunchKernelGGL((attend_wide<T, C, DP, R>), dim3(plan.wide.n * a.kv_heads),
-                         dim3(kThreads), bytes, stream, a, plan.wide.first);
+  const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
+  const int32_t narrow_blocks = narrow * (a.kv_heads / a.together);
+  // Both kinds in one launch while the narrow ones fit the card at once (24 sequences of two KV
+  // heads behind 512 tokens: 12.4 us against 18.4 in two); a long stream of them is better
+  // alone on it (128 sequences of the 8B shape: 215 us in two launches, 255 in one).
+  const bool both = wide && narrow && narrow_blocks <= 2 * compute_units();
+  if constexpr (sizeof(T) == 2) {
+    if (wide) {
+      const auto kernel = both ? attend_wide<T, C, DP, true> : attend_wide<T, C, DP, false>;
+      constexpr int of_wide = sizeof(typename Wide<T, DP>::Lds);
+      constexpr int of_both = std::max<int>(of_wide, sizeof(typename Narrow<T, C, DP>::Lds));
+      const int bytes = both ? of_both : of_wide;
+      static const hipError_t allowed[2] = {allow_lds(attend_wide<T, C, DP, false>, of_wide),
+                                            allow_lds(attend_wide<T, C, DP, true>, of_both)};
+      IEKV_OPS_HIP(allowed[both]);
+      hipLaunchKernelGGL(kernel, dim3(wide * a.kv_heads + (both ? narrow_blocks : 0)),
+                         dim3(kThreads), bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
+                         narrow);
       IEKV_OPS_HIP(hipGetLastError());
     }
   }
-  if (plan.narrow.n) {
+  if (narrow && !both) {
+    // Only 32-bit queries have narrow items of more than 16 heads.
     hipLaunchKernelGGL((attend_narrow<T, C, DP>),
-                       dim3(plan.narrow.n * a.kv_heads, (a.group + 15) / 16), dim3(kThreads), 0, stream, a, plan.narrow.first);
+                       dim3(narrow_blocks, (a.group + 15) / 16), dim3(kThreads), 0, stream, a,
+                       plan.narrow.first, narrow);
     IEKV_OPS_HIP(hipGetLastError());
   }
   if (plan.joined) {
+    // Few rows have many parts each: their loads are spread over four waves.
     const int64_t rows = int64_t(plan.joined) * a.kv_heads * a.group;
     const int32_t* w = a.words;
-    hipLaunchKernelGGL((join_parts<T>), dim3((rows + 3) / 4), dim3(kThreads), 0, stream, a,
+    const bool few = rows <= kJoinFew;
+    hipLaunchKernelGGL((few ? join_parts<T, kWaves> : join_parts<T, 1>),
+                       dim3(few ? rows : (rows + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a,
                        w + plan.join_tokens_at, w + plan.join_starts_at, w + plan.join_parts_at,
                        plan.joined);
     IEKV_OPS_HIP(hipGetLastError());
@@ -134,20 +164,6 @@ int check_shape(const iekv_attention_shape& s) {
   return IEKV_OK;
 }
 
-int compute_units() {
-  static const int units = [] {
-    int device = 0, n = 0;
-    if (hipGetDevice(&device) != hipSuccess ||
-        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
-        n <= 0) {
-      (void)hipGetLastError();
-      return 256;   // no GPU in sight: a plan made to be looked at
-    }
-    return n;
-  }();
-  return units;
-}
-
 int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* context_lens,
          const int32_t* query_lens, const int32_t* tables, const int64_t* starts,
          iekv_attention_plan** out) {
@@ -201,6 +217,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
   plan->shape = shape;
   plan->narrow = made.narrow;
   plan->wide = made.wide;
+  plan->together = made.together;
   plan->joined = static_cast<int32_t>(made.join_tokens.size());
   plan->tokens = tokens;
   plan->slots = made.slots;
@@ -302,6 +319,7 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
   a.group = s.num_heads / s.num_kv_heads;
   a.head_dim = s.head_dim;
   a.block_size = s.block_size;
+  a.together = plan->together;
   // Division by a constant as a product (Granlund and Montgomery), for numerators below 2^31.
   while ((uint64_t(1) << a.block_shift) < static_cast<uint64_t>(s.block_size)) ++a.block_shift;
   a.block_magic = static_cast<uint32_t>(

@@ -34,6 +34,7 @@ struct Args {
   int64_t q_token_stride, q_head_stride;
   int32_t window, sinks;      // window: INT32_MAX for all keys
   int32_t kv_heads, group, head_dim, block_size;
+  int32_t together;           // KV heads of a narrow item that a workgroup takes: 1, 2 or 4
   uint32_t block_magic, block_shift;  // j / block_size = (mulhi(j, magic) + j) >> shift
   uint32_t q_sign;            // flips the sign of q (in each half for 16 bits): scale >= 0
   float scale;                // |scale| log2(e)
@@ -61,6 +62,18 @@ __device__ __forceinline__ Words<(BYTES + 3) / 4> load_bytes(const void* p) {
   r.w[(BYTES - 1) / 4] = 0;
   __builtin_memcpy(&r, p, BYTES);
   return r;
+}
+
+// The same of a stream that is read once.
+template <int BYTES>
+__device__ __forceinline__ Words<(BYTES + 3) / 4> stream_bytes(const void* p) {
+  if constexpr (BYTES % 4) {
+    return load_bytes<BYTES>(p);
+  } else {
+    typedef uint32_t Vec __attribute__((ext_vector_type(BYTES / 4), aligned(1)));
+    return __builtin_bit_cast(Words<BYTES / 4>,
+                              __builtin_nontemporal_load(static_cast<const Vec*>(p)));
+  }
 }
 
 // Two elements of the compute type in a word, rounded to nearest even.
@@ -213,6 +226,22 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
+// The larger of two lanes 16 or 32 apart, by the row swaps of the vector unit: an LDS shuffle
+// would put its latency into every step's chain. (The halves of a swap are named: a bit cast
+// of a vector's element takes its first.)
+__device__ __forceinline__ float max_across32(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t low = r[0], high = r[1];
+  return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
+__device__ __forceinline__ float max_across16(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const uint32_t low = r[0], high = r[1];
+  return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
+
 __device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // --- one row key by key ------------------------------------------------------------------
@@ -294,43 +323,49 @@ __device__ __forceinline__ void store_out(T* out, const float* x) {
 
 // What bounds it is the cache's stream: each wave has a step's K or V (64 keys; 32 of 32-bit
 // caches) in flight at any time, straight into the registers the products read, and nothing
-// but block ids passes through LDS. A wave takes every fourth step, and the four join at the
-// end. Of a pair of key tiles (32 keys), lane group g = lane / 16 holds the weights of keys
-// 8 g .. 8 g + 7: a lane loads those keys' V, EV dimensions each, and turns them in its own
-// registers into the EV operands of V^T (dimension c EV + t at place c of tile t).
+// but block ids passes through LDS. A workgroup takes 1, 2 or 4 neighbouring KV heads: its
+// waves go through the same keys, whose rows are neighbours in memory (64 sequences of 16,000
+// tokens of the 8B shape: 5.5 TB/s with four waves on one head), and waves of the same head
+// take steps in turn and join at the end. Of a pair of key tiles (32 keys), lane group
+// g = lane / 16 holds the weights of keys 8 g .. 8 g + 7: a lane loads those keys' V, EV
+// dimensions each, and turns them in its own registers into the EV operands of V^T (dimension
+// c EV + t at place c of tile t).
 template <typename T, typename C, int DP>
 struct Narrow {
   static constexpr int EK = sizeof(T) == 4 ? 4 : 8;       // K elements a lane feeds at a time
-  static constexpr int NK = DP / (4 * EK);                // and how many times
+  // and brings at a time: 16 bytes, so that the four lanes of a key read 64 bytes on end
+  static constexpr int EL = 16 / int(sizeof(C)) * 4 <= DP ? 16 / int(sizeof(C)) : DP / 4;
+  static constexpr int NL = (DP + 4 * EL - 1) / (4 * EL), MF = EL / EK, NK = NL * MF;
   static constexpr int EV = DP <= 32 ? 2 : DP <= 64 ? 4 : 8;
   static constexpr int KT = sizeof(C) == 4 ? 2 : 4;       // key tiles of 16 in a step
   static constexpr int KS = 16 * KT;
-  using RawK = Words<EK * int(sizeof(C)) / 4>;
+  using RawK = Words<EL * int(sizeof(C)) / 4>;
   using RawV = Words<(EV * int(sizeof(C)) + 3) / 4>;
   static constexpr int LDO = DP + 4;                      // floats of a row of o in LDS
   struct Lds {
     alignas(16) uint32_t rows[kWaves][2][KS];
     float2 ml[kWaves][16];
     alignas(16) float o[kWaves][16][LDO];
-    int32_t redo;
+    int32_t redo[kWaves];
   };
 };
 
+// A group of more than 16 heads takes several workgroups for each of its tokens, `head0` on.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_narrow(
-    Args a, int32_t first) {
+__device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds, const Args& a,
+                                            int32_t item, int32_t kv_head0, int32_t head0) {
   using N = Narrow<T, C, DP>;
-  constexpr int EK = N::EK, NK = N::NK, EV = N::EV, KT = N::KT, KS = N::KS;
-  __shared__ typename N::Lds lds;
-  // A group of more than 16 heads takes several workgroups for each of its tokens.
-  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
-  const int32_t kv_head = blockIdx.x % a.kv_heads;
-  const int32_t head0 = blockIdx.y * 16, heads = a.group - head0 < 16 ? a.group - head0 : 16;
+  constexpr int EK = N::EK, EL = N::EL, NL = N::NL, MF = N::MF, NK = N::NK;
+  constexpr int EV = N::EV, KT = N::KT, KS = N::KS;
+  const Item it = item_of(a, item);
+  const int32_t heads = a.group - head0 < 16 ? a.group - head0 : 16;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
+  const int32_t together = a.together, turns = kWaves / together;
+  const int32_t kv_head = kv_head0 + wave % together, turn = wave / together;
   const int32_t d = a.head_dim, rows = it.tokens * heads;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
   const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
-  if (threadIdx.x == 0) lds.redo = 0;
+  if (threadIdx.x < kWaves) lds.redo[threadIdx.x] = 0;
 
   // Q^T: row c, zeros past the rows and past the dimensions.
   Words<4> q[NK];
@@ -342,11 +377,11 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int32_t d0 = (4 * i + g) * EK;
+      const int32_t d0 = (4 * (i / MF) + g) * EL + i % MF * EK;
       const bool in = c < rows && d0 < d;
       q[i] = load_bytes<EK * sizeof(T)>(at + (d0 < d ? d0 : 0));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[i].w[e] = in ? q[i].w[e] ^ a.q_sign : 0;
+      for (int e = 0; e < 4; ++e) q[i].w[e] = (q[i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
     }
   }
   const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
@@ -362,7 +397,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  typename N::RawK k[KT][NK];
+  typename N::RawK k[KT][NL];
   const auto load_k = [&](int half) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -370,13 +405,30 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
           lds.rows[wave][half][t / 2 * 32 + (c >> 2) * 8 + t % 2 * 4 + (c & 3)];
       const C* at = kc + row * width;
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const int32_t d0 = (4 * i + g) * EK;
-        k[t][i] = load_bytes<EK * sizeof(C)>(at + (d0 < d ? d0 : 0));
-        if (i == NK - 1 || sizeof(T) == 4)
-          for (uint32_t& w : k[t][i].w) w = d0 < d ? w : 0;
+      for (int i = 0; i < NL; ++i) {
+        const int32_t d0 = (4 * i + g) * EL;
+        // 16 elements past the head's end would be past the cache's at its last row.
+        const int32_t from = d0 >= d ? 0 : EL == 16 && d0 + 8 == d ? d0 - 8 : d0;
+        k[t][i] = stream_bytes<EL * sizeof(C)>(at + from);
       }
     }
+  };
+
+  // The elements of feed `e` of a load; zeros past the head's dimensions. Not where they are
+  // loaded, or they would be waited for there.
+  constexpr int KW = EK * int(sizeof(C)) / 4;
+  const auto feed = [&](const typename N::RawK& x, int i, int e) {
+    Words<KW> r;
+    const int32_t d0 = (4 * i + g) * EL + e * EK;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      r.w[w] = x.w[e * KW + w];
+      if ((i + 1) * 4 * EL > DP - 32) {
+        if (EL == 16 && e * EK < 8) r.w[w] = d0 - e * EK + 8 == d ? x.w[(e * EK + 8) / 4 + w] : r.w[w];
+        r.w[w] &= d0 < d ? ~0u : 0u;
+      }
+    }
+    return r;
   };
 
   f32x4 o[EV];
@@ -386,12 +438,12 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
 
   int half = 0;
   Place next{0, 0};
-  if (wave < steps) {
-    keep(0, place(wave));
+  if (turn < steps) {
+    keep(0, place(turn));
     load_k(0);
-    next = place(wave + kWaves);
+    next = place(turn + turns);
   }
-  for (int32_t s = wave; s < steps; s += kWaves, half ^= 1) {
+  for (int32_t s = turn; s < steps; s += turns, half ^= 1) {
     keep(half ^ 1, next);
     typename N::RawV v[KT / 2][8];
 #pragma unroll
@@ -399,18 +451,22 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t row = lds.rows[wave][half][p * 32 + g * 8 + e];
-        v[p][e] = load_bytes<EV * sizeof(C)>(vc + row * width);
+        v[p][e] = stream_bytes<EV * sizeof(C)>(vc + row * width);
       }
+    __builtin_amdgcn_sched_barrier(0);          // no wait for K's before V's are on their way
     f32x4 sc[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NK; ++i)
-        sc[t] = mma16(Convert<T, C, EK>::of(k[t][i]), q[i], sc[t], T{});
+        sc[t] = mma16(Convert<T, C, EK>::of(feed(k[t][i / MF], i / MF, i % MF)), q[i], sc[t], T{});
     }
-    if (s + kWaves < steps) load_k(half ^ 1);
-    next = place(s + 2 * kWaves);
+    // In this order: loads return in theirs, and the block's id is what is needed first. Past
+    // the last step these read the last key: a branch would make the next wait one for all.
+    next = place(s + 2 * turns);
+    load_k(half ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
 
     const int32_t v0 = s * KS;
     if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
@@ -429,8 +485,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][r]);
-      x = fmaxf(x, __shfl_xor(x, 16));
-      x = fmaxf(x, __shfl_xor(x, 32));
+      x = max_across32(max_across16(x));
       top = fmaxf(m, x * a.scale);
     }
     const float base = top == -INFINITY ? 0.f : top;
@@ -482,13 +537,13 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     }
   }
 
-  // The waves' parts.
+  // The parts of each head's waves.
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if (lane < 16) lds.ml[wave][lane] = {m, l};
   __syncthreads();
   float all = -INFINITY;
-  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, lds.ml[w][c].x);
+  for (int w = wave % together; w < kWaves; w += together) all = fmaxf(all, lds.ml[w][c].x);
   const float fade = power2(m - (all == -INFINITY ? 0.f : all));
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -496,46 +551,46 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
     for (int t = 0; t < EV; ++t)
       if ((g * 4 + r) * EV + t < DP) lds.o[wave][c][(g * 4 + r) * EV + t] = o[t][r] * fade;
   __syncthreads();
-  // Eight dimensions a thread.
+  // Eight dimensions of a row a thread.
   const int32_t row = threadIdx.x / 16, d0 = threadIdx.x % 16 * 8;
-  const bool mine = row < rows && d0 < d;
-  float x[8], total = 0.f, most = -INFINITY;
-  if (mine) {
-    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, lds.ml[w][row].x);
-    const float from = most == -INFINITY ? 0.f : most;
-    for (int w = 0; w < kWaves; ++w)
-      total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
-    bool odd = total != total;
+  const int32_t in_group = head0 + row % heads, token = row / heads;
+  if (row < rows && d0 < d) {
+    for (int k = 0; k < together; ++k) {
+      float x[8], total = 0.f, most = -INFINITY;
+      for (int w = k; w < kWaves; w += together) most = fmaxf(most, lds.ml[w][row].x);
+      const float from = most == -INFINITY ? 0.f : most;
+      for (int w = k; w < kWaves; w += together)
+        total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
+      bool odd = total != total;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = lds.o[0][row][d0 + i];
+      for (int i = 0; i < 8; ++i) x[i] = lds.o[k][row][d0 + i];
+      for (int w = k + together; w < kWaves; w += together)
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) x[i] += lds.o[w][row][d0 + i];
-      odd = odd || x[i] != x[i];
+        for (int i = 0; i < 8; ++i) x[i] += lds.o[w][row][d0 + i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) odd = odd || x[i] != x[i];
+      if (odd) lds.redo[k] = 1;
+      const int64_t kv = kv_head0 + k;
+      if (it.slot >= 0) {
+        const int64_t slot =
+            static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv;
+        __builtin_memcpy(a.part_o + slot * d + d0, x, 32);
+        if (d0 == 0) a.part_ml[slot] = {most, total};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] /= total;
+        const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
+                           kv * a.group + in_group;
+        store_out<T, 8>(static_cast<T*>(a.out) + at * d + d0, x);
+      }
     }
-    if (odd) lds.redo = 1;
   }
   __syncthreads();
-  if (lds.redo) {
+  for (int k = 0; k < together; ++k) {
+    if (!lds.redo[k]) continue;
     for (int32_t r = wave; r < rows; r += kWaves)
-      attend_row<T, C>(a, it, kv_head, r / heads * a.group + head0 + r % heads, lane);
-    return;
+      attend_row<T, C>(a, it, kv_head0 + k, r / heads * a.group + head0 + r % heads, lane);
   }
-  if (!mine) return;
-  const int32_t in_group = head0 + row % heads;
-  if (it.slot >= 0) {
-    const int64_t slot =
-        static_cast<int64_t>(it.slot + row / heads * a.group + in_group) * a.kv_heads + kv_head;
-    __builtin_memcpy(a.part_o + slot * d + d0, x, 32);
-    if (d0 == 0) a.part_ml[slot] = {most, total};
-    return;
-  }
-  const int64_t token = it.token0 + row / heads;
-  const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] /= total;
-  store_out<T, 8>(static_cast<T*>(a.out) +
-                      (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d + d0, x);
 }
 
 // --- wide: many rows ---------------------------------------------------------------------
@@ -568,14 +623,12 @@ __device__ __forceinline__ Words<2> transposed(const char* lds) {
 }
 
 template <typename T, typename C, int DP, int R>
-__global__ __launch_bounds__(kThreads, R == 1 ? 2 : 1) void attend_wide(Args a, int32_t first) {
+__device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const Args& a,
+                                          int32_t item, int32_t kv_head) {
   using W = Wide<T, DP>;
   constexpr int KS = W::KS, KW = W::KW, VW = W::VW, CHUNKS = W::CHUNKS, LOADS = W::LOADS;
   constexpr int NQ = DP / 16, ND = DP / 32;
-  extern __shared__ __attribute__((aligned(16))) char shared[];
-  auto& lds = *reinterpret_cast<typename W::Lds*>(shared);
-  const Item it = item_of(a, first + blockIdx.x / a.kv_heads);
-  const int32_t kv_head = blockIdx.x % a.kv_heads;
+  const Item it = item_of(a, item);
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, h = lane / 32, c = lane % 32;
   const int32_t d = a.head_dim, rows = it.tokens * a.group;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
@@ -597,7 +650,7 @@ __global__ __launch_bounds__(kThreads, R == 1 ? 2 : 1) void attend_wide(Args a, 
       const bool in = r < rows && d0 < d;
       q[u][i] = load_bytes<16>(at + (d0 < d ? d0 : 0));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[u][i].w[e] = in ? q[u][i].w[e] ^ a.q_sign : 0;
+      for (int e = 0; e < 4; ++e) q[u][i].w[e] = (q[u][i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
     }
   }
 
@@ -694,7 +747,7 @@ __global__ __launch_bounds__(kThreads, R == 1 ? 2 : 1) void attend_wide(Args a, 
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) x = fmaxf(x, sc[u][t][r]);
-      x = fmaxf(x, __shfl_xor(x, 32));
+      x = max_across32(x);
       const float top = fmaxf(m[u], x * a.scale), base = top == -INFINITY ? 0.f : top;
       if (__any(top > m[u])) {
         const float fade = power2(m[u] - base);
@@ -775,37 +828,124 @@ __global__ __launch_bounds__(kThreads, R == 1 ? 2 : 1) void attend_wide(Args a, 
   }
 }
 
-// --- join --------------------------------------------------------------------------------
+// --- kernels -----------------------------------------------------------------------------
 
-// Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, in
-// the order of the parts. One wave a row.
-template <typename T>
+// A block is one or more KV heads of an item. Blocks go to the XCDs in turn: the ones of a
+// narrow item, which read neighbouring rows of the cache, go to the same one.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_narrow(
+    Args a, int32_t first, int32_t n) {
+  __shared__ typename Narrow<T, C, DP>::Lds lds;
+  constexpr int kXcds = 8;
+  const int32_t each = a.kv_heads / a.together, b = blockIdx.x;
+  const bool whole = b < n / kXcds * kXcds * each;
+  const int32_t item = whole ? b / kXcds / each * kXcds + b % kXcds : b / each;
+  const int32_t part = whole ? b / kXcds % each : b % each;
+  narrow_item<T, C, DP>(lds, a, first + item, part * a.together, blockIdx.y * 16);
+}
+
+constexpr int kWideTiles = 1;                    // R of the kernels below
+constexpr int kWideRows = kWaves * 32 * kWideTiles;
+
+// `n_wide` wide items from `wide` on, and with BOTH `n_narrow` from `narrow` on in the same
+// launch: the matrix units work on the former while the latter wait for memory. Of a wide
+// item neighbouring blocks are its heads, and where there are eight, all blocks of an XCD are
+// of one head, whose keys the items share in its L2.
+template <typename T, typename C, int DP, bool BOTH>
+__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_wide(
+    Args a, int32_t wide, int32_t n_wide, int32_t narrow, int32_t n_narrow) {
+  extern __shared__ __attribute__((aligned(16))) char shared[];
+  auto& of_wide = *reinterpret_cast<typename Wide<T, DP>::Lds*>(shared);
+  if constexpr (!BOTH) {
+    wide_item<T, C, DP, kWideTiles>(of_wide, a, wide + blockIdx.x / a.kv_heads,
+                                    blockIdx.x % a.kv_heads);
+    return;
+  }
+  // Runs of as many blocks as a narrow item has; a wide item is `together` such runs. Those
+  // of the wide items come at even distances among the first three quarters.
+  const uint32_t each = a.kv_heads / a.together, run = blockIdx.x / each, part = blockIdx.x % each;
+  const uint32_t wides = n_wide * a.together, runs = wides + n_narrow;
+  const uint32_t span = wides > runs - runs / 4 ? wides : runs - runs / 4;
+  const uint32_t before = run < span ? uint64_t(run) * wides / span : wides;
+  const uint32_t after = run < span ? uint64_t(run + 1) * wides / span : wides;
+  if (after > before)
+    wide_item<T, C, DP, kWideTiles>(of_wide, a, wide + before / a.together,
+                                    before % a.together * each + part);
+  else
+    narrow_item<T, C, DP>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared), a,
+                          narrow + run - before, part * a.together, 0);
+}
+
+// Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, W
+// waves a row. The loads of a row's parts are what takes time, so they are independent of one
+// another: a lane holds 4 dimensions of every 64 / lanes-th part (of each 64, whose maxima
+// and sums the lanes hold), and the waves take turns. The order of the sums is fixed.
+template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* tokens,
                                                        const int32_t* starts,
                                                        const int32_t* parts, int32_t n) {
-  const int lane = threadIdx.x % kWave;
+  __shared__ float sums[kWaves][IEKV_ATTENTION_MAX_DIM];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, turn = wave % W;
   const int32_t heads = a.kv_heads * a.group, d = a.head_dim;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + threadIdx.x / kWave;
-  if (row >= static_cast<int64_t>(n) * heads) return;
-  const int32_t entry = static_cast<int32_t>(row / heads), head = static_cast<int32_t>(row % heads);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWaves / W) + wave / W;
+  const bool real = row < static_cast<int64_t>(n) * heads;
+  const int32_t entry = real ? static_cast<int32_t>(row / heads) : 0;
+  const int32_t head = real ? static_cast<int32_t>(row % heads) : 0;
   const int32_t kv_head = head / a.group, in_group = head % a.group;
   const int32_t p0 = starts[entry], p1 = starts[entry + 1];
+  const int32_t lanes = d <= 32 ? 8 : d <= 64 ? 16 : 32, each = kWave / lanes;
+  const int32_t which = lane / lanes, d0 = lane % lanes * 4;
+  const auto slot_of = [&](int32_t p) {
+    return static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
+  };
   float m = -INFINITY;
-  for (int32_t p = p0; p < p1; ++p)
-    m = fmaxf(m, a.part_ml[static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head].x);
+  for (int32_t p = p0 + lane; p < p1; p += kWave) m = fmaxf(m, a.part_ml[slot_of(p)].x);
+  m = wave_max(m);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int32_t p = p0; p < p1; ++p) {
-    const int64_t slot = static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
+  float l = 0.f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  for (int32_t q0 = p0; q0 < p1; q0 += kWave) {
+    const int32_t count = p1 - q0 < kWave ? p1 - q0 : kWave;
+    const int32_t p = q0 + (lane < count ? lane : 0);
+    const int64_t slot = slot_of(p);
     const float2 ml = a.part_ml[slot];
-    const float w = exp2f(ml.x - base);
-    l = fmaf(w, ml.y, l);
-    if (lane < d) o0 = fmaf(w, a.part_o[slot * d + lane], o0);
-    if (lane + kWave < d) o1 = fmaf(w, a.part_o[slot * d + lane + kWave], o1);
+    const float weight = power2(ml.x - base);
+    if (lane < count) l = fmaf(weight, ml.y, l);
+    for (int32_t q = turn * each; q < count; q += 4 * W * each) {
+      f32x4 x[4];
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t mine = q + i * W * each + which;
+        const int64_t at = __shfl(slot, mine < count ? mine : 0) * d + (d0 < d ? d0 : 0);
+        w[i] = __shfl(weight, mine < count ? mine : 0);
+        __builtin_memcpy(&x[i], a.part_o + at, 16);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (q + i * W * each + which < count) o += x[i] * w[i];
+    }
   }
-  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(tokens[entry]) * heads + head) * d;
-  if (lane < d) out[lane] = from_float<T>(o0 / l);
-  if (lane + kWave < d) out[lane + kWave] = from_float<T>(o1 / l);
+  l = wave_sum(l);
+  for (int s = lanes; s < kWave; s *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], s);
+  if constexpr (W > 1) {
+    if (which == 0)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[wave][d0 + i] = o[i];
+    __syncthreads();
+    if (turn == 0)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        for (int w = 1; w < W; ++w) o[i] += sums[wave + w][d0 + i];
+  }
+  if (!real || turn || which || d0 >= d) return;
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = o[i] / l;
+  store_out<T, 4>(static_cast<T*>(a.out) +
+                      (static_cast<int64_t>(tokens[entry]) * heads + head) * d + d0, x);
 }
 
 }  // namespace iekv_ops

@@ -45,6 +45,7 @@ struct Launch {
 struct Plan {
   std::vector<Item> items;
   Launch narrow, wide;
+  int32_t together = 1;                // KV heads a workgroup of the narrow kernel takes
   std::vector<int32_t> positions;      // per token
   std::vector<int32_t> join_tokens;    // tokens with several parts
   std::vector<int32_t> join_starts;    // n + 1: where each one's parts begin
@@ -53,6 +54,7 @@ struct Plan {
 };
 
 constexpr int kNarrowRows = 16;
+constexpr int kNarrowWaves = 4;
 
 // Keys of [lo, hi) that any of positions low..high sees.
 inline void visible(const Shape& sh, int64_t low, int64_t high, int64_t lo, int64_t hi, Item* it) {
@@ -131,15 +133,38 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
     add_tiles(sh, plan.positions, token0, n, table, lo, hi,
               is_wide ? sh.wide_rows : kNarrowRows, is_wide ? &wide : &narrow);
   };
-  if (sh.shared && tokens) {
-    const auto first = std::find_if(seqs.begin(), seqs.end(),
-                                    [](const Sequence& s) { return s.queries > 0; });
-    add(0, tokens, first->table, 0, sh.shared);
+  // Sequences whose own rows fill a tile gain nothing from a tile shared with others: they
+  // read the shared keys with their own, and leave no partial results. The rest are taken in
+  // runs.
+  const auto shares = [&](const Sequence& s) {
+    return sh.shared && int64_t(s.queries) * sh.group < (sh.wide_rows ? sh.wide_rows : kNarrowRows);
+  };
+  int32_t leading = -1, run0 = 0, run = 0;
+  for (const Sequence& s : seqs) {
+    if (!s.queries) continue;
+    if (leading < 0) leading = s.table;
+    if (shares(s)) {
+      if (!run) run0 = s.token0;
+      run += s.queries;
+    } else if (run) {
+      add(run0, run, leading, 0, sh.shared);
+      run = 0;
+    }
+    add(s.token0, s.queries, s.table, shares(s) ? sh.shared : 0, s.context);
   }
-  for (const Sequence& s : seqs)
-    if (s.queries) add(s.token0, s.queries, s.table, sh.shared, s.context);
-  narrow = split(narrow, sh.kv_heads, 4 * compute_units, 256, 64);
-  wide = split(wide, sh.kv_heads, 2 * compute_units, 512, 64);
+  if (run) add(run0, run, leading, 0, sh.shared);
+  // A workgroup of several heads reads longer runs of the cache, and each of its waves leaves
+  // a part of its own: worth it where a wave has steps enough to outweigh the part.
+  int64_t narrow_keys = 0;
+  for (const Item& it : narrow) narrow_keys += keys_of(it);
+  const int64_t blocks = 4 * compute_units;
+  if (narrow_keys * sh.kv_heads >= blocks * kNarrowWaves * 256)
+    plan.together = sh.kv_heads % 4 == 0 ? 4 : sh.kv_heads % 2 == 0 ? 2 : 1;
+  narrow = split(narrow, sh.kv_heads / plan.together, blocks, 256, 64);
+  // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
+  // are: they are cut only where more than half of the compute units would have none.
+  if (int64_t(wide.size()) * sh.kv_heads * 2 < compute_units)
+    wide = split(wide, sh.kv_heads, 2 * compute_units, 128, 64);
   // The longest first: the last workgroups to start are short ones.
   auto longer = [](const Item& x, const Item& y) { return keys_of(x) > keys_of(y); };
   std::stable_sort(narrow.begin(), narrow.end(), longer);
