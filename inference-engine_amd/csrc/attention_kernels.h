@@ -703,28 +703,40 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
   store(0);
   __syncthreads();
   for (int32_t s = 0; s < steps; ++s) {
+    // No branch around these loads, or every wait after them would be one for all: past the
+    // last step they read the last key.
     const int half = s & 1;
-    const bool more = s + 1 < steps;
-    if (more) load(half ^ 1);
-    Place next{0, 0};
-    if (wave == 0 && more) next = place(s + 2);
+    const Place next = place(s + 2);
+    load(half ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
 
     f32x16 sc[R][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int u = 0; u < R; ++u)
 #pragma unroll
-      for (int u = 0; u < R; ++u)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[u][t][r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         const Words<4> k = __builtin_bit_cast(
             Words<4>,
             *reinterpret_cast<const u32x4*>(lds.k[half] + (t * 32 + c) * KW + i * 32 + h * 16));
 #pragma unroll
         for (int u = 0; u < R; ++u) sc[u][t] = mma32(k, q[u][i], sc[u][t], T{});
       }
+    // Half of K's reads at once, then one behind each product: left to itself the compiler
+    // waits for every read before its product.
+    constexpr int kDsRead = 0x100, kMfma = 0x8;
+    __builtin_amdgcn_sched_group_barrier(kDsRead, NQ, 0);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, R, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(kMfma, NQ * R, 0);
 
     const int32_t v0 = s * KS;
     if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
@@ -778,8 +790,9 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
 #pragma unroll
         for (int u = 0; u < R; ++u) o[u][t] = mma32(v, p[u][i], o[u][t], T{});
       }
-    if (more) store(half ^ 1);
-    if (wave == 0 && more) lds.rows[half][lane] = row_of(a, next);
+    __builtin_amdgcn_sched_barrier(0);
+    store(half ^ 1);
+    if (wave == 0) lds.rows[half][lane] = row_of(a, next);
     __syncthreads();
   }
 
