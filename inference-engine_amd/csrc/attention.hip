@@ -81,16 +81,20 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   const bool both = wide && narrow && narrow_blocks <= 2 * compute_units();
   if constexpr (sizeof(T) == 2) {
     if (wide) {
-      const auto kernel = both ? attend_wide<T, C, DP, true> : attend_wide<T, C, DP, false>;
-      constexpr int of_wide = sizeof(typename Wide<T, DP>::Lds);
-      constexpr int of_both = std::max<int>(of_wide, sizeof(typename Narrow<T, C, DP>::Lds));
-      const int bytes = both ? of_both : of_wide;
-      static const hipError_t allowed[2] = {allow_lds(attend_wide<T, C, DP, false>, of_wide),
-                                            allow_lds(attend_wide<T, C, DP, true>, of_both)};
-      IEKV_OPS_HIP(allowed[both]);
-      hipLaunchKernelGGL(kernel, dim3(wide * a.kv_heads + (both ? narrow_blocks : 0)),
-                         dim3(kThreads), bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
-                         narrow);
+      const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+      if (!both && sizeof(C) == 2 && aligned(a.k) && aligned(a.v)) {
+        hipLaunchKernelGGL((attend_wide<T, C, DP>), dim3(wide * a.kv_heads), dim3(kThreads), 0,
+                           stream, a, plan.wide.first);
+      } else {
+        constexpr int bytes = std::max<int>(sizeof(typename Wide<T, DP>::Lds),
+                                            sizeof(typename Narrow<T, C, DP>::Lds));
+        static const hipError_t allowed = allow_lds(attend_both<T, C, DP>, bytes);
+        IEKV_OPS_HIP(allowed);
+        hipLaunchKernelGGL((attend_both<T, C, DP>),
+                           dim3(wide * a.kv_heads + (both ? narrow_blocks : 0)), dim3(kThreads),
+                           bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
+                           both ? narrow : 0);
+      }
       IEKV_OPS_HIP(hipGetLastError());
     }
   }

@@ -193,7 +193,7 @@ __device__ __forceinline__ int32_t key_at(const Item& it, int32_t v) {
 }
 
 __device__ __forceinline__ bool sees(const Args& a, int32_t position, int32_t key) {
-  return key <= position && (key > position - a.window || key < a.sinks);
+  return (key <= position) & ((key > position - a.window) | (key < a.sinks));
 }
 
 // Every position of the item sees every one of its keys v0 .. v1 - 1.
@@ -596,21 +596,30 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 // --- wide: many rows ---------------------------------------------------------------------
 
 // Four waves, 32 R rows each, share tiles of 64 keys in LDS, two tiles in turn: a tile's
-// loads are issued before the products of the one before it and stored to LDS after them.
-// V^T is read from V's rows by the transposing LDS load (a group of 16 lanes reads 4 keys of
-// 16 dimensions, and each lane gets one dimension of the four). Row strides in LDS put what
-// the lanes read at a time into different banks: 16 bytes past a multiple of 128 for K's
-// 16-byte reads, 32 bytes past for V's four rows of 32 bytes.
+// loads are issued before the products of the one before it. V^T is read from V's rows by the
+// transposing LDS load (a group of 16 lanes reads 4 keys of 16 dimensions, and each lane gets
+// one dimension of the four). A tile lies in LDS without gaps, so that the loads can go there
+// directly (DIRECT; 8-bit caches are converted on their way, and caches that begin at any
+// element are copied through registers); its rows' 16-byte chunks change places by key, so
+// that what the lanes read at a time lies in different banks: eight keys' chunks of K,
+// and four keys' pairs of chunks of V.
 template <typename T, int DP>
 struct Wide {
   static constexpr int KS = 64;
-  static constexpr int KW = DP * 2 + 16, VW = DP * 2 + 32;   // bytes of a row in LDS
   static constexpr int CHUNKS = DP / 8;                      // of eight elements, a row's
   static constexpr int LOADS = KS * CHUNKS / kThreads;       // chunks a thread brings
+  static constexpr bool POWER = DP == 64 || DP == 128;
+  static __device__ __forceinline__ int place_k(int key, int chunk) {
+    return chunk ^ (POWER ? key & 7 : key >> 1 & 3);
+  }
+  static __device__ __forceinline__ int place_v(int key, int chunk) {
+    return chunk ^ (POWER ? (key & 3) * 2 : (key >> 1 & 1) * 2);
+  }
+  using Tile = u32x4[KS * CHUNKS];
+  using Rows = int64_t[2][KS];                               // bytes to the keys' rows
   struct Lds {
-    alignas(16) char k[2][KS * KW];
-    alignas(16) char v[2][KS * VW];
-    uint32_t rows[2][KS];
+    Tile k[2], v[2];
+    Rows rows;
     int32_t redo;
   };
 };
@@ -622,18 +631,36 @@ __device__ __forceinline__ Words<2> transposed(const char* lds) {
                     (__attribute__((address_space(3))) s16x4*)const_cast<char*>(lds)));
 }
 
-template <typename T, typename C, int DP, int R>
-__device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const Args& a,
-                                          int32_t item, int32_t kv_head) {
+// 16 bytes of each lane into LDS, the wave's in a row from `to` on.
+__device__ __forceinline__ void bring16(const char* from, u32x4* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) uint32_t*)reinterpret_cast<uintptr_t>(from),
+      (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
+}
+
+// A barrier that the wave's loads into LDS have ended at, too.
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_s_waitcnt(0xf70);      // vmcnt 0; the other counters are not waited for
+  __syncthreads();
+}
+
+// K's and V's buffers are arguments of their own: the compiler then knows that a load into one
+// leaves the others alone, and does not wait for it before it reads them.
+template <typename T, typename C, int DP, int R, bool DIRECT>
+__device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
+                                          typename Wide<T, DP>::Tile& k1,
+                                          typename Wide<T, DP>::Tile& v0,
+                                          typename Wide<T, DP>::Tile& v1,
+                                          typename Wide<T, DP>::Rows& lds_rows, int32_t& redo,
+                                          const Args& a, int32_t item, int32_t kv_head) {
   using W = Wide<T, DP>;
-  constexpr int KS = W::KS, KW = W::KW, VW = W::VW, CHUNKS = W::CHUNKS, LOADS = W::LOADS;
+  constexpr int KS = W::KS, CHUNKS = W::CHUNKS, LOADS = W::LOADS;
   constexpr int NQ = DP / 16, ND = DP / 32;
   const Item it = item_of(a, item);
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, h = lane / 32, c = lane % 32;
   const int32_t d = a.head_dim, rows = it.tokens * a.group;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
-  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
-  if (threadIdx.x == 0) lds.redo = 0;
+  if (threadIdx.x == 0) redo = 0;
 
   Words<4> q[R][NQ];
   int32_t position[R];
@@ -654,31 +681,45 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
     }
   }
 
-  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
-  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * d * sizeof(C);
+  const char* kc = static_cast<const char*>(a.k) + static_cast<int64_t>(kv_head) * d * sizeof(C);
+  const char* vc = static_cast<const char*>(a.v) + static_cast<int64_t>(kv_head) * d * sizeof(C);
   const auto place = [&](int32_t s) {
     const int32_t v = s * KS + lane;
     return place_of(a, it, key_at(it, v < n ? v : n - 1));
   };
+  // The thread's chunks of a tile. Chunks past the head's dimensions hold its first ones: Q is
+  // zero there, and nothing of V there is written.
   using Raw = Words<8 * int(sizeof(C)) / 4>;
-  Raw kr[LOADS], vr[LOADS];
-  const auto load = [&](int half) {
+  struct Staged {
+    Raw k[LOADS], v[LOADS];
+  };
+  const auto load = [&](int64_t (&row)[KS], typename W::Tile& kt, typename W::Tile& vt, Staged& x) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int32_t at = threadIdx.x + i * kThreads, d0 = at % CHUNKS * 8;
-      const int64_t from = lds.rows[half][at / CHUNKS] * width + (d0 < d ? d0 : 0);
-      kr[i] = load_bytes<8 * sizeof(C)>(kc + from);
-      vr[i] = load_bytes<8 * sizeof(C)>(vc + from);
+      const int32_t at = threadIdx.x + i * kThreads, key = at / CHUNKS, to = at % CHUNKS;
+      const int32_t dk = W::place_k(key, to) * 8, dv = W::place_v(key, to) * 8;
+      const int64_t from = row[key];
+      const char* ks = kc + from + (dk < d ? dk : 0) * sizeof(C);
+      const char* vs = vc + from + (dv < d ? dv : 0) * sizeof(C);
+      if constexpr (DIRECT) {
+        const int32_t first = wave * kWave + i * kThreads;       // lane l's goes l places on
+        bring16(ks, &kt[first]);
+        bring16(vs, &vt[first]);
+      } else {
+        x.k[i] = load_bytes<8 * sizeof(C)>(ks);
+        x.v[i] = load_bytes<8 * sizeof(C)>(vs);
+      }
     }
   };
-  const auto store = [&](int half) {
+  const auto store = [&](const Staged& x, typename W::Tile& kt, typename W::Tile& vt) {
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int32_t at = threadIdx.x + i * kThreads, key = at / CHUNKS, ch = at % CHUNKS;
-      Words<4> k = Convert<T, C, 8>::of(kr[i]), v = Convert<T, C, 8>::of(vr[i]);
-      if (ch * 8 >= d) k = v = Words<4>{};
-      *reinterpret_cast<u32x4*>(lds.k[half] + key * KW + ch * 16) = __builtin_bit_cast(u32x4, k);
-      *reinterpret_cast<u32x4*>(lds.v[half] + key * VW + ch * 16) = __builtin_bit_cast(u32x4, v);
+      for (int i = 0; i < LOADS; ++i) {
+        const int32_t at = threadIdx.x + i * kThreads;
+        kt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.k[i]));
+        vt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.v[i]));
+      }
     }
   };
 
@@ -694,20 +735,22 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
       for (int r = 0; r < 16; ++r) o[u][t][r] = 0.f;
   }
 
-  if (wave == 0) {
-    lds.rows[0][lane] = row_of(a, place(0));
-    lds.rows[1][lane] = row_of(a, place(1));
+  if (wave < 2) lds_rows[wave][lane] = row_of(a, place(wave)) * row_bytes;
+  __syncthreads();
+  {
+    Staged x;
+    load(lds_rows[0], k0, v0, x);
+    store(x, k0, v0);
   }
-  __syncthreads();
-  load(0);
-  store(0);
-  __syncthreads();
-  for (int32_t s = 0; s < steps; ++s) {
+  arrive();
+  // Tile s, in `kt` and `vt`; the next one goes to `kn` and `vn`.
+  const auto step = [&](int32_t s, int half, typename W::Tile& kt, typename W::Tile& vt,
+                        typename W::Tile& kn, typename W::Tile& vn) {
     // No branch around these loads, or every wait after them would be one for all: past the
     // last step they read the last key.
-    const int half = s & 1;
     const Place next = place(s + 2);
-    load(half ^ 1);
+    Staged x;
+    load(lds_rows[half ^ 1], kn, vn, x);
     __builtin_amdgcn_sched_barrier(0);
 
     f32x16 sc[R][2];
@@ -722,8 +765,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Words<4> k = __builtin_bit_cast(
-            Words<4>,
-            *reinterpret_cast<const u32x4*>(lds.k[half] + (t * 32 + c) * KW + i * 32 + h * 16));
+            Words<4>, kt[(t * 32 + c) * CHUNKS + W::place_k(c, i * 2 + h)]);
 #pragma unroll
         for (int u = 0; u < R; ++u) sc[u][t] = mma32(k, q[u][i], sc[u][t], T{});
       }
@@ -738,17 +780,17 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
     }
     __builtin_amdgcn_sched_group_barrier(kMfma, NQ * R, 0);
 
-    const int32_t v0 = s * KS;
-    if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
+    const int32_t first = s * KS;
+    if (first + KS > n || !all_see(a, it, first, first + KS)) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int32_t at = v0 + t * 32 + r / 4 * 8 + h * 4 + r % 4;
+          const int32_t at = first + t * 32 + r / 4 * 8 + h * 4 + r % 4;
           const int32_t j = key_at(it, at);
 #pragma unroll
           for (int u = 0; u < R; ++u)
-            if (at >= n || !sees(a, position[u], j)) sc[u][t][r] = -INFINITY;
+            sc[u][t][r] = (at < n) & sees(a, position[u], j) ? sc[u][t][r] : -INFINITY;
         }
     }
     Words<4> p[R][4];
@@ -759,15 +801,18 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) x = fmaxf(x, sc[u][t][r]);
-      x = max_across32(x);
-      const float top = fmaxf(m[u], x * a.scale), base = top == -INFINITY ? 0.f : top;
-      if (__any(top > m[u])) {
-        const float fade = power2(m[u] - base);
+      // The maximum that weights are taken relative to follows only when a row's has grown by
+      // a factor of 2^8: weights, their sum and O are floating point and as exact relative to
+      // any of them, and of 32 rows one or another would grow at almost every tile.
+      const float top = max_across32(x) * a.scale;
+      if (__any(top > m[u] + 8.f)) {
+        const float next = fmaxf(m[u], top), fade = next == -INFINITY ? 1.f : power2(m[u] - next);
         l[u] *= fade;
 #pragma unroll
         for (int t = 0; t < ND; ++t) o[u][t] *= fade;
-        m[u] = top;
+        m[u] = next;
       }
+      const float base = m[u] == -INFINITY ? 0.f : m[u];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -783,17 +828,24 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int t = 0; t < ND; ++t) {
-        const char* at = lds.v[half] + (i * 16 + h * 4 + c % 16 / 4) * VW + t * 64 +
-                         c / 16 * 32 + c % 4 * 8;
-        const Words<2> lo = transposed(at), hi = transposed(at + 8 * VW);
+        const int key = i * 16 + h * 4 + c % 16 / 4, chunk = t * 4 + c / 16 * 2 + c % 4 / 2;
+        const char* at = reinterpret_cast<const char*>(&vt[key * CHUNKS + W::place_v(key, chunk)]) +
+                         c % 2 * 8;
+        const Words<2> lo = transposed(at), hi = transposed(at + 8 * CHUNKS * 16);
         const Words<4> v{{lo.w[0], lo.w[1], hi.w[0], hi.w[1]}};
 #pragma unroll
         for (int u = 0; u < R; ++u) o[u][t] = mma32(v, p[u][i], o[u][t], T{});
       }
     __builtin_amdgcn_sched_barrier(0);
-    store(half ^ 1);
-    if (wave == 0) lds.rows[half][lane] = row_of(a, next);
-    __syncthreads();
+    store(x, kn, vn);
+    if (wave == 0) lds_rows[half][lane] = row_of(a, next) * row_bytes;
+    arrive();
+  };
+  for (int32_t s = 0;;) {
+    step(s, 0, k0, v0, k1, v1);
+    if (++s >= steps) break;
+    step(s, 1, k1, v1, k0, v0);
+    if (++s >= steps) break;
   }
 
   bool odd = false;
@@ -808,9 +860,9 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Lds& lds, const 
       for (int r = 0; r < 16; ++r)
         odd = odd || (t * 32 + r / 4 * 8 < d && o[u][t][r] != o[u][t][r]);
   }
-  if (odd) lds.redo = 1;
+  if (odd) redo = 1;
   __syncthreads();
-  if (lds.redo) {
+  if (redo) {
     for (int32_t r = wave; r < rows; r += kWaves) attend_row<T, C>(a, it, kv_head, r, lane);
     return;
   }
@@ -860,20 +912,27 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
 constexpr int kWideTiles = 1;                    // R of the kernels below
 constexpr int kWideRows = kWaves * 32 * kWideTiles;
 
-// `n_wide` wide items from `wide` on, and with BOTH `n_narrow` from `narrow` on in the same
-// launch: the matrix units work on the former while the latter wait for memory. Of a wide
-// item neighbouring blocks are its heads, and where there are eight, all blocks of an XCD are
-// of one head, whose keys the items share in its L2.
-template <typename T, typename C, int DP, bool BOTH>
-__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_wide(
+// Wide items from `wide` on, of 16-bit caches at 16-byte addresses. Neighbouring blocks are the
+// heads of an item, and where there are eight, all blocks of an XCD are of one head, whose
+// keys the items share in its L2.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_wide(Args a,
+                                                                                 int32_t wide) {
+  using W = Wide<T, DP>;
+  __shared__ typename W::Tile k0, k1, v0, v1;
+  __shared__ typename W::Rows rows;
+  __shared__ int32_t redo;
+  wide_item<T, C, DP, kWideTiles, true>(k0, k1, v0, v1, rows, redo, a, wide + blockIdx.x / a.kv_heads,
+                                        blockIdx.x % a.kv_heads);
+}
+
+// `n_wide` wide items from `wide` on and `n_narrow` narrow ones from `narrow` on in one launch:
+// the matrix units work on the former while the latter wait for memory.
+template <typename T, typename C, int DP>
+__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_both(
     Args a, int32_t wide, int32_t n_wide, int32_t narrow, int32_t n_narrow) {
   extern __shared__ __attribute__((aligned(16))) char shared[];
   auto& of_wide = *reinterpret_cast<typename Wide<T, DP>::Lds*>(shared);
-  if constexpr (!BOTH) {
-    wide_item<T, C, DP, kWideTiles>(of_wide, a, wide + blockIdx.x / a.kv_heads,
-                                    blockIdx.x % a.kv_heads);
-    return;
-  }
   // Runs of as many blocks as a narrow item has; a wide item is `together` such runs. Those
   // of the wide items come at even distances among the first three quarters.
   const uint32_t each = a.kv_heads / a.together, run = blockIdx.x / each, part = blockIdx.x % each;
@@ -882,8 +941,10 @@ __global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_wide
   const uint32_t before = run < span ? uint64_t(run) * wides / span : wides;
   const uint32_t after = run < span ? uint64_t(run + 1) * wides / span : wides;
   if (after > before)
-    wide_item<T, C, DP, kWideTiles>(of_wide, a, wide + before / a.together,
-                                    before % a.together * each + part);
+    wide_item<T, C, DP, kWideTiles, false>(of_wide.k[0], of_wide.k[1], of_wide.v[0], of_wide.v[1],
+                                           of_wide.rows, of_wide.redo, a,
+                                           wide + before / a.together,
+                                           before % a.together * each + part);
   else
     narrow_item<T, C, DP>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared), a,
                           narrow + run - before, part * a.together, 0);
