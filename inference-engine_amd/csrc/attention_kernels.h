@@ -217,31 +217,6 @@ __device__ __forceinline__ uint32_t row_of(const Args& a, Place p) {
   return static_cast<uint32_t>(p.block) * static_cast<uint32_t>(a.block_size) + p.within;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
-  return x;
-}
-
-// The larger of two lanes 16 or 32 apart, by the row swaps of the vector unit: an LDS shuffle
-// would put its latency into every step's chain. (The halves of a swap are named: a bit cast
-// of a vector's element takes its first.)
-__device__ __forceinline__ float max_across32(float x) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  const uint32_t low = r[0], high = r[1];
-  return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
-}
-__device__ __forceinline__ float max_across16(float x) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-  const uint32_t low = r[0], high = r[1];
-  return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
-}
-
 __device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // --- one row key by key ------------------------------------------------------------------
@@ -485,7 +460,8 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][r]);
-      x = max_across32(max_across16(x));
+      x = fmaxf(x, lane_xor<16>(x));
+      x = fmaxf(x, lane_xor<32>(x));
       top = fmaxf(m, x * a.scale);
     }
     const float base = top == -INFINITY ? 0.f : top;
@@ -538,8 +514,8 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
   }
 
   // The parts of each head's waves.
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
+  l += lane_xor<16>(l);
+  l += lane_xor<32>(l);
   if (lane < 16) lds.ml[wave][lane] = {m, l};
   __syncthreads();
   float all = -INFINITY;
@@ -804,7 +780,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
       // The maximum that weights are taken relative to follows only when a row's has grown by
       // a factor of 2^8: weights, their sum and O are floating point and as exact relative to
       // any of them, and of 32 rows one or another would grow at almost every tile.
-      const float top = max_across32(x) * a.scale;
+      const float top = fmaxf(x, lane_xor<32>(x)) * a.scale;
       if (__any(top > m[u] + 8.f)) {
         const float next = fmaxf(m[u], top), fade = next == -INFINITY ? 1.f : power2(m[u] - next);
         l[u] *= fade;
@@ -851,7 +827,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
   bool odd = false;
 #pragma unroll
   for (int u = 0; u < R; ++u) {
-    l[u] += __shfl_xor(l[u], 32);
+    l[u] += lane_xor<32>(l[u]);
     if ((wave * R + u) * 32 + c >= rows) continue;
     odd = odd || l[u] != l[u];
 #pragma unroll

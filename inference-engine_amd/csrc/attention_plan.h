@@ -161,10 +161,13 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   if (narrow_keys * sh.kv_heads >= blocks * kNarrowWaves * 256)
     plan.together = sh.kv_heads % 4 == 0 ? 4 : sh.kv_heads % 2 == 0 ? 2 : 1;
   narrow = split(narrow, sh.kv_heads / plan.together, blocks, 256, 64);
+  const int64_t narrow_blocks = int64_t(narrow.size()) * sh.kv_heads / plan.together;
   // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
-  // are: they are cut only where more than half of the compute units would have none.
+  // are: they are cut only where more than half of the compute units would have none, and so
+  // that those of a step run at once, two to a compute unit.
   if (int64_t(wide.size()) * sh.kv_heads * 2 < compute_units)
-    wide = split(wide, sh.kv_heads, 2 * compute_units, 128, 64);
+    wide = split(wide, sh.kv_heads, std::max<int64_t>(compute_units, 2 * compute_units - narrow_blocks), 128,
+                 64);
   // The longest first: the last workgroups to start are short ones.
   auto longer = [](const Item& x, const Item& y) { return keys_of(x) > keys_of(y); };
   std::stable_sort(narrow.begin(), narrow.end(), longer);

@@ -46,38 +46,20 @@ __device__ __forceinline__ uint32_t index_of(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
 }
 
-__device__ __forceinline__ uint64_t shuffled(uint64_t k, int mask) {
-  return __shfl_xor(static_cast<unsigned long long>(k), mask);
-}
 __device__ __forceinline__ uint64_t wave_top(uint64_t k) {
-  for (int s = 32; s; s >>= 1) {
-    const uint64_t other = shuffled(k, s);
-    k = other > k ? other : k;
-  }
-  return k;
-}
-__device__ __forceinline__ float wave_max(float x) {
-  for (int s = 32; s; s >>= 1) x = fmaxf(x, __shfl_xor(x, s));
-  return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-  for (int s = 32; s; s >>= 1) x += __shfl_xor(x, s);
-  return x;
+  return wave_all(k, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 
-// The lanes' values in falling order (Batcher's bitonic network).
-template <typename V>
-__device__ __forceinline__ V wave_sorted(V x, int lane) {
-#pragma unroll
-  for (int size = 2; size <= kWave; size *= 2)
-#pragma unroll
-    for (int step = size / 2; step; step /= 2) {
-      const V other = __shfl_xor(x, step);
-      const bool first = !(lane & step), falling = !(lane & size);
-      const bool larger = other > x;
-      x = (first == falling) == larger ? other : x;
-    }
-  return x;
+// The lanes' values in falling order (Batcher's bitonic network: runs of SIZE, compared at
+// distance STEP).
+template <int SIZE = 2, int STEP = 1>
+__device__ __forceinline__ float wave_sorted(float x) {
+  const float other = lane_xor<STEP>(x);
+  const bool first = !(threadIdx.x & STEP), falling = !(threadIdx.x & SIZE) || SIZE == kWave;
+  x = first == falling ? fmaxf(x, other) : fminf(x, other);
+  if constexpr (STEP > 1) return wave_sorted<SIZE, STEP / 2>(x);
+  else if constexpr (SIZE < kWave) return wave_sorted<SIZE * 2, SIZE>(x);
+  else return x;
 }
 
 // Sums of a part of a row: m, s and w above.
@@ -113,11 +95,17 @@ __device__ __forceinline__ float logprob_of(float x, const Sums& a, float log_s)
   return a.s == 0.f ? -INFINITY : (x - a.m) - log_s;
 }
 
+// The logit of the row's token, NaN for one outside the vocabulary. Read before the sums, so
+// that nothing waits for it.
 template <typename T>
-__device__ __forceinline__ void write_row(const Scores& out, const T* x, int64_t row,
-                                          const Sums& a, float log_s) {
+__device__ __forceinline__ float given_of(const Scores& out, const T* x, int64_t row) {
   const int64_t t = out.tokens[row];
-  out.logprobs[row] = t < 0 || t >= out.vocab ? NAN : logprob_of(to_float(x[t]), a, log_s);
+  return t < 0 || t >= out.vocab ? NAN : to_float(x[t]);
+}
+
+__device__ __forceinline__ void write_row(const Scores& out, float given, int64_t row,
+                                          const Sums& a, float log_s) {
+  out.logprobs[row] = given != given ? NAN : logprob_of(given, a, log_s);
   out.entropy[row] = a.s == 0.f ? 0.f : log_s - a.w / a.s;
 }
 
@@ -133,6 +121,17 @@ struct Parts {
   uint64_t* keys;    // [rows][parts][top], falling; 0 past the part's logits
   int32_t parts, size;
 };
+
+// How many keys of a list are larger. The list goes on for `kPad` zeros: eight keys are read
+// at a time, or each would be waited for.
+constexpr int kPad = 8;
+__device__ __forceinline__ int32_t rank_of(uint64_t key, const uint64_t* list, int32_t count) {
+  int32_t rank = 0;
+  for (int32_t j = 0; j < count; j += kPad)
+#pragma unroll
+    for (int i = 0; i < kPad; ++i) rank += list[j + i] > key;
+  return rank;
+}
 
 // One part of a row by one workgroup.
 //
@@ -154,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   const T* x = logits + row * stride;
   __shared__ float most[kWaves];
   __shared__ float2 sums[kWaves], bounds[kWaves];
-  __shared__ uint64_t list[kCandidates];
+  __shared__ uint64_t list[kCandidates + kPad];
   __shared__ int32_t listed;
 
   // Logit v (of this thread's `HELD`) is number (v / VEC * kThreads + tid) * VEC + v % VEC.
@@ -173,6 +172,8 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
         held[i * VEC + j] = at + j < n ? to_float(x[first + at + j]) : -INFINITY;
     }
   }
+  const bool whole = parts.parts == 1;
+  const float given = whole ? given_of(out, x, row) : 0.f;
   const auto index = [&](int v) { return (v / VEC * kThreads + tid) * VEC + v % VEC; };
 
   float mine = -INFINITY;
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   if (top) {
     float each = of_wave, alone = of_wave;  // the wave's ceil(k / 4)-th and k-th largest lane
     if (top > 1) {
-      const float sorted = wave_sorted(mine, lane);
+      const float sorted = wave_sorted(mine);
       each = __shfl(sorted, (top + kWaves - 1) / kWaves - 1);
       alone = __shfl(sorted, top - 1);
     }
@@ -209,10 +210,9 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   all.s = (sums[0].x + sums[1].x) + (sums[2].x + sums[3].x);
   all.w = (sums[0].y + sums[1].y) + (sums[2].y + sums[3].y);
   const float log_s = logf(all.s);
-  const bool whole = parts.parts == 1;
   if (tid == 0) {
     if (whole)
-      write_row(out, x, row, all, log_s);
+      write_row(out, given, row, all, log_s);
     else
       parts.sums[blockIdx.x] = all;
   }
@@ -227,21 +227,35 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   const float bound =
       fmaxf(fminf(fminf(bounds[0].x, bounds[1].x), fminf(bounds[2].x, bounds[3].x)),
             fmaxf(fmaxf(bounds[0].y, bounds[1].y), fmaxf(bounds[2].y, bounds[3].y)));
-  if (mine >= bound) {
+  // Each wave takes as many places of the list as its lanes have candidates.
+  int32_t own = 0;
+#pragma unroll
+  for (int v = 0; v < HELD; ++v) own += held[v] >= bound && index(v) < n;
+  int32_t before = 0, of_lanes = 0;
+#pragma unroll
+  for (int bit = 0; HELD >> bit; ++bit) {
+    const uint64_t with = __ballot(own >> bit & 1);
+    before += __popcll(with & ((uint64_t(1) << lane) - 1)) << bit;
+    of_lanes += __popcll(with) << bit;
+  }
+  int32_t at = lane == 0 && of_lanes ? atomicAdd(&listed, of_lanes) : 0;
+  at = __builtin_amdgcn_readfirstlane(at) + before;
+  if (own) {
 #pragma unroll
     for (int v = 0; v < HELD; ++v)
       if (held[v] >= bound && index(v) < n) {
-        const int at = atomicAdd(&listed, 1);
         if (at < kCandidates) list[at] = key_of(held[v], first + index(v));
+        ++at;
       }
   }
   __syncthreads();
   const int32_t count = listed;
   if (count <= kCandidates && all.s == all.s) {
+    if (tid < kPad) list[count + tid] = 0;
+    __syncthreads();
     for (int32_t i = tid; i < count; i += kThreads) {
       const uint64_t key = list[i];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < count; ++j) rank += list[j] > key;
+      const int32_t rank = rank_of(key, list, count);
       if (rank < top) put(rank, key);
     }
     // A part of fewer logits than alternatives (of a row of several parts).
@@ -271,13 +285,14 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_rows(const T* logits, int64_t stride,
                                                       int64_t n_rows, Scores out, Parts parts) {
-  __shared__ uint64_t lists[kWaves][kCandidates];
+  __shared__ uint64_t lists[kWaves][kCandidates + kPad];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
   if (row >= n_rows) return;
   const Sums* sums = parts.sums + row * parts.parts;
   const int32_t n = parts.parts, top = out.top;
   const uint64_t* keys = parts.keys + row * n * top;
+  const float given = given_of(out, logits + row * stride, row);
   uint64_t any = 0, least = ~uint64_t(0);
   const int32_t each = (top + n - 1) / n;
   float m = -INFINITY;
@@ -299,7 +314,7 @@ __global__ __launch_bounds__(kThreads) void join_rows(const T* logits, int64_t s
   all.s = wave_sum(all.s);
   all.w = wave_sum(all.w);
   const float log_s = logf(all.s);
-  if (lane == 0) write_row(out, logits + row * stride, row, all, log_s);
+  if (lane == 0) write_row(out, given, row, all, log_s);
   if (!top) return;
 
   any = wave_top(any);
@@ -308,20 +323,31 @@ __global__ __launch_bounds__(kThreads) void join_rows(const T* logits, int64_t s
   uint64_t* list = lists[wave];
   int32_t count = 0;
   const int32_t total = n * top;
-  for (int32_t i = 0; i < total && count <= kCandidates; i += kWave) {
-    const uint64_t key = i + lane < total ? keys[i + lane] : 0;
-    const uint64_t in = __ballot(key && key >= bound);
-    const int32_t at = count + __popcll(in & ((uint64_t(1) << lane) - 1));
-    if (key && key >= bound && at < kCandidates) list[at] = key;
-    count += __popcll(in);
+  constexpr int kAtOnce = 8;                  // loads on their way
+  for (int32_t i0 = 0; i0 < total && count <= kCandidates; i0 += kAtOnce * kWave) {
+    uint64_t key[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int32_t at = i0 + i * kWave + lane;
+      key[i] = keys[at < total ? at : total - 1];
+      if (at >= total) key[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const bool in = key[i] && key[i] >= bound;
+      const uint64_t who = __ballot(in);
+      const int32_t at = count + __popcll(who & ((uint64_t(1) << lane) - 1));
+      if (in && at < kCandidates) list[at] = key[i];
+      count += __popcll(who);
+    }
   }
+  if (lane < kPad && count <= kCandidates) list[count + lane] = 0;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   if (count <= kCandidates) {
     for (int32_t i = lane; i < count; i += kWave) {
       const uint64_t key = list[i];
-      int32_t rank = 0;
-      for (int32_t j = 0; j < count; ++j) rank += list[j] > key;
+      const int32_t rank = rank_of(key, list, count);
       if (rank < top) write_top(out, row, rank, key, all, log_s);
     }
     return;

@@ -189,7 +189,7 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
     if q.stride(2) != 1 or q.is_neg():
         q = q.contiguous().resolve_neg()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or \
             not out.is_contiguous() or out.is_neg():
         raise ValueError("out must be a contiguous tensor of the queries' shape, type and device")
@@ -200,7 +200,7 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
         plan._used_on(stream)
     need, workspace = plan._workspace_bytes, None
     if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=pool.device)
+        workspace = q.new_empty(need, dtype=torch.uint8)
     k, v = plan._layers[layer]
     _ops.call("iekv_attend", plan._handle, plan._words.data_ptr(), k, v, q.data_ptr(), q.stride(0),
               q.stride(1), 1.0 / math.sqrt(plan.head_dim) if scale is None else scale,

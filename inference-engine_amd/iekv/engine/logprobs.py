@@ -8,6 +8,7 @@ alternatives. The reference draws its tokens from the logits on the host
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -28,6 +29,11 @@ class TokenLogprobs:
     top_ids: torch.Tensor         # [rows, top] int64
 
 
+@lru_cache(maxsize=256)
+def _workspace_bytes(kind: int, rows: int, vocab: int, top: int) -> int:
+    return _ops.lib().iekv_logprobs_workspace(kind, rows, vocab, top)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
     """Score ``tokens[i]`` under ``softmax(logits[i])``, for every row.
 
@@ -38,7 +44,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     a NaN or +inf is NaN; a token outside the vocabulary (a padding mark) has log
     probability NaN. Runs on the device's current stream.
     """
-    if logits.dim() != 2 or logits.dtype not in _TYPES or logits.device.type != "cuda":
+    if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda:
         raise ValueError(f"logits must be [rows, vocab] float32, float16 or bfloat16 on the GPU, "
                          f"got {tuple(logits.shape)} {logits.dtype} on {logits.device}")
     rows, vocab = logits.shape
@@ -53,20 +59,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
                            "no_grad")
     if logits.stride(1) != 1 or logits.is_neg():
         logits = logits.contiguous().resolve_neg()
-    tokens = tokens.contiguous().resolve_neg()
-    device = logits.device
-    scores = torch.empty((2, rows), dtype=torch.float32, device=device)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
-    result = TokenLogprobs(scores[0], scores[1], top_logprobs, top_ids)
-    if not rows:
-        return result
-    kind = _TYPES[logits.dtype]
-    need = _ops.lib().iekv_logprobs_workspace(kind, rows, vocab, top)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    base = scores.data_ptr()
-    _ops.call("iekv_logprobs", kind, logits.data_ptr(), logits.stride(0), rows, vocab,
-              tokens.data_ptr(), top, base, base + 4 * rows, top_logprobs.data_ptr(),
-              top_ids.data_ptr(), workspace.data_ptr() if need else None, need,
-              current_stream_handle(device))
-    return result
+    if not tokens.is_contiguous() or tokens.is_neg():
+        tokens = tokens.contiguous().resolve_neg()
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    top_ids = logits.new_empty((rows, top), dtype=torch.int64)
+    if rows:
+        kind = _TYPES[logits.dtype]
+        need, workspace = _workspace_bytes(kind, rows, vocab, top), None
+        if need:
+            workspace = logits.new_empty(need, dtype=torch.uint8)
+        _ops.call("iekv_logprobs", kind, logits.data_ptr(), logits.stride(0), rows, vocab,
+                  tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(),
+                  top_logprobs.data_ptr(), top_ids.data_ptr(),
+                  workspace.data_ptr() if need else None, need,
+                  current_stream_handle(logits.device))
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
