@@ -65,7 +65,8 @@ class Sequence:
     is the physical block holding logical block ``i``. ``swapped`` is set while
     a swap preemption keeps the sequence's KV in host memory:
     ``(host payload of its first ceil(num_computed / block_size) blocks,
-    num_computed at swap-out)``.
+    num_computed at swap-out)``. ``scores[i]`` is what an engine that scores its answers
+    (``EngineConfig.logprobs``) says of generated token ``i``.
     """
 
     def __init__(self, prompt_ids: list[int], block_size: int, max_new_tokens: int = 64,
@@ -84,6 +85,7 @@ class Sequence:
         self.num_scheduled = 0
         self.block_table: list[int] = []
         self.swapped: tuple | None = None
+        self.scores: list = []
 
     # -- sizes ---------------------------------------------------------------------
     @property

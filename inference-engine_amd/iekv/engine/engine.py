@@ -31,6 +31,10 @@ class EngineConfig:
 
     ``preemption`` is this build's addition: ``"recompute"`` (the reference's
     behaviour) or ``"swap"`` (preempted sequences keep their KV in host memory).
+    ``logprobs`` is another: with a number ``k``, every generated token is scored on the
+    GPU (``iekv.engine.logprobs``) and ``Sequence.scores`` holds its log probability, the
+    entropy of the distribution at temperature 1 and the ``k`` most likely tokens; None
+    scores nothing.
     """
 
     block_size: int = 16
@@ -41,6 +45,17 @@ class EngineConfig:
     offload_blocks: int = 0
     capture_graphs: bool = False
     preemption: str = "recompute"
+    logprobs: int | None = None
+
+
+@dataclass(slots=True)
+class TokenScore:
+    """What the model thought of a token it generated."""
+
+    token_id: int
+    logprob: float
+    entropy: float
+    top: list[tuple[int, float]]          # (token, log probability), most likely first
 
 
 def sample_from_logits(logits: np.ndarray, temperatures: np.ndarray,
@@ -86,6 +101,8 @@ class Engine:
         self.copier_factory = copier_factory or default_copier_factory
         if self.config.preemption not in ("recompute", "swap"):
             raise ValueError("preemption must be 'recompute' or 'swap'")
+        if self.config.logprobs is not None and self.config.logprobs < 0:
+            raise ValueError(f"logprobs {self.config.logprobs} must not be negative")
         self.blocks = BlockManager(self.config.num_blocks, self.config.block_size)
         self.generator = np.random.default_rng(self.config.seed)
         if caches is None:
@@ -135,11 +152,15 @@ class Engine:
         """
         self.blocks.flush_pending()
 
-    def forward(self, batch):
-        """Run the model over a scheduled batch; returns (layout, last-token logits)."""
+    def _hidden(self, batch):
         self.flush_offloads()
         layout = build_layout(batch, self.config.block_size)
-        hidden = self.model.forward(layout, self.k_caches, self.v_caches, self.config.block_size)
+        return layout, self.model.forward(layout, self.k_caches, self.v_caches,
+                                          self.config.block_size)
+
+    def forward(self, batch):
+        """Run the model over a scheduled batch; returns (layout, last-token logits)."""
+        layout, hidden = self._hidden(batch)
         return layout, self.model.logits_for_last_token_of_each(hidden, layout.query_lens)
 
     def _advance(self):
@@ -148,11 +169,37 @@ class Engine:
         batch = self.scheduler.schedule()
         if not batch:
             return None, []
-        _, logits = self.forward(batch)
+        on_device = None
+        if self.config.logprobs is None:
+            _, logits = self.forward(batch)
+        else:
+            layout, hidden = self._hidden(batch)
+            on_device = self.model.last_token_logits(hidden, layout.query_lens)
+            logits = on_device.cpu().numpy()
         temps = np.fromiter((s.temperature for s in batch.sequences), dtype=np.float32,
                             count=len(batch))
-        tokens = sample_from_logits(logits, temps, self.generator)
-        return batch, self.scheduler.finish_step(batch, [int(t) for t in tokens])
+        tokens = [int(t) for t in sample_from_logits(logits, temps, self.generator)]
+        scores = None if on_device is None else self._score(on_device, tokens)
+        lengths = [len(s) for s in batch.sequences]
+        finished = self.scheduler.finish_step(batch, tokens)
+        if scores is not None:
+            # A chunk in the middle of a prompt got no token.
+            for seq, length, score in zip(batch.sequences, lengths, scores):
+                if len(seq) > length:
+                    seq.scores.append(score)
+        return batch, finished
+
+    def _score(self, logits, tokens: list[int]) -> list[TokenScore]:
+        """Score the tokens sampled from ``logits`` (a device tensor, a row each)."""
+        import torch
+
+        from .logprobs import token_logprobs
+
+        given = torch.tensor(tokens, dtype=torch.int64, device=logits.device)
+        s = token_logprobs(logits, given, top=self.config.logprobs)
+        columns = (t.tolist() for t in (s.logprobs, s.entropy, s.top_ids, s.top_logprobs))
+        return [TokenScore(token, logprob, entropy, list(zip(ids, values)))
+                for token, (logprob, entropy, ids, values) in zip(tokens, zip(*columns))]
 
     def step(self) -> list[Sequence]:
         """Run one step; returns the sequences it finished."""

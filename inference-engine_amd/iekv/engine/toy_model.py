@@ -11,7 +11,11 @@ drawn from ``numpy.random.default_rng(seed)`` in the same order). Attention
 math runs in float32 whatever the cache dtype. It is support code: the
 handoff never calls it. With ``hip_kv=True`` its KV writes and context reads go
 through libiekv's slot kernels (``iekv.engine.slots``) instead of torch's
-``index_copy_`` / ``index_select``.
+``index_copy_`` / ``index_select``. With ``hip_attention=True`` each layer attends
+straight over its paged cache (``iekv.engine.attention``): one plan per step serves
+every layer, and the leading blocks that all sequences of a step share are attended
+once for all. ``window`` and ``sinks`` make every layer's attention a sliding window
+that keeps the first keys visible, on either path.
 """
 from __future__ import annotations
 
@@ -99,11 +103,20 @@ class ToyTransformer:
     """Paged toy decoder on ``device`` with KV caches of ``cache_dtype``."""
 
     def __init__(self, config: ModelConfig, seed: int = 0, device: str | torch.device = "cuda",
-                 cache_dtype: torch.dtype = torch.float32, hip_kv: bool = False) -> None:
+                 cache_dtype: torch.dtype = torch.float32, hip_kv: bool = False,
+                 hip_attention: bool = False, window: int | None = None,
+                 sinks: int = 0) -> None:
+        if window is not None and window < 1:
+            raise ValueError(f"window {window} must be at least 1 (None for no window)")
+        if sinks < 0:
+            raise ValueError(f"sinks {sinks} is negative")
         self.config = config
         self.device = torch.device(device)
         self.cache_dtype = cache_dtype
         self.hip_kv = hip_kv
+        self.hip_attention = hip_attention
+        self.window = window
+        self.sinks = sinks
         # Registered pools by cache address; an engine holds each one (bind_caches).
         self._pools: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
         rng = np.random.default_rng(seed)
@@ -137,11 +150,11 @@ class ToyTransformer:
                                   device=self.device)
 
     def bind_caches(self, k_caches, v_caches, block_size: int):
-        """Register a pool for the slot kernels; the caller keeps the returned
-        handle for as long as it uses the caches (an Engine holds it for its
+        """Register a pool for the slot and attention kernels; the caller keeps the
+        returned handle for as long as it uses the caches (an Engine holds it for its
         lifetime). The model itself keeps only a weak reference, so a pool is
-        released with the engine that owns it. None without ``hip_kv``."""
-        if not self.hip_kv:
+        released with the engine that owns it. None where torch does both."""
+        if not (self.hip_kv or self.hip_attention):
             return None
         from .pools import KVPool
 
@@ -187,11 +200,24 @@ class ToyTransformer:
             scores = torch.matmul(qh, kt) / float(np.sqrt(c.head_dim))
             rows = torch.arange(query_len, device=self.device)[:, None] + (context_len - query_len)
             cols = torch.arange(context_len, device=self.device)[None, :]
-            scores = scores.masked_fill(~(cols <= rows), float("-inf"))
+            seen = cols <= rows
+            if self.window is not None:
+                seen &= (cols > rows - self.window) | (cols < self.sinks)
+            scores = scores.masked_fill(~seen, float("-inf"))
             weights = torch.softmax(scores, dim=-1)
             outputs.append(torch.matmul(weights, vh).permute(1, 0, 2))
             start += query_len
         return torch.cat(outputs, dim=0)
+
+    def _plan(self, pool, layout: BatchLayout):
+        """The step's attention plan, for every layer."""
+        from .attention import AttentionPlan, common_blocks
+
+        return AttentionPlan(pool, layout.block_tables, layout.context_lens, layout.query_lens,
+                             self.config.num_heads, window=self.window, sinks=self.sinks,
+                             shared_blocks=common_blocks(layout.block_tables, layout.context_lens,
+                                                         pool.block_size),
+                             query_dtype=torch.float32)
 
     @torch.no_grad()
     def forward(self, layout: BatchLayout, k_caches, v_caches, block_size: int) -> torch.Tensor:
@@ -205,16 +231,25 @@ class ToyTransformer:
         attends over that context followed by this step's rows, cast to the cache
         dtype exactly as a cache read returns them; after the layers, one
         iekv_write_slots_layers writes every layer's new rows.
+
+        With ``hip_attention`` each layer's rows are written before it attends (by
+        iekv_write_slots_layers with ``hip_kv``), and iekv_attend reads the cache
+        through the block tables; nothing is gathered.
         """
         c = self.config
         tokens = torch.as_tensor(layout.token_ids, device=self.device, dtype=torch.long)
         positions = torch.as_tensor(layout.positions, device=self.device, dtype=torch.long)
         slots = torch.as_tensor(layout.slot_mapping, device=self.device, dtype=torch.long)
         x = self.embedding[tokens]
-        pool = self._pool(k_caches, v_caches, block_size) if self.hip_kv else None
-        if pool is not None:
-            from .slots import gather_rows_arrays, write_slots_layers
-
+        pool = self._pool(k_caches, v_caches, block_size) \
+            if self.hip_kv or self.hip_attention else None
+        plan = self._plan(pool, layout) if self.hip_attention else None
+        gathers = pool is not None and plan is None
+        if self.hip_kv:
+            from .slots import gather_rows_arrays, write_slots, write_slots_layers
+        if plan is not None:
+            from .attention import attend
+        if gathers:
             earlier = [gather_rows_arrays(pool, table, ctx - n) if ctx > n else None
                        for table, ctx, n in zip(layout.block_tables, layout.context_lens,
                                                 layout.query_lens)]
@@ -228,7 +263,7 @@ class ToyTransformer:
             q = _rope(q, positions, self.cos, self.sin, c.rope_halved)
             k = _rope(k, positions, self.cos, self.sin, c.rope_halved)
             kc, vc = k.to(k_cache.dtype), v.to(v_cache.dtype)
-            if pool is not None:
+            if gathers:
                 new_k.append(kc)
                 new_v.append(vc)
                 contexts = []
@@ -238,23 +273,33 @@ class ToyTransformer:
                         ks = torch.cat((prior[index], ks))
                         vs = torch.cat((prior[c.num_layers + index], vs))
                     contexts.append((ks, vs))
+            elif self.hip_kv:
+                write_slots(pool, index, kc, vc, slots)
             else:
                 k_cache.index_copy_(0, slots, kc)
                 v_cache.index_copy_(0, slots, vc)
+            if plan is not None:
+                attended = attend(plan, index, q)
+            elif not gathers:
                 contexts = [(self._cached_rows(k_cache, t, n, block_size),
                              self._cached_rows(v_cache, t, n, block_size))
                             for t, n in zip(layout.block_tables, layout.context_lens)]
-            attended = self._attend(q, contexts, layout)
+            if plan is None:
+                attended = self._attend(q, contexts, layout)
             x = x + attended.reshape(-1, c.num_heads * c.head_dim) @ layer.o_proj
             normed = _rms_norm(x, layer.mlp_norm, c.norm_eps)
             gate = normed @ layer.gate_proj
             x = x + (gate / (1.0 + torch.exp(-gate)) * (normed @ layer.up_proj)) @ layer.down_proj
-        if pool is not None and layout.num_tokens:
+        if gathers and layout.num_tokens:
             write_slots_layers(pool, torch.stack(new_k), torch.stack(new_v), slots)
         return _rms_norm(x, self.final_norm, c.norm_eps)
 
     @torch.no_grad()
+    def last_token_logits(self, hidden: torch.Tensor, query_lens: list[int]) -> torch.Tensor:
+        """``[sequences, vocab]`` float32, on the device."""
+        ends = torch.as_tensor(np.cumsum(query_lens) - 1, device=self.device, dtype=torch.long)
+        return (hidden[ends] @ self.lm_head).float()
+
     def logits_for_last_token_of_each(self, hidden: torch.Tensor,
                                       query_lens: list[int]) -> np.ndarray:
-        ends = torch.as_tensor(np.cumsum(query_lens) - 1, device=self.device, dtype=torch.long)
-        return (hidden[ends] @ self.lm_head).float().cpu().numpy()
+        return self.last_token_logits(hidden, query_lens).cpu().numpy()

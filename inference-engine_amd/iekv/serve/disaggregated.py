@@ -43,7 +43,7 @@ Transfer modes (``mode=``):
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Callable
 
 from ..core.sequence import Sequence, Status
@@ -120,7 +120,9 @@ class KVTransfer:
     (None for a direct-mode transfer, whose ``source`` names the blocks).
     ``first_block`` is the index in the sequence's table of the first moved
     block (non-zero only for prefix-aware transfers). ``bytes_moved`` is the
-    payload size of the moved blocks, one direction (B x 2L x T).
+    payload size of the moved blocks, one direction (B x 2L x T). ``scores`` are the
+    prefill worker's of the tokens it generated (``Sequence.scores``; they do not go over
+    the wire format).
     """
 
     token_ids: list[int]
@@ -129,6 +131,7 @@ class KVTransfer:
     bytes_moved: int = 0
     first_block: int = 0
     source: DirectSource | None = None
+    scores: list = field(default_factory=list)
 
     @property
     def num_blocks(self) -> int:
@@ -192,11 +195,12 @@ class PrefillWorker:
             source = DirectSource(self.copier, list(moved), release=lambda: self._retire(seq))
             return KVTransfer(token_ids=list(seq.token_ids), num_computed=seq.num_computed,
                               block_payloads=None, bytes_moved=nbytes,
-                              first_block=skip_blocks, source=source)
+                              first_block=skip_blocks, source=source,
+                              scores=list(seq.scores))
         payloads = self._read(moved, payload_buffer)
         transfer = KVTransfer(token_ids=list(seq.token_ids), num_computed=seq.num_computed,
                               block_payloads=payloads, bytes_moved=nbytes,
-                              first_block=skip_blocks)
+                              first_block=skip_blocks, scores=list(seq.scores))
         self._retire(seq)
         return transfer
 
@@ -266,6 +270,7 @@ class DecodeWorker:
 
         seq.token_ids = list(transfer.token_ids)
         seq.num_computed = transfer.num_computed
+        seq.scores = list(transfer.scores)
         engine.scheduler.waiting.remove(seq)
         copied = True
         if deferred:

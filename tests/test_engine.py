@@ -208,3 +208,31 @@ def test_the_paged_view_indexes_block_tiles_without_a_copy():
     assert (k[1][8:12] == -1).all() and (k[1][:8] >= 0).all()
     with pytest.raises(ValueError):
         paged_view(k[1], 5)
+
+
+def test_answers_are_scored_only_when_asked():
+    """Without ``logprobs`` nothing is scored; a negative number of alternatives is refused."""
+    eng = engine()
+    eng.generate([[1, 2, 3]], max_new_tokens=2, temperature=0.0)
+    assert all(s.scores == [] for s in eng.scheduler.finished)
+    with pytest.raises(ValueError, match="logprobs -1"):
+        engine(logprobs=-1)
+
+
+def test_a_window_hides_earlier_keys_on_the_torch_path():
+    """With a window that holds every key the output is that of no window; a window of one
+    key sees neither; windows and sinks out of range are refused."""
+    from iekv.engine.engine import Engine, EngineConfig
+    from iekv.engine.toy_model import ModelConfig, ToyTransformer
+
+    def generate(**options):
+        toy = ToyTransformer(ModelConfig(), seed=3, device="cpu", **options)
+        return Engine(toy, EngineConfig(num_blocks=64)).generate(
+            [[5, 9, 2, 77, 31, 8, 100, 4]], max_new_tokens=10, temperature=0.0)
+
+    whole = generate()
+    assert generate(window=1000) == whole == generate(window=4, sinks=1000)
+    assert generate(window=1) != whole
+    for bad in (dict(window=0), dict(sinks=-1)):
+        with pytest.raises(ValueError):
+            ToyTransformer(ModelConfig(), device="cpu", **bad)
