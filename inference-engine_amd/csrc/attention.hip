@@ -39,6 +39,7 @@ using iekv_attention::Launch;
 struct iekv_attention_plan {
   iekv_attention_shape shape;
   Launch narrow, wide;
+  bool streams;                  // the narrow items are a long stream
   int32_t together;              // KV heads a workgroup of the narrow kernel takes
   int32_t joined;                // tokens with several parts
   int64_t tokens, slots;
@@ -75,10 +76,10 @@ template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
   const int32_t narrow_blocks = narrow * (a.kv_heads / a.together);
-  // Both kinds in one launch while the narrow ones fit the card at once (24 sequences of two KV
-  // heads behind 512 tokens: 12.4 us against 18.4 in two); a long stream of them is better
-  // alone on it (128 sequences of the 8B shape: 215 us in two launches, 255 in one).
-  const bool both = wide && narrow && narrow_blocks <= 2 * compute_units();
+  // Both kinds in one launch where the narrow ones are soon done (24 sequences of two KV heads
+  // behind 512 tokens: 12.4 us against 18.4 in two); a long stream of them is better alone on
+  // the card (128 sequences of the 8B shape: 206 us in two launches, 246 in one).
+  const bool both = wide && narrow && !plan.streams;
   if constexpr (sizeof(T) == 2) {
     if (wide) {
       const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -221,6 +222,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
   plan->shape = shape;
   plan->narrow = made.narrow;
   plan->wide = made.wide;
+  plan->streams = made.streams;
   plan->together = made.together;
   plan->joined = static_cast<int32_t>(made.join_tokens.size());
   plan->tokens = tokens;

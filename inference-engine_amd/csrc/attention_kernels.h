@@ -414,9 +414,10 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
   int half = 0;
   Place next{0, 0};
   if (turn < steps) {
-    keep(0, place(turn));
+    const Place now = place(turn);
+    next = place(turn + turns);                 // before K's loads: see below
+    keep(0, now);
     load_k(0);
-    next = place(turn + turns);
   }
   for (int32_t s = turn; s < steps; s += turns, half ^= 1) {
     keep(half ^ 1, next);
@@ -948,32 +949,39 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* to
   const auto slot_of = [&](int32_t p) {
     return static_cast<int64_t>(parts[p] + in_group) * a.kv_heads + kv_head;
   };
-  float m = -INFINITY;
-  for (int32_t p = p0 + lane; p < p1; p += kWave) m = fmaxf(m, a.part_ml[slot_of(p)].x);
-  m = wave_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
   for (int32_t q0 = p0; q0 < p1; q0 += kWave) {
     const int32_t count = p1 - q0 < kWave ? p1 - q0 : kWave;
-    const int32_t p = q0 + (lane < count ? lane : 0);
-    const int64_t slot = slot_of(p);
+    const int64_t slot = slot_of(q0 + (lane < count ? lane : 0));
     const float2 ml = a.part_ml[slot];
-    const float weight = power2(ml.x - base);
-    if (lane < count) l = fmaf(weight, ml.y, l);
-    for (int32_t q = turn * each; q < count; q += 4 * W * each) {
-      f32x4 x[4];
-      float w[4];
+    // The first parts' sums are on their way while the maximum is found.
+    constexpr int kAtOnce = 4;
+    f32x4 x[kAtOnce];
+    const auto load = [&](int32_t q) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kAtOnce; ++i) {
         const int32_t mine = q + i * W * each + which;
         const int64_t at = __shfl(slot, mine < count ? mine : 0) * d + (d0 < d ? d0 : 0);
-        w[i] = __shfl(weight, mine < count ? mine : 0);
         __builtin_memcpy(&x[i], a.part_o + at, 16);
       }
+    };
+    load(turn * each);
+    const float top = fmaxf(m, wave_max(lane < count ? ml.x : -INFINITY));
+    const float base = top == -INFINITY ? 0.f : top, fade = power2(m - base);
+    m = top;
+    l *= fade;
+    o *= fade;
+    const float weight = power2(ml.x - base);
+    if (lane < count) l = fmaf(weight, ml.y, l);
+    for (int32_t q = turn * each; q < count; q += kAtOnce * W * each) {
+      if (q != turn * each) load(q);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (q + i * W * each + which < count) o += x[i] * w[i];
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int32_t mine = q + i * W * each + which;
+        const float w = __shfl(weight, mine < count ? mine : 0);
+        if (mine < count) o += x[i] * w;
+      }
     }
   }
   l = wave_sum(l);

@@ -45,6 +45,7 @@ struct Launch {
 struct Plan {
   std::vector<Item> items;
   Launch narrow, wide;
+  bool streams = false;                // the narrow items keep the card's memory busy for long
   int32_t together = 1;                // KV heads a workgroup of the narrow kernel takes
   std::vector<int32_t> positions;      // per token
   std::vector<int32_t> join_tokens;    // tokens with several parts
@@ -103,18 +104,35 @@ inline void add_tiles(const Shape& sh, const std::vector<int32_t>& positions, in
   }
 }
 
-// Splits long items so that a launch has enough workgroups.
-inline std::vector<Item> split(const std::vector<Item>& in, int32_t kv_heads, int64_t want,
-                               int32_t least, int32_t step) {
-  int64_t keys = 0;
-  for (const Item& it : in) keys += keys_of(it);
-  const int64_t items = std::max<int64_t>(1, (want + kv_heads - 1) / kv_heads);
-  const int64_t each = std::max<int64_t>(least, (keys + items - 1) / items);
+// Splits items into parts of at most `each` keys, the smallest such number (a multiple of
+// `step`, `least` or more, and no less than a workgroup's share of them all) that keeps to
+// `want` workgroups, so that they run at once and none is much longer than another. Where
+// there are more items than that, half as many again are allowed: one long sequence among
+// many short ones is cut all the same.
+inline std::vector<Item> split(const std::vector<Item>& in, int64_t blocks_per_item, int64_t want,
+                               int64_t least, int64_t step) {
+  int64_t longest = 0, keys = 0;
+  for (const Item& it : in) {
+    longest = std::max<int64_t>(longest, keys_of(it));
+    keys += keys_of(it);
+  }
+  const int64_t items = static_cast<int64_t>(in.size());
+  const int64_t share = std::max<int64_t>(1, want / blocks_per_item);
+  const int64_t most = std::max(share, items + items / 2);
+  least = (std::max(least, keys / share) + step - 1) / step * step;
+  const auto parts = [](const Item& it, int64_t each) { return (keys_of(it) + each - 1) / each; };
+  // In steps: too small, and large enough.
+  int64_t low = least / step - 1, high = std::max((longest + step - 1) / step, least / step);
+  while (high - low > 1) {
+    const int64_t middle = (low + high) / 2;
+    int64_t total = 0;
+    for (const Item& it : in) total += parts(it, middle * step);
+    (total <= most ? high : low) = middle;
+  }
   std::vector<Item> out;
   for (const Item& it : in) {
-    const int64_t n = keys_of(it);
-    const int64_t parts = std::max<int64_t>(1, (n + each / 2) / each);
-    const int64_t size = ((n + parts - 1) / parts + step - 1) / step * step;
+    const int64_t n = keys_of(it), count = parts(it, high * step);
+    const int64_t size = ((n + count - 1) / count + step - 1) / step * step;
     for (int64_t v = 0; v < n; v += size)
       out.push_back(cut(it, static_cast<int32_t>(v), static_cast<int32_t>(std::min(n, v + size))));
   }
@@ -157,17 +175,20 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // a part of its own: worth it where a wave has steps enough to outweigh the part.
   int64_t narrow_keys = 0;
   for (const Item& it : narrow) narrow_keys += keys_of(it);
-  const int64_t blocks = 4 * compute_units;
-  if (narrow_keys * sh.kv_heads >= blocks * kNarrowWaves * 256)
+  plan.streams = narrow_keys * sh.kv_heads >= int64_t(4) * compute_units * kNarrowWaves * 256;
+  if (plan.streams)
     plan.together = sh.kv_heads % 4 == 0 ? 4 : sh.kv_heads % 2 == 0 ? 2 : 1;
-  narrow = split(narrow, sh.kv_heads / plan.together, blocks, 256, 64);
+  // Two workgroups fit a compute unit. Long streams are cut for half as many again: 128
+  // sequences of unlike lengths 182 us against 191 with two, of one length 175 against 173.
+  narrow = split(narrow, sh.kv_heads / plan.together, (plan.streams ? 3 : 2) * compute_units, 256,
+                 64);
   const int64_t narrow_blocks = int64_t(narrow.size()) * sh.kv_heads / plan.together;
   // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
   // are: they are cut only where more than half of the compute units would have none, and so
   // that those of a step run at once, two to a compute unit.
   if (int64_t(wide.size()) * sh.kv_heads * 2 < compute_units)
-    wide = split(wide, sh.kv_heads, std::max<int64_t>(compute_units, 2 * compute_units - narrow_blocks), 128,
-                 64);
+    wide = split(wide, sh.kv_heads,
+                 std::max<int64_t>(compute_units, 2 * compute_units - narrow_blocks), 128, 64);
   // The longest first: the last workgroups to start are short ones.
   auto longer = [](const Item& x, const Item& y) { return keys_of(x) > keys_of(y); };
   std::stable_sort(narrow.begin(), narrow.end(), longer);
