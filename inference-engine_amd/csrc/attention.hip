@@ -81,21 +81,25 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   // the card (128 sequences of the 8B shape: 206 us in two launches, 246 in one).
   const bool both = wide && narrow && !plan.streams;
   if constexpr (sizeof(T) == 2) {
-    if (wide) {
+    const dim3 wide_blocks(wide * a.kv_heads);
+    bool done = !wide;
+    if constexpr (sizeof(C) == 2) {
       const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-      if (!both && sizeof(C) == 2 && aligned(a.k) && aligned(a.v)) {
-        hipLaunchKernelGGL((attend_wide<T, C, DP>), dim3(wide * a.kv_heads), dim3(kThreads), 0,
-                           stream, a, plan.wide.first);
-      } else {
-        constexpr int bytes = std::max<int>(sizeof(typename Wide<T, DP>::Lds),
-                                            sizeof(typename Narrow<T, C, DP>::Lds));
-        static const hipError_t allowed = allow_lds(attend_both<T, C, DP>, bytes);
-        IEKV_OPS_HIP(allowed);
-        hipLaunchKernelGGL((attend_both<T, C, DP>),
-                           dim3(wide * a.kv_heads + (both ? narrow_blocks : 0)), dim3(kThreads),
-                           bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
-                           both ? narrow : 0);
+      if (wide && !both && aligned(a.k) && aligned(a.v)) {
+        hipLaunchKernelGGL((attend_wide<T, C, DP>), wide_blocks, dim3(kThreads), 0, stream, a,
+                           plan.wide.first);
+        IEKV_OPS_HIP(hipGetLastError());
+        done = true;
       }
+    }
+    if (!done) {
+      constexpr int bytes = std::max<int>(sizeof(typename Wide<T, DP>::Lds),
+                                          sizeof(typename Narrow<T, C, DP>::Lds));
+      static const hipError_t allowed = allow_lds(attend_both<T, C, DP>, bytes);
+      IEKV_OPS_HIP(allowed);
+      hipLaunchKernelGGL((attend_both<T, C, DP>), dim3(wide_blocks.x + (both ? narrow_blocks : 0)),
+                         dim3(kThreads), bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
+                         both ? narrow : 0);
       IEKV_OPS_HIP(hipGetLastError());
     }
   }

@@ -572,7 +572,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 
 // --- wide: many rows ---------------------------------------------------------------------
 
-// Four waves, 32 R rows each, share tiles of 64 keys in LDS, two tiles in turn: a tile's
+// Four waves, 32 rows each, share tiles of 64 keys in LDS, two tiles in turn: a tile's
 // loads are issued before the products of the one before it. V^T is read from V's rows by the
 // transposing LDS load (a group of 16 lanes reads 4 keys of 16 dimensions, and each lane gets
 // one dimension of the four). A tile lies in LDS without gaps, so that the loads can go there
@@ -623,7 +623,7 @@ __device__ __forceinline__ void arrive() {
 
 // K's and V's buffers are arguments of their own: the compiler then knows that a load into one
 // leaves the others alone, and does not wait for it before it reads them.
-template <typename T, typename C, int DP, int R, bool DIRECT>
+template <typename T, typename C, int DP, bool DIRECT>
 __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
                                           typename Wide<T, DP>::Tile& k1,
                                           typename Wide<T, DP>::Tile& v0,
@@ -639,22 +639,22 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
   if (threadIdx.x == 0) redo = 0;
 
-  Words<4> q[R][NQ];
-  int32_t position[R];
-#pragma unroll
-  for (int u = 0; u < R; ++u) {
-    const int32_t r = (wave * R + u) * 32 + c, row = r < rows ? r : 0;
-    const int32_t token = it.token0 + row / a.group;
+  // Q^T: row `mine`, zeros past the rows and past the dimensions.
+  const int32_t mine = wave * 32 + c;
+  Words<4> q[NQ];
+  int32_t position;
+  {
+    const int32_t row = mine < rows ? mine : 0, token = it.token0 + row / a.group;
     const int64_t head = static_cast<int64_t>(kv_head) * a.group + row % a.group;
-    position[u] = a.words[a.positions_at + token];
+    position = a.words[a.positions_at + token];
     const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       const int32_t d0 = i * 16 + h * 8;
-      const bool in = r < rows && d0 < d;
-      q[u][i] = load_bytes<16>(at + (d0 < d ? d0 : 0));
+      const bool in = mine < rows && d0 < d;
+      q[i] = load_bytes<16>(at + (d0 < d ? d0 : 0));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[u][i].w[e] = (q[u][i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
+      for (int e = 0; e < 4; ++e) q[i].w[e] = (q[i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
     }
   }
 
@@ -700,17 +700,12 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     }
   };
 
-  f32x16 o[R][ND];
-  float m[R], l[R];
+  f32x16 o[ND];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {
-    m[u] = -INFINITY;
-    l[u] = 0.f;
+  for (int t = 0; t < ND; ++t)
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[u][t][r] = 0.f;
-  }
+    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
 
   if (wave < 2) lds_rows[wave][lane] = row_of(a, place(wave)) * row_bytes;
   __syncthreads();
@@ -726,25 +721,22 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     // No branch around these loads, or every wait after them would be one for all: past the
     // last step they read the last key.
     const Place next = place(s + 2);
-    Staged x;
-    load(lds_rows[half ^ 1], kn, vn, x);
+    Staged staged;
+    load(lds_rows[half ^ 1], kn, vn, staged);
     __builtin_amdgcn_sched_barrier(0);
 
-    f32x16 sc[R][2];
+    f32x16 sc[2];
 #pragma unroll
-    for (int u = 0; u < R; ++u)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[u][t][r] = 0.f;
+      for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Words<4> k = __builtin_bit_cast(
             Words<4>, kt[(t * 32 + c) * CHUNKS + W::place_k(c, i * 2 + h)]);
-#pragma unroll
-        for (int u = 0; u < R; ++u) sc[u][t] = mma32(k, q[u][i], sc[u][t], T{});
+        sc[t] = mma32(k, q[i], sc[t], T{});
       }
     // Half of K's reads at once, then one behind each product: left to itself the compiler
     // waits for every read before its product.
@@ -752,10 +744,10 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     __builtin_amdgcn_sched_group_barrier(kDsRead, NQ, 0);
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kMfma, R, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
       __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(kMfma, NQ * R, 0);
+    __builtin_amdgcn_sched_group_barrier(kMfma, NQ, 0);
 
     const int32_t first = s * KS;
     if (first + KS > n || !all_see(a, it, first, first + KS)) {
@@ -764,42 +756,37 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int32_t at = first + t * 32 + r / 4 * 8 + h * 4 + r % 4;
-          const int32_t j = key_at(it, at);
-#pragma unroll
-          for (int u = 0; u < R; ++u)
-            sc[u][t][r] = (at < n) & sees(a, position[u], j) ? sc[u][t][r] : -INFINITY;
+          const bool seen = (at < n) & sees(a, position, key_at(it, at));
+          sc[t][r] = seen ? sc[t][r] : -INFINITY;
         }
     }
-    Words<4> p[R][4];
+    float x = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
-      float x = -INFINITY;
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int r = 0; r < 16; ++r) x = fmaxf(x, sc[t][r]);
+    // The maximum that weights are taken relative to follows only when a row's has grown by a
+    // factor of 2^8: weights, their sum and O are floating point and as exact relative to any
+    // of them, and of 32 rows one or another would grow at almost every tile.
+    const float top = fmaxf(x, lane_xor<32>(x)) * a.scale;
+    if (__any(top > m + 8.f)) {
+      const float to = fmaxf(m, top), fade = to == -INFINITY ? 1.f : power2(m - to);
+      l *= fade;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x = fmaxf(x, sc[u][t][r]);
-      // The maximum that weights are taken relative to follows only when a row's has grown by
-      // a factor of 2^8: weights, their sum and O are floating point and as exact relative to
-      // any of them, and of 32 rows one or another would grow at almost every tile.
-      const float top = fmaxf(x, lane_xor<32>(x)) * a.scale;
-      if (__any(top > m[u] + 8.f)) {
-        const float next = fmaxf(m[u], top), fade = next == -INFINITY ? 1.f : power2(m[u] - next);
-        l[u] *= fade;
+      for (int t = 0; t < ND; ++t) o[t] *= fade;
+      m = to;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    Words<4> p[4];
 #pragma unroll
-        for (int t = 0; t < ND; ++t) o[u][t] *= fade;
-        m[u] = next;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = power2(fmaf(sc[t][r], a.scale, -base));
+        const float p1 = power2(fmaf(sc[t][r + 1], a.scale, -base));
+        l += p0 + p1;
+        p[t * 2 + r / 8].w[r % 8 / 2] = pack2<T>(p0, p1);
       }
-      const float base = m[u] == -INFINITY ? 0.f : m[u];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float p0 = power2(fmaf(sc[u][t][r], a.scale, -base));
-          const float p1 = power2(fmaf(sc[u][t][r + 1], a.scale, -base));
-          l[u] += p0 + p1;
-          p[u][t * 2 + r / 8].w[r % 8 / 2] = pack2<T>(p0, p1);
-        }
-    }
     // Of 16 keys, half h holds the weights of 4 h .. 4 h + 3 and 8 + 4 h ..
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -809,12 +796,10 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
         const char* at = reinterpret_cast<const char*>(&vt[key * CHUNKS + W::place_v(key, chunk)]) +
                          c % 2 * 8;
         const Words<2> lo = transposed(at), hi = transposed(at + 8 * CHUNKS * 16);
-        const Words<4> v{{lo.w[0], lo.w[1], hi.w[0], hi.w[1]}};
-#pragma unroll
-        for (int u = 0; u < R; ++u) o[u][t] = mma32(v, p[u][i], o[u][t], T{});
+        o[t] = mma32(Words<4>{{lo.w[0], lo.w[1], hi.w[0], hi.w[1]}}, p[i], o[t], T{});
       }
     __builtin_amdgcn_sched_barrier(0);
-    store(x, kn, vn);
+    store(staged, kn, vn);
     if (wave == 0) lds_rows[half][lane] = row_of(a, next) * row_bytes;
     arrive();
   };
@@ -825,49 +810,39 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     if (++s >= steps) break;
   }
 
-  bool odd = false;
+  l += lane_xor<32>(l);
+  bool odd = l != l;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {
-    l[u] += lane_xor<32>(l[u]);
-    if ((wave * R + u) * 32 + c >= rows) continue;
-    odd = odd || l[u] != l[u];
+  for (int t = 0; t < ND; ++t)
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        odd = odd || (t * 32 + r / 4 * 8 < d && o[u][t][r] != o[u][t][r]);
-  }
-  if (odd) redo = 1;
+    for (int r = 0; r < 16; ++r) odd = odd || (t * 32 + r / 4 * 8 < d && o[t][r] != o[t][r]);
+  if (odd && mine < rows) redo = 1;
   __syncthreads();
   if (redo) {
     for (int32_t r = wave; r < rows; r += kWaves) attend_row<T, C>(a, it, kv_head, r, lane);
     return;
   }
+  if (mine >= rows) return;
+  const int64_t token = it.token0 + mine / a.group;
+  const int64_t head = static_cast<int64_t>(kv_head) * a.group + mine % a.group;
+  const int64_t slot = static_cast<int64_t>(it.slot + mine) * a.kv_heads + kv_head;
+  T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
+  const float inverse = 1.f / l;
 #pragma unroll
-  for (int u = 0; u < R; ++u) {
-    const int32_t row = (wave * R + u) * 32 + c;
-    if (row >= rows) continue;
-    const int64_t token = it.token0 + row / a.group;
-    const int64_t head = static_cast<int64_t>(kv_head) * a.group + row % a.group;
-    const int64_t slot = static_cast<int64_t>(it.slot + row) * a.kv_heads + kv_head;
-    T* out = static_cast<T*>(a.out) + (token * static_cast<int64_t>(a.kv_heads) * a.group + head) * d;
-    const float inverse = 1.f / l[u];
+  for (int t = 0; t < ND; ++t)
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
+    for (int r = 0; r < 16; r += 4) {
+      const int32_t d0 = t * 32 + r * 2 + h * 4;
+      if (d0 >= d) continue;
+      float x[4];
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int32_t d0 = t * 32 + r * 2 + h * 4;
-        if (d0 >= d) continue;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = it.slot >= 0 ? o[u][t][r + e] : o[u][t][r + e] * inverse;
-        if (it.slot >= 0)
-          __builtin_memcpy(a.part_o + slot * d + d0, x, 16);
-        else
-          store_out<T, 4>(out + d0, x);
-      }
-    if (it.slot >= 0 && h == 0) a.part_ml[slot] = {m[u], l[u]};
-  }
+      for (int e = 0; e < 4; ++e) x[e] = it.slot >= 0 ? o[t][r + e] : o[t][r + e] * inverse;
+      if (it.slot >= 0)
+        __builtin_memcpy(a.part_o + slot * d + d0, x, 16);
+      else
+        store_out<T, 4>(out + d0, x);
+    }
+  if (it.slot >= 0 && h == 0) a.part_ml[slot] = {m, l};
 }
 
 // --- kernels -----------------------------------------------------------------------------
@@ -886,27 +861,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void a
   narrow_item<T, C, DP>(lds, a, first + item, part * a.together, blockIdx.y * 16);
 }
 
-constexpr int kWideTiles = 1;                    // R of the kernels below
-constexpr int kWideRows = kWaves * 32 * kWideTiles;
+constexpr int kWideRows = kWaves * 32;
 
 // Wide items from `wide` on, of 16-bit caches at 16-byte addresses. Neighbouring blocks are the
 // heads of an item, and where there are eight, all blocks of an XCD are of one head, whose
 // keys the items share in its L2.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_wide(Args a,
+__global__ __launch_bounds__(kThreads, 2) void attend_wide(Args a,
                                                                                  int32_t wide) {
   using W = Wide<T, DP>;
   __shared__ typename W::Tile k0, k1, v0, v1;
   __shared__ typename W::Rows rows;
   __shared__ int32_t redo;
-  wide_item<T, C, DP, kWideTiles, true>(k0, k1, v0, v1, rows, redo, a, wide + blockIdx.x / a.kv_heads,
+  wide_item<T, C, DP, true>(k0, k1, v0, v1, rows, redo, a, wide + blockIdx.x / a.kv_heads,
                                         blockIdx.x % a.kv_heads);
 }
 
 // `n_wide` wide items from `wide` on and `n_narrow` narrow ones from `narrow` on in one launch:
 // the matrix units work on the former while the latter wait for memory.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_both(
+__global__ __launch_bounds__(kThreads, 2) void attend_both(
     Args a, int32_t wide, int32_t n_wide, int32_t narrow, int32_t n_narrow) {
   extern __shared__ __attribute__((aligned(16))) char shared[];
   auto& of_wide = *reinterpret_cast<typename Wide<T, DP>::Lds*>(shared);
@@ -918,7 +892,7 @@ __global__ __launch_bounds__(kThreads, kWideTiles == 1 ? 2 : 1) void attend_both
   const uint32_t before = run < span ? uint64_t(run) * wides / span : wides;
   const uint32_t after = run < span ? uint64_t(run + 1) * wides / span : wides;
   if (after > before)
-    wide_item<T, C, DP, kWideTiles, false>(of_wide.k[0], of_wide.k[1], of_wide.v[0], of_wide.v[1],
+    wide_item<T, C, DP, false>(of_wide.k[0], of_wide.k[1], of_wide.v[0], of_wide.v[1],
                                            of_wide.rows, of_wide.redo, a,
                                            wide + before / a.together,
                                            before % a.together * each + part);
