@@ -578,19 +578,19 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 // one dimension of the four). A tile lies in LDS without gaps, so that the loads can go there
 // directly (DIRECT; 8-bit caches are converted on their way, and caches that begin at any
 // element are copied through registers); its rows' 16-byte chunks change places by key, so
-// that what the lanes read at a time lies in different banks: eight keys' chunks of K,
-// and four keys' pairs of chunks of V.
+// that the 256 bytes that are read at a time lie in different banks: a chunk of K of 16 keys
+// each, four chunks of V of four keys each.
 template <typename T, int DP>
 struct Wide {
   static constexpr int KS = 64;
   static constexpr int CHUNKS = DP / 8;                      // of eight elements, a row's
   static constexpr int LOADS = KS * CHUNKS / kThreads;       // chunks a thread brings
-  static constexpr bool POWER = DP == 64 || DP == 128;
+  // The place of a chunk, and the chunk at a place.
   static __device__ __forceinline__ int place_k(int key, int chunk) {
-    return chunk ^ (POWER ? key & 7 : key >> 1 & 3);
+    return chunk ^ (DP == 128 ? key & 15 : DP == 64 ? key >> 1 & 7 : key >> 2 & 3);
   }
   static __device__ __forceinline__ int place_v(int key, int chunk) {
-    return chunk ^ (POWER ? (key & 3) * 2 : (key >> 1 & 1) * 2);
+    return chunk ^ (DP == 128 ? (key & 3) * 4 : DP == 64 ? (key >> 1 & 1) * 4 : 0);
   }
   using Tile = u32x4[KS * CHUNKS];
   using Rows = int64_t[2][KS];                               // bytes to the keys' rows
