@@ -15,6 +15,7 @@
 #include "ops_common.h"
 
 #include <cmath>
+#include <type_traits>
 
 using namespace iekv_ops;
 
@@ -23,7 +24,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWave = 64;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kCandidates = 512;   // of a part, or of a row's parts, that are ranked at once
+constexpr int kCandidates = 512;   // of a row's parts that are ranked at once
+constexpr int kEach = 128;         // and of a wave's share of a part
 constexpr int kSmall = 8, kLarge = 32;  // logits a thread holds
 
 // A logit as an unsigned number of the same order; NaN is the largest. Zeros of both signs
@@ -138,9 +140,9 @@ __device__ __forceinline__ int32_t rank_of(uint64_t key, const uint64_t* list, i
 // The alternatives: a lower bound of the part's k-th largest logit is found from the lanes'
 // own largest ones. Each wave sorts its 64: if every wave has ceil(k / 4) lanes of at least
 // b, or one wave has k, there are k logits of at least b. What reaches the bound, a few more
-// than k as a rule, is put on a list in LDS and ranked by counting the larger keys. Where
-// more reach it than the list holds (rows of equal logits, all but barred rows) or the part
-// holds a NaN, the largest key is taken k times instead.
+// than k as a rule, is put on the waves' lists in LDS and ranked by counting the larger keys.
+// Where more reach it than a list holds (rows of equal logits, all but barred rows) or the
+// part holds a NaN, the largest key is taken k times instead.
 template <typename T, int HELD>
 __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t stride, Scores out,
                                                        Parts parts) {
@@ -153,8 +155,8 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   const T* x = logits + row * stride;
   __shared__ float most[kWaves];
   __shared__ float2 sums[kWaves], bounds[kWaves];
-  __shared__ uint64_t list[kCandidates + kPad];
-  __shared__ int32_t listed;
+  __shared__ uint64_t lists[kWaves][kEach + kPad];
+  __shared__ int32_t listed[kWaves];
 
   // Logit v (of this thread's `HELD`) is number (v / VEC * kThreads + tid) * VEC + v % VEC.
   float held[HELD];
@@ -181,7 +183,6 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   for (int v = 0; v < HELD; ++v) mine = fmaxf(mine, held[v]);
   const float of_wave = wave_max(mine);
   if (lane == 0) most[wave] = of_wave;
-  if (tid == 0) listed = 0;
   __syncthreads();
   Sums all;
   all.m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
@@ -227,35 +228,39 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   const float bound =
       fmaxf(fminf(fminf(bounds[0].x, bounds[1].x), fminf(bounds[2].x, bounds[3].x)),
             fmaxf(fmaxf(bounds[0].y, bounds[1].y), fmaxf(bounds[2].y, bounds[3].y)));
-  // Each wave takes as many places of the list as its lanes have candidates.
+  // Each wave lists its own. Only where nothing bounds them could what fills the part up, -inf,
+  // be among them.
+  uint64_t* list = lists[wave];
   int32_t own = 0;
+  const auto collect = [&](auto unbounded) {
 #pragma unroll
-  for (int v = 0; v < HELD; ++v) own += held[v] >= bound && index(v) < n;
-  int32_t before = 0, of_lanes = 0;
-#pragma unroll
-  for (int bit = 0; HELD >> bit; ++bit) {
-    const uint64_t with = __ballot(own >> bit & 1);
-    before += __popcll(with & ((uint64_t(1) << lane) - 1)) << bit;
-    of_lanes += __popcll(with) << bit;
-  }
-  int32_t at = lane == 0 && of_lanes ? atomicAdd(&listed, of_lanes) : 0;
-  at = __builtin_amdgcn_readfirstlane(at) + before;
-  if (own) {
-#pragma unroll
-    for (int v = 0; v < HELD; ++v)
-      if (held[v] >= bound && index(v) < n) {
-        if (at < kCandidates) list[at] = key_of(held[v], first + index(v));
-        ++at;
-      }
-  }
+    for (int v = 0; v < HELD; ++v) {
+      const bool in = held[v] >= bound && (!unbounded || index(v) < n);
+      const uint64_t who = __ballot(in);
+      if (!who) continue;
+      const int32_t at = own + __popcll(who & ((uint64_t(1) << lane) - 1));
+      if (in && at < kEach) list[at] = key_of(held[v], first + index(v));
+      own += __popcll(who);
+    }
+  };
+  if (bound == -INFINITY)
+    collect(std::true_type{});
+  else if (__any(mine >= bound))
+    collect(std::false_type{});
+  if (lane < kPad && own <= kEach) list[own + lane] = 0;
+  if (lane == 0) listed[wave] = own;
   __syncthreads();
-  const int32_t count = listed;
-  if (count <= kCandidates && all.s == all.s) {
-    if (tid < kPad) list[count + tid] = 0;
-    __syncthreads();
-    for (int32_t i = tid; i < count; i += kThreads) {
+  int32_t count = 0;
+  bool fits = all.s == all.s;
+  for (int w = 0; w < kWaves; ++w) {
+    count += listed[w];
+    fits = fits && listed[w] <= kEach;
+  }
+  if (fits) {
+    for (int32_t i = lane; i < own; i += kWave) {
       const uint64_t key = list[i];
-      const int32_t rank = rank_of(key, list, count);
+      int32_t rank = 0;
+      for (int w = 0; w < kWaves; ++w) rank += rank_of(key, lists[w], listed[w]);
       if (rank < top) put(rank, key);
     }
     // A part of fewer logits than alternatives (of a row of several parts).
@@ -272,9 +277,9 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
     }
     key = wave_top(key);
     __syncthreads();
-    if (lane == 0) list[wave] = key;
+    if (lane == 0) lists[0][wave] = key;
     __syncthreads();
-    for (int i = 0; i < kWaves; ++i) key = list[i] > key ? list[i] : key;
+    for (int i = 0; i < kWaves; ++i) key = lists[0][i] > key ? lists[0][i] : key;
     below = key;
     if (tid == 0) put(rank, key);
   }
