@@ -40,7 +40,7 @@ typedef struct iekv_attention_shape {
   int32_t num_kv_heads;  /* head h reads KV head h / (num_heads / num_kv_heads) */
   int32_t head_dim;
   int32_t block_size;    /* cache rows per block */
-  int64_t num_blocks;    /* blocks of the pool: every table entry is below */
+  int64_t num_blocks;    /* blocks of the pool (fewer than 2^32 rows): every table entry is below */
   int32_t query_type;    /* IEKV_TYPE_F32, _F16 or _BF16: of q and of the output */
   int32_t cache_type;    /* the query type, or _E4M3; any type for F32 queries */
   int64_t window;        /* a query sees the last `window` keys up to its own (0: all) */
@@ -88,8 +88,8 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
  * top_ids [n_rows][top]. Logits of -inf have probability zero. A row of nothing but -inf
  * has log probabilities of -inf and entropy 0; a row with a NaN or +inf has NaN log
  * probabilities and entropy (its alternatives put NaN first); a token outside 0..vocab-1
- * has log probability NaN. The workspace (iekv_logprobs_workspace bytes, aligned to 16) is used until the
- * call's kernels end. */
+ * has log probability NaN. The workspace (iekv_logprobs_workspace bytes, aligned to 16) is
+ * used until the call's kernels end. */
 int64_t iekv_logprobs_workspace(int32_t type, int64_t n_rows, int64_t vocab, int32_t top);
 int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,
                   int64_t vocab, const int64_t* tokens, int32_t top, float* logprobs,

@@ -116,8 +116,8 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
     const int32_t* w = a.words;
     const bool few = rows <= kJoinFew;
     hipLaunchKernelGGL((few ? join_parts<T, kWaves> : join_parts<T, 1>),
-                       dim3(few ? rows : (rows + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a,
-                       w + plan.join_tokens_at, w + plan.join_starts_at, w + plan.join_parts_at,
+                       dim3(few ? rows : (rows + kWaves - 1) / kWaves), dim3(kThreads), 0, stream,
+                       a, w + plan.join_tokens_at, w + plan.join_starts_at, w + plan.join_parts_at,
                        plan.joined);
     IEKV_OPS_HIP(hipGetLastError());
   }
