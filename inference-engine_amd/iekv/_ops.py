@@ -85,12 +85,23 @@ def lib() -> ctypes.CDLL:
 _functions: dict[str, ctypes._CFuncPtr] = {}
 
 
-def call(function: str, *args) -> None:
-    """Call an entry point; raises as :func:`iekv._native.call` does."""
+def entry(function: str) -> ctypes._CFuncPtr:
+    """An entry point itself, for callers that are called often: pass a code other than 0
+    to :func:`fail`."""
     f = _functions.get(function)
     if f is None:
         f = _functions[function] = getattr(lib(), function)
-    code = f(*args)
+    return f
+
+
+def fail(function: str, code: int) -> None:
+    """Raise what :func:`iekv._native.call` raises for the code of a failed call."""
+    message = lib().iekv_ops_last_error().decode(errors="replace")
+    raise _native._ERRORS.get(code, _native.NativeError)(function, code, message)
+
+
+def call(function: str, *args) -> None:
+    """Call an entry point; raises as :func:`iekv._native.call` does."""
+    code = entry(function)(*args)
     if code:
-        message = lib().iekv_ops_last_error().decode(errors="replace")
-        raise _native._ERRORS.get(code, _native.NativeError)(function, code, message)
+        fail(function, code)

@@ -137,6 +137,11 @@ class AttentionPlan:
             host = torch.empty(n.value, dtype=torch.int32, pin_memory=True)
             ctypes.memmove(host.data_ptr(), words, 4 * n.value)
             self._words = host.to(pool.device, non_blocking=True)
+        self._words_at = self._words.data_ptr() if n.value else None
+        # What attend needs of these for each call.
+        self._shape = torch.Size((self.num_tokens, num_heads, dim))
+        self._scale = 1.0 / math.sqrt(dim)
+        self._attend = _ops.entry("iekv_attend")
         self._stream = current_stream_handle(pool.device)
         self._uploaded = torch.cuda.Event()
         self._uploaded.record(torch.cuda.current_stream(pool.device))
@@ -176,33 +181,41 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
     type. Runs on the device's current stream.
     """
     pool = plan.pool
-    if q.dtype != plan.query_dtype or q.device != pool.device:
+    device, shape = pool.device, plan._shape
+    if q.dtype != plan.query_dtype or q.device != device:
         raise ValueError(f"queries of {q.dtype} on {q.device}, the plan is for "
-                         f"{plan.query_dtype} on {pool.device}")
-    if q.shape != (plan.num_tokens, plan.num_heads, plan.head_dim):
-        raise ValueError(f"queries of shape {tuple(q.shape)}, the plan is for "
-                         f"{(plan.num_tokens, plan.num_heads, plan.head_dim)}")
+                         f"{plan.query_dtype} on {device}")
+    if q.shape != shape:
+        raise ValueError(f"queries of shape {tuple(q.shape)}, the plan is for {tuple(shape)}")
     if not 0 <= layer < pool.num_layers:
         raise IndexError(f"layer {layer} out of range for {pool.num_layers} layers")
     if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("attend has no backward pass: detach the queries or use no_grad")
-    if q.stride(2) != 1 or q.is_neg():
-        q = q.contiguous().resolve_neg()
+    if q.is_neg():
+        q = q.resolve_neg()
+    if q.is_contiguous():
+        token_stride, head_stride = shape[1] * shape[2], shape[2]
+    else:
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        token_stride, head_stride = q.stride(0), q.stride(1)
     if out is None:
-        out = q.new_empty(q.shape)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or \
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != q.dtype or out.device != device or \
             not out.is_contiguous() or out.is_neg():
         raise ValueError("out must be a contiguous tensor of the queries' shape, type and device")
-    if not plan.num_tokens:
+    if not shape[0]:
         return out
-    stream = current_stream_handle(pool.device)
+    stream = current_stream_handle(device)
     if stream != plan._stream:
         plan._used_on(stream)
     need, workspace = plan._workspace_bytes, None
     if need:
         workspace = q.new_empty(need, dtype=torch.uint8)
     k, v = plan._layers[layer]
-    _ops.call("iekv_attend", plan._handle, plan._words.data_ptr(), k, v, q.data_ptr(), q.stride(0),
-              q.stride(1), 1.0 / math.sqrt(plan.head_dim) if scale is None else scale,
-              out.data_ptr(), workspace.data_ptr() if need else None, need, stream)
+    code = plan._attend(plan._handle, plan._words_at, k, v, q.data_ptr(), token_stride, head_stride,
+                        plan._scale if scale is None else scale, out.data_ptr(),
+                        workspace.data_ptr() if need else None, need, stream)
+    if code:
+        _ops.fail("iekv_attend", code)
     return out

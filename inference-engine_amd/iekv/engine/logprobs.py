@@ -70,9 +70,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
         need, workspace = _workspace_bytes(kind, rows, vocab, top), None
         if need:
             workspace = logits.new_empty(need, dtype=torch.uint8)
-        _ops.call("iekv_logprobs", kind, logits.data_ptr(), logits.stride(0), rows, vocab,
-                  tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(),
-                  top_logprobs.data_ptr(), top_ids.data_ptr(),
-                  workspace.data_ptr() if need else None, need,
-                  current_stream_handle(logits.device))
+        code = _ops.entry("iekv_logprobs")(
+            kind, logits.data_ptr(), logits.stride(0), rows, vocab, tokens.data_ptr(), top,
+            logprobs.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(),
+            workspace.data_ptr() if need else None, need, current_stream_handle(logits.device))
+        if code:
+            _ops.fail("iekv_logprobs", code)
     return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
