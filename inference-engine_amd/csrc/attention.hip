@@ -173,6 +173,15 @@ int check_shape(const iekv_attention_shape& s) {
   return IEKV_OK;
 }
 
+// Keys that one workgroup takes for less than the parts and their join cost: four steps of its
+// four waves, or what a compute unit's loads bring in that time (one sequence of 700 tokens of
+// eight bf16 heads of 128, 350 KB a workgroup: 13.5 us against 15.8 in parts; of 1,000 tokens
+// 19 against 14, and of 1,000 on an 8-bit cache 16.7 against 19.2).
+int32_t few_keys(const iekv_attention_shape& s) {
+  const int32_t bytes = s.cache_type == IEKV_TYPE_F32 ? 4 : s.cache_type == IEKV_TYPE_E4M3 ? 1 : 2;
+  return std::min(bytes == 4 ? 512 : 1024, (384 << 10) / (2 * s.head_dim * bytes));
+}
+
 int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* context_lens,
          const int32_t* query_lens, const int32_t* tables, const int64_t* starts,
          iekv_attention_plan** out) {
@@ -217,7 +226,8 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
   iekv_attention::Shape sh{shape.num_heads / shape.num_kv_heads, shape.num_kv_heads,
                            shape.block_size, shape.window, shape.sinks,
                            static_cast<int32_t>(shape.shared_blocks * bs),
-                           shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows};
+                           shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
+                           few_keys(shape)};
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units());
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||
       made.slots > INT32_MAX)

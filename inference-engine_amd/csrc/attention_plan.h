@@ -31,6 +31,7 @@ struct Shape {
   int64_t window, sinks;  // window 0: every key up to the query's own
   int32_t shared;         // keys of the shared blocks (0: none)
   int32_t wide_rows;      // rows an item of the wide kernel holds at most (0: there is none)
+  int32_t few_keys = 1024;  // that a narrow workgroup takes whole rather than leave parts
 };
 
 struct Sequence {
@@ -56,6 +57,7 @@ struct Plan {
 
 constexpr int kNarrowRows = 16;
 constexpr int kNarrowWaves = 4;
+constexpr int64_t kFewKeys = 1 << 16;   // of all KV heads, read again rather than joined
 
 // Keys of [lo, hi) that any of positions low..high sees.
 inline void visible(const Shape& sh, int64_t low, int64_t high, int64_t lo, int64_t hi, Item* it) {
@@ -154,9 +156,18 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // Sequences whose own rows fill a tile gain nothing from a tile shared with others: they
   // read the shared keys with their own, and leave no partial results. The rest are taken in
   // runs.
-  const auto shares = [&](const Sequence& s) {
-    return sh.shared && int64_t(s.queries) * sh.group < (sh.wide_rows ? sh.wide_rows : kNarrowRows);
+  const auto could = [&](const Sequence& s) {
+    return sh.shared && s.queries &&
+           int64_t(s.queries) * sh.group < (sh.wide_rows ? sh.wide_rows : kNarrowRows);
   };
+  // Nor do short contexts, where what is read again for each is less than a join's launch is
+  // worth (24 sequences of two KV heads behind 512 tokens: 9.5 us against 11.3).
+  int64_t sharing = 0;
+  int32_t longest = 0;
+  for (const Sequence& s : seqs)
+    if (could(s)) ++sharing, longest = std::max(longest, s.context);
+  const bool worth = longest > sh.few_keys || sharing * sh.shared * sh.kv_heads > kFewKeys;
+  const auto shares = [&](const Sequence& s) { return worth && could(s); };
   int32_t leading = -1, run0 = 0, run = 0;
   for (const Sequence& s : seqs) {
     if (!s.queries) continue;
@@ -178,10 +189,15 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   plan.streams = narrow_keys * sh.kv_heads >= int64_t(4) * compute_units * kNarrowWaves * 256;
   if (plan.streams)
     plan.together = sh.kv_heads % 4 == 0 ? 4 : sh.kv_heads % 2 == 0 ? 2 : 1;
+  // Few keys take less time in turn than a join does, if there is none yet.
+  int32_t longest_item = 0;
+  for (const Item& it : narrow) longest_item = std::max(longest_item, keys_of(it));
+  const bool whole = longest_item <= sh.few_keys && !(worth && sharing);
   // Two workgroups fit a compute unit. Long streams are cut for half as many again: 128
   // sequences of unlike lengths 182 us against 191 with two, of one length 175 against 173.
-  narrow = split(narrow, sh.kv_heads / plan.together, (plan.streams ? 3 : 2) * compute_units, 256,
-                 64);
+  if (!whole)
+    narrow = split(narrow, sh.kv_heads / plan.together, (plan.streams ? 3 : 2) * compute_units, 256,
+                   64);
   const int64_t narrow_blocks = int64_t(narrow.size()) * sh.kv_heads / plan.together;
   // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
   // are: they are cut only where more than half of the compute units would have none, and so

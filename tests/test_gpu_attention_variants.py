@@ -142,3 +142,29 @@ def test_a_scale_of_zero_weighs_all_keys_alike(gpu, query, cache):
     q = queries_of(141, 8, 64, query, 68)
     check(q, k[0], v[0], pool, tables, contexts, queries, scale=0.0)
     check(q, k[0], v[0], pool, tables, contexts, queries, scale=-0.0, window=30, sinks=2)
+
+
+def test_prompts_and_tokens_behind_a_long_prefix(gpu):
+    """As above behind a prefix that is worth sharing."""
+    bs, shared = 16, 90
+    own, queries = [40, 300, 7, 1, 200, 90, 3], [1, 300, 7, 1, 150, 2, 3]
+    contexts = [shared * bs + c for c in own]
+    blocks = shared + sum(-(-c // bs) for c in contexts) + 2
+    for query, cache in ((BF16, BF16), (F16, FP8), (F32, F16)):
+        pool, k, v = make_pool(blocks, bs, 2, 64, cache, 69)
+        tables = make_tables(contexts, bs, blocks, 70, shared)
+        q = queries_of(sum(queries), 8, 64, query, 71)
+        check(q, k[0], v[0], pool, tables, contexts, queries, shared_blocks=shared)
+        check(q, k[0], v[0], pool, tables, contexts, queries, shared_blocks=shared, window=1250,
+              sinks=17)
+
+
+@pytest.mark.parametrize("context", [255, 256, 257, 511, 513, 767, 769, 1023, 1025, 1300])
+@pytest.mark.parametrize("query, cache, dim", [(BF16, BF16, 128), (BF16, FP8, 128), (F32, F32, 32)])
+def test_contexts_around_what_one_workgroup_takes(gpu, context, query, cache, dim):
+    contexts = [context, 3, context // 2]
+    blocks = sum(-(-c // 16) for c in contexts) + 2
+    pool, k, v = make_pool(blocks, 16, 2, dim, cache, 72)
+    tables = make_tables(contexts, 16, blocks, 73)
+    q = queries_of(3, 8, dim, query, 74)
+    check(q, k[0], v[0], pool, tables, contexts, [1, 1, 1])
