@@ -12,7 +12,7 @@
 // launch that joins a row's parts in their order. Rows of one part are done in one launch.
 // How a row is cut depends on the vocabulary alone, so a row's result does not depend on the
 // rows beside it. Bound by the stream of logits where there are many (2,001 rows of 100,003 in
-// fp32: 132 us, 6.0 TB/s), by the two launches otherwise (64 rows of 128,000 in bf16 with 20
+// fp32: 117 us, 6.8 TB/s), by the two launches otherwise (64 rows of 128,000 in bf16 with 20
 // alternatives: 12 us for the parts, whose sums and alternatives follow one another, 7 to join).
 #include "ops_common.h"
 
@@ -28,7 +28,9 @@ constexpr int kWave = 64;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kCandidates = 512;   // of a row's parts that are ranked at once
 constexpr int kEach = 128;         // and of a wave's share of a part
+constexpr int kOneByOne = 5;       // largest lanes that are found by so many reductions
 constexpr int kSmall = 8, kLarge = 32;  // logits a thread holds
+constexpr int64_t kCacheBytes = 256 << 20;  // of the last-level cache
 
 // A logit as an unsigned number of the same order; NaN is the largest. Zeros of both signs
 // are equal.
@@ -145,7 +147,11 @@ __device__ __forceinline__ int32_t rank_of(uint64_t key, const uint64_t* list, i
 // than k as a rule, is put on the waves' lists in LDS and ranked by counting the larger keys.
 // Where more reach it than a list holds (rows of equal logits, all but barred rows) or the
 // part holds a NaN, the largest key is taken k times instead.
-template <typename T, int HELD>
+//
+// STREAM reads past the caches: logits that no cache holds come 13% faster so (2,001 rows of
+// 100,003 in fp32 117 us against 132), those that one may hold 10% slower (512 rows of 128,000
+// in bf16 57 us against 51).
+template <typename T, int HELD, bool STREAM>
 __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t stride, Scores out,
                                                        Parts parts) {
   constexpr int VEC = 16 / sizeof(T), LOADS = HELD / VEC;
@@ -167,7 +173,10 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
     const int32_t at = (i * kThreads + tid) * VEC;
     T e[VEC];
     if (at + VEC <= n) {
-      __builtin_memcpy(e, x + first + at, sizeof(e));
+      typedef uint32_t Chunk __attribute__((ext_vector_type(4), aligned(2)));
+      const Chunk* from = reinterpret_cast<const Chunk*>(x + first + at);
+      const Chunk chunk = STREAM ? __builtin_nontemporal_load(from) : *from;
+      __builtin_memcpy(e, &chunk, sizeof(e));
 #pragma unroll
       for (int j = 0; j < VEC; ++j) held[i * VEC + j] = to_float(e[j]);
     } else {
@@ -180,9 +189,15 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   const float given = whole ? given_of(out, x, row) : 0.f;
   const auto index = [&](int v) { return (v / VEC * kThreads + tid) * VEC + v % VEC; };
 
-  float mine = -INFINITY;
+  constexpr int GROUP = 8;
+  float of_group[HELD / GROUP], mine = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < HELD; ++v) mine = fmaxf(mine, held[v]);
+  for (int g = 0; g < HELD / GROUP; ++g) {
+    of_group[g] = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < GROUP; ++v) of_group[g] = fmaxf(of_group[g], held[g * GROUP + v]);
+    mine = fmaxf(mine, of_group[g]);
+  }
   const float of_wave = wave_max(mine);
   if (lane == 0) most[wave] = of_wave;
   __syncthreads();
@@ -194,18 +209,29 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   for (int v = 0; v < HELD; ++v) {
     const float d = held[v] - base, e = exponential(d);
     s += e;
-    w = fmaf(e, fmaxf(d, -200.f), w);     // e is 0 from -104 on; 0 * -inf would be NaN
+    // e is 0 from -104 on, and 0 * -inf would be NaN.
+    w = fmaf(e, __builtin_amdgcn_fmed3f(d, -200.f, 0.f), w);
   }
   s = wave_sum(s);
   w = wave_sum(w);
   if (lane == 0) sums[wave] = {s, w};
   const int32_t top = out.top;
   if (top) {
-    float each = of_wave, alone = of_wave;  // the wave's ceil(k / 4)-th and k-th largest lane
-    if (top > 1) {
+    // The wave's ceil(k / 4)-th largest lane, and where some wave has few lanes with logits its
+    // k-th. Few are found one by one, more by a sort.
+    const int32_t share = (top + kWaves - 1) / kWaves;
+    float each = of_wave, alone = top == 1 ? of_wave : -INFINITY;
+    if (top > 1 && (n < kThreads * VEC || share > kOneByOne)) {
       const float sorted = wave_sorted(mine);
-      each = __shfl(sorted, (top + kWaves - 1) / kWaves - 1);
+      each = __shfl(sorted, share - 1);
       alone = __shfl(sorted, top - 1);
+    } else {
+      float left = mine;
+      for (int32_t i = 1; i < share; ++i) {
+        const uint64_t who = __ballot(left == each);
+        if (lane == __ffsll(static_cast<unsigned long long>(who)) - 1) left = -INFINITY;
+        each = wave_max(left);
+      }
     }
     if (lane == 0) bounds[wave] = {each, alone};
   }
@@ -236,13 +262,17 @@ __global__ __launch_bounds__(kThreads) void score_part(const T* logits, int64_t 
   int32_t own = 0;
   const auto collect = [&](auto unbounded) {
 #pragma unroll
-    for (int v = 0; v < HELD; ++v) {
-      const bool in = held[v] >= bound && (!unbounded || index(v) < n);
-      const uint64_t who = __ballot(in);
-      if (!who) continue;
-      const int32_t at = own + __popcll(who & ((uint64_t(1) << lane) - 1));
-      if (in && at < kEach) list[at] = key_of(held[v], first + index(v));
-      own += __popcll(who);
+    for (int g = 0; g < HELD / GROUP; ++g) {
+      if (!__any(of_group[g] >= bound)) continue;
+#pragma unroll
+      for (int v = g * GROUP; v < (g + 1) * GROUP; ++v) {
+        const bool in = held[v] >= bound && (!unbounded || index(v) < n);
+        const uint64_t who = __ballot(in);
+        if (!who) continue;
+        const int32_t at = own + __popcll(who & ((uint64_t(1) << lane) - 1));
+        if (in && at < kEach) list[at] = key_of(held[v], first + index(v));
+        own += __popcll(who);
+      }
     }
   };
   if (bound == -INFINITY)
@@ -389,12 +419,11 @@ int launch(const Cut& cut, const T* logits, int64_t stride, int64_t n_rows, cons
   auto* keys = static_cast<uint64_t*>(workspace);
   Parts parts{reinterpret_cast<Sums*>(keys + n_rows * count * out.top), keys, count, cut.size};
   const dim3 grid(static_cast<uint32_t>(n_rows * count));
-  if (cut.held == kSmall)
-    hipLaunchKernelGGL((score_part<T, kSmall>), grid, dim3(kThreads), 0, stream, logits, stride, out,
-                       parts);
-  else
-    hipLaunchKernelGGL((score_part<T, kLarge>), grid, dim3(kThreads), 0, stream, logits, stride, out,
-                       parts);
+  const bool stream_past = n_rows * out.vocab * int64_t(sizeof(T)) > kCacheBytes;
+  const auto kernel = cut.held == kSmall ? score_part<T, kSmall, false>
+                      : stream_past      ? score_part<T, kLarge, true>
+                                         : score_part<T, kLarge, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, logits, stride, out, parts);
   IEKV_OPS_HIP(hipGetLastError());
   if (count > 1) {
     hipLaunchKernelGGL((join_rows<T>), dim3(static_cast<uint32_t>((n_rows + kWaves - 1) / kWaves)),
