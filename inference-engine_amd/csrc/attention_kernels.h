@@ -11,6 +11,8 @@
 #ifndef IEKV_ATTENTION_KERNELS_H_
 #define IEKV_ATTENTION_KERNELS_H_
 
+#include <type_traits>
+
 #include "attention_plan.h"
 #include "ops_common.h"
 
@@ -219,6 +221,16 @@ __device__ __forceinline__ uint32_t row_of(const Args& a, Place p) {
 
 __device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// float16 ends at 2^-25: of weights relative to a largest one of about 1, a long flat tail beside
+// a single high key would be lost from O while their sum holds it. So m is held that many powers
+// of two below the maximum, and the weights as many above, up to 2^15: O and the sum carry the
+// factor alike. What is lost then is less than 2^-39 (narrow) and 2^-32 (wide, where the maximum
+// may be 2^8 more) of the largest weight. The other types reach as far down as the power does.
+template <typename T>
+constexpr float lift(float narrow_or_wide) {
+  return std::is_same_v<T, _Float16> ? narrow_or_wide : 0.f;
+}
+
 // --- one row key by key ------------------------------------------------------------------
 
 // One query row by one wave: a lane scores a key of each 64, then holds two dimensions of
@@ -320,6 +332,7 @@ struct Narrow {
   static constexpr int EV = DP <= 32 ? 2 : DP <= 64 ? 4 : 8;
   static constexpr int KT = sizeof(C) == 4 ? 2 : 4;       // key tiles of 16 in a step
   static constexpr int KS = 16 * KT;
+  static constexpr float LIFT = lift<T>(14.f);
   using RawK = Words<EL * int(sizeof(C)) / 4>;
   using RawV = Words<(EV * int(sizeof(C)) + 3) / 4>;
   static constexpr int LDO = DP + 4;                      // floats of a row of o in LDS
@@ -469,7 +482,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
         for (int r = 0; r < 4; ++r) x = fmaxf(x, sc[t][r]);
       x = fmaxf(x, lane_xor<16>(x));
       x = fmaxf(x, lane_xor<32>(x));
-      top = fmaxf(m, x * a.scale);
+      top = fmaxf(m, x * a.scale - N::LIFT);
     }
     const float base = top == -INFINITY ? 0.f : top;
     if (__any(top > m)) {
@@ -604,6 +617,7 @@ struct Wide {
   static constexpr int KS = 64;
   static constexpr int CHUNKS = DP / 8;                      // of eight elements, a row's
   static constexpr int LOADS = KS * CHUNKS / kThreads;       // chunks a thread brings
+  static constexpr float LIFT = lift<T>(7.f);
   // The place of a chunk, and the chunk at a place.
   static __device__ __forceinline__ int place_k(int key, int chunk) {
     return chunk ^ (DP == 128 ? key & 15 : DP == 64 ? key >> 1 & 7 : key >> 2 & 3);
@@ -787,7 +801,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     // The maximum that weights are taken relative to follows only when a row's has grown by a
     // factor of 2^8: weights, their sum and O are floating point and as exact relative to any
     // of them, and of 32 rows one or another would grow at almost every tile.
-    const float top = fmaxf(x, lane_xor<32>(x)) * a.scale;
+    const float top = fmaxf(x, lane_xor<32>(x)) * a.scale - W::LIFT;
     if (__any(top > m + 8.f)) {
       const float to = fmaxf(m, top), fade = to == -INFINITY ? 1.f : power2(m - to);
       l *= fade;

@@ -57,3 +57,82 @@ def test_weights_of_single_tokens_keep_their_bits(gpu, query, cache, contexts):
             if query == F16:
                 tol += 2.0 ** -24
             assert ((got[i, rows] - o).abs() <= tol).all()
+
+
+def tail(v, hot_v, counts, score):
+    """Output and A of a key of weight one and ``counts`` keys of e^-score beside it, whose
+    values' sums (and sums of absolute values) are ``v``."""
+    import math
+
+    w = math.exp(-score)
+    total = 1.0 + counts.double() * w
+    return tuple((h + w * s) / total for h, s in zip((hot_v, hot_v.abs()), v))
+
+
+# A key 17 nats above 60,000 others, whose weights are below half of float16's smallest number.
+TAIL, SCORE = 60000, 17.375
+
+
+@pytest.mark.parametrize("hot", [0.0, 0.25])
+@pytest.mark.parametrize("query, cache", [(F16, F16), (F16, FP8), (BF16, BF16), (F32, F32)])
+def test_a_long_tail_counts_for_single_tokens(gpu, query, cache, hot):
+    """800 sequences over one table: enough for a wave to take a whole context."""
+    from iekv.engine.attention import AttentionPlan, attend
+    from iekv.engine.pools import KVPool
+
+    bs, kv_heads, dim, n = 16, 4, 64, TAIL + 1
+    blocks = -(-n // bs)
+    k = torch.zeros((blocks * bs, kv_heads, dim), device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(83)
+    v = (torch.rand(k.shape, generator=gen, device="cuda") + 0.5).to(cache)
+    k[5, :, 0] = SCORE * (2 if cache == FP8 else 1)      # 34.75 is no fp8 number, 36 is
+    k, v[5] = k.to(cache), torch.full((kv_heads, dim), hot, device="cuda").to(cache)
+    score = k[5, 0, 0].item() * (0.5 if cache == FP8 else 1)
+    q = torch.zeros((800, kv_heads, dim), dtype=query, device="cuda")
+    q[:, :, 0] = 1.0
+    plan = AttentionPlan(KVPool([k], [v], bs), [list(range(blocks))] * 800, [n] * 800, [1] * 800,
+                         kv_heads, query_dtype=query)
+    got = attend(plan, 0, q, scale=0.5 if cache == FP8 else 1.0).double()
+    assert torch.equal(got, got[:1].expand_as(got))
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[5] = False
+    sums = v[:n][rest].double().sum(0)
+    o, a = tail((sums, sums), v[5].double(), torch.tensor(TAIL, device="cuda"), score)
+    u = torch.finfo(query).eps / 2
+    ds = score * (dim + 2) * 2.0 ** -24
+    tol = u * o + (u * u + 2 * ds + (2 * n + 16) * 2.0 ** -24) * a + (2.0 ** -24 if query == F16
+                                                                      else 0.0)
+    assert ((got[0] - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("hot", [0.0, 0.25])
+@pytest.mark.parametrize("query, cache", [(F16, F16), (F16, FP8), (BF16, BF16)])
+def test_a_long_tail_counts_for_prompts(gpu, query, cache, hot):
+    """512 queries of eight KV heads: as many workgroups as take a context in one piece.
+    float16 weights are steps of 2^-24 there, 2^7 or more times the weights."""
+    from iekv.engine.attention import AttentionPlan, attend
+    from iekv.engine.pools import KVPool
+
+    bs, kv_heads, group, dim, n, queries = 16, 8, 4, 64, TAIL + 1, 512
+    blocks = -(-n // bs)
+    k = torch.zeros((blocks * bs, kv_heads, dim), device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(84)
+    v = (torch.rand(k.shape, generator=gen, device="cuda") + 0.5).to(cache)
+    k[0, :, 0] = SCORE * (2 if cache == FP8 else 1)
+    k, v[0] = k.to(cache), torch.full((kv_heads, dim), hot, device="cuda").to(cache)
+    score = k[0, 0, 0].item() * (0.5 if cache == FP8 else 1)
+    q = torch.zeros((queries, kv_heads * group, dim), dtype=query, device="cuda")
+    q[:, :, 0] = 1.0
+    plan = AttentionPlan(KVPool([k], [v], bs), [list(range(blocks))], [n], [queries],
+                         kv_heads * group, query_dtype=query)
+    got = attend(plan, 0, q, scale=0.5 if cache == FP8 else 1.0).double()
+    got = got.view(queries, kv_heads, group, dim)
+    sums = v[1:n].double().cumsum(0)[-queries:]
+    counts = torch.arange(n - queries, n, device="cuda")[:, None, None]
+    o, a = tail((sums, sums), v[0].double(), counts, score)
+    u = torch.finfo(query).eps / 2
+    ds = score * (dim + 2) * 2.0 ** -24
+    tol = u * o + (u + 2 * ds + (n + 16) * 2.0 ** -24) * a
+    if query == F16:
+        tol = tol + 2.0 ** -24 + 2.0 ** -25 / 2 ** 7 * sums
+    assert ((got - o[:, :, None]).abs() <= tol[:, :, None]).all()
