@@ -233,11 +233,17 @@ constexpr float lift(float narrow_or_wide) {
 
 // --- one row key by key ------------------------------------------------------------------
 
+// The matrix kernels take s - m of a score that is not rounded first (one operation less a
+// key), where m is: off by half a step of m, which past this many powers of two would leave a
+// row's largest weight far above or below 1, in the end infinite or zero.
+constexpr float kFar = 1 << 20;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && fabsf(m) < INFINITY; }
+
 // One query row by one wave: a lane scores a key of each 64, then holds two dimensions of
 // the output. A key the row does not see is not read for it at all, so that whatever the
 // cache holds there (infinities, NaN) stays out. The matrix kernels multiply such a V by a
-// weight of zero; where that, or anything else, leaves a NaN in their output they come here
-// for the item's rows, at a hundredth of their speed.
+// weight of zero; where that, or anything else, leaves a NaN in their output, or where a row's
+// maximum is far, they come here for the item's rows, at a hundredth of their speed.
 template <typename T, typename C>
 __device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32_t row, int lane) {
   const int32_t token = it.token0 + row / a.group, in_group = row % a.group;
@@ -562,7 +568,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
       const float from = most == -INFINITY ? 0.f : most;
       for (int w = k; w < kWaves; w += together)
         total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
-      bool odd = total != total;
+      bool odd = total != total || is_far(most);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = lds.o[k][row][d0 + i];
       for (int w = k + together; w < kWaves; w += together)
@@ -844,7 +850,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
   }
 
   l += lane_xor<32>(l);
-  bool odd = l != l;
+  bool odd = l != l || is_far(m);
 #pragma unroll
   for (int t = 0; t < ND; ++t)
 #pragma unroll

@@ -136,3 +136,35 @@ def test_a_long_tail_counts_for_prompts(gpu, query, cache, hot):
     if query == F16:
         tol = tol + 2.0 ** -24 + 2.0 ** -25 / 2 ** 7 * sums
     assert ((got - o[:, :, None]).abs() <= tol[:, :, None]).all()
+
+
+@pytest.mark.parametrize("query, cache, size", [(F16, F16, 6e4), (BF16, BF16, 1e6),
+                                                (F32, F32, 1e8), (F32, F16, 6e4)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("contexts, queries", [([150], [150]), ([5001, 40], [1, 1]),
+                                               ([1500, 900], [700, 2])])
+def test_scores_far_past_24_bits(gpu, query, cache, size, sign, contexts, queries):
+    """Finite scores between whose neighbours in 32 bits lie many powers of e: the largest takes
+    all, and its row is its V to the bit."""
+    from iekv.engine.attention import AttentionPlan, attend
+
+    bs, kv_heads, group, dim = 16, 2, 4, 64
+    blocks = sum(-(-c // bs) for c in contexts) + 2
+    pool, k, v = make_pool(blocks, bs, kv_heads, dim, cache, 85)
+    tables = make_tables(contexts, bs, blocks, 86)
+    k[0].zero_()
+    gen = torch.Generator(device="cuda").manual_seed(87)
+    k[0][:, :, 0] = (torch.rand(k[0].shape[:2], generator=gen, device="cuda") * -size).to(cache)
+    for table in tables:
+        k[0][table[0] * bs + 3, :, 0] = size
+    q = torch.zeros((sum(queries), kv_heads * group, dim), dtype=query, device="cuda")
+    q[:, :, 0] = size * sign
+    plan = AttentionPlan(pool, tables, contexts, queries, kv_heads * group, query_dtype=query)
+    got = attend(plan, 0, q, scale=sign * dim ** -0.5)
+    at = 0
+    for table, n, m in zip(tables, contexts, queries):
+        first = max(0, 3 - (n - m))              # queries before the key do not see it
+        want = v[0][table[0] * bs + 3].to(query).repeat_interleave(group, 0)
+        assert torch.equal(got[at + first:at + m], want.expand(m - first, -1, -1))
+        assert torch.isfinite(got[at:at + m]).all()
+        at += m
