@@ -73,8 +73,9 @@ int iekv_attention_plan_info(const iekv_attention_plan* plan, const int32_t** wo
 /* out[t][h] = softmax(scale * q[t][h] . K) V over the keys the row sees.
  * `words` is the device copy of the plan's words; k and v one layer's arrays
  * [num_blocks * block_size][num_kv_heads][head_dim]; q is [tokens][num_heads][head_dim]
- * with the given strides in elements (head_dim contiguous); out is contiguous. The
- * workspace is used until the call's kernels end. */
+ * with the given strides in elements (head_dim contiguous); out is contiguous, and may be
+ * q itself where that is too, but not overlap it otherwise. The workspace is used until the
+ * call's kernels end. */
 int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const void* k,
                 const void* v, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                 float scale, void* out, void* workspace, int64_t workspace_bytes,

@@ -134,6 +134,30 @@ int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   }
 }
 
+// Whether the output lies over queries of other rows: a workgroup writes its rows when it has
+// read their queries, and not when others have read theirs.
+bool overlaps(const iekv_attention_plan& plan, const void* q, int64_t token_stride,
+              int64_t head_stride, const void* out) {
+  const iekv_attention_shape& s = plan.shape;
+  const int64_t tokens = plan.tokens, heads = s.num_heads, size = s.query_type == IEKV_TYPE_F32 ? 4 : 2;
+  const int64_t row = s.head_dim * size, bytes = tokens * heads * row;
+  const auto at = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
+  const int64_t q0 = at(q), out0 = at(out);
+  const int64_t along = (tokens - 1) * token_stride * size, across = (heads - 1) * head_stride * size;
+  const int64_t lo = q0 + std::min<int64_t>(along, 0) + std::min<int64_t>(across, 0);
+  const int64_t hi = q0 + std::max<int64_t>(along, 0) + std::max<int64_t>(across, 0) + row;
+  if (hi <= out0 || out0 + bytes <= lo) return false;
+  if (q0 == out0 && (tokens == 1 || token_stride == heads * s.head_dim) &&
+      (heads == 1 || head_stride == s.head_dim))
+    return false;                    // row over row
+  for (int64_t t = 0; t < tokens; ++t)
+    for (int64_t h = 0; h < heads; ++h) {
+      const int64_t first = q0 + (t * token_stride + h * head_stride) * size;
+      if (first < out0 + bytes && out0 < first + row) return true;
+    }
+  return false;
+}
+
 int64_t workspace_bytes_of(const iekv_attention_plan& p) {
   return p.slots * p.shape.num_kv_heads * (p.shape.head_dim + 2) * int64_t(sizeof(float));
 }
@@ -320,6 +344,8 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
                      static_cast<long long>(need));
   if (need && reinterpret_cast<uintptr_t>(workspace) % 16)
     return set_error(IEKV_ERR_INVALID, "workspace is not aligned to 16 bytes");
+  if (overlaps(*plan, q, q_token_stride, q_head_stride, out))
+    return set_error(IEKV_ERR_INVALID, "out overlaps q without being in its place");
   const iekv_attention_shape& s = plan->shape;
   Args a{};
   a.words = words;

@@ -558,41 +558,52 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     for (int t = 0; t < EV; ++t)
       if ((g * 4 + r) * EV + t < DP) lds.o[wave][c][(g * 4 + r) * EV + t] = o[t][r] * fade;
   __syncthreads();
-  // Eight dimensions of a row a thread.
+  // Eight dimensions of a row a thread, of each head.
   const int32_t row = threadIdx.x / 16, d0 = threadIdx.x % 16 * 8;
   const int32_t in_group = head0 + row % heads, token = row / heads;
-  if (row < rows && d0 < d) {
-    for (int k = 0; k < together; ++k) {
-      float x[8], total = 0.f, most = -INFINITY;
-      for (int w = k; w < kWaves; w += together) most = fmaxf(most, lds.ml[w][row].x);
-      const float from = most == -INFINITY ? 0.f : most;
-      for (int w = k; w < kWaves; w += together)
-        total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
-      bool odd = total != total || is_far(most);
+  const bool mine = row < rows && d0 < d;
+  float x[kWaves][8];
+  float2 ml[kWaves];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = lds.o[k][row][d0 + i];
-      for (int w = k + together; w < kWaves; w += together)
+  for (int k = 0; k < kWaves; ++k) {
+    if (!mine || k >= together) break;
+    float total = 0.f, most = -INFINITY;
+    for (int w = k; w < kWaves; w += together) most = fmaxf(most, lds.ml[w][row].x);
+    const float from = most == -INFINITY ? 0.f : most;
+    for (int w = k; w < kWaves; w += together)
+      total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
+    ml[k] = {most, total};
+    bool odd = total != total || is_far(most);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += lds.o[w][row][d0 + i];
+    for (int i = 0; i < 8; ++i) x[k][i] = lds.o[k][row][d0 + i];
+    for (int w = k + together; w < kWaves; w += together)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) odd = odd || x[i] != x[i];
-      if (odd) lds.redo[k] = 1;
-      const int64_t kv = kv_head0 + k;
-      if (it.slot >= 0) {
-        const int64_t slot =
-            static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv;
-        __builtin_memcpy(a.part_o + slot * d + d0, x, 32);
-        if (d0 == 0) a.part_ml[slot] = {most, total};
-      } else {
+      for (int i = 0; i < 8; ++i) x[k][i] += lds.o[w][row][d0 + i];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] /= total;
-        const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
-                           kv * a.group + in_group;
-        store_out<T, 8>(static_cast<T*>(a.out) + at * d + d0, x);
-      }
-    }
+    for (int i = 0; i < 8; ++i) odd = odd || x[k][i] != x[k][i];
+    if (odd) lds.redo[k] = 1;
   }
   __syncthreads();
+  // Nothing is written of a head whose rows are done again: the output may lie where their
+  // queries do.
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    if (!mine || k >= together) break;
+    if (lds.redo[k]) continue;
+    const int64_t kv = kv_head0 + k;
+    if (it.slot >= 0) {
+      const int64_t slot =
+          static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv;
+      __builtin_memcpy(a.part_o + slot * d + d0, x[k], 32);
+      if (d0 == 0) a.part_ml[slot] = ml[k];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[k][i] /= ml[k].y;
+      const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
+                         kv * a.group + in_group;
+      store_out<T, 8>(static_cast<T*>(a.out) + at * d + d0, x[k]);
+    }
+  }
   for (int k = 0; k < together; ++k) {
     if (!lds.redo[k]) continue;
     for (int32_t r = wave; r < rows; r += kWaves)

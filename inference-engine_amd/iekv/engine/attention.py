@@ -178,7 +178,7 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
     one after the other, head ``h`` reading KV head ``h // (num_heads / kv_heads)``; any
     strides (a last dimension that is not contiguous is copied first). ``scale`` defaults to
     ``1 / sqrt(head_dim)``. Returns ``out``, or a new contiguous tensor of q's shape and
-    type. Runs on the device's current stream.
+    type; ``out`` may be ``q`` itself, and overlap it in no other way. Runs on the device's current stream.
     """
     pool = plan.pool
     device, shape = pool.device, plan._shape
