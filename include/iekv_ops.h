@@ -49,7 +49,8 @@ typedef struct iekv_attention_shape {
 } iekv_attention_shape;
 
 /* How a step's attention is cut into workgroups: made once per step, used by every
- * layer. Holds no device memory. */
+ * layer. Holds no device memory. It is for the device that is current when it is made:
+ * iekv_attend runs there, whatever device is current then. */
 typedef struct iekv_attention_plan iekv_attention_plan;
 
 /* Plan the attention of n_seqs sequences (HOST arrays). Sequence s has context_lens[s]
@@ -89,7 +90,8 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
  * top_ids [n_rows][top]. Logits of -inf have probability zero. A row of nothing but -inf
  * has log probabilities of -inf and entropy 0; a row with a NaN or +inf has NaN log
  * probabilities and entropy (its alternatives put NaN first); a token outside 0..vocab-1
- * has log probability NaN. The workspace (iekv_logprobs_workspace bytes, aligned to 16) is
+ * has log probability NaN. Runs on the current device, which has to be the arrays'. The
+ * workspace (iekv_logprobs_workspace bytes, aligned to 16) is
  * used until the call's kernels end. */
 int64_t iekv_logprobs_workspace(int32_t type, int64_t n_rows, int64_t vocab, int32_t top);
 int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t n_rows,

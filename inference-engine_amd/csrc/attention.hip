@@ -6,6 +6,7 @@
 #include "ops_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -38,6 +39,7 @@ using iekv_attention::Launch;
 
 struct iekv_attention_plan {
   iekv_attention_shape shape;
+  int device;                    // whose arrays it is for
   Launch narrow, wide;
   bool streams;                  // the narrow items are a long stream
   int32_t together;              // KV heads a workgroup of the narrow kernel takes
@@ -51,25 +53,31 @@ namespace {
 
 constexpr int64_t kJoinFew = 2048;  // rows that are joined by four waves each
 
-int compute_units() {
-  static const int units = [] {
-    int device = 0, n = 0;
-    if (hipGetDevice(&device) != hipSuccess ||
-        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
-        n <= 0) {
-      (void)hipGetLastError();
-      return 256;   // no GPU in sight: a plan made to be looked at
-    }
-    return n;
-  }();
-  return units;
+int current_device() {
+  int device = 0;
+  if (hipGetDevice(&device) == hipSuccess) return device;
+  (void)hipGetLastError();
+  return 0;         // no GPU in sight: a plan made to be looked at
 }
 
-// More LDS than a kernel may have without asking.
+int compute_units(int device) {
+  int n = 0;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) == hipSuccess &&
+      n > 0)
+    return n;
+  (void)hipGetLastError();
+  return 256;
+}
+
+// More LDS than a kernel may have without asking: asked for once on each device.
 template <typename K>
-hipError_t allow_lds(K kernel, int bytes) {
-  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+hipError_t allow_lds(K kernel, int bytes, int device, std::atomic<uint64_t>* asked) {
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (asked->load() & bit) return hipSuccess;
+  const hipError_t error = hipFuncSetAttribute(
+      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (error == hipSuccess) asked->fetch_or(bit);
+  return error;
 }
 
 template <typename T, typename C, int DP>
@@ -95,8 +103,8 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
     if (!done) {
       constexpr int bytes = std::max<int>(sizeof(typename Wide<T, DP>::Lds),
                                           sizeof(typename Narrow<T, C, DP>::Lds));
-      static const hipError_t allowed = allow_lds(attend_both<T, C, DP>, bytes);
-      IEKV_OPS_HIP(allowed);
+      static std::atomic<uint64_t> asked{0};
+      IEKV_OPS_HIP(allow_lds(attend_both<T, C, DP>, bytes, plan.device, &asked));
       hipLaunchKernelGGL((attend_both<T, C, DP>), dim3(wide_blocks.x + (both ? narrow_blocks : 0)),
                          dim3(kThreads), bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
                          both ? narrow : 0);
@@ -252,12 +260,14 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
                            few_keys(shape)};
-  iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units());
+  const int device = current_device();
+  iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||
       made.slots > INT32_MAX)
     return set_error(IEKV_ERR_INVALID, "too many work items in one step");
   auto plan = new iekv_attention_plan{};
   plan->shape = shape;
+  plan->device = device;
   plan->narrow = made.narrow;
   plan->wide = made.wide;
   plan->streams = made.streams;
@@ -374,6 +384,8 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
   // is held above it, so that it leaves the -inf of a hidden key alone.
   a.q_sign = !std::signbit(scale) ? 0 : s.query_type == IEKV_TYPE_F32 ? 0x80000000u : 0x80008000u;
   a.scale = std::max(std::fabs(scale) * 1.4426950408889634f, FLT_MIN);
+  const DeviceGuard guard(plan->device);
+  IEKV_OPS_HIP(guard.error());
   switch (s.query_type * 8 + s.cache_type) {
     case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F32: return launch<float, float>(*plan, a, stream);
     case IEKV_TYPE_F32 * 8 + IEKV_TYPE_F16: return launch<float, _Float16>(*plan, a, stream);

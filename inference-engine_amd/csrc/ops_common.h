@@ -23,6 +23,30 @@ int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3
     }                                                                                      \
   } while (0)
 
+// Makes a device current for a call that launches on it, and the caller's again after.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device) {
+    error_ = hipGetDevice(&before_);
+    if (error_ == hipSuccess && before_ != device) {
+      error_ = hipSetDevice(device);
+      switched_ = error_ == hipSuccess;
+    }
+    if (error_ != hipSuccess) (void)hipGetLastError();
+  }
+  ~DeviceGuard() {
+    if (switched_) (void)hipSetDevice(before_);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+  hipError_t error() const { return error_; }
+
+ private:
+  int before_ = 0;
+  hipError_t error_;
+  bool switched_ = false;
+};
+
 // Element types as they lie in memory.
 struct E4m3 {
   uint8_t bits;

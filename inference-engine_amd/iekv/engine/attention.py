@@ -118,14 +118,16 @@ class AttentionPlan:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("an attention plan is uploaded, which a stream under capture "
                                    "cannot do: make it before the capture")
+            self._handle = ctypes.c_void_p()
+            # For the device that is current: attend runs there.
+            _ops.call("iekv_attention_plan_create", ctypes.byref(shape), len(contexts),
+                      contexts.buffer_info()[0], queries.buffer_info()[0],
+                      flat.buffer_info()[0], starts.buffer_info()[0],
+                      ctypes.byref(self._handle))
         self.pool = pool
         self.num_heads = num_heads
         self.query_dtype = query_dtype
         self.head_dim = dim
-        self._handle = ctypes.c_void_p()
-        _ops.call("iekv_attention_plan_create", ctypes.byref(shape), len(contexts),
-                  contexts.buffer_info()[0], queries.buffer_info()[0], flat.buffer_info()[0],
-                  starts.buffer_info()[0], ctypes.byref(self._handle))
         words, n = ctypes.POINTER(ctypes.c_int32)(), ctypes.c_int64()
         tokens, workspace = ctypes.c_int64(), ctypes.c_int64()
         _ops.call("iekv_attention_plan_info", self._handle, ctypes.byref(words), ctypes.byref(n),
@@ -178,7 +180,8 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
     one after the other, head ``h`` reading KV head ``h // (num_heads / kv_heads)``; any
     strides (a last dimension that is not contiguous is copied first). ``scale`` defaults to
     ``1 / sqrt(head_dim)``. Returns ``out``, or a new contiguous tensor of q's shape and
-    type; ``out`` may be ``q`` itself, and overlap it in no other way. Runs on the device's current stream.
+    type; ``out`` may be ``q`` itself, and overlap it in no other way. Runs on the
+    current stream of the pool's device, whichever device is current.
     """
     pool = plan.pool
     device, shape = pool.device, plan._shape

@@ -42,7 +42,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     ordered by logit, equal ones by index. Barred tokens (logits of -inf) have probability
     zero; a row that bars every token has log probabilities of -inf and entropy 0; a row with
     a NaN or +inf is NaN; a token outside the vocabulary (a padding mark) has log
-    probability NaN. Runs on the device's current stream.
+    probability NaN. Runs on the current stream of the logits' device, whichever device is
+    current.
     """
     if logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda:
         raise ValueError(f"logits must be [rows, vocab] float32, float16 or bfloat16 on the GPU, "
@@ -54,6 +55,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if not 0 <= top <= min(vocab, _ops.LOGPROBS_MAX_TOP):
         raise ValueError(f"top {top} out of range for a vocabulary of {vocab} (at most "
                          f"{_ops.LOGPROBS_MAX_TOP})")
+    if logits.device.index != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, tokens, top=top)
     if logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("token_logprobs has no backward pass: detach the logits or use "
                            "no_grad")
