@@ -66,7 +66,8 @@ class Sequence:
     a swap preemption keeps the sequence's KV in host memory:
     ``(host payload of its first ceil(num_computed / block_size) blocks,
     num_computed at swap-out)``. ``scores[i]`` is what an engine that scores its answers
-    (``EngineConfig.logprobs``) says of generated token ``i``.
+    (``EngineConfig.logprobs``) says of generated token ``i``, None where nobody scored it
+    (an engine before, that had not been asked to).
     """
 
     def __init__(self, prompt_ids: list[int], block_size: int, max_new_tokens: int = 64,
@@ -98,6 +99,10 @@ class Sequence:
     @property
     def num_generated(self) -> int:
         return len(self) - self.num_prompt
+
+    def reach_scores(self, n: int) -> None:
+        """None for each of the first ``n`` generated tokens that no score has come for."""
+        self.scores += [None] * (n - len(self.scores))
 
     @property
     def last_token(self) -> int:

@@ -186,6 +186,7 @@ class Engine:
             # A chunk in the middle of a prompt got no token.
             for seq, length, score in zip(batch.sequences, lengths, scores):
                 if len(seq) > length:
+                    seq.reach_scores(seq.num_generated - 1)
                     seq.scores.append(score)
         return batch, finished
 

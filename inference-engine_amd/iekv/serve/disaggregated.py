@@ -121,8 +121,8 @@ class KVTransfer:
     ``first_block`` is the index in the sequence's table of the first moved
     block (non-zero only for prefix-aware transfers). ``bytes_moved`` is the
     payload size of the moved blocks, one direction (B x 2L x T). ``scores`` are the
-    prefill worker's of the tokens it generated (``Sequence.scores``; they do not go over
-    the wire format).
+    prefill worker's of the tokens it generated (``Sequence.scores``; none where it was not
+    asked to score).
     """
 
     token_ids: list[int]
@@ -270,7 +270,10 @@ class DecodeWorker:
 
         seq.token_ids = list(transfer.token_ids)
         seq.num_computed = transfer.num_computed
-        seq.scores = list(transfer.scores)
+        # The last of its tokens is the one generated so far.
+        seq.scores = list(transfer.scores)[-seq.num_generated:]
+        if engine.config.logprobs is not None:
+            seq.reach_scores(seq.num_generated)
         engine.scheduler.waiting.remove(seq)
         copied = True
         if deferred:

@@ -8,7 +8,10 @@ messages:
 1. a self-describing header: magic ``b"IEKV"``, a little-endian u32 format
    version, a u32 length, then UTF-8 JSON with the sequence state
    (``token_ids``, ``num_computed``, ``first_block``, ``bytes_moved``) and the
-   payload layout (blocks, layers, tile shape, dtype, tile bytes);
+   payload layout (blocks, layers, tile shape, dtype, tile bytes); where the prefill
+   worker scored its tokens also ``scores``, a ``[token, log probability, entropy,
+   [[token, log probability], ...]]`` or null each (infinities and NaN, which JSON has no
+   numbers for, as "-inf", "inf" and "nan");
 2. the payload itself: the block-major byte image ``[B, 2L, T]`` that
    ``iekv_pack`` writes (K tiles of layers 0..L-1, then V tiles, per block), so
    the receiver unpacks it with one ``iekv_unpack`` and nothing is re-laid-out.
@@ -21,6 +24,7 @@ payload goes GPU to GPU over xGMI; with gloo they are host tensors.
 from __future__ import annotations
 
 import json
+import math
 import struct
 from typing import Any
 
@@ -61,6 +65,26 @@ def _packed_of(transfer: KVTransfer):
     raise TypeError("wire transfers need PackedBlocks payloads (the HIP copier's)")
 
 
+def _number(x: float) -> float | str:
+    return x if math.isfinite(x) else str(x)
+
+
+def _encode_score(score):
+    if score is None:
+        return None
+    return [int(score.token_id), _number(float(score.logprob)), _number(float(score.entropy)),
+            [[int(t), _number(float(x))] for t, x in score.top]]
+
+
+def _decode_score(item):
+    from ..engine.engine import TokenScore
+
+    if item is None:
+        return None
+    token, logprob, entropy, top = item
+    return TokenScore(token, float(logprob), float(entropy), [(t, float(x)) for t, x in top])
+
+
 def encode_header(transfer: KVTransfer, packed) -> bytes:
     dtype = _NAMES.get(packed.dtype)
     if dtype is None:
@@ -76,7 +100,9 @@ def encode_header(transfer: KVTransfer, packed) -> bytes:
         "dtype": dtype,
         "tile_bytes": packed.tile_bytes,
     }
-    body = json.dumps(meta, separators=(",", ":")).encode()
+    if transfer.scores:
+        meta["scores"] = [_encode_score(s) for s in transfer.scores]
+    body = json.dumps(meta, separators=(",", ":"), allow_nan=False).encode()
     return _PREFIX.pack(MAGIC, WIRE_VERSION, len(body)) + body
 
 
@@ -118,7 +144,8 @@ def from_wire(header: bytes, payload: torch.Tensor) -> KVTransfer:
                           _DTYPES[meta["dtype"]])
     return KVTransfer(token_ids=list(meta["token_ids"]), num_computed=meta["num_computed"],
                       block_payloads=packed, bytes_moved=meta["bytes_moved"],
-                      first_block=meta["first_block"])
+                      first_block=meta["first_block"],
+                      scores=[_decode_score(s) for s in meta.get("scores", [])])
 
 
 def send_transfer(transfer: KVTransfer, dst: int, group=None,
