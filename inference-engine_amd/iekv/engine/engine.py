@@ -33,8 +33,8 @@ class EngineConfig:
     behaviour) or ``"swap"`` (preempted sequences keep their KV in host memory).
     ``logprobs`` is another: with a number ``k``, every generated token is scored on the
     GPU (``iekv.engine.logprobs``) and ``Sequence.scores`` holds its log probability, the
-    entropy of the distribution at temperature 1 and the ``k`` most likely tokens; None
-    scores nothing.
+    entropy of the distribution at temperature 1 and the ``k`` most likely tokens (at most 64
+    and the vocabulary); None scores nothing.
     """
 
     block_size: int = 16
@@ -101,8 +101,6 @@ class Engine:
         self.copier_factory = copier_factory or default_copier_factory
         if self.config.preemption not in ("recompute", "swap"):
             raise ValueError("preemption must be 'recompute' or 'swap'")
-        if self.config.logprobs is not None and self.config.logprobs < 0:
-            raise ValueError(f"logprobs {self.config.logprobs} must not be negative")
         self.blocks = BlockManager(self.config.num_blocks, self.config.block_size)
         self.generator = np.random.default_rng(self.config.seed)
         if caches is None:
@@ -112,6 +110,8 @@ class Engine:
         if (len(self.k_caches) != len(self.v_caches)
                 or any(len(t) != rows for t in list(self.k_caches) + list(self.v_caches))):
             raise ValueError(f"caches must hold {rows} rows per array, K and V per layer")
+        if self.config.logprobs is not None:
+            self._check_logprobs(self.config.logprobs)
         # Per-pool state the model keeps for these caches (the toy model's slot-kernel
         # pool registration); held here so it lives exactly as long as the engine.
         bind = getattr(model, "bind_caches", None)
@@ -131,6 +131,22 @@ class Engine:
                                               self.config.block_size, "offload")
             self.blocks.tier = KVTier(self.config.offload_blocks)
             self.blocks.copier = self.copier
+
+    def _check_logprobs(self, top: int) -> None:
+        """Refuse here what the first step could not be scored with."""
+        from .._ops import LOGPROBS_MAX_TOP
+
+        if top < 0:
+            raise ValueError(f"logprobs {top} must not be negative")
+        if top > LOGPROBS_MAX_TOP:
+            raise ValueError(f"logprobs {top}: at most {LOGPROBS_MAX_TOP} alternatives are found")
+        vocab = getattr(getattr(self.model, "config", None), "vocab_size", None)
+        if vocab is not None and top > vocab:
+            raise ValueError(f"logprobs {top} of a vocabulary of {vocab}")
+        device = getattr(self.k_caches[0], "device", "cpu") if len(self.k_caches) else "cpu"
+        if not str(device).startswith("cuda"):
+            raise ValueError(f"tokens are scored on the GPU that holds the caches, these are on "
+                             f"{device}")
 
     def make_copier(self, role: str = "transfer"):
         return self.copier_factory(self.k_caches, self.v_caches, self.config.block_size, role)
@@ -152,15 +168,12 @@ class Engine:
         """
         self.blocks.flush_pending()
 
-    def _hidden(self, batch):
-        self.flush_offloads()
-        layout = build_layout(batch, self.config.block_size)
-        return layout, self.model.forward(layout, self.k_caches, self.v_caches,
-                                          self.config.block_size)
-
     def forward(self, batch):
         """Run the model over a scheduled batch; returns (layout, last-token logits)."""
-        layout, hidden = self._hidden(batch)
+        self.flush_offloads()
+        layout = build_layout(batch, self.config.block_size)
+        hidden = self.model.forward(layout, self.k_caches, self.v_caches,
+                                    self.config.block_size)
         return layout, self.model.logits_for_last_token_of_each(hidden, layout.query_lens)
 
     def _advance(self):
@@ -169,17 +182,11 @@ class Engine:
         batch = self.scheduler.schedule()
         if not batch:
             return None, []
-        on_device = None
-        if self.config.logprobs is None:
-            _, logits = self.forward(batch)
-        else:
-            layout, hidden = self._hidden(batch)
-            on_device = self.model.last_token_logits(hidden, layout.query_lens)
-            logits = on_device.cpu().numpy()
+        _, logits = self.forward(batch)
         temps = np.fromiter((s.temperature for s in batch.sequences), dtype=np.float32,
                             count=len(batch))
         tokens = [int(t) for t in sample_from_logits(logits, temps, self.generator)]
-        scores = None if on_device is None else self._score(on_device, tokens)
+        scores = None if self.config.logprobs is None else self._score(logits, tokens)
         lengths = [len(s) for s in batch.sequences]
         finished = self.scheduler.finish_step(batch, tokens)
         if scores is not None:
@@ -191,13 +198,16 @@ class Engine:
         return batch, finished
 
     def _score(self, logits, tokens: list[int]) -> list[TokenScore]:
-        """Score the tokens sampled from ``logits`` (a device tensor, a row each)."""
+        """Score the tokens sampled from ``logits`` (what :meth:`forward` returned, whatever
+        model or subclass made it)."""
         import torch
 
         from .logprobs import token_logprobs
 
-        given = torch.tensor(tokens, dtype=torch.int64, device=logits.device)
-        s = token_logprobs(logits, given, top=self.config.logprobs)
+        device = self.k_caches[0].device
+        rows = torch.from_numpy(np.ascontiguousarray(logits, dtype=np.float32)).to(device)
+        given = torch.tensor(tokens, dtype=torch.int64, device=device)
+        s = token_logprobs(rows, given, top=min(self.config.logprobs, rows.shape[1]))
         columns = (t.tolist() for t in (s.logprobs, s.entropy, s.top_ids, s.top_logprobs))
         return [TokenScore(token, logprob, entropy, list(zip(ids, values)))
                 for token, (logprob, entropy, ids, values) in zip(tokens, zip(*columns))]

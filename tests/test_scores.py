@@ -87,3 +87,47 @@ def test_scores_of_a_prefill_stay_where_decode_does_not_score(monkeypatch):
     seq = decode.admit(transfer, 3, 0.0)
     both.decode_until_done()
     assert [s.token_id for s in seq.scores] == [seq.token_ids[seq.num_prompt]]
+
+
+@pytest.mark.parametrize("logprobs, said", [
+    (65, "at most 64"), (-1, "logprobs -1"), (33, "vocabulary of 32"), (3, "on cpu")])
+def test_engines_refuse_what_no_step_could_be_scored_with(logprobs, said):
+    """Before anything is scheduled: a step that raises has computed and committed nothing."""
+    from iekv.engine.engine import Engine, EngineConfig
+    from iekv.engine.toy_model import ModelConfig, ToyTransformer
+    from test_engine import SMALL
+
+    model = ToyTransformer(ModelConfig(**dict(SMALL, vocab_size=32)), seed=0, device="cpu")
+    with pytest.raises(ValueError, match=said):
+        Engine(model, EngineConfig(block_size=8, num_blocks=16, logprobs=logprobs))
+
+
+def test_scores_are_of_the_logits_that_forward_returned(monkeypatch):
+    """An engine whose forward changes the logits, and a model that has no logits but
+    those forward takes from it."""
+    import numpy as np
+
+    from iekv.engine.engine import Engine
+
+    seen = []
+
+    class Barring(Engine):
+        def forward(self, batch):
+            layout, logits = super().forward(batch)
+            logits = logits.copy()
+            logits[:, ::2] = -np.inf
+            return layout, logits
+
+    eng = engine()
+    eng.__class__ = Barring
+    monkeypatch.delattr(type(eng.model), "last_token_logits")
+    monkeypatch.setattr(type(eng.model), "logits_for_last_token_of_each",
+                        lambda self, hidden, lens: np.tile(
+                            np.arange(64, dtype=np.float32), (len(lens), 1)))
+    monkeypatch.setattr(eng.config, "logprobs", 2)
+    monkeypatch.setattr(eng, "_score", lambda logits, tokens: seen.append(logits) or
+                        [score(t) for t in tokens])
+    seq = eng.submit([1, 2, 3], max_new_tokens=3, temperature=0.0)
+    eng.run()
+    assert seq.token_ids[3:] == [63, 63, 63] and len(seq.scores) == 3
+    assert all(np.isneginf(x[:, ::2]).all() and (x[:, 1] == 1).all() for x in seen)
