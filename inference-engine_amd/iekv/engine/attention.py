@@ -18,8 +18,8 @@ block table begins with the same so many blocks, as the block manager's prefix s
 makes them: their keys are read and scored once for all sequences' queries together. The
 result is the same, up to rounding.
 
-Forward only: the package serves and trains nothing, and queries that require a gradient
-are refused.
+Forward only: the package serves and trains nothing, and queries that require a gradient or
+carry a tangent are refused.
 """
 from __future__ import annotations
 
@@ -30,7 +30,7 @@ from array import array as _ints
 import torch
 
 from .. import _native, _ops
-from .pools import KVPool, current_stream_handle, integer_ids
+from .pools import KVPool, current_stream_handle, integer_ids, refuse_derivatives
 
 _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
           torch.bfloat16: _native.IEKV_TYPE_BF16, torch.float8_e4m3fn: _native.IEKV_TYPE_E4M3}
@@ -192,8 +192,7 @@ def attend(plan: AttentionPlan, layer: int, q: torch.Tensor, *, scale: float | N
         raise ValueError(f"queries of shape {tuple(q.shape)}, the plan is for {tuple(shape)}")
     if not 0 <= layer < pool.num_layers:
         raise IndexError(f"layer {layer} out of range for {pool.num_layers} layers")
-    if q.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("attend has no backward pass: detach the queries or use no_grad")
+    refuse_derivatives(q, "attend")
     if q.is_neg():
         q = q.resolve_neg()
     if q.is_contiguous():

@@ -13,7 +13,7 @@ from functools import lru_cache
 import torch
 
 from .. import _native, _ops
-from .pools import current_stream_handle
+from .pools import current_stream_handle, refuse_derivatives
 
 _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
           torch.bfloat16: _native.IEKV_TYPE_BF16}
@@ -58,9 +58,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if logits.device.index != torch.cuda.current_device():
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top=top)
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("token_logprobs has no backward pass: detach the logits or use "
-                           "no_grad")
+    refuse_derivatives(logits, "token_logprobs")
     if logits.stride(1) != 1 or logits.is_neg():
         logits = logits.contiguous().resolve_neg()
     if not tokens.is_contiguous() or tokens.is_neg():

@@ -17,6 +17,7 @@ from typing import Sequence as Seq
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from .. import _native
 
@@ -389,6 +390,17 @@ def stage_ids(device: torch.device, *arrays: np.ndarray) -> list[torch.Tensor]:
         out.append(on_device[at:at + n])
         at += n
     return out
+
+
+def refuse_derivatives(tensor: torch.Tensor, call: str) -> None:
+    """RuntimeError for an input whose derivative ``call``, which has none, would drop: one
+    that requires a gradient, or one with a tangent of forward mode."""
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{call} has no backward pass: detach its input or use no_grad")
+    # Outside of forward mode no tensor has one, and asking each costs more.
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and \
+            _forward_ad.unpack_dual(tensor).tangent is not None:
+        raise RuntimeError(f"{call} has no derivative in forward mode: unpack its input")
 
 
 def stream_handle(device: torch.device, stream: torch.cuda.Stream | None = None) -> int:

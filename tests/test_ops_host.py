@@ -170,3 +170,24 @@ def test_logprobs_run_on_the_logits_device(monkeypatch):
                                      Elsewhere((2,), torch.int64), top=3)
     assert scored.top_ids.shape == (2, 3)
     assert ran_on == [("iekv_logprobs", 1)] and current == [0]
+
+
+def test_inputs_with_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    from iekv.engine.pools import refuse_derivatives
+
+    x = torch.ones(3)
+    refuse_derivatives(x, "attend")
+    with pytest.raises(RuntimeError, match="attend has no backward"):
+        refuse_derivatives(x.clone().requires_grad_(), "attend")
+    with torch.no_grad():
+        refuse_derivatives(x.clone().requires_grad_(), "attend")
+    with forward_ad.dual_level():
+        refuse_derivatives(x, "attend")
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            refuse_derivatives(dual, "attend")
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+            refuse_derivatives(dual * 2, "attend")
+        refuse_derivatives(forward_ad.unpack_dual(dual).primal, "attend")
