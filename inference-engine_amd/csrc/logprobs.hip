@@ -16,6 +16,7 @@
 // alternatives: 12 us for the parts, whose sums and alternatives follow one another, 7 to join).
 #include "ops_common.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -417,18 +418,26 @@ int launch(const Cut& cut, const T* logits, int64_t stride, int64_t n_rows, cons
   // Parts of the rounded size may be one fewer.
   const int32_t count = (out.vocab + cut.size - 1) / cut.size;
   auto* keys = static_cast<uint64_t*>(workspace);
-  Parts parts{reinterpret_cast<Sums*>(keys + n_rows * count * out.top), keys, count, cut.size};
-  const dim3 grid(static_cast<uint32_t>(n_rows * count));
+  auto* sums = reinterpret_cast<Sums*>(keys + n_rows * count * out.top);
   const bool stream_past = n_rows * out.vocab * int64_t(sizeof(T)) > kCacheBytes;
   const auto kernel = cut.held == kSmall ? score_part<T, kSmall, false>
                       : stream_past      ? score_part<T, kLarge, true>
                                          : score_part<T, kLarge, false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, logits, stride, out, parts);
-  IEKV_OPS_HIP(hipGetLastError());
-  if (count > 1) {
-    hipLaunchKernelGGL((join_rows<T>), dim3(static_cast<uint32_t>((n_rows + kWaves - 1) / kWaves)),
-                       dim3(kThreads), 0, stream, logits, stride, n_rows, out, parts);
+  for (int64_t first = 0; first < n_rows; first += kMaxGrid / count) {
+    const int64_t rows = std::min(n_rows - first, kMaxGrid / count);
+    const T* x = logits + first * stride;
+    const Scores to{out.tokens + first, out.logprobs + first, out.entropy + first,
+                    out.top_logprobs + first * out.top, out.top_ids + first * out.top,
+                    out.vocab, out.top};
+    const Parts parts{sums + first * count, keys + first * count * out.top, count, cut.size};
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(rows * count)), dim3(kThreads), 0, stream,
+                       x, stride, to, parts);
     IEKV_OPS_HIP(hipGetLastError());
+    if (count > 1) {
+      hipLaunchKernelGGL((join_rows<T>), dim3(static_cast<uint32_t>((rows + kWaves - 1) / kWaves)),
+                         dim3(kThreads), 0, stream, x, stride, rows, to, parts);
+      IEKV_OPS_HIP(hipGetLastError());
+    }
   }
   return IEKV_OK;
 }
@@ -463,9 +472,6 @@ int iekv_logprobs(int32_t type, const void* logits, int64_t row_stride, int64_t 
   if (!logits || !tokens || !logprobs || !entropy || (top && (!top_logprobs || !top_ids)))
     return set_error(IEKV_ERR_INVALID, "null argument");
   const Cut cut = cut_of(vocab);
-  if (n_rows * cut.parts > INT32_MAX)
-    return set_error(IEKV_ERR_INVALID, "%lld rows of %lld logits: too many in one call",
-                     static_cast<long long>(n_rows), static_cast<long long>(vocab));
   const int64_t need = iekv_logprobs_workspace(type, n_rows, vocab, top);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(IEKV_ERR_CAPACITY, "workspace of %lld bytes, %lld are needed",

@@ -23,6 +23,10 @@ int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3
     }                                                                                      \
   } while (0)
 
+// A dispatch counts its work-items in 32 bits: workgroups of 256 threads that one launch may
+// have. What needs more is launched in several.
+constexpr int64_t kMaxGrid = static_cast<int64_t>(UINT32_MAX) / 256;
+
 // Makes a device current for a call that launches on it, and the caller's again after.
 class DeviceGuard {
  public:

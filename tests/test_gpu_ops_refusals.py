@@ -30,3 +30,22 @@ def test_tangents_are_refused(gpu):
         token_logprobs(logits, tokens)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: attend(plan, 0, x), (q,), (torch.ones_like(q),))
+
+
+@pytest.mark.parametrize("vocab, top", [(5, 2), (3, 0)])
+def test_more_rows_than_a_launch_has_workgroups(gpu, vocab, top):
+    """2^24 and some rows: the last ones, of a second launch, and the first are scored alike."""
+    from iekv.engine.logprobs import token_logprobs
+
+    rows = (1 << 24) + 1000
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((2000, vocab), generator=gen, device="cuda").to(BF16)
+    logits = x.repeat(rows // 2000 + 1, 1)[:rows]
+    tokens = (torch.arange(rows, device="cuda") % 2000) % vocab
+    got = token_logprobs(logits, tokens, top=top)
+    want = token_logprobs(x, tokens[:2000].clone(), top=top)
+    index = torch.arange(rows, device="cuda") % 2000
+    for name in ("logprobs", "entropy", "top_logprobs", "top_ids"):
+        assert torch.equal(getattr(got, name), getattr(want, name)[index])
+    lp = torch.log_softmax(x.double(), 1)
+    assert ((want.logprobs - lp.gather(1, tokens[:2000, None])[:, 0]).abs() < 1e-6).all()

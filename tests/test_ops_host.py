@@ -191,3 +191,27 @@ def test_inputs_with_derivatives_are_refused():
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
             refuse_derivatives(dual * 2, "attend")
         refuse_derivatives(forward_ad.unpack_dual(dual).primal, "attend")
+
+
+MOST = (2 ** 32 - 1) // 256          # workgroups of a launch
+
+
+@pytest.mark.parametrize("rows, vocab, top, joins", [
+    (MOST + 1, 5, 2, False), (2 * MOST + 3, 2000, 0, False), (MOST // 16 + 1, 128000, 3, True),
+    (MOST // 2, 10000, 0, True), (MOST, 100, 1, False)])
+def test_logprobs_of_many_rows_run_in_several_launches(on_stub, rows, vocab, top, joins):
+    got = on_stub(f"""
+A = 1 << 48
+need = ops.iekv_logprobs_workspace(1, {rows}, {vocab}, {top})
+rc = ops.iekv_logprobs(1, A, {vocab}, {rows}, {vocab}, 2 * A, {top}, 3 * A, 4 * A, 5 * A, 6 * A,
+                       7 * A, need, 77)
+print(json.dumps([rc, ops.iekv_ops_last_error().decode() if rc else "", launches()]))
+""")
+    rc, message, launches = got
+    assert rc == 0, message
+    parts, each = launches[::2 if joins else 1], 1 if not joins else -(-vocab // 8192)
+    assert all(x[0] == 0 and x[4] == 77 and x[1] <= MOST for x in launches)
+    assert sum(x[1] for x in parts) == rows * each
+    if joins:
+        assert len(launches) == 2 * len(parts)
+        assert [-(-x[1] // each // 4) for x in parts] == [x[1] for x in launches[1::2]]
