@@ -83,20 +83,31 @@ hipError_t allow_lds(K kernel, int bytes, int device, std::atomic<uint64_t>* ask
 template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
-  const int32_t narrow_blocks = narrow * (a.kv_heads / a.together);
+  const int64_t each = a.kv_heads / a.together;     // workgroups of a narrow item
+  const int64_t blocks = wide * int64_t(a.kv_heads) + narrow * each;
   // Both kinds in one launch where the narrow ones are soon done (24 sequences of two KV heads
   // behind 512 tokens: 12.4 us against 18.4 in two); a long stream of them is better alone on
   // the card (128 sequences of the 8B shape: 206 us in two launches, 246 in one).
-  const bool both = wide && narrow && !plan.streams;
+  const bool both = wide && narrow && !plan.streams && blocks <= kMaxGrid;
+  // As many of n items at a time as a launch has workgroups for.
+  const auto in_launches = [](int64_t n, int64_t blocks_each, const auto& run) {
+    const int64_t most = kMaxGrid / blocks_each;
+    for (int64_t first = 0; first < n; first += most) {
+      run(first, std::min(most, n - first));
+      IEKV_OPS_HIP(hipGetLastError());
+    }
+    return int(IEKV_OK);
+  };
   if constexpr (sizeof(T) == 2) {
-    const dim3 wide_blocks(wide * a.kv_heads);
     bool done = !wide;
     if constexpr (sizeof(C) == 2) {
       const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
       if (wide && !both && aligned(a.k) && aligned(a.v)) {
-        hipLaunchKernelGGL((attend_wide<T, C, DP>), wide_blocks, dim3(kThreads), 0, stream, a,
-                           plan.wide.first);
-        IEKV_OPS_HIP(hipGetLastError());
+        if (const int rc = in_launches(wide, a.kv_heads, [&](int64_t first, int64_t n) {
+              hipLaunchKernelGGL((attend_wide<T, C, DP>), dim3(n * a.kv_heads), dim3(kThreads), 0,
+                                 stream, a, static_cast<int32_t>(plan.wide.first + first));
+            }))
+          return rc;
         done = true;
       }
     }
@@ -105,29 +116,37 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
                                           sizeof(typename Narrow<T, C, DP>::Lds));
       static std::atomic<uint64_t> asked{0};
       IEKV_OPS_HIP(allow_lds(attend_both<T, C, DP>, bytes, plan.device, &asked));
-      hipLaunchKernelGGL((attend_both<T, C, DP>), dim3(wide_blocks.x + (both ? narrow_blocks : 0)),
-                         dim3(kThreads), bytes, stream, a, plan.wide.first, wide, plan.narrow.first,
-                         both ? narrow : 0);
-      IEKV_OPS_HIP(hipGetLastError());
+      if (const int rc = in_launches(wide, a.kv_heads, [&](int64_t first, int64_t n) {
+            hipLaunchKernelGGL((attend_both<T, C, DP>),
+                               dim3(both ? blocks : n * a.kv_heads), dim3(kThreads), bytes, stream,
+                               a, static_cast<int32_t>(plan.wide.first + first),
+                               static_cast<int32_t>(n), plan.narrow.first, both ? narrow : 0);
+          }))
+        return rc;
     }
   }
   if (narrow && !both) {
     // Only 32-bit queries have narrow items of more than 16 heads.
-    hipLaunchKernelGGL((attend_narrow<T, C, DP>),
-                       dim3(narrow_blocks, (a.group + 15) / 16), dim3(kThreads), 0, stream, a,
-                       plan.narrow.first, narrow);
-    IEKV_OPS_HIP(hipGetLastError());
+    if (const int rc = in_launches(narrow, each, [&](int64_t first, int64_t n) {
+          hipLaunchKernelGGL((attend_narrow<T, C, DP>), dim3(n * each, (a.group + 15) / 16),
+                             dim3(kThreads), 0, stream, a,
+                             static_cast<int32_t>(plan.narrow.first + first),
+                             static_cast<int32_t>(n));
+        }))
+      return rc;
   }
   if (plan.joined) {
     // Few rows have many parts each: their loads are spread over four waves.
     const int64_t rows = int64_t(plan.joined) * a.kv_heads * a.group;
     const int32_t* w = a.words;
     const bool few = rows <= kJoinFew;
-    hipLaunchKernelGGL((few ? join_parts<T, kWaves> : join_parts<T, 1>),
-                       dim3(few ? rows : (rows + kWaves - 1) / kWaves), dim3(kThreads), 0, stream,
-                       a, w + plan.join_tokens_at, w + plan.join_starts_at, w + plan.join_parts_at,
-                       plan.joined);
-    IEKV_OPS_HIP(hipGetLastError());
+    if (const int rc = in_launches(few ? rows : (rows + kWaves - 1) / kWaves, 1,
+                                   [&](int64_t first, int64_t n) {
+          hipLaunchKernelGGL((few ? join_parts<T, kWaves> : join_parts<T, 1>), dim3(n),
+                             dim3(kThreads), 0, stream, a, w + plan.join_tokens_at,
+                             w + plan.join_starts_at, w + plan.join_parts_at, plan.joined, first);
+        }))
+      return rc;
   }
   return IEKV_OK;
 }

@@ -954,15 +954,17 @@ __global__ __launch_bounds__(kThreads, 2) void attend_both(
 // Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, W
 // waves a row. The loads of a row's parts are what takes time, so they are independent of one
 // another: a lane holds 4 dimensions of every 64 / lanes-th part (of each 64, whose maxima
-// and sums the lanes hold), and the waves take turns. The order of the sums is fixed.
+// and sums the lanes hold), and the waves take turns. The order of the sums is fixed. The
+// launch's workgroups are the `first` one and on.
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void join_parts(Args a, const int32_t* tokens,
                                                        const int32_t* starts,
-                                                       const int32_t* parts, int32_t n) {
+                                                       const int32_t* parts, int32_t n,
+                                                       int64_t first) {
   __shared__ float sums[kWaves][IEKV_ATTENTION_MAX_DIM];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, turn = wave % W;
   const int32_t heads = a.kv_heads * a.group, d = a.head_dim;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWaves / W) + wave / W;
+  const int64_t row = (first + blockIdx.x) * (kWaves / W) + wave / W;
   const bool real = row < static_cast<int64_t>(n) * heads;
   const int32_t entry = real ? static_cast<int32_t>(row / heads) : 0;
   const int32_t head = real ? static_cast<int32_t>(row % heads) : 0;

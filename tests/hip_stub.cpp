@@ -12,7 +12,7 @@ constexpr int kMost = 1 << 16;
 struct Launch {
   int64_t device, grid_x, grid_y, block_x, stream;
 } launches[kMost];
-int n_launches = 0, current = 0, units_asked_of = -1, lds_asked_on = 0, devices = 8;
+int n_launches = 0, current = 0, units_asked_of = -1, lds_asked_on = 0, devices = 8, last = 0;
 Dim3 grid, block;
 size_t shared;
 void* stream;
@@ -35,7 +35,7 @@ int hipGetDevice(int* device) {
   return 0;
 }
 int hipSetDevice(int device) {
-  if (device < 0 || device >= devices) return 101;   // hipErrorInvalidDevice
+  if (device < 0 || device >= devices) return last = 101;   // hipErrorInvalidDevice
   current = device;
   return 0;
 }
@@ -44,7 +44,11 @@ int hipDeviceGetAttribute(int* value, int, int device) {
   *value = 256 >> device;
   return 0;
 }
-int hipGetLastError() { return 0; }
+int hipGetLastError() {
+  const int error = last;
+  last = 0;
+  return error;
+}
 const char* hipGetErrorString(int error) { return error == 101 ? "invalid device" : "invalid launch"; }
 int hipFuncSetAttribute(const void*, int, int) {
   lds_asked_on |= 1 << current;
@@ -60,7 +64,7 @@ int __hipPopCallConfiguration(Dim3* g, Dim3* b, size_t* s, void** on) {
 }
 int hipLaunchKernel(const void*, Dim3 g, Dim3 b, void**, size_t, void* on) {
   // A dispatch counts its work-items in 32 bits.
-  if (uint64_t(g.x) * b.x > UINT32_MAX || !g.x || !g.y || n_launches == kMost) return 9;
+  if (uint64_t(g.x) * b.x > UINT32_MAX || !g.x || !g.y || n_launches == kMost) return last = 9;
   launches[n_launches++] = {current, g.x, g.y, b.x, reinterpret_cast<int64_t>(on)};
   return 0;
 }

@@ -215,3 +215,28 @@ print(json.dumps([rc, ops.iekv_ops_last_error().decode() if rc else "", launches
     if joins:
         assert len(launches) == 2 * len(parts)
         assert [-(-x[1] // each // 4) for x in parts] == [x[1] for x in launches[1::2]]
+
+
+@pytest.mark.parametrize("step, blocks", [
+    ("[1] * 16385, [1] * 16385", [16385 * 1024]),               # four heads a workgroup
+    ("[17] * 4100, [17] * 4100", [4100 * 4096]),
+    ("[17] * 4097 + [5], [17] * 4097 + [1]", [4097 * 4096, 4096]),   # not in one launch
+    # Rows that are joined, four a workgroup: prompts of 120 behind 512 keys.
+    ("[632] * 140, [120] * 140, 16, 32", [None, 140 * 120 * 1024]),
+])
+def test_steps_of_any_size_run_in_several_launches(on_stub, step, blocks):
+    got = on_stub(f"""
+p = plan({step}, num_heads=4096, num_kv_heads=4096, head_dim=8)
+rc = ops.iekv_attend(p, 1 << 44, 1 << 45, 1 << 46, 1 << 47, 4096 * 8, 8, 1.0, 3 << 46, 5 << 46,
+                     1 << 46, 77)
+print(json.dumps([rc, ops.iekv_ops_last_error().decode() if rc else "", launches()]))
+""")
+    rc, message, launches = got
+    assert rc == 0, message
+    assert all(x[0] == 0 and x[4] == 77 and x[1] <= MOST and x[2] == 1 for x in launches)
+    total = sum(b for b in blocks if b is not None)
+    if blocks[0] is None:
+        assert sum(x[1] for x in launches) > total and launches[-1][1] == total - MOST
+    else:
+        assert sum(x[1] for x in launches) == total
+    assert len(launches) > len(blocks) or blocks[-1] == 4096
