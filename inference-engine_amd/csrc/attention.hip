@@ -251,6 +251,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
       return set_error(IEKV_ERR_RANGE, "sequence %d: context of %lld needs %lld blocks, table has %lld",
                        s, static_cast<long long>(context), static_cast<long long>(used),
                        static_cast<long long>(held));
+    if (!tables && (used || held)) return set_error(IEKV_ERR_INVALID, "tables is null");
     const int32_t* table = tables + starts[s];
     for (int64_t b = 0; b < used; ++b)
       if (table[b] < 0 || table[b] >= shape.num_blocks)
@@ -329,8 +330,6 @@ int iekv_attention_plan_create(const iekv_attention_shape* shape, int32_t n_seqs
   if (n_seqs < 0) return set_error(IEKV_ERR_INVALID, "n_seqs %d is negative", n_seqs);
   if (n_seqs && (!context_lens || !query_lens || !table_starts))
     return set_error(IEKV_ERR_INVALID, "context_lens, query_lens or table_starts is null");
-  if (n_seqs && !tables && table_starts[n_seqs] > 0)
-    return set_error(IEKV_ERR_INVALID, "tables is null");
   if (const int rc = check_shape(*shape)) return rc;
   try {
     return make(*shape, n_seqs, context_lens, query_lens, tables, table_starts, out);

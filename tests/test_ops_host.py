@@ -240,3 +240,25 @@ print(json.dumps([rc, ops.iekv_ops_last_error().decode() if rc else "", launches
     else:
         assert sum(x[1] for x in launches) == total
     assert len(launches) > len(blocks) or blocks[-1] == 4096
+
+
+def test_tables_that_are_missing_are_refused(on_stub):
+    """Also where their lengths end at zero: a table is read by what it is said to hold."""
+    got = on_stub("""
+got = []
+for starts, contexts in (([0, 2, 2], [20, 0]), ([0, 2, 0], [20, 0]), ([0, 0, 1], [0, 5])):
+    out = ctypes.c_void_p()
+    shape = _ops.AttentionShape(8, 2, 64, 16, 10, 3, 3, 0, 0, 0)
+    rc = ops.iekv_attention_plan_create(
+        ctypes.byref(shape), 2, (ctypes.c_int32 * 2)(*contexts), (ctypes.c_int32 * 2)(0, 0), None,
+        (ctypes.c_int64 * 3)(*starts), ctypes.byref(out))
+    got.append([rc, out.value, ops.iekv_ops_last_error().decode()])
+out = ctypes.c_void_p()
+rc = ops.iekv_attention_plan_create(
+    ctypes.byref(shape), 2, (ctypes.c_int32 * 2)(0, 0), (ctypes.c_int32 * 2)(0, 0), None,
+    (ctypes.c_int64 * 3)(0, 0, 0), ctypes.byref(out))
+print(json.dumps([got, rc]))
+""")
+    for rc, plan, message in got[0]:
+        assert rc == INVALID and plan is None and "tables is null" in message
+    assert got[1] == 0
