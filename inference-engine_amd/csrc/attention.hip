@@ -161,12 +161,16 @@ int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   }
 }
 
+int32_t bytes_of(int32_t type) {
+  return type == IEKV_TYPE_F32 ? 4 : type == IEKV_TYPE_E4M3 ? 1 : 2;
+}
+
 // Whether the output lies over queries of other rows: a workgroup writes its rows when it has
 // read their queries, and not when others have read theirs.
 bool overlaps(const iekv_attention_plan& plan, const void* q, int64_t token_stride,
               int64_t head_stride, const void* out) {
   const iekv_attention_shape& s = plan.shape;
-  const int64_t tokens = plan.tokens, heads = s.num_heads, size = s.query_type == IEKV_TYPE_F32 ? 4 : 2;
+  const int64_t tokens = plan.tokens, heads = s.num_heads, size = bytes_of(s.query_type);
   const int64_t row = s.head_dim * size, bytes = tokens * heads * row;
   const auto at = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
   const int64_t q0 = at(q), out0 = at(out);
@@ -229,7 +233,7 @@ int check_shape(const iekv_attention_shape& s) {
 // eight bf16 heads of 128, 350 KB a workgroup: 13.5 us against 15.8 in parts; of 1,000 tokens
 // 19 against 14, and of 1,000 on an 8-bit cache 16.7 against 19.2).
 int32_t few_keys(const iekv_attention_shape& s) {
-  const int32_t bytes = s.cache_type == IEKV_TYPE_F32 ? 4 : s.cache_type == IEKV_TYPE_E4M3 ? 1 : 2;
+  const int32_t bytes = bytes_of(s.cache_type);
   return std::min(bytes == 4 ? 512 : 1024, (384 << 10) / (2 * s.head_dim * bytes));
 }
 
@@ -279,7 +283,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            shape.block_size, shape.window, shape.sinks,
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
-                           few_keys(shape)};
+                           few_keys(shape), 2 * shape.head_dim * bytes_of(shape.cache_type)};
   const int device = current_device();
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||

@@ -32,6 +32,7 @@ struct Shape {
   int32_t shared;         // keys of the shared blocks (0: none)
   int32_t wide_rows;      // rows an item of the wide kernel holds at most (0: there is none)
   int32_t few_keys = 1024;  // that a narrow workgroup takes whole rather than leave parts
+  int32_t key_bytes = 512;  // K and V of a key in one KV head
 };
 
 struct Sequence {
@@ -57,7 +58,8 @@ struct Plan {
 
 constexpr int kNarrowRows = 16;
 constexpr int kNarrowWaves = 4;
-constexpr int64_t kFewKeys = 1 << 16;   // of all KV heads, read again rather than joined
+constexpr int64_t kSharedBytes = 256 << 10;  // of shared keys in a KV head that are worth a join
+constexpr int64_t kSavedBytes = 8 << 20;     // and of reads that sharing them saves
 
 // Keys of [lo, hi) that any of positions low..high sees.
 inline void visible(const Shape& sh, int64_t low, int64_t high, int64_t lo, int64_t hi, Item* it) {
@@ -160,13 +162,17 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
     return sh.shared && s.queries &&
            int64_t(s.queries) * sh.group < (sh.wide_rows ? sh.wide_rows : kNarrowRows);
   };
-  // Nor do short contexts, where what is read again for each is less than a join's launch is
-  // worth (24 sequences of two KV heads behind 512 tokens: 9.5 us against 11.3).
+  // Nor do short prefixes, or those of few sequences, where what is read again for each is less
+  // than the parts of every row, their join and a second launch take. Of eight bf16 heads of 128
+  // alone and shared: 96 sequences of 1,200 tokens behind 16 of them 85 us and 94, behind 512 76
+  // and 70, behind 1,024 68 and 32; eight of 612 behind 512 16.9 and 12.0, four 11.7 and 11.7.
+  // 8-bit keys pay from twice as many on: 64 sequences of 612 behind 512 17 us and 23, 128 of
+  // 1,124 behind 1,024 50 and 38. Between, some gain a tenth and some lose one.
   int64_t sharing = 0;
-  int32_t longest = 0;
-  for (const Sequence& s : seqs)
-    if (could(s)) ++sharing, longest = std::max(longest, s.context);
-  const bool worth = longest > sh.few_keys || sharing * sh.shared * sh.kv_heads > kFewKeys;
+  for (const Sequence& s : seqs) sharing += could(s);
+  const int64_t shared_bytes = int64_t(sh.shared) * sh.key_bytes;
+  const bool worth = shared_bytes >= kSharedBytes &&
+                     (sharing - 1) * shared_bytes * sh.kv_heads >= kSavedBytes;
   const auto shares = [&](const Sequence& s) { return worth && could(s); };
   int32_t leading = -1, run0 = 0, run = 0;
   for (const Sequence& s : seqs) {

@@ -15,8 +15,8 @@ step, a prompt or a chunk of one in a prefill step.
 A query at position ``p`` sees the keys ``j <= p`` with ``j > p - window`` or
 ``j < sinks``; without a window every key up to its own. ``shared_blocks`` says that every
 block table begins with the same so many blocks, as the block manager's prefix sharing
-makes them: their keys are read and scored once for all sequences' queries together. The
-result is the same, up to rounding.
+makes them: where that saves more than it costs, their keys are read and scored once for all
+sequences' queries together. The result is the same, up to rounding.
 
 Forward only: the package serves and trains nothing, and queries that require a gradient or
 carry a tangent are refused.
