@@ -13,7 +13,7 @@ from functools import lru_cache
 import torch
 
 from .. import _native, _ops
-from .pools import current_stream_handle, refuse_derivatives
+from .pools import current_device, current_stream_handle, refuse_derivatives
 
 _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
           torch.bfloat16: _native.IEKV_TYPE_BF16}
@@ -55,7 +55,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if not 0 <= top <= min(vocab, _ops.LOGPROBS_MAX_TOP):
         raise ValueError(f"top {top} out of range for a vocabulary of {vocab} (at most "
                          f"{_ops.LOGPROBS_MAX_TOP})")
-    if logits.device.index != torch.cuda.current_device():
+    if logits.device.index != current_device():
         with torch.cuda.device(logits.device):
             return token_logprobs(logits, tokens, top=top)
     refuse_derivatives(logits, "token_logprobs")

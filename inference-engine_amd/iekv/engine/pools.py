@@ -392,14 +392,18 @@ def stage_ids(device: torch.device, *arrays: np.ndarray) -> list[torch.Tensor]:
     return out
 
 
+# The current device, without the check of torch.cuda's own accessor that there is one: for
+# callers that hold a tensor of it.
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def refuse_derivatives(tensor: torch.Tensor, call: str) -> None:
     """RuntimeError for an input whose derivative ``call``, which has none, would drop: one
     that requires a gradient, or one with a tangent of forward mode."""
     if tensor.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{call} has no backward pass: detach its input or use no_grad")
     # Outside of forward mode no tensor has one, and asking each costs more.
-    if getattr(_forward_ad, "_current_level", 0) >= 0 and \
-            _forward_ad.unpack_dual(tensor).tangent is not None:
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(tensor).tangent is not None:
         raise RuntimeError(f"{call} has no derivative in forward mode: unpack its input")
 
 

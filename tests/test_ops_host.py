@@ -161,7 +161,7 @@ def test_logprobs_run_on_the_logits_device(monkeypatch):
         def __exit__(self, *_):
             current[0] = self.before
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(logprobs, "current_device", lambda: current[0])
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(logprobs, "current_stream_handle", lambda device: 0)
     monkeypatch.setattr(logprobs._ops, "entry",
@@ -221,8 +221,8 @@ print(json.dumps([rc, ops.iekv_ops_last_error().decode() if rc else "", launches
     ("[1] * 16385, [1] * 16385", [16385 * 1024]),               # four heads a workgroup
     ("[17] * 4100, [17] * 4100", [4100 * 4096]),
     ("[17] * 4097 + [5], [17] * 4097 + [1]", [4097 * 4096, 4096]),   # not in one launch
-    # Rows that are joined, four a workgroup: prompts of 120 behind 512 keys.
-    ("[632] * 140, [120] * 140, 16, 32", [None, 140 * 120 * 1024]),
+    # Rows that are joined, four a workgroup: prompts of 120 behind a prefix worth sharing.
+    ("[8312] * 140, [120] * 140, 16, 512", [None, 140 * 120 * 1024]),
 ])
 def test_steps_of_any_size_run_in_several_launches(on_stub, step, blocks):
     got = on_stub(f"""
