@@ -45,7 +45,8 @@ typedef struct iekv_attention_shape {
   int32_t cache_type;    /* the query type, or _E4M3; any type for F32 queries */
   int64_t window;        /* a query sees the last `window` keys up to its own (0: all) */
   int64_t sinks;         /* and the first `sinks` keys */
-  int64_t shared_blocks; /* leading blocks that every table shares, attended once for all */
+  int64_t shared_blocks; /* leading blocks that every table shares: attended once for all where
+                          * that saves more than joining the results takes */
 } iekv_attention_shape;
 
 /* How a step's attention is cut into workgroups: made once per step, used by every

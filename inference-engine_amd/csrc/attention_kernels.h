@@ -621,8 +621,8 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 // element are copied through registers); its rows' 16-byte chunks change places by key, so
 // that the 256 bytes that are read at a time lie in different banks: a chunk of K of 16 keys
 // each, four chunks of V of four keys each. A prompt of 7,777 tokens in a window of 4,096, 32
-// bf16 heads of 128: 985 TFLOP/s, the matrix units busy for 46% of the cycles and the vector
-// units for 48%: two waves to a SIMD, one with its products and one with its weights. Scoring
+// bf16 heads of 128: 398-406 us by the box, 950-965 TFLOP/s, the matrix units busy for 46% of the
+// cycles and the vector units for 48%: two waves to a SIMD, one with its products and one with its weights. Scoring
 // a tile while the one before is weighted in the same wave was 3-12% slower.
 //
 // Weights are rounded to the queries' type, by at most half a step of it each: an output is off

