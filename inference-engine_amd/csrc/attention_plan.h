@@ -168,11 +168,17 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // and 70, behind 1,024 68 and 32; eight of 612 behind 512 16.9 and 12.0, four 11.7 and 11.7.
   // 8-bit keys pay from twice as many on: 64 sequences of 612 behind 512 17 us and 23, 128 of
   // 1,124 behind 1,024 50 and 38. Between, some gain a tenth and some lose one.
-  int64_t sharing = 0;
-  for (const Sequence& s : seqs) sharing += could(s);
-  const int64_t shared_bytes = int64_t(sh.shared) * sh.key_bytes;
-  const bool worth = shared_bytes >= kSharedBytes &&
-                     (sharing - 1) * shared_bytes * sh.kv_heads >= kSavedBytes;
+  // What counts is what the sequences see: a window may have left most of the prefix behind.
+  int64_t seen = 0, longest = 0;
+  for (const Sequence& s : seqs) {
+    if (!could(s)) continue;
+    Item it{};
+    visible(sh, s.context - s.queries, s.context - 1, 0, sh.shared, &it);
+    seen += keys_of(it);
+    longest = std::max<int64_t>(longest, keys_of(it));
+  }
+  const bool worth = longest * sh.key_bytes >= kSharedBytes &&
+                     (seen - longest) * sh.key_bytes * sh.kv_heads >= kSavedBytes;
   const auto shares = [&](const Sequence& s) { return worth && could(s); };
   int32_t leading = -1, run0 = 0, run = 0;
   for (const Sequence& s : seqs) {
@@ -198,7 +204,7 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // Few keys take less time in turn than a join does, if there is none yet.
   int32_t longest_item = 0;
   for (const Item& it : narrow) longest_item = std::max(longest_item, keys_of(it));
-  const bool whole = longest_item <= sh.few_keys && !(worth && sharing);
+  const bool whole = longest_item <= sh.few_keys && !worth;
   // Two workgroups fit a compute unit. Long streams are cut for half as many again: 128
   // sequences of unlike lengths 182 us against 191 with two, of one length 175 against 173.
   if (!whole)

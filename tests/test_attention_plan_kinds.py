@@ -64,6 +64,16 @@ def test_steps_of_every_kind_read_every_visible_key_once(checker):
         assert found.get(kind, 0) >= 10, found
 
 
+@pytest.mark.parametrize("window, sinks, shares", [
+    (0, 0, True), (4000, 4, True), (1100, 4, True), (600, 4, False), (100, 4, False),
+    (100, 2000, True), (1, 0, False)])
+def test_prefixes_that_a_window_has_left_behind_are_not_shared(checker, window, sinks, shares):
+    """96 sequences of 2,560 tokens behind 2,048: what of them the last tokens see counts."""
+    shape = (1024, 512, 4, 8, 16, window, sinks, 2048, 128, 256)
+    kinds, = run(checker, [(shape, [(2560, 1)] * 96)])
+    assert ("shared" in kinds) == shares, kinds
+
+
 @pytest.mark.parametrize("key_bytes, kv_heads, group, shared, contexts, shares", [
     (512, 8, 4, 16, [1200] * 96, False),             # one block of many sequences
     (512, 8, 4, 256, [1200] * 96, False),
