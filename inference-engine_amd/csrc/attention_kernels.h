@@ -326,7 +326,7 @@ __device__ __forceinline__ void store_out(T* out, const float* x) {
 // operands of V^T (dimension c EV + t at place c of tile t).
 //
 // 16-bit operands hold a weight as two, its value rounded to the type and what that leaves:
-// together off by 2^-17 (bf16) of it, as good as 32 bits beside V's own. The second product is
+// together off by 2^-16 (bf16) of it, as good as 32 bits beside V's own. The second product is
 // hidden behind the stream: 48 sequences of 6,000 tokens of eight bf16 heads 129.9 us against
 // 130.1 with the rounded weights alone, one of 16,384 on an 8-bit cache 16.0 against 15.7.
 template <typename T, typename C, int DP>
@@ -622,8 +622,8 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 // that the 256 bytes that are read at a time lie in different banks: a chunk of K of 16 keys
 // each, four chunks of V of four keys each. A prompt of 7,777 tokens in a window of 4,096, 32
 // bf16 heads of 128: 398-406 us by the box, 950-965 TFLOP/s, the matrix units busy for 46% of the
-// cycles and the vector units for 48%: two waves to a SIMD, one with its products and one with its weights. Scoring
-// a tile while the one before is weighted in the same wave was 3-12% slower.
+// cycles and the vector units for 48%: two waves to a SIMD, one with its products and one with
+// its weights. Scoring a tile while the one before is weighted in the same wave was 3-12% slower.
 //
 // Weights are rounded to the queries' type, by at most half a step of it each: an output is off
 // by no more than that of the mean of |v|, as it is by its own rounding. The remainders' product
