@@ -4,6 +4,7 @@
  *
  *   attention   of one layer of a step, read through block tables: sliding window
  *               with sink tokens, batches that share leading blocks
+ *   microscaled caches: rows quantised as they are written, and read back as values
  *   logprobs    log probabilities of given tokens, entropy, most likely alternatives
  *
  * The conventions are those of iekv.h: IEKV_OK or a negative IEKV_ERR_* code, a
@@ -23,12 +24,23 @@
 extern "C" {
 #endif
 
-#define IEKV_OPS_ABI_VERSION 1
+#define IEKV_OPS_ABI_VERSION 2
 
 int iekv_ops_abi_version(void);
 
 /* Message for the last failed call on this thread ("" if none). */
 const char* iekv_ops_last_error(void);
+
+/* Element types of caches only (beside IEKV_TYPE_*): microscaled. 32 dimensions of a head (the
+ * last of a head may be fewer) share a power of two 2^e; an element x is held as x / 2^e rounded
+ * to nearest even, in 8 bits (e4m3 of at most 448; integers of at most 127) or 4 (e2m1 of at
+ * most 6; the even dimension in a byte's low half). e is the smallest from -100 on with which
+ * the group's largest magnitude is within the type's. A head's record is the bytes of its
+ * elements, then 4 bytes of which byte g is group g's e + 127 and those past the last group are
+ * 0. A group with a NaN or an infinity has the byte 255, and its elements 0, and reads as NaN.
+ * A cache is [num_blocks * block_size][num_kv_heads] records: rows like any other for the
+ * handoff and whatever else moves bytes. */
+enum { IEKV_TYPE_MXFP8 = 5, IEKV_TYPE_MXINT8 = 6, IEKV_TYPE_MXFP4 = 7 };
 
 #define IEKV_ATTENTION_MAX_DIM 128   /* largest head dimension (multiples of 8) */
 #define IEKV_ATTENTION_MAX_GROUP 128 /* most query heads per KV head */
@@ -42,7 +54,8 @@ typedef struct iekv_attention_shape {
   int32_t block_size;    /* cache rows per block */
   int64_t num_blocks;    /* blocks of the pool (fewer than 2^32 rows): every table entry is below */
   int32_t query_type;    /* IEKV_TYPE_F32, _F16 or _BF16: of q and of the output */
-  int32_t cache_type;    /* the query type, or _E4M3; any type for F32 queries */
+  int32_t cache_type;    /* the query type, _E4M3 or microscaled; any type for F32 queries.
+                          * Microscaled elements are taken as the query type holds them */
   int64_t window;        /* a query sees the last `window` keys up to its own (0: all) */
   int64_t sinks;         /* and the first `sinks` keys */
   int64_t shared_blocks; /* leading blocks that every table shares: attended once for all where
@@ -82,6 +95,40 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
                 const void* v, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                 float scale, void* out, void* workspace, int64_t workspace_bytes,
                 hipStream_t stream);
+
+/* Bytes of a record of head_dim dimensions (a multiple of 8 up to IEKV_ATTENTION_MAX_DIM):
+ * head_dim + 4, or head_dim / 2 + 4 of MXFP4; 0 for any other type or size. */
+int64_t iekv_mx_head_bytes(int32_t cache_type, int32_t head_dim);
+
+/* What a pool's microscaled arrays have in common. */
+typedef struct iekv_mx_cache {
+  int32_t cache_type;   /* IEKV_TYPE_MX* */
+  int32_t num_kv_heads, head_dim;
+  int32_t block_size;   /* rows per block */
+  int64_t num_blocks;
+} iekv_mx_cache;
+
+/* Quantise rows into slots, for n_layers layers: K and V of layer l and token t, the
+ * num_kv_heads * head_dim values of row_type (F32, F16 or BF16) at k + l * k_strides[0] +
+ * t * k_strides[1] + head * k_strides[2] elements (HOST arrays of three strides, head_dim
+ * contiguous) and at v likewise, become the records of row slots[t] (int64, device memory) of
+ * the arrays at k_arrays[l] and v_arrays[l] (HOST arrays of device addresses). Rows whose slot is
+ * outside the pool are skipped; of rows with the same slot any may be held, or parts of several.
+ * Runs on the current device, which has to be the arrays'. */
+int iekv_mx_write_slots(const iekv_mx_cache* cache, const uint64_t* k_arrays,
+                        const uint64_t* v_arrays, int32_t n_layers, int32_t row_type,
+                        const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
+                        hipStream_t stream);
+
+/* Read a context back as values: out [n_arrays][context_len][num_kv_heads][head_dim] of out_type
+ * (F32, F16 or BF16; rounded to nearest even), row j of array i from the array at arrays[i]
+ * (HOST array of device addresses), row table[j / block_size] * block_size + j % block_size
+ * (int32, device memory). Rows of blocks outside the pool are left untouched. A context of
+ * 2^32 / (num_kv_heads * head_dim / 8) rows or more is refused. */
+int iekv_mx_read_rows(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
+                      const int32_t* table, int64_t context_len, int32_t out_type, void* out,
+                      hipStream_t stream);
 
 #define IEKV_LOGPROBS_MAX_TOP 64
 

@@ -100,7 +100,7 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   };
   if constexpr (sizeof(T) == 2) {
     bool done = !wide;
-    if constexpr (sizeof(C) == 2) {
+    if constexpr (std::is_same_v<T, C>) {
       const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
       if (wide && !both && aligned(a.k) && aligned(a.v)) {
         if (const int rc = in_launches(wide, a.kv_heads, [&](int64_t first, int64_t n) {
@@ -165,6 +165,13 @@ int32_t bytes_of(int32_t type) {
   return type == IEKV_TYPE_F32 ? 4 : type == IEKV_TYPE_E4M3 ? 1 : 2;
 }
 
+// Bytes of a head of a key in the cache.
+int32_t head_bytes_of(const iekv_attention_shape& s) {
+  return s.cache_type >= IEKV_TYPE_MXFP8
+             ? static_cast<int32_t>(iekv_mx_head_bytes(s.cache_type, s.head_dim))
+             : s.head_dim * bytes_of(s.cache_type);
+}
+
 // Whether the output lies over queries of other rows: a workgroup writes its rows when it has
 // read their queries, and not when others have read theirs.
 bool overlaps(const iekv_attention_plan& plan, const void* q, int64_t token_stride,
@@ -194,9 +201,9 @@ int64_t workspace_bytes_of(const iekv_attention_plan& p) {
 }
 
 bool known_types(int32_t query, int32_t cache) {
-  if (query == IEKV_TYPE_F32) return cache >= IEKV_TYPE_F32 && cache <= IEKV_TYPE_E4M3;
+  if (query == IEKV_TYPE_F32) return cache >= IEKV_TYPE_F32 && cache <= IEKV_TYPE_MXFP4;
   return (query == IEKV_TYPE_F16 || query == IEKV_TYPE_BF16) &&
-         (cache == query || cache == IEKV_TYPE_E4M3);
+         (cache == query || (cache >= IEKV_TYPE_E4M3 && cache <= IEKV_TYPE_MXFP4));
 }
 
 int check_shape(const iekv_attention_shape& s) {
@@ -233,8 +240,7 @@ int check_shape(const iekv_attention_shape& s) {
 // eight bf16 heads of 128, 350 KB a workgroup: 13.5 us against 15.8 in parts; of 1,000 tokens
 // 19 against 14, and of 1,000 on an 8-bit cache 16.7 against 19.2).
 int32_t few_keys(const iekv_attention_shape& s) {
-  const int32_t bytes = bytes_of(s.cache_type);
-  return std::min(bytes == 4 ? 512 : 1024, (384 << 10) / (2 * s.head_dim * bytes));
+  return std::min(s.cache_type == IEKV_TYPE_F32 ? 512 : 1024, (384 << 10) / (2 * head_bytes_of(s)));
 }
 
 int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* context_lens,
@@ -283,7 +289,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            shape.block_size, shape.window, shape.sinks,
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
-                           few_keys(shape), 2 * shape.head_dim * bytes_of(shape.cache_type)};
+                           few_keys(shape), 2 * head_bytes_of(shape)};
   const int device = current_device();
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||
@@ -416,7 +422,16 @@ int iekv_attend(const iekv_attention_plan* plan, const int32_t* words, const voi
     case IEKV_TYPE_F16 * 8 + IEKV_TYPE_F16: return launch<_Float16, _Float16>(*plan, a, stream);
     case IEKV_TYPE_F16 * 8 + IEKV_TYPE_E4M3: return launch<_Float16, E4m3>(*plan, a, stream);
     case IEKV_TYPE_BF16 * 8 + IEKV_TYPE_BF16: return launch<Bf16, Bf16>(*plan, a, stream);
-    default: return launch<Bf16, E4m3>(*plan, a, stream);
+    case IEKV_TYPE_BF16 * 8 + IEKV_TYPE_E4M3: return launch<Bf16, E4m3>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_MXFP8: return launch<float, Mxfp8>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_MXINT8: return launch<float, Mxint8>(*plan, a, stream);
+    case IEKV_TYPE_F32 * 8 + IEKV_TYPE_MXFP4: return launch<float, Mxfp4>(*plan, a, stream);
+    case IEKV_TYPE_F16 * 8 + IEKV_TYPE_MXFP8: return launch<_Float16, Mxfp8>(*plan, a, stream);
+    case IEKV_TYPE_F16 * 8 + IEKV_TYPE_MXINT8: return launch<_Float16, Mxint8>(*plan, a, stream);
+    case IEKV_TYPE_F16 * 8 + IEKV_TYPE_MXFP4: return launch<_Float16, Mxfp4>(*plan, a, stream);
+    case IEKV_TYPE_BF16 * 8 + IEKV_TYPE_MXFP8: return launch<Bf16, Mxfp8>(*plan, a, stream);
+    case IEKV_TYPE_BF16 * 8 + IEKV_TYPE_MXINT8: return launch<Bf16, Mxint8>(*plan, a, stream);
+    default: return launch<Bf16, Mxfp4>(*plan, a, stream);
   }
 }
 

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "attention_plan.h"
+#include "microscaled.h"
 #include "ops_common.h"
 
 namespace iekv_ops {
@@ -47,15 +48,8 @@ struct Args {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-template <int N>
-struct Words {
-  uint32_t w[N];
-};
 
 // BYTES from any address (caches and queries may begin at any element).
 template <int BYTES>
@@ -69,25 +63,14 @@ __device__ __forceinline__ Words<(BYTES + 3) / 4> load_bytes(const void* p) {
 // The same of a stream that is read once.
 template <int BYTES>
 __device__ __forceinline__ Words<(BYTES + 3) / 4> stream_bytes(const void* p) {
-  if constexpr (BYTES % 4) {
+  // (Vectors of three are loaded as four.)
+  if constexpr (BYTES % 4 || BYTES == 12) {
     return load_bytes<BYTES>(p);
   } else {
     typedef uint32_t Vec __attribute__((ext_vector_type(BYTES / 4), aligned(1)));
     return __builtin_bit_cast(Words<BYTES / 4>,
                               __builtin_nontemporal_load(static_cast<const Vec*>(p)));
   }
-}
-
-// Two elements of the compute type in a word, rounded to nearest even.
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<Bf16>(float a, float b) {
-  return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<_Float16>(float a, float b) {
-  return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
 }
 
 // N elements of type C as elements of the compute type T (exact: T holds every value of C).
@@ -239,6 +222,20 @@ constexpr float lift(float narrow_or_wide) {
 constexpr float kFar = 1 << 20;
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && fabsf(m) < INFINITY; }
 
+// Dimension `i` of a head of `d` in the cache, as T holds it.
+template <typename T, typename C>
+__device__ __forceinline__ float cached(const char* head, int32_t d, int32_t i) {
+  if constexpr (!kScaled<C>) {
+    return to_float(reinterpret_cast<const C*>(head)[i]);
+  } else {
+    const uint8_t code = head[code_bytes<C>(i)];
+    const uint32_t w = kBits<C> == 4 ? code >> i % 2 * 4 : code;
+    const float scale = scale_of(static_cast<uint8_t>(head[code_bytes<C>(d) + i / kGroup]), 0);
+    const float x = __builtin_bit_cast(float, pair_of<float, C>(&w, 0, scale).w[0]);
+    return to_float(from_float<T>(x));
+  }
+}
+
 // One query row by one wave: a lane scores a key of each 64, then holds two dimensions of
 // the output. A key the row does not see is not read for it at all, so that whatever the
 // cache holds there (infinities, NaN) stays out. The matrix kernels multiply such a V by a
@@ -249,23 +246,24 @@ __device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32
   const int32_t token = it.token0 + row / a.group, in_group = row % a.group;
   const int32_t position = a.words[a.positions_at + token];
   const int32_t d = a.head_dim;
-  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  const int32_t size = head_bytes<C>(d);
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * size;
   const int64_t head = static_cast<int64_t>(kv_head) * a.group + in_group;
   const T* q = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
-  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
-  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d;
+  const char* kc = static_cast<const char*>(a.k) + static_cast<int64_t>(kv_head) * size;
+  const char* vc = static_cast<const char*>(a.v) + static_cast<int64_t>(kv_head) * size;
   const float scale = a.q_sign ? -a.scale : a.scale;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0);
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int32_t v0 = 0; v0 < n; v0 += kWave) {
     const bool in = v0 + lane < n;
     const int32_t j = key_at(it, in ? v0 + lane : n - 1);
-    const int64_t at = row_of(a, place_of(a, it, j)) * width;
+    const int64_t at = row_of(a, place_of(a, it, j)) * row_bytes;
     const bool seen = in && sees(a, position, j);
     float s = -INFINITY;
     if (seen) {
       float dot = 0.f;
-      for (int32_t i = 0; i < d; ++i) dot = fmaf(to_float(q[i]), to_float(kc[at + i]), dot);
+      for (int32_t i = 0; i < d; ++i) dot = fmaf(to_float(q[i]), cached<T, C>(kc + at, d, i), dot);
       s = dot * scale;
     }
     // A score that is NaN stays in the sum, and the row is NaN as it has to be.
@@ -283,8 +281,8 @@ __device__ void attend_row(const Args& a, const Item& it, int32_t kv_head, int32
       left &= left - 1;
       const float pi = __shfl(p, i);
       const int64_t ai = __shfl(at, i);
-      if (lane < d) o0 = fmaf(pi, to_float(vc[ai + lane]), o0);
-      if (lane + kWave < d) o1 = fmaf(pi, to_float(vc[ai + lane + kWave]), o1);
+      if (lane < d) o0 = fmaf(pi, cached<T, C>(vc + ai, d, lane), o0);
+      if (lane + kWave < d) o1 = fmaf(pi, cached<T, C>(vc + ai, d, lane + kWave), o1);
     }
   }
   if (it.slot >= 0) {
@@ -333,20 +331,21 @@ template <typename T, typename C, int DP>
 struct Narrow {
   static constexpr int EK = sizeof(T) == 4 ? 4 : 8;       // K elements a lane feeds at a time
   // and brings at a time: 16 bytes, so that the four lanes of a key read 64 bytes on end
-  static constexpr int EL = 16 / int(sizeof(C)) * 4 <= DP ? 16 / int(sizeof(C)) : DP / 4;
+  static constexpr int EL = 128 / kBits<C> * 4 <= DP ? 128 / kBits<C> : DP / 4;
   static constexpr int NL = (DP + 4 * EL - 1) / (4 * EL), MF = EL / EK, NK = NL * MF;
   static constexpr int EV = DP <= 32 ? 2 : DP <= 64 ? 4 : 8;
-  static constexpr int KT = sizeof(C) == 4 ? 2 : 4;       // key tiles of 16 in a step
+  static constexpr int KT = kBits<C> == 32 ? 2 : 4;       // key tiles of 16 in a step
   static constexpr int KS = 16 * KT;
   static constexpr float LIFT = lift<T>(14.f);
-  using RawK = Words<EL * int(sizeof(C)) / 4>;
-  using RawV = Words<(EV * int(sizeof(C)) + 3) / 4>;
+  using RawK = Words<EL * kBits<C> / 32>;
+  using RawV = Words<(EV * kBits<C> / 8 + 3) / 4>;
   static constexpr int LDO = DP + 4;                      // floats of a row of o in LDS
   struct Lds {
     alignas(16) uint32_t rows[kWaves][2][KS];
     float2 ml[kWaves][16];
     alignas(16) float o[kWaves][16][LDO];
     int32_t redo[kWaves];
+    alignas(16) uint32_t scales[kScaled<C> ? kWaves : 1][KS];   // of the step's V
   };
 };
 
@@ -364,9 +363,16 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
   const int32_t kv_head = kv_head0 + wave % together, turn = wave / together;
   const int32_t d = a.head_dim, rows = it.tokens * heads;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
-  const int64_t width = static_cast<int64_t>(a.kv_heads) * d;
+  const int32_t size = head_bytes<C>(d);
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * size;
   if (threadIdx.x < kWaves) lds.redo[threadIdx.x] = 0;
 
+  // The first dimension that the lane brings at load i. Of microscaled caches a load that would
+  // end behind the head begins sooner, and Q is zero where it repeats what another lane brings.
+  const auto begin = [&](int i) {
+    const int32_t d0 = (4 * i + g) * EL;
+    return !kScaled<C> || d0 + EL <= d ? d0 : d0 < d ? d - EL : 0;
+  };
   // Q^T: row c, zeros past the rows and past the dimensions.
   Words<4> q[NK];
   int32_t position;
@@ -377,16 +383,16 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int32_t d0 = (4 * (i / MF) + g) * EL + i % MF * EK;
-      const bool in = c < rows && d0 < d;
+      const int32_t d0 = begin(i / MF) + i % MF * EK;
+      const bool in = c < rows && d0 < d && (!kScaled<C> || d0 >= (4 * (i / MF) + g) * EL);
       q[i] = load_bytes<EK * sizeof(T)>(at + (d0 < d ? d0 : 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i].w[e] = (q[i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
     }
   }
-  const C* kc = static_cast<const C*>(a.k) + static_cast<int64_t>(kv_head) * d;
-  const C* vc = static_cast<const C*>(a.v) + static_cast<int64_t>(kv_head) * d +
-                (c * EV < d ? c * EV : 0);
+  const char* kc = static_cast<const char*>(a.k) + static_cast<int64_t>(kv_head) * size;
+  const char* vh = static_cast<const char*>(a.v) + static_cast<int64_t>(kv_head) * size;
+  const char* vc = vh + code_bytes<C>(c * EV < d ? c * EV : 0);
 
   const auto place = [&](int32_t s) {
     const int32_t v = s * KS + lane % KS;
@@ -398,27 +404,35 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     __builtin_amdgcn_wave_barrier();
   };
   typename N::RawK k[KT][NL];
+  uint32_t k_scales[kScaled<C> ? KT : 1];
   const auto load_k = [&](int half) {
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       const uint32_t row =
           lds.rows[wave][half][t / 2 * 32 + (c >> 2) * 8 + t % 2 * 4 + (c & 3)];
-      const C* at = kc + row * width;
+      const char* at = kc + row * row_bytes;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int32_t d0 = (4 * i + g) * EL;
+        const int32_t d0 = begin(i);
         // 16 elements past the head's end would be past the cache's at its last row.
         const int32_t from = d0 >= d ? 0 : EL == 16 && d0 + 8 == d ? d0 - 8 : d0;
-        k[t][i] = stream_bytes<EL * sizeof(C)>(at + from);
+        k[t][i] = stream_bytes<code_bytes<C>(EL)>(at + code_bytes<C>(from));
       }
+      if constexpr (kScaled<C>) k_scales[t] = load_bytes<kScaleBytes>(at + code_bytes<C>(d)).w[0];
     }
   };
 
   // The elements of feed `e` of a load; zeros past the head's dimensions. Not where they are
   // loaded, or they would be waited for there.
-  constexpr int KW = EK * int(sizeof(C)) / 4;
+  constexpr int KW = (EK * kBits<C> / 8 + 3) / 4;
   const auto feed = [&](const typename N::RawK& x, int i, int e) {
     Words<KW> r;
+    if constexpr (kScaled<C>) {
+#pragma unroll
+      for (int w = 0; w < KW; ++w) r.w[w] = x.w[e * EK * kBits<C> / 32 + w];
+      if (EK * kBits<C> < 32) r.w[0] >>= e * EK * kBits<C> % 32;
+      return r;
+    }
     const int32_t d0 = (4 * i + g) * EL + e * EK;
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
@@ -446,13 +460,17 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
   }
   for (int32_t s = turn; s < steps; s += turns, half ^= 1) {
     keep(half ^ 1, next);
+    uint32_t v_scales = 0;                      // of the key that is the lane's in `rows`
+    if constexpr (kScaled<C>)
+      v_scales = load_bytes<kScaleBytes>(vh + lds.rows[wave][half][lane % KS] * row_bytes +
+                                         code_bytes<C>(d)).w[0];
     typename N::RawV v[KT / 2][8];
 #pragma unroll
     for (int p = 0; p < KT / 2; ++p)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t row = lds.rows[wave][half][p * 32 + g * 8 + e];
-        v[p][e] = stream_bytes<EV * sizeof(C)>(vc + row * width);
+        v[p][e] = stream_bytes<code_bytes<C>(EV)>(vc + row * row_bytes);
       }
     __builtin_amdgcn_sched_barrier(0);          // no wait for K's before V's are on their way
     f32x4 sc[KT];
@@ -460,14 +478,34 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     for (int t = 0; t < KT; ++t) {
       sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < NK; ++i)
-        sc[t] = mma16(Convert<T, C, EK>::of(feed(k[t][i / MF], i / MF, i % MF)), q[i], sc[t], T{});
+      for (int i = 0; i < NK; ++i) {
+        const auto raw = feed(k[t][i / MF], i / MF, i % MF);
+        if constexpr (kScaled<C>)
+          sc[t] = mma16(scaled<T, C, EK>(raw, scale_of(k_scales[t], (begin(i / MF) + i % MF * EK) /
+                                                                        kGroup * 8)),
+                        q[i], sc[t], T{});
+        else
+          sc[t] = mma16(Convert<T, C, EK>::of(raw), q[i], sc[t], T{});
+      }
     }
     // In this order: loads return in theirs, and the block's id is what is needed first. Past
     // the last step these read the last key: a branch would make the next wait one for all.
     next = place(s + 2 * turns);
     load_k(half ^ 1);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kScaled<C>) {
+      if (lane < KS) lds.scales[wave][lane] = v_scales;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    // V of key `e` of the lane's eight of pair `p`.
+    const auto v_of = [&](int p, int e) {
+      if constexpr (kScaled<C>)
+        return scaled<T, C, EV>(v[p][e], scale_of(lds.scales[wave][p * 32 + g * 8 + e],
+                                                  c * EV / kGroup * 8));
+      else
+        return Convert<T, C, EV>::of(v[p][e]);
+    };
 
     const int32_t v0 = s * KS;
     if (v0 + KS > n || !all_see(a, it, v0, v0 + KS)) {
@@ -511,7 +549,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
       if constexpr (sizeof(T) == 4) {
         Words<EV> x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = Convert<T, C, EV>::of(v[pr][e]);
+        for (int e = 0; e < 8; ++e) x[e] = v_of(pr, e);
 #pragma unroll
         for (int t = 0; t < EV; ++t)
 #pragma unroll
@@ -521,7 +559,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
       } else {
         Words<EV / 2> x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = Convert<T, C, EV>::of(v[pr][e]);
+        for (int e = 0; e < 8; ++e) x[e] = v_of(pr, e);
         Words<4> w, rest;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -708,18 +746,20 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     }
   }
 
-  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * d * sizeof(C);
-  const char* kc = static_cast<const char*>(a.k) + static_cast<int64_t>(kv_head) * d * sizeof(C);
-  const char* vc = static_cast<const char*>(a.v) + static_cast<int64_t>(kv_head) * d * sizeof(C);
+  const int32_t size = head_bytes<C>(d);
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * size;
+  const char* kc = static_cast<const char*>(a.k) + static_cast<int64_t>(kv_head) * size;
+  const char* vc = static_cast<const char*>(a.v) + static_cast<int64_t>(kv_head) * size;
   const auto place = [&](int32_t s) {
     const int32_t v = s * KS + lane;
     return place_of(a, it, key_at(it, v < n ? v : n - 1));
   };
   // The thread's chunks of a tile. Chunks past the head's dimensions hold its first ones: Q is
   // zero there, and nothing of V there is written.
-  using Raw = Words<8 * int(sizeof(C)) / 4>;
+  using Raw = Words<8 * kBits<C> / 32>;
   struct Staged {
     Raw k[LOADS], v[LOADS];
+    uint8_t k_scale[LOADS], v_scale[LOADS];      // of microscaled caches
   };
   const auto load = [&](int64_t (&row)[KS], typename W::Tile& kt, typename W::Tile& vt, Staged& x) {
 #pragma unroll
@@ -727,15 +767,19 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
       const int32_t at = threadIdx.x + i * kThreads, key = at / CHUNKS, to = at % CHUNKS;
       const int32_t dk = W::place_k(key, to) * 8, dv = W::place_v(key, to) * 8;
       const int64_t from = row[key];
-      const char* ks = kc + from + (dk < d ? dk : 0) * sizeof(C);
-      const char* vs = vc + from + (dv < d ? dv : 0) * sizeof(C);
+      const char* ks = kc + from + code_bytes<C>(dk < d ? dk : 0);
+      const char* vs = vc + from + code_bytes<C>(dv < d ? dv : 0);
       if constexpr (DIRECT) {
         const int32_t first = wave * kWave + i * kThreads;       // lane l's goes l places on
         bring16(ks, &kt[first]);
         bring16(vs, &vt[first]);
       } else {
-        x.k[i] = load_bytes<8 * sizeof(C)>(ks);
-        x.v[i] = load_bytes<8 * sizeof(C)>(vs);
+        x.k[i] = load_bytes<code_bytes<C>(8)>(ks);
+        x.v[i] = load_bytes<code_bytes<C>(8)>(vs);
+        if constexpr (kScaled<C>) {
+          x.k_scale[i] = kc[from + code_bytes<C>(d) + (dk < d ? dk : 0) / kGroup];
+          x.v_scale[i] = vc[from + code_bytes<C>(d) + (dv < d ? dv : 0) / kGroup];
+        }
       }
     }
   };
@@ -744,8 +788,13 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int32_t at = threadIdx.x + i * kThreads;
-        kt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.k[i]));
-        vt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.v[i]));
+        if constexpr (kScaled<C>) {
+          kt[at] = __builtin_bit_cast(u32x4, scaled<T, C, 8>(x.k[i], scale_of(x.k_scale[i], 0)));
+          vt[at] = __builtin_bit_cast(u32x4, scaled<T, C, 8>(x.v[i], scale_of(x.v_scale[i], 0)));
+        } else {
+          kt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.k[i]));
+          vt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.v[i]));
+        }
       }
     }
   };

@@ -1,0 +1,317 @@
+// Writing rows into a microscaled cache and reading them back (C-ABI in iekv_ops.h, the format
+// in microscaled.h).
+#include "microscaled.h"
+
+#include <algorithm>
+
+namespace iekv_ops {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kEach = 8;                       // dimensions a lane takes
+constexpr int kLanes = kGroup / kEach;         // lanes of a group
+
+struct Fp8Limits {
+  static constexpr int kPower = 8;             // the largest element is 1.75 2^8,
+  static constexpr uint32_t kPart = 0x600000;  // its part after the leading one in 23 bits
+};
+struct Int8Limits {
+  static constexpr int kPower = 6;
+  static constexpr uint32_t kPart = 0x7e0000;  // 127 = 1.984375 2^6
+};
+struct Fp4Limits {
+  static constexpr int kPower = 2;
+  static constexpr uint32_t kPart = 0x400000;  // 6 = 1.5 2^2
+};
+template <typename C>
+using Limits = std::conditional_t<std::is_same_v<C, Mxfp8>, Fp8Limits,
+                                  std::conditional_t<std::is_same_v<C, Mxint8>, Int8Limits,
+                                                     Fp4Limits>>;
+
+// e + 127 of a group whose largest magnitude has these bits: its own exponent less the largest
+// element's, and one more where its part is the larger (the sum carries into the exponent).
+template <typename C>
+__device__ __forceinline__ uint32_t exponent_byte(uint32_t largest) {
+  if (largest >= 0x7f800000u) return 255;      // an infinity or a NaN
+  const int32_t e = static_cast<int32_t>((largest + (0x7fffffu - Limits<C>::kPart)) >> 23) -
+                    Limits<C>::kPower;
+  return max(e, kLeastExponent + 127);
+}
+
+// Eight elements as codes.
+template <typename C>
+__device__ __forceinline__ Words<kEach * kBits<C> / 32> encode(const float (&x)[kEach],
+                                                                uint32_t byte) {
+  Words<kEach * kBits<C> / 32> r{};
+  if (byte == 255) return r;
+  if constexpr (std::is_same_v<C, Mxint8>) {
+    const float inverse = __builtin_bit_cast(float, (254 - byte) << 23);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int32_t c = static_cast<int32_t>(rintf(x[i] * inverse));
+      r.w[i / 4] |= (static_cast<uint32_t>(c) & 255u) << i % 4 * 8;
+    }
+  } else if constexpr (std::is_same_v<C, Mxfp8>) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const float scale = __builtin_bit_cast(float, byte << 23);
+#pragma unroll
+    for (int i = 0; i < kEach / 4; ++i) {
+      s16x2 w{};
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[4 * i], x[4 * i + 1], scale, false);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[4 * i + 2], x[4 * i + 3], scale, true);
+      r.w[i] = __builtin_bit_cast(uint32_t, w);
+    }
+  } else {
+    const float scale = __builtin_bit_cast(float, byte << 23);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+    r.w[0] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
+  }
+  return r;
+}
+
+struct WriteArgs {
+  uint64_t k_cache, v_cache;                   // of the first layer
+  int64_t k_cache_stride, v_cache_stride;      // bytes from one layer's to the next
+  const void* k;
+  const void* v;
+  int64_t k_layer, k_token, k_head, v_layer, v_token, v_head;   // strides in elements
+  const int64_t* slots;
+  int64_t n_slots;
+  uint32_t n;                                  // tokens
+  int32_t heads, head_dim, lanes;              // lanes: of a head, a multiple of kLanes
+};
+
+// Bound by memory: a lane brings eight dimensions of K and of V of one token's head, the four
+// lanes of a group find its largest magnitude, and each writes its codes.
+template <typename T, typename C>
+__global__ __launch_bounds__(kThreads) void write_rows(WriteArgs a) {
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint32_t row_lanes = a.heads * a.lanes;
+  const uint32_t t = static_cast<uint32_t>(at / row_lanes), in_row = at % row_lanes;
+  if (t >= a.n) return;                        // whole groups of lanes: the rest of a group too
+  const uint32_t head = in_row / a.lanes, lane = in_row % a.lanes;
+  const int32_t d0 = lane * kEach, layer = blockIdx.y;
+  const bool in = d0 < a.head_dim;
+  float x[2][kEach];
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+    const T* from = static_cast<const T*>(o ? a.v : a.k) +
+                    layer * (o ? a.v_layer : a.k_layer) + t * (o ? a.v_token : a.k_token) +
+                    head * (o ? a.v_head : a.k_head);
+    T raw[kEach];
+    __builtin_memcpy(raw, from + (in ? d0 : 0), sizeof(raw));
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[o][i] = in ? to_float(raw[i]) : 0.f;
+  }
+  const int64_t slot = a.slots[t];
+  const int32_t codes = code_bytes<C>(a.head_dim), record = head_bytes<C>(a.head_dim);
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+    // Magnitudes as integers: a NaN is the largest of all.
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      largest = max(largest, __builtin_bit_cast(uint32_t, x[o][i]) & 0x7fffffffu);
+    largest = max(largest, lane_xor<1>(largest));
+    largest = max(largest, lane_xor<2>(largest));
+    const uint32_t byte = exponent_byte<C>(largest);
+    const auto code = encode<C>(x[o], byte);
+    if (static_cast<uint64_t>(slot) >= static_cast<uint64_t>(a.n_slots)) continue;
+    char* to = reinterpret_cast<char*>((o ? a.v_cache : a.k_cache) +
+                                       layer * (o ? a.v_cache_stride : a.k_cache_stride)) +
+               (slot * a.heads + head) * record;
+    if (in) __builtin_memcpy(to + code_bytes<C>(d0), &code, sizeof(code));
+    if (lane % kLanes == 0) to[codes + lane / kLanes] = static_cast<char>(byte);
+    // Bytes past the last group.
+    if (lane == 0)
+      for (int32_t g = a.lanes / kLanes; g < kScaleBytes; ++g) to[codes + g] = 0;
+  }
+}
+
+struct ReadArgs {
+  uint64_t cache;                              // the first array
+  int64_t cache_stride;
+  void* out;                                   // [arrays][n][heads][head_dim]
+  const int32_t* table;
+  uint32_t n;                                  // rows
+  int32_t heads, head_dim, lanes;              // lanes: of a head
+  int32_t block_size;
+  int64_t num_blocks;
+};
+
+// Bound by memory: a lane turns eight dimensions into values.
+template <typename T, typename C>
+__global__ __launch_bounds__(kThreads) void read_rows(ReadArgs a) {
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const uint32_t row_lanes = a.heads * a.lanes;
+  const uint32_t j = static_cast<uint32_t>(at / row_lanes), in_row = at % row_lanes;
+  if (j >= a.n) return;
+  const uint32_t head = in_row / a.lanes;
+  const int32_t d0 = in_row % a.lanes * kEach, array = blockIdx.y;
+  const int32_t block = a.table[j / a.block_size];
+  if (block < 0 || block >= a.num_blocks) return;
+  const int64_t row = static_cast<int64_t>(block) * a.block_size + j % a.block_size;
+  const char* from = reinterpret_cast<const char*>(a.cache + array * a.cache_stride) +
+                     (row * a.heads + head) * head_bytes<C>(a.head_dim);
+  Words<kEach * kBits<C> / 32> code;
+  __builtin_memcpy(&code, from + code_bytes<C>(d0), sizeof(code));
+  uint32_t scales;
+  __builtin_memcpy(&scales, from + code_bytes<C>(a.head_dim), sizeof(scales));
+  const auto value = scaled<T, C, kEach>(code, scale_of(scales, d0 / kGroup * 8));
+  T* to = static_cast<T*>(a.out) +
+          ((static_cast<int64_t>(array) * a.n + j) * a.heads + head) * a.head_dim + d0;
+  __builtin_memcpy(to, &value, sizeof(value));
+}
+
+int check_cache(const iekv_mx_cache* c) {
+  if (!c) return set_error(IEKV_ERR_INVALID, "cache is null");
+  if (c->cache_type < IEKV_TYPE_MXFP8 || c->cache_type > IEKV_TYPE_MXFP4)
+    return set_error(IEKV_ERR_INVALID, "%d is no microscaled type", c->cache_type);
+  if (c->num_kv_heads < 1 || c->num_kv_heads > 4096)
+    return set_error(IEKV_ERR_INVALID, "num_kv_heads %d out of range", c->num_kv_heads);
+  if (c->head_dim < 8 || c->head_dim > IEKV_ATTENTION_MAX_DIM || c->head_dim % 8)
+    return set_error(IEKV_ERR_INVALID, "head_dim %d is not a multiple of 8 up to %d", c->head_dim,
+                     IEKV_ATTENTION_MAX_DIM);
+  if (c->block_size < 1 || c->block_size > (1 << 20))
+    return set_error(IEKV_ERR_INVALID, "block_size %d out of range", c->block_size);
+  if (c->num_blocks < 1 || c->num_blocks > INT32_MAX)
+    return set_error(IEKV_ERR_INVALID, "num_blocks %lld out of range",
+                     static_cast<long long>(c->num_blocks));
+  return IEKV_OK;
+}
+
+bool is_float(int32_t type) { return type >= IEKV_TYPE_F32 && type <= IEKV_TYPE_BF16; }
+
+// How many of the arrays from `first` on lie at even distances, and that distance: all of a
+// pool's that one allocation holds, two at least of others.
+int32_t run_of(const uint64_t* arrays, int32_t first, int32_t n, int64_t* stride) {
+  *stride = first + 1 < n ? static_cast<int64_t>(arrays[first + 1] - arrays[first]) : 0;
+  int32_t last = first;
+  while (last + 1 < n && static_cast<int64_t>(arrays[last + 1] - arrays[last]) == *stride) ++last;
+  return last - first + 1;
+}
+
+// Calls f with a row type and a cache type.
+template <typename F>
+void with_types(int32_t row, int32_t cache, F f) {
+  const auto with_cache = [&](auto t) {
+    switch (cache) {
+      case IEKV_TYPE_MXFP8: return f(t, Mxfp8{});
+      case IEKV_TYPE_MXINT8: return f(t, Mxint8{});
+      default: return f(t, Mxfp4{});
+    }
+  };
+  switch (row) {
+    case IEKV_TYPE_F32: return with_cache(float{});
+    case IEKV_TYPE_F16: return with_cache(_Float16{});
+    default: return with_cache(Bf16{});
+  }
+}
+
+constexpr int32_t kMostLayers = 65535;         // of a launch: its grid's second dimension
+
+}  // namespace
+}  // namespace iekv_ops
+
+using namespace iekv_ops;
+
+extern "C" {
+
+int64_t iekv_mx_head_bytes(int32_t cache_type, int32_t head_dim) {
+  if (cache_type < IEKV_TYPE_MXFP8 || cache_type > IEKV_TYPE_MXFP4 || head_dim < 8 ||
+      head_dim > IEKV_ATTENTION_MAX_DIM || head_dim % 8)
+    return 0;
+  return cache_type == IEKV_TYPE_MXFP4 ? head_bytes<Mxfp4>(head_dim) : head_bytes<Mxfp8>(head_dim);
+}
+
+int iekv_mx_write_slots(const iekv_mx_cache* cache, const uint64_t* k_arrays,
+                        const uint64_t* v_arrays, int32_t n_layers, int32_t row_type,
+                        const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
+                        hipStream_t stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (!is_float(row_type)) return set_error(IEKV_ERR_INVALID, "rows of type %d", row_type);
+  if (n_layers < 0 || n_tokens < 0)
+    return set_error(IEKV_ERR_INVALID, "%d layers of %lld tokens", n_layers,
+                     static_cast<long long>(n_tokens));
+  if (!n_layers || !n_tokens) return IEKV_OK;
+  if (!k_arrays || !v_arrays || !k || !k_strides || !v || !v_strides || !slots)
+    return set_error(IEKV_ERR_INVALID, "null argument");
+  const int64_t size = row_type == IEKV_TYPE_F32 ? 4 : 2;
+  const int32_t lanes = (cache->head_dim + kGroup - 1) / kGroup * kLanes;
+  const int64_t most = kMaxGrid * kThreads / (cache->num_kv_heads * lanes);  // tokens of a launch
+  for (int32_t l = 0; l < n_layers;) {
+    WriteArgs a{};
+    const int32_t run = std::min(std::min(run_of(k_arrays, l, n_layers, &a.k_cache_stride),
+                                          run_of(v_arrays, l, n_layers, &a.v_cache_stride)),
+                                 kMostLayers);
+    for (int64_t t = 0; t < n_tokens; t += most) {
+      a.k_cache = k_arrays[l];
+      a.v_cache = v_arrays[l];
+      a.k_layer = k_strides[0], a.k_token = k_strides[1], a.k_head = k_strides[2];
+      a.v_layer = v_strides[0], a.v_token = v_strides[1], a.v_head = v_strides[2];
+      a.k = static_cast<const char*>(k) + (l * a.k_layer + t * a.k_token) * size;
+      a.v = static_cast<const char*>(v) + (l * a.v_layer + t * a.v_token) * size;
+      a.slots = slots + t;
+      a.n_slots = cache->num_blocks * cache->block_size;
+      a.n = static_cast<uint32_t>(std::min(most, n_tokens - t));
+      a.heads = cache->num_kv_heads;
+      a.head_dim = cache->head_dim;
+      a.lanes = lanes;
+      const int64_t threads = static_cast<int64_t>(a.n) * a.heads * lanes;
+      const dim3 grid((threads + kThreads - 1) / kThreads, run);
+      with_types(row_type, cache->cache_type, [&](auto row, auto code) {
+        hipLaunchKernelGGL((write_rows<decltype(row), decltype(code)>), grid, dim3(kThreads), 0,
+                           stream, a);
+      });
+      IEKV_OPS_HIP(hipGetLastError());
+    }
+    l += run;
+  }
+  return IEKV_OK;
+}
+
+int iekv_mx_read_rows(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
+                      const int32_t* table, int64_t context_len, int32_t out_type, void* out,
+                      hipStream_t stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (!is_float(out_type)) return set_error(IEKV_ERR_INVALID, "values of type %d", out_type);
+  if (n_arrays < 0 || context_len < 0 || context_len > IEKV_ATTENTION_MAX_CONTEXT)
+    return set_error(IEKV_ERR_INVALID, "%d arrays of a context of %lld", n_arrays,
+                     static_cast<long long>(context_len));
+  if (!n_arrays || !context_len) return IEKV_OK;
+  if (!arrays || !table || !out) return set_error(IEKV_ERR_INVALID, "null argument");
+  const int64_t size = out_type == IEKV_TYPE_F32 ? 4 : 2;
+  const int32_t lanes = cache->head_dim / kEach;
+  for (int32_t i = 0; i < n_arrays;) {
+    ReadArgs a{};
+    const int32_t run = std::min(run_of(arrays, i, n_arrays, &a.cache_stride), kMostLayers);
+    a.cache = arrays[i];
+    a.out = static_cast<char*>(out) +
+            i * context_len * cache->num_kv_heads * cache->head_dim * size;
+    a.table = table;
+    a.n = static_cast<uint32_t>(context_len);
+    a.heads = cache->num_kv_heads;
+    a.head_dim = cache->head_dim;
+    a.lanes = lanes;
+    a.block_size = cache->block_size;
+    a.num_blocks = cache->num_blocks;
+    const int64_t threads = context_len * a.heads * lanes;
+    if ((threads + kThreads - 1) / kThreads > kMaxGrid)
+      return set_error(IEKV_ERR_INVALID, "a context of %lld rows of %d heads is too long",
+                       static_cast<long long>(context_len), a.heads);
+    const dim3 grid((threads + kThreads - 1) / kThreads, run);
+    with_types(out_type, cache->cache_type, [&](auto value, auto code) {
+      hipLaunchKernelGGL((read_rows<decltype(value), decltype(code)>), grid, dim3(kThreads), 0,
+                         stream, a);
+    });
+    IEKV_OPS_HIP(hipGetLastError());
+    i += run;
+  }
+  return IEKV_OK;
+}
+
+}  // extern "C"

@@ -1,5 +1,5 @@
-"""ctypes binding of libiekv_ops.so: attention over the paged cache and the scoring of
-answers (C-ABI in include/iekv_ops.h).
+"""ctypes binding of libiekv_ops.so: attention over the paged cache, caches in microscaled
+formats and the scoring of answers (C-ABI in include/iekv_ops.h).
 
 Loaded like the handoff library (:mod:`iekv._native`): after torch, with no fallback, and
 with the same kinds of exception for the same status codes.
@@ -14,7 +14,10 @@ from pathlib import Path
 from . import _native
 
 LIBRARY = Path(__file__).resolve().parent / "libiekv_ops.so"
-ABI_VERSION = 1
+ABI_VERSION = 2
+
+# Element types of caches beside IEKV_TYPE_* (microscaled).
+IEKV_TYPE_MXFP8, IEKV_TYPE_MXINT8, IEKV_TYPE_MXFP4 = 5, 6, 7
 
 ATTENTION_MAX_DIM = 128              # IEKV_ATTENTION_MAX_DIM
 ATTENTION_MAX_GROUP = 128            # IEKV_ATTENTION_MAX_GROUP
@@ -31,6 +34,13 @@ class AttentionShape(ctypes.Structure):
                 ("shared_blocks", c_int64)]
 
 
+class MxCache(ctypes.Structure):
+    """iekv_mx_cache."""
+
+    _fields_ = [("cache_type", c_int32), ("num_kv_heads", c_int32), ("head_dim", c_int32),
+                ("block_size", c_int32), ("num_blocks", c_int64)]
+
+
 # Every entry point of include/iekv_ops.h: name -> (restype, argtypes).
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "iekv_ops_abi_version": (c_int, []),
@@ -42,6 +52,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                          POINTER(c_int64), POINTER(c_int64)]),
     "iekv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                             c_float, c_void_p, c_void_p, c_int64, c_void_p]),
+    "iekv_mx_head_bytes": (c_int64, [c_int32, c_int32]),
+    "iekv_mx_write_slots": (c_int, [POINTER(MxCache), c_void_p, c_void_p, c_int32, c_int32,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                    c_void_p]),
+    "iekv_mx_read_rows": (c_int, [POINTER(MxCache), c_void_p, c_int32, c_void_p, c_int64, c_int32,
+                                  c_void_p, c_void_p]),
     "iekv_logprobs_workspace": (c_int64, [c_int32, c_int64, c_int64, c_int32]),
     "iekv_logprobs": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,

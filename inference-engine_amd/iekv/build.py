@@ -2,8 +2,9 @@
 
 The libraries are compiled with hipcc straight from ``csrc/`` into ``iekv/`` next to
 this file, so they travel with the source tree and are the files ``iekv._native`` (the
-handoff, from ``csrc/kv_handoff.hip``) and ``iekv._ops`` (attention and scoring, from
-``csrc/attention.hip`` and ``csrc/logprobs.hip``) load. Run ``python -m iekv.build`` (with
+handoff, from ``csrc/kv_handoff.hip``) and ``iekv._ops`` (attention, scoring and
+microscaled caches, from ``csrc/attention.hip``, ``csrc/logprobs.hip`` and
+``csrc/microscaled.hip``) load. Run ``python -m iekv.build`` (with
 ``inference-engine_amd`` on ``sys.path``) or call :func:`build`.
 """
 from __future__ import annotations
@@ -21,7 +22,7 @@ INCLUDE_DIR = REPO_ROOT / "include"
 LIBRARY = PACKAGE_DIR / "libiekv.so"
 SOURCES = [SOURCE_DIR / "kv_handoff.hip"]
 OPS_LIBRARY = PACKAGE_DIR / "libiekv_ops.so"
-OPS_SOURCES = [SOURCE_DIR / "attention.hip", SOURCE_DIR / "logprobs.hip"]
+OPS_SOURCES = [SOURCE_DIR / name for name in ("attention.hip", "logprobs.hip", "microscaled.hip")]
 ARCH = "gfx950"
 
 

@@ -31,6 +31,7 @@ import torch
 
 from .. import _native, _ops
 from .pools import KVPool, current_stream_handle, integer_ids, refuse_derivatives
+from .quantized import FORMATS, QuantizedPool
 
 _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
           torch.bfloat16: _native.IEKV_TYPE_BF16, torch.float8_e4m3fn: _native.IEKV_TYPE_E4M3}
@@ -81,8 +82,10 @@ class AttentionPlan:
     ``block_tables`` (host lists or arrays; entries past a context are not read),
     ``context_lens`` and ``query_lens`` are the step's, per sequence; a sequence without
     queries takes no part. ``query_dtype`` is the queries' type: float32 on any cache,
-    float16 or bfloat16 on a cache of the same type or float8_e4m3fn (default: the cache's
-    type, bfloat16 on an fp8 cache). IndexError for a block outside the pool or a table
+    float16 or bfloat16 on a cache of the same type, float8_e4m3fn or a quantised pool
+    (default: the cache's type, bfloat16 on an fp8 cache and a quantised pool). A quantised
+    pool's values are taken as :func:`~iekv.engine.slots.gather_rows` reads them back in the
+    queries' type. IndexError for a block outside the pool or a table
     too short for its context, ValueError for tables that do not begin with the shared
     blocks and for arguments out of range.
 
@@ -102,9 +105,11 @@ class AttentionPlan:
                              f"of {pool.tile_shape}")
         if window is not None and window < 1:
             raise ValueError(f"window {window} must be at least 1 (None for no window)")
+        quantized = isinstance(pool, QuantizedPool)
         if query_dtype is None:
-            query_dtype = torch.bfloat16 if pool.dtype == torch.float8_e4m3fn else pool.dtype
-        if query_dtype not in _TYPES or pool.dtype not in _TYPES:
+            query_dtype = torch.bfloat16 if quantized or pool.dtype == torch.float8_e4m3fn \
+                else pool.dtype
+        if query_dtype not in _TYPES or not quantized and pool.dtype not in _TYPES:
             raise ValueError(f"attention of {query_dtype} queries on a {pool.dtype} cache")
         if not len(block_tables) == len(context_lens) == len(query_lens):
             raise ValueError(f"{len(block_tables)} block tables for {len(context_lens)} contexts "
@@ -112,9 +117,13 @@ class AttentionPlan:
         contexts = _lengths(context_lens, "context lengths")
         queries = _lengths(query_lens, "query lengths")
         flat, starts = _flat_tables(block_tables, contexts, pool.block_size)
-        _, kv_heads, dim = pool.tile_shape
+        if quantized:
+            kv_heads, dim, cache_type = pool.num_kv_heads, pool.head_dim, FORMATS[pool.format]
+        else:
+            _, kv_heads, dim = pool.tile_shape
+            cache_type = _TYPES[pool.dtype]
         shape = _ops.AttentionShape(num_heads, kv_heads, dim, pool.block_size, pool.num_blocks,
-                                    _TYPES[query_dtype], _TYPES[pool.dtype],
+                                    _TYPES[query_dtype], cache_type,
                                     min(window or 0, 1 << 40), min(sinks, 1 << 40),
                                     shared_blocks)
         with torch.cuda.device(pool.device):

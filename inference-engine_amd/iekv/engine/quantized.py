@@ -1,0 +1,218 @@
+"""KV pools in microscaled formats: quantised as they are written, read back as values.
+
+The reference's caches hold the model's type (ie/kernels/reference.py:39-42,
+ie/model/torch_transformer.py:82-86). A :class:`QuantizedPool` holds half of a 16-bit cache's
+bytes, or a quarter: 32 dimensions of a head share a power of two, and an element is what is
+left in 8 or 4 bits, rounded to nearest even.
+
+    ``mxfp8``    e4m3: 3 bits after the leading one, off by 2^-4 of a value at most
+    ``mxint8``   integers up to 127: off by 2^-7 of the group's largest value at most
+    ``mxfp4``    e2m1: 1 bit after the leading one, off by 2^-2 of a value, or a twelfth of the
+                 group's largest
+
+A head's record is its elements and four bytes of exponents, so that a cache is an ordinary
+array ``[num_blocks * block_size, num_kv_heads, record]`` of bytes: the handoff, the offload
+tier and the wire move its blocks as they move any other's.
+
+    k, v = allocate_quantized_pool(num_blocks, 16, layers, kv_heads, head_dim, format="mxfp8")
+    pool = QuantizedPool(k, v, 16, "mxfp8")
+    write_slots(pool, layer, k_rows, v_rows, slots)          # iekv.engine.slots
+    plan = AttentionPlan(pool, tables, contexts, queries, num_heads)
+    out = attend(plan, layer, q)                             # iekv.engine.attention
+    rows = gather_rows(pool, layer, table, context_len, dtype=torch.bfloat16)
+
+Both pools of a handoff have to be of one format: their records may be of the same size in
+another.
+"""
+from __future__ import annotations
+
+import ctypes
+from array import array as _ints
+from typing import Sequence as Seq
+
+import numpy as np
+import torch
+
+from .. import _native, _ops
+from .pools import (KVPool, allocate_pool, allocate_pool_pair, current_device,
+                    current_stream_handle, integer_ids, refuse_derivatives)
+
+FORMATS = {"mxfp8": _ops.IEKV_TYPE_MXFP8, "mxint8": _ops.IEKV_TYPE_MXINT8,
+           "mxfp4": _ops.IEKV_TYPE_MXFP4}
+_CODE_BITS = {"mxfp8": 8, "mxint8": 8, "mxfp4": 4}
+_SCALE_BYTES = 4
+
+_TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
+          torch.bfloat16: _native.IEKV_TYPE_BF16}
+
+
+def record_bytes(format: str, head_dim: int) -> int:
+    """Bytes of one head of one token: its elements and the groups' exponents."""
+    if format not in FORMATS:
+        raise ValueError(f"no format {format!r}: one of {', '.join(FORMATS)}")
+    if not 8 <= head_dim <= _ops.ATTENTION_MAX_DIM or head_dim % 8:
+        raise ValueError(f"head_dim {head_dim} is not a multiple of 8 up to "
+                         f"{_ops.ATTENTION_MAX_DIM}")
+    return head_dim * _CODE_BITS[format] // 8 + _SCALE_BYTES
+
+
+def allocate_quantized_pool(num_blocks: int, block_size: int, num_layers: int,
+                            num_kv_heads: int, head_dim: int, *, format: str,
+                            device: str | torch.device = "cuda", zero: bool = True
+                            ) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
+    """Per-layer K and V caches of records, views of one slab (zero-filled: every value 0)."""
+    return allocate_pool(num_blocks, block_size, num_layers, num_kv_heads,
+                         record_bytes(format, head_dim), dtype=torch.uint8, device=device,
+                         zero=zero)
+
+
+def allocate_quantized_pool_pair(first_blocks: int, second_blocks: int, block_size: int,
+                                 num_layers: int, num_kv_heads: int, head_dim: int, *,
+                                 format: str, device: str | torch.device = "cuda",
+                                 zero: bool = True):
+    """Two such pools in one allocation (:func:`iekv.engine.pools.allocate_pool_pair`)."""
+    return allocate_pool_pair(first_blocks, second_blocks, block_size, num_layers, num_kv_heads,
+                              record_bytes(format, head_dim), dtype=torch.uint8, device=device,
+                              zero=zero)
+
+
+class QuantizedPool(KVPool):
+    """A registered set of per-layer caches whose rows are records of ``format``.
+
+    ``k_caches`` and ``v_caches`` are ``[rows, num_kv_heads, record]`` uint8, as
+    :func:`allocate_quantized_pool` makes them. The slot calls of :mod:`iekv.engine.slots` and
+    the attention of :mod:`iekv.engine.attention` take and return values; the copiers move the
+    records.
+    """
+
+    def __init__(self, k_caches: Seq[torch.Tensor], v_caches: Seq[torch.Tensor],
+                 block_size: int, format: str) -> None:
+        if format not in FORMATS:
+            raise ValueError(f"no format {format!r}: one of {', '.join(FORMATS)}")
+        super().__init__(k_caches, v_caches, block_size)
+        if self.dtype != torch.uint8 or len(self.tile_shape) != 3:
+            raise ValueError(f"caches of records are [rows, KV heads, record] uint8, got tiles of "
+                             f"{self.tile_shape} {self.dtype}")
+        _, heads, record = self.tile_shape
+        head_dim = (record - _SCALE_BYTES) * 8 // _CODE_BITS[format]
+        try:
+            fits = record_bytes(format, head_dim) == record
+        except ValueError:
+            fits = False
+        if not fits:
+            raise ValueError(f"records of {record} bytes are none of {format}: head_dim is a "
+                             f"multiple of 8 up to {_ops.ATTENTION_MAX_DIM}")
+        self.format = format
+        self.num_kv_heads = heads
+        self.head_dim = head_dim
+        self._shape = _ops.MxCache(FORMATS[format], heads, head_dim, block_size, self.num_blocks)
+        self._addresses = (ctypes.c_uint64 * len(self._ptrs))(*self._ptrs)
+        self._at = ctypes.addressof(self._addresses)
+
+    def same_shape(self, other: KVPool) -> bool:
+        return super().same_shape(other) and self.format == getattr(other, "format", self.format)
+
+    def _arrays_from(self, array: int) -> int:
+        """Where the addresses of the arrays from ``array`` on begin."""
+        return self._at + 8 * array
+
+    def _rows(self, t: torch.Tensor, what: str) -> torch.Tensor:
+        """Rows as the library reads them: as they are where their heads are contiguous."""
+        if t.device != self.device:
+            raise ValueError(f"{what} on {t.device}, pool on {self.device}")
+        if t.dtype not in _TYPES:
+            raise ValueError(f"{what} of {t.dtype}: float32, float16 or bfloat16 are quantised")
+        refuse_derivatives(t, "a quantised cache")
+        if t.is_neg():
+            t = t.resolve_neg()
+        return t if t.stride(-1) == 1 else t.contiguous()
+
+    def _slots(self, slots) -> torch.Tensor:
+        """Slots on the device: a device tensor as it is, host ones checked and uploaded."""
+        if isinstance(slots, torch.Tensor) and slots.device.type != "cpu":
+            if slots.device != self.device:
+                raise ValueError(f"slots on {slots.device}, pool on {self.device}")
+            if slots.dim() != 1 or slots.dtype.is_floating_point or slots.dtype.is_complex or \
+                    slots.dtype == torch.bool:
+                raise TypeError(f"slots must be integers in one dimension, got "
+                                f"{tuple(slots.shape)} {slots.dtype}")
+            return slots.to(torch.int64).contiguous()
+        host = integer_ids(slots, "slot")
+        rows = self.num_blocks * self.block_size
+        bad = host[(host < 0) | (host >= rows)]
+        if bad.size:
+            raise IndexError(f"slot {bad[0]} out of range for a pool of {rows} slots")
+        if np.unique(host).size != host.size:
+            raise ValueError("slots must be distinct")
+        return self._upload(host, "slots")
+
+    def _table(self, block_table, context_len: int) -> torch.Tensor:
+        """The entries of a block table that a context uses, on the device."""
+        if context_len < 0:
+            raise ValueError(f"context of {context_len}")
+        needed = -(-context_len // self.block_size)
+        if len(block_table) < needed:
+            raise IndexError(f"context of {context_len} needs {needed} blocks, table has "
+                             f"{len(block_table)}")
+        used = block_table[:needed]
+        if isinstance(used, torch.Tensor) and used.device.type != "cpu":
+            if used.device != self.device:
+                raise ValueError(f"block table on {used.device}, pool on {self.device}")
+            if used.dim() != 1 or used.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"a device block table must be int32 or int64 in one dimension, "
+                                f"got {tuple(used.shape)} {used.dtype}")
+            return used.to(torch.int32).contiguous()
+        return self._upload(self.host_ids(used, what="context block").astype(np.int32),
+                            "a block table")
+
+    def _upload(self, host: np.ndarray, what: str) -> torch.Tensor:
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what} on the host are uploaded, which a stream under "
+                                   "capture cannot do: pass a device tensor")
+            if not host.size:
+                return torch.empty(0, dtype=torch.int64, device=self.device)
+            return torch.from_numpy(np.ascontiguousarray(host)).pin_memory().to(
+                self.device, non_blocking=True)
+
+    def _call(self, function: str, *args) -> None:
+        """Call an entry point with the pool's shape first and its stream last, on its device."""
+        f, stream = _ops.entry(function), current_stream_handle(self.device)
+        shape = ctypes.byref(self._shape)
+        if self.device.index == current_device():
+            code = f(shape, *args, stream)
+        else:
+            with torch.cuda.device(self.device):
+                code = f(shape, *args, stream)
+        if code:
+            _ops.fail(function, code)
+
+
+def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tensor,
+          slots) -> None:
+    """``[n_layers, n, H, D]`` rows into the slots of layers ``first_layer`` and on (the calls
+    of :mod:`iekv.engine.slots` have checked their shapes)."""
+    k, v = pool._rows(k, "K rows"), pool._rows(v, "V rows")
+    if k.dtype != v.dtype:
+        raise ValueError(f"K rows of {k.dtype} and V rows of {v.dtype}")
+    where = pool._slots(slots)
+    n_layers, n = k.shape[:2]
+    strides = (_ints("q", k.stride()[:3]), _ints("q", v.stride()[:3]))
+    pool._call("iekv_mx_write_slots", pool._arrays_from(first_layer),
+               pool._arrays_from(pool.num_layers + first_layer), n_layers, _TYPES[k.dtype],
+               k.data_ptr(), strides[0].buffer_info()[0], v.data_ptr(),
+               strides[1].buffer_info()[0], where.data_ptr(), n)
+
+
+def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, context_len: int,
+         dtype: torch.dtype | None) -> torch.Tensor:
+    """``[n_arrays, context_len, H, D]`` values of a context (default: bfloat16)."""
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype not in _TYPES:
+        raise ValueError(f"values of {dtype}: float32, float16 or bfloat16 are read back")
+    table = pool._table(block_table, context_len)
+    out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim), dtype=dtype,
+                      device=pool.device)
+    pool._call("iekv_mx_read_rows", pool._arrays_from(first_array), n_arrays, table.data_ptr(),
+               context_len, _TYPES[dtype], out.data_ptr())
+    return out

@@ -11,6 +11,9 @@ bytes the handoff moves.
 ``write_slots_layers`` and ``gather_rows_arrays`` do the same for many layers or
 arrays in one launch: a forward pass's KV writes for every layer at once, and
 a sequence's context in every layer's K and V cache at once.
+
+On a :class:`~iekv.engine.quantized.QuantizedPool` all four take and return values: rows are
+quantised on their way into their slots, and a context is read back in the type asked for.
 """
 from __future__ import annotations
 
@@ -20,7 +23,9 @@ import numpy as np
 import torch
 
 from .. import _native
+from . import quantized
 from .pools import KVPool, current_stream_handle
+from .quantized import QuantizedPool
 
 
 # Longest host slot list the library carries in its launches' arguments (IEKV_INLINE_IDS
@@ -116,21 +121,40 @@ def _write(pool: KVPool, first_layer: int, n_layers: int, n: int, k: torch.Tenso
                  current_stream_handle(pool.device))
 
 
+def _row_shape(pool: KVPool) -> tuple[int, ...]:
+    """What a row of the pool holds: its values' shape, where the cache holds records."""
+    if isinstance(pool, QuantizedPool):
+        return pool.num_kv_heads, pool.head_dim
+    return pool.tile_shape[1:]
+
+
+def _cache_dtype_only(pool: KVPool, dtype: torch.dtype | None) -> None:
+    if dtype is not None and dtype != pool.dtype:
+        raise ValueError(f"rows of a {pool.dtype} cache are read as they are, not as {dtype}")
+
+
 def write_slots(pool: KVPool, layer: int, k: torch.Tensor, v: torch.Tensor, slots) -> None:
     """Scatter rows ``k[i]``, ``v[i]`` ([n, H, D]) into slot ``slots[i]`` of ``layer``.
 
     The rows are cast to the cache dtype (as ``index_copy_`` of
     ``k.to(cache dtype)`` does), on their way where the library has the cast;
     slots are range-checked on the host when given as a list.
+
+    Rows for a quantised pool are float32, float16 or bfloat16 on its device, with any strides;
+    host slots given twice raise ValueError there (on the device, any of the rows may be held,
+    or parts of several), and device slots outside the pool are skipped.
     """
     n = k.shape[0]
     if v.shape[0] != n or len(slots) != n:
         raise ValueError(f"{len(slots)} slots for {n} K rows and {v.shape[0]} V rows")
-    if tuple(k.shape[1:]) != pool.tile_shape[1:] or tuple(v.shape[1:]) != pool.tile_shape[1:]:
-        raise ValueError(f"rows of shape {tuple(k.shape[1:])} do not fit a pool of "
-                         f"{pool.tile_shape[1:]}")
+    row = _row_shape(pool)
+    if tuple(k.shape[1:]) != row or tuple(v.shape[1:]) != row:
+        raise ValueError(f"rows of shape {tuple(k.shape[1:])} do not fit a pool of {row}")
     if not 0 <= layer < pool.num_layers:
         raise IndexError(f"layer {layer} out of range for {pool.num_layers} layers")
+    if isinstance(pool, QuantizedPool):
+        quantized.write(pool, layer, k[None], v[None], slots)
+        return
     _write(pool, layer, 1, n, k, v, slots)
 
 
@@ -164,13 +188,22 @@ def _address(table) -> int:
     return table.data_ptr() if isinstance(table, torch.Tensor) else table.buffer_info()[0]
 
 
-def gather_rows(pool: KVPool, array: int, block_table, context_len: int) -> torch.Tensor:
+def gather_rows(pool: KVPool, array: int, block_table, context_len: int, *,
+                dtype: torch.dtype | None = None) -> torch.Tensor:
     """Rows ``0..context_len-1`` of a sequence in array ``array`` (K of layer l is l, V is L+l).
 
     Returns a new ``[context_len, H, D]`` tensor of the cache dtype. Raises
     IndexError when the table is too short for ``context_len`` (as the
     reference does) or holds a block outside the pool.
+
+    A quantised pool's values come in ``dtype`` (float32, float16, bfloat16; default bfloat16),
+    rounded to nearest even. Rows of blocks of a device table outside the pool are left as
+    the memory was.
     """
+    if isinstance(pool, QuantizedPool):
+        _check_arrays(pool, array, 1)
+        return quantized.read(pool, array, 1, block_table, context_len, dtype)[0]
+    _cache_dtype_only(pool, dtype)
     table, fn = _context_table(pool, block_table, context_len)
     out = torch.empty((context_len, *pool.tile_shape[1:]), dtype=pool.dtype, device=pool.device)
     _native.call(fn, pool.native.handle, array, 1, pool.block_size, _address(table),
@@ -189,24 +222,36 @@ def write_slots_layers(pool: KVPool, k: torch.Tensor, v: torch.Tensor, slots,
     n_layers, n = k.shape[0], k.shape[1]
     if len(slots) != n:
         raise ValueError(f"{len(slots)} slots for {n} rows per layer")
-    if tuple(k.shape[2:]) != pool.tile_shape[1:]:
+    if tuple(k.shape[2:]) != _row_shape(pool):
         raise ValueError(f"rows of shape {tuple(k.shape[2:])} do not fit a pool of "
-                         f"{pool.tile_shape[1:]}")
+                         f"{_row_shape(pool)}")
     if first_layer < 0 or first_layer + n_layers > pool.num_layers:
         raise IndexError(f"layers {first_layer}..{first_layer + n_layers - 1} out of range for "
                          f"{pool.num_layers} layers")
+    if isinstance(pool, QuantizedPool):
+        quantized.write(pool, first_layer, k, v, slots)
+        return
     _write(pool, first_layer, n_layers, n, k, v, slots)
 
 
-def gather_rows_arrays(pool: KVPool, block_table, context_len: int, first_array: int = 0,
-                       n_arrays: int | None = None) -> torch.Tensor:
-    """Rows ``0..context_len-1`` of a sequence in arrays ``first_array ..`` (all 2L by
-    default: K of layers 0..L-1, then V), in one launch; a new
-    ``[n_arrays, context_len, H, D]`` tensor of the cache dtype."""
-    n_arrays = pool.n_arrays - first_array if n_arrays is None else n_arrays
+def _check_arrays(pool: KVPool, first_array: int, n_arrays: int) -> None:
     if first_array < 0 or n_arrays <= 0 or first_array + n_arrays > pool.n_arrays:
         raise IndexError(f"arrays {first_array}..{first_array + n_arrays - 1} out of range for "
                          f"{pool.n_arrays} arrays")
+
+
+def gather_rows_arrays(pool: KVPool, block_table, context_len: int, first_array: int = 0,
+                       n_arrays: int | None = None, *,
+                       dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Rows ``0..context_len-1`` of a sequence in arrays ``first_array ..`` (all 2L by
+    default: K of layers 0..L-1, then V), in one launch; a new
+    ``[n_arrays, context_len, H, D]`` tensor of the cache dtype, of a quantised pool's values
+    in ``dtype`` as :func:`gather_rows` has them."""
+    n_arrays = pool.n_arrays - first_array if n_arrays is None else n_arrays
+    _check_arrays(pool, first_array, n_arrays)
+    if isinstance(pool, QuantizedPool):
+        return quantized.read(pool, first_array, n_arrays, block_table, context_len, dtype)
+    _cache_dtype_only(pool, dtype)
     table, fn = _context_table(pool, block_table, context_len)
     out = torch.empty((n_arrays, context_len, *pool.tile_shape[1:]), dtype=pool.dtype,
                       device=pool.device)

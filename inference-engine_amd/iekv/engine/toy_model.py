@@ -14,8 +14,10 @@ through libiekv's slot kernels (``iekv.engine.slots``) instead of torch's
 ``index_copy_`` / ``index_select``. With ``hip_attention=True`` each layer attends
 straight over its paged cache (``iekv.engine.attention``): one plan per step serves
 every layer, and the leading blocks that all sequences of a step share are attended
-once for all. ``window`` and ``sinks`` make every layer's attention a sliding window
-that keeps the first keys visible, on either path.
+once for all. ``cache_format`` holds the caches in a microscaled format
+(``iekv.engine.quantized``): rows are quantised as each layer writes them, and either path
+attends over the values that the cache then holds. ``window`` and ``sinks`` make every
+layer's attention a sliding window that keeps the first keys visible, on either path.
 """
 from __future__ import annotations
 
@@ -105,14 +107,22 @@ class ToyTransformer:
     def __init__(self, config: ModelConfig, seed: int = 0, device: str | torch.device = "cuda",
                  cache_dtype: torch.dtype = torch.float32, hip_kv: bool = False,
                  hip_attention: bool = False, window: int | None = None,
-                 sinks: int = 0) -> None:
+                 sinks: int = 0, cache_format: str | None = None) -> None:
         if window is not None and window < 1:
             raise ValueError(f"window {window} must be at least 1 (None for no window)")
         if sinks < 0:
             raise ValueError(f"sinks {sinks} is negative")
+        if cache_format is not None:
+            from .quantized import record_bytes
+
+            record_bytes(cache_format, config.head_dim)        # a format, and heads it takes
+            if not (hip_kv or hip_attention):
+                raise ValueError("caches in a microscaled format are written by the slot kernels: "
+                                 "hip_kv or hip_attention")
         self.config = config
         self.device = torch.device(device)
         self.cache_dtype = cache_dtype
+        self.cache_format = cache_format
         self.hip_kv = hip_kv
         self.hip_attention = hip_attention
         self.window = window
@@ -139,15 +149,32 @@ class ToyTransformer:
 
     def allocate_caches(self, num_blocks: int, block_size: int):
         c = self.config
-        return allocate_pool(num_blocks, block_size, c.num_layers, c.num_kv_heads, c.head_dim,
-                             dtype=self.cache_dtype, device=self.device)
+        shape = (num_blocks, block_size, c.num_layers, c.num_kv_heads, c.head_dim)
+        if self.cache_format is not None:
+            from .quantized import allocate_quantized_pool
+
+            return allocate_quantized_pool(*shape, format=self.cache_format, device=self.device)
+        return allocate_pool(*shape, dtype=self.cache_dtype, device=self.device)
 
     def allocate_cache_pair(self, first_blocks: int, second_blocks: int, block_size: int):
         """Two pools in one reservation (prefill first); see ``allocate_pool_pair``."""
         c = self.config
-        return allocate_pool_pair(first_blocks, second_blocks, block_size, c.num_layers,
-                                  c.num_kv_heads, c.head_dim, dtype=self.cache_dtype,
-                                  device=self.device)
+        shape = (first_blocks, second_blocks, block_size, c.num_layers, c.num_kv_heads, c.head_dim)
+        if self.cache_format is not None:
+            from .quantized import allocate_quantized_pool_pair
+
+            return allocate_quantized_pool_pair(*shape, format=self.cache_format,
+                                                device=self.device)
+        return allocate_pool_pair(*shape, dtype=self.cache_dtype, device=self.device)
+
+    def _registered(self, k_caches, v_caches, block_size: int):
+        if self.cache_format is not None:
+            from .quantized import QuantizedPool
+
+            return QuantizedPool(k_caches, v_caches, block_size, self.cache_format)
+        from .pools import KVPool
+
+        return KVPool(k_caches, v_caches, block_size)
 
     def bind_caches(self, k_caches, v_caches, block_size: int):
         """Register a pool for the slot and attention kernels; the caller keeps the
@@ -156,12 +183,10 @@ class ToyTransformer:
         released with the engine that owns it. None where torch does both."""
         if not (self.hip_kv or self.hip_attention):
             return None
-        from .pools import KVPool
-
         key = (k_caches[0].data_ptr(), v_caches[0].data_ptr(), block_size)
         pool = self._pools.get(key)
         if pool is None:
-            pool = KVPool(k_caches, v_caches, block_size)
+            pool = self._registered(k_caches, v_caches, block_size)
             self._pools[key] = pool
         return pool
 
@@ -169,9 +194,7 @@ class ToyTransformer:
         key = (k_caches[0].data_ptr(), v_caches[0].data_ptr(), block_size)
         pool = self._pools.get(key)
         if pool is None:      # caches nobody bound: a pool for this call only
-            from .pools import KVPool
-
-            pool = KVPool(k_caches, v_caches, block_size)
+            pool = self._registered(k_caches, v_caches, block_size)
         return pool
 
     def _cached_rows(self, cache: torch.Tensor, table: list[int], context_len: int,
@@ -234,7 +257,9 @@ class ToyTransformer:
 
         With ``hip_attention`` each layer's rows are written before it attends (by
         iekv_write_slots_layers with ``hip_kv``), and iekv_attend reads the cache
-        through the block tables; nothing is gathered.
+        through the block tables; nothing is gathered. So it is with ``cache_format``, where
+        without ``hip_attention`` each layer's contexts are read back when its rows are
+        written.
         """
         c = self.config
         tokens = torch.as_tensor(layout.token_ids, device=self.device, dtype=torch.long)
@@ -244,9 +269,10 @@ class ToyTransformer:
         pool = self._pool(k_caches, v_caches, block_size) \
             if self.hip_kv or self.hip_attention else None
         plan = self._plan(pool, layout) if self.hip_attention else None
-        gathers = pool is not None and plan is None
-        if self.hip_kv:
-            from .slots import gather_rows_arrays, write_slots, write_slots_layers
+        quantized = self.cache_format is not None
+        gathers = pool is not None and plan is None and not quantized
+        if self.hip_kv or quantized:
+            from .slots import gather_rows, gather_rows_arrays, write_slots, write_slots_layers
         if plan is not None:
             from .attention import attend
         if gathers:
@@ -262,7 +288,7 @@ class ToyTransformer:
             v = (normed @ layer.v_proj).view(-1, c.num_kv_heads, c.head_dim)
             q = _rope(q, positions, self.cos, self.sin, c.rope_halved)
             k = _rope(k, positions, self.cos, self.sin, c.rope_halved)
-            kc, vc = k.to(k_cache.dtype), v.to(v_cache.dtype)
+            kc, vc = (k, v) if quantized else (k.to(k_cache.dtype), v.to(v_cache.dtype))
             if gathers:
                 new_k.append(kc)
                 new_v.append(vc)
@@ -273,13 +299,17 @@ class ToyTransformer:
                         ks = torch.cat((prior[index], ks))
                         vs = torch.cat((prior[c.num_layers + index], vs))
                     contexts.append((ks, vs))
-            elif self.hip_kv:
+            elif self.hip_kv or quantized:
                 write_slots(pool, index, kc, vc, slots)
             else:
                 k_cache.index_copy_(0, slots, kc)
                 v_cache.index_copy_(0, slots, vc)
             if plan is not None:
                 attended = attend(plan, index, q)
+            elif quantized:
+                contexts = [tuple(gather_rows(pool, array, t, n, dtype=x.dtype)
+                                  for array in (index, c.num_layers + index))
+                            for t, n in zip(layout.block_tables, layout.context_lens)]
             elif not gathers:
                 contexts = [(self._cached_rows(k_cache, t, n, block_size),
                              self._cached_rows(v_cache, t, n, block_size))

@@ -1,0 +1,98 @@
+"""Serving from microscaled caches (GPU): the toy model's rows are quantised as they are written
+and attended over, colocated and after a handoff, from the offload tier and over the wire."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from quantized_reference import FORMATS, decode, encode
+from test_gpu_scored_serving import G, decided, engine_config, model
+
+pytestmark = pytest.mark.gpu
+
+
+def agree(got, want):
+    assert [g[:len(w)] for g, w in zip(got, want)] == want
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("window, sinks", [(None, 0), (9, 2)])
+def test_the_model_decodes_alike_on_every_path(gpu, format, window, sinks):
+    """Contexts that are read back and attended in torch, attention over the records, and a
+    handoff of the records between the two workers: the same tokens."""
+    from iekv.engine.engine import Engine
+    from iekv.serve.disaggregated import DisaggregatedEngine
+
+    options = dict(cache_format=format, window=window, sinks=sinks)
+    want = decided(gpu, G["prompts"], 8, hip_kv=True, **options)
+    assert sum(map(len, want)) > 4 * len(want)
+    for m in (model(gpu, hip_attention=True, **options),
+              model(gpu, hip_kv=True, hip_attention=True, **options),
+              model(gpu, hip_kv=True, **options)):
+        for engine in (Engine(m, engine_config()), DisaggregatedEngine(m, engine_config()),
+                       DisaggregatedEngine(m, engine_config(), mode="direct"),
+                       DisaggregatedEngine(m, engine_config(), mode="queue")):
+            agree(engine.generate(G["prompts"], max_new_tokens=8, temperature=0.0), want)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_the_caches_hold_what_the_formats_make_of_the_rows(gpu, format):
+    """Of the first layer, whose rows no attention comes before."""
+    from iekv.engine.engine import Engine
+
+    prompt = G["prompts"][0]
+    plain = Engine(model(gpu), engine_config())
+    scaled = Engine(model(gpu, hip_attention=True, cache_format=format), engine_config())
+    tables = []
+    for engine in (plain, scaled):
+        seq = engine.submit(prompt, max_new_tokens=4, temperature=0.0)
+        engine.step()
+        tables.append(list(seq.block_table))
+    assert tables[0] == tables[1]
+    bs = plain.config.block_size
+    rows = [tables[0][j // bs] * bs + j % bs for j in range(len(prompt))]
+    for a, b in ((plain.k_caches, scaled.k_caches), (plain.v_caches, scaled.v_caches)):
+        want = decode(encode(a[0][rows], format), format)
+        assert torch.equal(decode(b[0][rows], format), want)
+
+
+@pytest.mark.parametrize("over", [dict(offload_blocks=64, num_blocks=24),
+                                  dict(preemption="swap", num_blocks=24)], ids=["tier", "swap"])
+def test_records_come_back_from_host_memory(gpu, over):
+    from iekv.engine.engine import Engine
+
+    m = model(gpu, hip_kv=True, hip_attention=True, cache_format="mxint8")
+    want = Engine(m, engine_config()).generate(G["prompts"], max_new_tokens=8, temperature=0.0)
+    engine = Engine(m, engine_config(**over))
+    for _ in range(2):                       # the second time behind resident or offloaded blocks
+        got = engine.generate(G["prompts"], max_new_tokens=8, temperature=0.0)
+        close = sum(g != w for g, w in zip(got, want))
+        assert close <= 1                    # a token that rounding could decide
+
+
+def test_records_travel_over_the_wire(gpu):
+    from iekv.serve.disaggregated import DecodeWorker, PrefillWorker
+    from iekv.serve.wire import from_wire, to_wire
+
+    m = model(gpu, hip_attention=True, cache_format="mxfp8")
+    prefill, decode_side = PrefillWorker(m, engine_config()), DecodeWorker(m, engine_config())
+    prompt = G["prompts"][1]
+    transfer = prefill.prefill(prompt, 0.0)
+    header, payload = to_wire(transfer)
+    back = from_wire(header, payload.cpu())
+    seq = decode_side.admit(back, max_new_tokens=6, temperature=0.0)
+    n, bs = len(prompt), prefill.engine.config.block_size
+    sent = payload.cpu()
+    for index, block in enumerate(seq.block_table[:n // bs]):
+        for a, cache in enumerate(decode_side.engine.k_caches + decode_side.engine.v_caches):
+            assert torch.equal(cache[block * bs:(block + 1) * bs].cpu().view(-1), sent[index, a])
+    decode_side.engine.run()
+    want = decided(gpu, [prompt], 6, hip_kv=True, cache_format="mxfp8")
+    agree([seq.token_ids[seq.num_prompt:]], want)
+
+
+def test_models_without_the_slot_kernels_are_refused(gpu):
+    with pytest.raises(ValueError, match="hip_kv or hip_attention"):
+        model(gpu, cache_format="mxfp8")
+    with pytest.raises(ValueError, match="no format"):
+        model(gpu, hip_kv=True, cache_format="fp8")

@@ -1,0 +1,179 @@
+"""Microscaled caches: what the host decides and refuses (CPU)."""
+from __future__ import annotations
+
+import ctypes
+import re
+
+import pytest
+import torch
+
+from conftest import ROOT
+from quantized_reference import CODES, FORMATS, decode, encode
+from test_attention_plan import make, ops  # noqa: F401  (the library, and a plan of two sequences)
+from test_ops_host import on_stub  # noqa: F401  (the library over a HIP that runs nothing)
+
+INVALID = -1
+MOST = (2 ** 32 - 1) // 256          # workgroups of a launch
+
+
+def test_types_and_structure_agree_with_the_header():
+    from iekv import _ops
+
+    text = (ROOT / "include" / "iekv_ops.h").read_text()
+    for name in ("MXFP8", "MXINT8", "MXFP4"):
+        value = re.search(rf"IEKV_TYPE_{name} = (\d+)", text).group(1)
+        assert int(value) == getattr(_ops, f"IEKV_TYPE_{name}")
+    assert ctypes.sizeof(_ops.MxCache) == 24
+
+
+def test_records(ops):  # noqa: F811
+    from iekv.engine.quantized import FORMATS as TYPES
+    from iekv.engine.quantized import record_bytes
+
+    assert set(TYPES) == set(FORMATS)
+    for format in FORMATS:
+        for dim in range(8, 129, 8):
+            size = dim // (2 if format == "mxfp4" else 1) + 4
+            assert record_bytes(format, dim) == size == ops.iekv_mx_head_bytes(TYPES[format], dim)
+        for dim in (0, -8, 4, 12, 136):
+            with pytest.raises(ValueError, match=f"head_dim {dim}"):
+                record_bytes(format, dim)
+            assert ops.iekv_mx_head_bytes(TYPES[format], dim) == 0
+    with pytest.raises(ValueError, match="no format 'fp8'"):
+        record_bytes("fp8", 128)
+    assert ops.iekv_mx_head_bytes(4, 128) == ops.iekv_mx_head_bytes(8, 128) == 0
+
+
+def test_the_definition():
+    """The oracle's own rounding: nearest, ties to even codes, nothing past the largest."""
+    x = torch.zeros(1, 32, dtype=torch.float64)
+    x[0, :9] = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.26])
+    assert decode(encode(x, "mxfp4"), "mxfp4")[0, :9].tolist() == \
+        [6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, -0.5]
+    x[0, :4] = torch.tensor([127.0, 0.5, 1.5, -2.5])
+    assert decode(encode(x, "mxint8"), "mxint8")[0, :4].tolist() == [127.0, 0.0, 2.0, -2.0]
+    x[0, :4] = torch.tensor([448.0, 17.0, 19.0, -2.0 ** -10])
+    assert decode(encode(x, "mxfp8"), "mxfp8")[0, :4].tolist() == [448.0, 16.0, 20.0, 0.0]
+    gen = torch.Generator().manual_seed(1)
+    for format in FORMATS:
+        rows = torch.randn((50, 3, 80), generator=gen, dtype=torch.float64)
+        rows *= torch.exp2(torch.randn((50, 3, 1), generator=gen) * 12)
+        got = decode(encode(rows, format), format)
+        # By brute force over every code of a group's own exponent and of one less: its largest
+        # is within the type's, and would not be there.
+        scale = torch.ldexp(torch.ones((), dtype=torch.float64),
+                            encode(rows, format)[..., -4:].int() - 127)
+        top = {"mxfp8": 448.0, "mxint8": 127.0, "mxfp4": 6.0}[format]
+        values = CODES[format][torch.isfinite(CODES[format])]
+        values = values[values.abs() <= top]
+        for g in range(3):
+            part, s = rows[..., g * 32:g * 32 + 32], scale[..., g:g + 1]
+            assert (part.abs().amax(-1) <= top * s[..., 0]).all()
+            assert (part.abs().amax(-1) > top / 2 * s[..., 0]).all()
+            off = (part[..., None] - values * s[..., None]).abs().amin(-1)
+            assert torch.equal((part - got[..., g * 32:g * 32 + 32]).abs(), off)
+
+
+def test_pools_of_host_tensors_are_refused():
+    from iekv.engine.quantized import QuantizedPool, allocate_quantized_pool
+
+    k, v = allocate_quantized_pool(4, 8, 2, 2, 32, format="mxfp8", device="cpu")
+    assert len(k) == len(v) == 2 and k[0].shape == (32, 2, 36) and k[0].dtype == torch.uint8
+    with pytest.raises(ValueError, match="GPU"):
+        QuantizedPool(k, v, 8, "mxfp8")
+    with pytest.raises(ValueError, match="no format"):
+        QuantizedPool(k, v, 8, "int8")
+
+
+@pytest.mark.parametrize("cache_type, query_type, taken", [
+    *[(c, q, True) for c in (5, 6, 7) for q in (1, 2, 3)], (8, 3, False), (8, 1, False),
+    (5, 4, False), (7, 5, False), (6, 0, False)])
+def test_plans_take_microscaled_caches(ops, cache_type, query_type, taken):  # noqa: F811
+    rc, out, message = make(ops, cache_type=cache_type, query_type=query_type)
+    assert (rc == 0) == taken
+    if taken:
+        ops.iekv_attention_plan_destroy(out)
+    else:
+        assert rc == INVALID and f"cache of type {cache_type}" in message
+
+
+CALLS = """
+def cache(**over):
+    fields = dict(dict(cache_type=5, num_kv_heads=8, head_dim=128, block_size=16, num_blocks=100),
+                  **over)
+    return ctypes.byref(_ops.MxCache(**fields))
+
+def u64(*x):
+    return (ctypes.c_uint64 * len(x))(*x)
+
+def i64(*x):
+    return (ctypes.c_int64 * len(x))(*x)
+
+def write(k=u64(1 << 20), v=u64(1 << 21), layers=1, row=3, n=5, rows=1 << 22, slots=1 << 23,
+          strides=i64(5120, 1024, 128), **over):
+    return ops.iekv_mx_write_slots(cache(**over), k, v, layers, row, rows, strides, rows, strides,
+                                   slots, n, 77)
+
+def read(arrays=u64(1 << 20), n=1, table=1 << 21, context=20, out_type=3, out=1 << 22, **over):
+    return ops.iekv_mx_read_rows(cache(**over), arrays, n, table, context, out_type, out, 77)
+
+def said(rc):
+    return [rc, ops.iekv_ops_last_error().decode() if rc else ""]
+"""
+
+SHAPES = [("cache_type=4", "4 is no microscaled type"), ("cache_type=8", "8 is no microscaled"),
+          ("num_kv_heads=0", "num_kv_heads 0"), ("num_kv_heads=4097", "num_kv_heads 4097"),
+          ("head_dim=0", "head_dim 0"), ("head_dim=12", "head_dim 12"),
+          ("head_dim=136", "head_dim 136"), ("block_size=0", "block_size 0"),
+          ("num_blocks=0", "num_blocks 0"), ("num_blocks=1 << 31", "num_blocks 2147483648")]
+
+
+def test_refusals_come_before_anything_is_enqueued(on_stub):  # noqa: F811
+    cases = [(f"{f}({a})", want) for f in ("write", "read") for a, want in SHAPES]
+    cases += [("write(row=4)", "rows of type 4"), ("write(row=0)", "rows of type 0"),
+              ("write(layers=-1)", "-1 layers"), ("write(n=-1)", "of -1 tokens"),
+              *[(f"write({a}=None)", "null") for a in ("k", "v", "rows", "slots", "strides")],
+              ("read(out_type=5)", "values of type 5"), ("read(n=-2)", "-2 arrays"),
+              ("read(context=-1)", "context of -1"),
+              ("read(context=(1 << 30) + 1)", "context of 1073741825"),
+              ("read(context=1 << 26)", "too long"),
+              *[(f"read({a}=None)", "null") for a in ("arrays", "table", "out")]]
+    got = on_stub(CALLS + f"""
+bad = [said(eval(call)) for call in {[c for c, _ in cases]!r}]
+bad.append(said(ops.iekv_mx_write_slots(None, *[None] * 2, 0, 3, *[None] * 5, 0, None)))
+bad.append(said(ops.iekv_mx_read_rows(None, None, 0, None, 0, 3, None, None)))
+none = [write(n=0, k=None, rows=None), write(layers=0, v=None), read(context=0, out=None),
+        read(n=0, arrays=None)]
+print(json.dumps([bad, none, launches()]))
+""")
+    for (rc, message), (call, want) in zip(got[0], cases + [("", "cache is null")] * 2):
+        assert rc == INVALID and want in message, (call, rc, message)
+    assert got[1] == [0, 0, 0, 0] and got[2] == []
+
+
+def test_arrays_at_even_distances_share_a_launch(on_stub):  # noqa: F811
+    """All layers of a pool in one launch; of arrays in no order as many as lie so."""
+    got = on_stub(CALLS + """
+even = u64(*[(1 << 30) + 4096 * i for i in range(40)])
+odd = u64(*[(1 << 30) + 4096 * i for i in (0, 1, 2, 7, 9, 10, 5)])
+stub.hipSetDevice(3)
+rcs = [write(k=even, v=even, layers=40), write(k=even, v=odd, layers=7), write(layers=1),
+       read(arrays=odd, n=7), read(arrays=even, n=40)]
+print(json.dumps([rcs, launches()]))
+""")
+    assert got[0] == [0] * 5
+    grids = [x[1:4] for x in got[1]]
+    assert {x[0] for x in got[1]} == {3} and {x[4] for x in got[1]} == {77}
+    layers = [x[1] for x in grids]
+    assert layers == [40, 3, 2, 2, 1, 3, 2, 2, 40]
+
+
+def test_steps_of_any_size_run_in_several_launches(on_stub):  # noqa: F811
+    got = on_stub(CALLS + """
+rc = write(n=(1 << 28) + 5, num_kv_heads=16)
+print(json.dumps([said(rc), launches()]))
+""")
+    assert got[0][0] == 0, got[0]
+    lanes = 16 * 16                                  # of a token
+    assert len(got[1]) > 1 and all(x[1] <= MOST for x in got[1])
+    assert sum(x[1] for x in got[1]) == ((1 << 28) + 5) * lanes // 256
