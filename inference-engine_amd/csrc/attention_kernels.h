@@ -51,28 +51,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// BYTES from any address (caches and queries may begin at any element).
-template <int BYTES>
-__device__ __forceinline__ Words<(BYTES + 3) / 4> load_bytes(const void* p) {
-  Words<(BYTES + 3) / 4> r;
-  r.w[(BYTES - 1) / 4] = 0;
-  __builtin_memcpy(&r, p, BYTES);
-  return r;
-}
-
-// The same of a stream that is read once.
-template <int BYTES>
-__device__ __forceinline__ Words<(BYTES + 3) / 4> stream_bytes(const void* p) {
-  // (Vectors of three are loaded as four.)
-  if constexpr (BYTES % 4 || BYTES == 12) {
-    return load_bytes<BYTES>(p);
-  } else {
-    typedef uint32_t Vec __attribute__((ext_vector_type(BYTES / 4), aligned(1)));
-    return __builtin_bit_cast(Words<BYTES / 4>,
-                              __builtin_nontemporal_load(static_cast<const Vec*>(p)));
-  }
-}
-
 // N elements of type C as elements of the compute type T (exact: T holds every value of C).
 template <typename T, typename C, int N>
 struct Convert {                                 // T == C

@@ -61,6 +61,35 @@ struct Words {
   uint32_t w[N];
 };
 
+// BYTES from any address (caches and queries may begin at any element).
+template <int BYTES>
+__device__ __forceinline__ Words<(BYTES + 3) / 4> load_bytes(const void* p) {
+  Words<(BYTES + 3) / 4> r;
+  r.w[(BYTES - 1) / 4] = 0;
+  __builtin_memcpy(&r, p, BYTES);
+  return r;
+}
+
+// The same of a stream that is read once.
+template <int BYTES>
+__device__ __forceinline__ Words<(BYTES + 3) / 4> stream_bytes(const void* p) {
+  // (Vectors of three are loaded as four.)
+  if constexpr (BYTES % 4 || BYTES == 12) {
+    return load_bytes<BYTES>(p);
+  } else {
+    typedef uint32_t Vec __attribute__((ext_vector_type(BYTES / 4), aligned(1)));
+    return __builtin_bit_cast(Words<BYTES / 4>,
+                              __builtin_nontemporal_load(static_cast<const Vec*>(p)));
+  }
+}
+
+// BYTES (a multiple of 4) to any address, of a stream that nothing here reads again.
+template <int BYTES>
+__device__ __forceinline__ void stream_out(void* p, const Words<BYTES / 4>& x) {
+  typedef uint32_t Vec __attribute__((ext_vector_type(BYTES / 4), aligned(1)));
+  __builtin_nontemporal_store(__builtin_bit_cast(Vec, x), static_cast<Vec*>(p));
+}
+
 // Two elements of the compute type in a word, rounded to nearest even.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
