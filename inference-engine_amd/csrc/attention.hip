@@ -80,6 +80,29 @@ hipError_t allow_lds(K kernel, int bytes, int device, std::atomic<uint64_t>* ask
   return error;
 }
 
+int32_t bytes_of(int32_t type) {
+  return type == IEKV_TYPE_F32 ? 4 : type == IEKV_TYPE_E4M3 ? 1 : 2;
+}
+
+// Bytes of a head of a key in the cache.
+int32_t head_bytes_of(const iekv_attention_shape& s) {
+  return s.cache_type >= IEKV_TYPE_MXFP8
+             ? static_cast<int32_t>(iekv_mx_head_bytes(s.cache_type, s.head_dim))
+             : s.head_dim * bytes_of(s.cache_type);
+}
+
+// Whether narrow items of four KV heads are taken together: see Together.
+bool together_fits(const iekv_attention_shape& s) {
+  return s.cache_type >= IEKV_TYPE_MXFP8 && s.num_kv_heads % kWaves == 0 &&
+         s.head_dim % kGroup == 0;
+}
+
+// Workgroups of a long stream that a compute unit runs at once. Those that take four heads
+// together have the records of 64 keys in LDS.
+int32_t streams_at_once(const iekv_attention_shape& s) {
+  return !together_fits(s) ? 3 : head_bytes_of(s) * kWaves * 64 * 2 < (36 << 10) ? 4 : 2;
+}
+
 template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
@@ -100,8 +123,10 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   };
   if constexpr (sizeof(T) == 2) {
     bool done = !wide;
-    if constexpr (std::is_same_v<T, C>) {
-      const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if constexpr (std::is_same_v<T, C> || kScaled<C>) {
+      const auto aligned = [](const void* p) {
+        return kScaled<C> || reinterpret_cast<uintptr_t>(p) % 16 == 0;
+      };
       if (wide && !both && aligned(a.k) && aligned(a.v)) {
         if (const int rc = in_launches(wide, a.kv_heads, [&](int64_t first, int64_t n) {
               hipLaunchKernelGGL((attend_wide<T, C, DP>), dim3(n * a.kv_heads), dim3(kThreads), 0,
@@ -127,13 +152,26 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   }
   if (narrow && !both) {
     // Only 32-bit queries have narrow items of more than 16 heads.
-    if (const int rc = in_launches(narrow, each, [&](int64_t first, int64_t n) {
-          hipLaunchKernelGGL((attend_narrow<T, C, DP>), dim3(n * each, (a.group + 15) / 16),
-                             dim3(kThreads), 0, stream, a,
-                             static_cast<int32_t>(plan.narrow.first + first),
-                             static_cast<int32_t>(n));
-        }))
-      return rc;
+    const auto run = [&](auto kernel, size_t bytes, std::atomic<uint64_t>* asked) {
+      IEKV_OPS_HIP(allow_lds(kernel, static_cast<int>(bytes), plan.device, asked));
+      return in_launches(narrow, each, [&](int64_t first, int64_t n) {
+        hipLaunchKernelGGL(kernel, dim3(n * each, (a.group + 15) / 16), dim3(kThreads), bytes,
+                           stream, a, static_cast<int32_t>(plan.narrow.first + first),
+                           static_cast<int32_t>(n));
+      });
+    };
+    using N = Narrow<T, C, DP>;
+    static std::atomic<uint64_t> asked{0}, asked_together{0};
+    int rc = IEKV_OK;
+    if constexpr (kScaled<C>) {
+      if (a.together == kWaves && together_fits(plan.shape))
+        rc = run(attend_narrow<T, C, DP, true>, sizeof(typename N::LdsTogether), &asked_together);
+      else
+        rc = run(attend_narrow<T, C, DP, false>, sizeof(typename N::Lds), &asked);
+    } else {
+      rc = run(attend_narrow<T, C, DP, false>, sizeof(typename N::Lds), &asked);
+    }
+    if (rc) return rc;
   }
   if (plan.joined) {
     // Few rows have many parts each: their loads are spread over four waves.
@@ -159,17 +197,6 @@ int launch(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
     case 3: return launch_dim<T, C, 96>(plan, a, stream);
     default: return launch_dim<T, C, 128>(plan, a, stream);
   }
-}
-
-int32_t bytes_of(int32_t type) {
-  return type == IEKV_TYPE_F32 ? 4 : type == IEKV_TYPE_E4M3 ? 1 : 2;
-}
-
-// Bytes of a head of a key in the cache.
-int32_t head_bytes_of(const iekv_attention_shape& s) {
-  return s.cache_type >= IEKV_TYPE_MXFP8
-             ? static_cast<int32_t>(iekv_mx_head_bytes(s.cache_type, s.head_dim))
-             : s.head_dim * bytes_of(s.cache_type);
 }
 
 // Whether the output lies over queries of other rows: a workgroup writes its rows when it has
@@ -289,7 +316,8 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            shape.block_size, shape.window, shape.sinks,
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
-                           few_keys(shape), 2 * head_bytes_of(shape)};
+                           few_keys(shape), 2 * head_bytes_of(shape),
+                           streams_at_once(shape)};
   const int device = current_device();
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||

@@ -290,6 +290,155 @@ __device__ __forceinline__ void store_out(T* out, const float* x) {
   }
 }
 
+// The records of a step of a microscaled cache, on their way through LDS into the products'
+// operands. Records begin at any multiple of 4, and as operands sixteen lanes would take from
+// sixteen of them: what bounds such loads is the first cache, a line at a time. So a wave brings
+// the 64 records in chunks of 16 bytes laid end to end (of 32 dimensions 4), the last of each the
+// one that ends with the scales, and every lane's load is full.
+template <typename C, int DP>
+struct Staged {
+  static constexpr int KEYS = 64;
+  static constexpr int CODES = DP * kBits<C> / 8;            // bytes of a key; its scales' chunk
+  static constexpr int W = DP == 32 ? 4 : 16;                // follows them
+  static constexpr int CHUNKS = CODES / W + 1;               // and loads of a wave
+  // Reads of neighbouring keys meet in no bank.
+  static constexpr int PITCH = CODES + W + (CODES == 48 ? 16 : 0);
+  alignas(16) char bytes[kScaled<C> ? KEYS * PITCH : 16];
+
+  using Chunk = Words<W / 4>;
+  // Load n of a wave brings chunk (n + lane) % CHUNKS of key n * 64 / CHUNKS + ...: 64 n + lane in
+  // all.
+  struct Lane {
+    int32_t key[CHUNKS], from[CHUNKS], to[CHUNKS];
+  };
+
+  // Key 32 p + 8 a + 4 b + e lies at 32 p + 16 b + 4 a + e: in the order in which the lanes of
+  // two tiles of scores take them.
+  static __device__ __forceinline__ int32_t placed(int32_t key) {
+    return (key & 32) | (key & 4) << 2 | (key & 24) >> 1 | (key & 3);
+  }
+  static __device__ __forceinline__ Lane lane_of(int lane, int32_t d) {
+    Lane r;
+#pragma unroll
+    for (int n = 0; n < CHUNKS; ++n) {
+      const int32_t at = n * kWave + lane, key = at / CHUNKS, chunk = at % CHUNKS;
+      const int32_t codes = code_bytes<C>(d);
+      // The last of the codes begins sooner where it would end behind them.
+      const int32_t begin = chunk * W < codes - W ? chunk * W : codes - W;
+      const bool scales = chunk == CHUNKS - 1;
+      r.key[n] = key;
+      r.from[n] = scales ? codes + kScaleBytes - W : begin;
+      r.to[n] = placed(key) * PITCH + (scales ? CODES : begin);
+    }
+    return r;
+  }
+  // Zeros behind the dimensions, where nothing is brought.
+  __device__ __forceinline__ void clear(int lane) {
+    for (int32_t i = lane * 4; i < KEYS * PITCH; i += kWave * 4)
+      __builtin_memset(__builtin_assume_aligned(bytes + i, 4), 0, 4);
+  }
+  static __device__ __forceinline__ void load(Chunk (&x)[CHUNKS], const Lane& lane,
+                                              const char* head, const int64_t* rows) {
+#pragma unroll
+    for (int n = 0; n < CHUNKS; ++n) x[n] = load_bytes<W>(head + rows[lane.key[n]] + lane.from[n]);
+  }
+  __device__ __forceinline__ void put(const Chunk (&x)[CHUNKS], const Lane& lane, int32_t d) {
+    if (code_bytes<C>(d) % W == 0) {
+#pragma unroll
+      for (int n = 0; n < CHUNKS; ++n)
+        __builtin_memcpy(__builtin_assume_aligned(bytes + lane.to[n], W), &x[n], W);
+    } else {
+#pragma unroll
+      for (int n = 0; n < CHUNKS; ++n)
+        __builtin_memcpy(__builtin_assume_aligned(bytes + lane.to[n], 4), &x[n], W);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // BYTES of the codes of the key at a place, from dimension `d0` on; and 2^e of its group.
+  template <int BYTES>
+  __device__ __forceinline__ Words<(BYTES + 3) / 4> codes(int32_t place, int32_t d0) const {
+    constexpr int align = BYTES % 16 == 0 && PITCH % 16 == 0  ? 16
+                          : BYTES % 8 == 0 && PITCH % 8 == 0 ? 8
+                          : BYTES % 4 == 0                   ? 4
+                                                             : BYTES;
+    Words<(BYTES + 3) / 4> r;
+    r.w[(BYTES - 1) / 4] = 0;
+    __builtin_memcpy(&r, __builtin_assume_aligned(bytes + place * PITCH + code_bytes<C>(d0), align),
+                     BYTES);
+    return r;
+  }
+  __device__ __forceinline__ float scale(int32_t place, int32_t d0) const {
+    return scale_of(static_cast<uint8_t>(bytes[place * PITCH + CODES + W - kScaleBytes +
+                                               d0 / kGroup]), 0);
+  }
+};
+
+// The same of the four neighbouring heads that a workgroup takes: their records lie on end, and
+// of whole groups of 32 dimensions four are a multiple of 16 bytes. The workgroup brings them as
+// they lie, each line once and past the caches; a wave reads its own head's out of them.
+template <typename C, int DP>
+struct Together {
+  static constexpr int KEYS = 64, HEADS = 4;
+  static constexpr int CODES = DP * kBits<C> / 8, RECORD = head_bytes<C>(DP);
+  static constexpr int OF_KEY = HEADS * RECORD / 16;         // chunks
+  static constexpr int CHUNKS = (KEYS * OF_KEY + kThreads - 1) / kThreads;   // of a thread
+  static constexpr int PITCH = HEADS * RECORD;
+  static_assert(!kScaled<C> || PITCH % 16 == 0);
+  alignas(16) char k[kScaled<C> ? KEYS * PITCH : 16], v[kScaled<C> ? KEYS * PITCH : 16];
+
+  using Chunk = Words<4>;
+  struct Lane {
+    int32_t key[CHUNKS], from[CHUNKS], to[CHUNKS];
+  };
+  static __device__ __forceinline__ Lane lane_of() {
+    Lane r;
+#pragma unroll
+    for (int n = 0; n < CHUNKS; ++n) {
+      // The last threads bring the last chunk once more.
+      const int32_t all = KEYS * OF_KEY, i = n * kThreads + threadIdx.x, at = i < all ? i : all - 1;
+      r.key[n] = at / OF_KEY;
+      r.from[n] = at % OF_KEY * 16;
+      r.to[n] = Staged<C, DP>::placed(r.key[n]) * PITCH + r.from[n];
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void load(Chunk (&x)[CHUNKS], const Lane& lane,
+                                              const char* heads, const int64_t* rows) {
+#pragma unroll
+    for (int n = 0; n < CHUNKS; ++n) {
+      const char* at = heads + rows[lane.key[n]] + lane.from[n];
+      // Past the caches where the heads' bytes are long beside the lines at their ends, which
+      // another workgroup's heads have a part of.
+      if constexpr (PITCH >= 512)
+        x[n] = stream_bytes<16>(at);
+      else
+        x[n] = load_bytes<16>(at);
+    }
+  }
+  static __device__ __forceinline__ void put(char* tile, const Chunk (&x)[CHUNKS],
+                                             const Lane& lane) {
+#pragma unroll
+    for (int n = 0; n < CHUNKS; ++n)
+      __builtin_memcpy(__builtin_assume_aligned(tile + lane.to[n], 16), &x[n], 16);
+  }
+  // As Staged's, of a head.
+  template <int BYTES>
+  static __device__ __forceinline__ Words<(BYTES + 3) / 4> codes(const char* tile, int32_t place,
+                                                                 int32_t head, int32_t d0) {
+    Words<(BYTES + 3) / 4> r;
+    r.w[(BYTES - 1) / 4] = 0;
+    __builtin_memcpy(&r, __builtin_assume_aligned(tile + place * PITCH + head * RECORD +
+                                                  code_bytes<C>(d0), BYTES < 4 ? BYTES : 4), BYTES);
+    return r;
+  }
+  static __device__ __forceinline__ float scale(const char* tile, int32_t place, int32_t head,
+                                                int32_t d0) {
+    return scale_of(static_cast<uint8_t>(tile[place * PITCH + head * RECORD + CODES +
+                                              d0 / kGroup]), 0);
+  }
+};
+
 // What bounds it is the cache's stream: each wave has a step's K or V (64 keys; 32 of 32-bit
 // caches) in flight at any time, straight into the registers the products read, and nothing
 // but block ids passes through LDS. A workgroup takes 1, 2 or 4 neighbouring KV heads: its
@@ -319,25 +468,37 @@ struct Narrow {
   using RawV = Words<(EV * kBits<C> / 8 + 3) / 4>;
   static constexpr int LDO = DP + 4;                      // floats of a row of o in LDS
   struct Lds {
-    alignas(16) uint32_t rows[kWaves][2][KS];
+    alignas(16) int64_t rows[kWaves][2][KS];              // bytes to the keys' rows
     float2 ml[kWaves][16];
-    alignas(16) float o[kWaves][16][LDO];
+    union {
+      alignas(16) float o[kWaves][16][LDO];
+      Staged<C, DP> staged[kScaled<C> ? kWaves : 1];      // until the last step
+    };
     int32_t redo[kWaves];
-    alignas(16) uint32_t scales[kScaled<C> ? kWaves : 1][KS];   // of the step's V
+  };
+  struct LdsTogether {
+    alignas(16) int64_t rows[kWaves][2][KS];
+    float2 ml[kWaves][16];
+    union {
+      alignas(16) float o[kWaves][16][LDO];
+      Together<C, DP> staged;
+    };
+    int32_t redo[kWaves];
   };
 };
 
 // A group of more than 16 heads takes several workgroups for each of its tokens, `head0` on.
-template <typename T, typename C, int DP>
-__device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds, const Args& a,
-                                            int32_t item, int32_t kv_head0, int32_t head0) {
+// TOGETHER: four KV heads of a microscaled cache, of DP dimensions each.
+template <typename T, typename C, int DP, bool TOGETHER, typename Lds>
+__device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t item,
+                                            int32_t kv_head0, int32_t head0) {
   using N = Narrow<T, C, DP>;
   constexpr int EK = N::EK, EL = N::EL, NL = N::NL, MF = N::MF, NK = N::NK;
   constexpr int EV = N::EV, KT = N::KT, KS = N::KS;
   const Item it = item_of(a, item);
   const int32_t heads = a.group - head0 < 16 ? a.group - head0 : 16;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane / 16, c = lane % 16;
-  const int32_t together = a.together, turns = kWaves / together;
+  const int32_t together = TOGETHER ? kWaves : a.together, turns = kWaves / together;
   const int32_t kv_head = kv_head0 + wave % together, turn = wave / together;
   const int32_t d = a.head_dim, rows = it.tokens * heads;
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
@@ -345,12 +506,6 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
   const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * size;
   if (threadIdx.x < kWaves) lds.redo[threadIdx.x] = 0;
 
-  // The first dimension that the lane brings at load i. Of microscaled caches a load that would
-  // end behind the head begins sooner, and Q is zero where it repeats what another lane brings.
-  const auto begin = [&](int i) {
-    const int32_t d0 = (4 * i + g) * EL;
-    return !kScaled<C> || d0 + EL <= d ? d0 : d0 < d ? d - EL : 0;
-  };
   // Q^T: row c, zeros past the rows and past the dimensions.
   Words<4> q[NK];
   int32_t position;
@@ -361,8 +516,8 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     const T* at = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int32_t d0 = begin(i / MF) + i % MF * EK;
-      const bool in = c < rows && d0 < d && (!kScaled<C> || d0 >= (4 * (i / MF) + g) * EL);
+      const int32_t d0 = (4 * (i / MF) + g) * EL + i % MF * EK;
+      const bool in = c < rows && d0 < d;
       q[i] = load_bytes<EK * sizeof(T)>(at + (d0 < d ? d0 : 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i].w[e] = (q[i].w[e] ^ a.q_sign) & (in ? ~0u : 0u);
@@ -377,27 +532,56 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     return place_of(a, it, key_at(it, v < n ? v : n - 1));
   };
   const auto keep = [&](int half, Place p) {
-    if (lane < KS) lds.rows[wave][half][lane] = row_of(a, p);
+    if (lane < KS) lds.rows[wave][half][lane] = row_of(a, p) * row_bytes;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  typename N::RawK k[KT][NL];
-  uint32_t k_scales[kScaled<C> ? KT : 1];
+  typename N::RawK k[kScaled<C> ? 1 : KT][NL];
+  // Of microscaled caches: what a lane brings of a step's records, K's and V's.
+  using S = std::conditional_t<TOGETHER, Together<C, DP>, Staged<C, DP>>;
+  static_assert(!kScaled<C> || KS == S::KEYS);
+  typename S::Lane brings;
+  typename S::Chunk k_chunks[kScaled<C> ? S::CHUNKS : 1], v_chunks[kScaled<C> ? S::CHUNKS : 1];
+  if constexpr (TOGETHER) {
+    brings = S::lane_of();
+  } else if constexpr (kScaled<C>) {
+    brings = S::lane_of(lane, d);
+    if (d < DP) lds.staged[wave].clear(lane);
+  }
+  const char* const k_heads = TOGETHER ? kc - wave * size : kc;
+  const char* const v_heads = TOGETHER ? vh - wave * size : vh;
   const auto load_k = [&](int half) {
+    if constexpr (kScaled<C>) {
+      S::load(k_chunks, brings, k_heads, lds.rows[wave][half]);
+    } else {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const uint32_t row =
-          lds.rows[wave][half][t / 2 * 32 + (c >> 2) * 8 + t % 2 * 4 + (c & 3)];
-      const char* at = kc + row * row_bytes;
+      for (int t = 0; t < KT; ++t) {
+        const char* at =
+            kc + lds.rows[wave][half][t / 2 * 32 + (c >> 2) * 8 + t % 2 * 4 + (c & 3)];
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int32_t d0 = begin(i);
-        // 16 elements past the head's end would be past the cache's at its last row.
-        const int32_t from = d0 >= d ? 0 : EL == 16 && d0 + 8 == d ? d0 - 8 : d0;
-        k[t][i] = stream_bytes<code_bytes<C>(EL)>(at + code_bytes<C>(from));
+        for (int i = 0; i < NL; ++i) {
+          const int32_t d0 = (4 * i + g) * EL;
+          // 16 elements past the head's end would be past the cache's at its last row.
+          const int32_t from = d0 >= d ? 0 : EL == 16 && d0 + 8 == d ? d0 - 8 : d0;
+          k[t][i] = stream_bytes<code_bytes<C>(EL)>(at + code_bytes<C>(from));
+        }
       }
-      if constexpr (kScaled<C>) k_scales[t] = load_bytes<kScaleBytes>(at + code_bytes<C>(d)).w[0];
     }
+  };
+  const auto k_of = [&](int t, int i) {
+    if constexpr (TOGETHER)
+      return S::template codes<code_bytes<C>(EL)>(lds.staged.k, t * 16 + c, wave, (4 * i + g) * EL);
+    else if constexpr (kScaled<C>)
+      return lds.staged[wave].template codes<code_bytes<C>(EL)>(t * 16 + c, (4 * i + g) * EL);
+    else
+      return k[t][i];
+  };
+
+  const auto k_scale = [&](int t, int32_t d0) {
+    if constexpr (TOGETHER)
+      return S::scale(lds.staged.k, t * 16 + c, wave, d0);
+    else
+      return lds.staged[wave].scale(t * 16 + c, d0);
   };
 
   // The elements of feed `e` of a load; zeros past the head's dimensions. Not where they are
@@ -409,6 +593,10 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
 #pragma unroll
       for (int w = 0; w < KW; ++w) r.w[w] = x.w[e * EK * kBits<C> / 32 + w];
       if (EK * kBits<C> < 32) r.w[0] >>= e * EK * kBits<C> % 32;
+      // What lies behind 96 dimensions of 8 bits is no code.
+      if (4 * NL * EL > DP && (i + 1) * 4 * EL > DP)
+#pragma unroll
+        for (int w = 0; w < KW; ++w) r.w[w] &= (4 * i + g) * EL < DP ? ~0u : 0u;
       return r;
     }
     const int32_t d0 = (4 * i + g) * EL + e * EK;
@@ -435,54 +623,71 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
     next = place(turn + turns);                 // before K's loads: see below
     keep(0, now);
     load_k(0);
+    if constexpr (TOGETHER) S::load(v_chunks, brings, v_heads, lds.rows[wave][0]);
   }
   for (int32_t s = turn; s < steps; s += turns, half ^= 1) {
     keep(half ^ 1, next);
-    uint32_t v_scales = 0;                      // of the key that is the lane's in `rows`
-    if constexpr (kScaled<C>)
-      v_scales = load_bytes<kScaleBytes>(vh + lds.rows[wave][half][lane % KS] * row_bytes +
-                                         code_bytes<C>(d)).w[0];
-    typename N::RawV v[KT / 2][8];
+    typename N::RawV v[KT / 2][kScaled<C> ? 1 : 8];
+    if constexpr (TOGETHER) {
+      __syncthreads();                          // the step before has been read
+      S::put(lds.staged.k, k_chunks, brings);
+      S::put(lds.staged.v, v_chunks, brings);
+      __syncthreads();
+      next = place(s + 2);
+      load_k(half ^ 1);
+      S::load(v_chunks, brings, v_heads, lds.rows[wave][half ^ 1]);
+    } else if constexpr (kScaled<C>) {
+      S::load(v_chunks, brings, v_heads, lds.rows[wave][half]);
+      __builtin_amdgcn_sched_barrier(0);
+      lds.staged[wave].put(k_chunks, brings, d);
+    } else {
 #pragma unroll
-    for (int p = 0; p < KT / 2; ++p)
+      for (int p = 0; p < KT / 2; ++p)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t row = lds.rows[wave][half][p * 32 + g * 8 + e];
-        v[p][e] = stream_bytes<code_bytes<C>(EV)>(vc + row * row_bytes);
-      }
+        for (int e = 0; e < 8; ++e)
+          v[p][e] = stream_bytes<EV * kBits<C> / 8>(vc + lds.rows[wave][half][p * 32 + g * 8 + e]);
+    }
     __builtin_amdgcn_sched_barrier(0);          // no wait for K's before V's are on their way
     f32x4 sc[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const auto raw = feed(k[t][i / MF], i / MF, i % MF);
-        if constexpr (kScaled<C>)
-          sc[t] = mma16(scaled<T, C, EK>(raw, scale_of(k_scales[t], (begin(i / MF) + i % MF * EK) /
-                                                                        kGroup * 8)),
-                        q[i], sc[t], T{});
-        else
-          sc[t] = mma16(Convert<T, C, EK>::of(raw), q[i], sc[t], T{});
+      for (int i = 0; i < NL; ++i) {
+        const typename N::RawK whole = k_of(t, i);
+#pragma unroll
+        for (int e = 0; e < MF; ++e) {
+          const auto raw = feed(whole, i, e);
+          if constexpr (kScaled<C>)
+            sc[t] = mma16(scaled<T, C, EK>(raw, k_scale(t, (4 * i + g) * EL + e * EK)),
+                          q[i * MF + e], sc[t], T{});
+          else
+            sc[t] = mma16(Convert<T, C, EK>::of(raw), q[i * MF + e], sc[t], T{});
+        }
       }
     }
     // In this order: loads return in theirs, and the block's id is what is needed first. Past
     // the last step these read the last key: a branch would make the next wait one for all.
-    next = place(s + 2 * turns);
-    load_k(half ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (kScaled<C>) {
-      if (lane < KS) lds.scales[wave][lane] = v_scales;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+    if constexpr (!TOGETHER) {
+      next = place(s + 2 * turns);
+      load_k(half ^ 1);
     }
+    __builtin_amdgcn_sched_barrier(0);
     // V of key `e` of the lane's eight of pair `p`.
     const auto v_of = [&](int p, int e) {
-      if constexpr (kScaled<C>)
-        return scaled<T, C, EV>(v[p][e], scale_of(lds.scales[wave][p * 32 + g * 8 + e],
-                                                  c * EV / kGroup * 8));
-      else
+      if constexpr (kScaled<C>) {
+        const int32_t at = p * 32 + e / 4 * 16 + g * 4 + e % 4;
+        if constexpr (TOGETHER)
+          return scaled<T, C, EV>(
+              S::template codes<EV * kBits<C> / 8>(lds.staged.v, at, wave, c * EV),
+              S::scale(lds.staged.v, at, wave, c * EV));
+        else
+          return scaled<T, C, EV>(
+              lds.staged[wave].template codes<EV * kBits<C> / 8>(at, c * EV),
+              lds.staged[wave].scale(at, c * EV));
+      } else {
         return Convert<T, C, EV>::of(v[p][e]);
+      }
     };
 
     const int32_t v0 = s * KS;
@@ -522,6 +727,7 @@ __device__ __forceinline__ void narrow_item(typename Narrow<T, C, DP>::Lds& lds,
         p[t][r] = power2(fmaf(sc[t][r], a.scale, -base));
         l += p[t][r];
       }
+    if constexpr (kScaled<C> && !TOGETHER) lds.staged[wave].put(v_chunks, brings, d);
 #pragma unroll
     for (int pr = 0; pr < KT / 2; ++pr) {
       if constexpr (sizeof(T) == 4) {
@@ -649,7 +855,11 @@ template <typename T, int DP>
 struct Wide {
   static constexpr int KS = 64;
   static constexpr int CHUNKS = DP / 8;                      // of eight elements, a row's
-  static constexpr int LOADS = KS * CHUNKS / kThreads;       // chunks a thread brings
+  // Dimensions that a thread brings at a time, and how often for a tile.
+  template <typename C>
+  static constexpr int EACH = kScaled<C> && DP > 32 ? 16 : 8;
+  template <typename C>
+  static constexpr int LOADS = (KS * DP / EACH<C> + kThreads - 1) / kThreads;
   static constexpr float LIFT = lift<T>(7.f);
   // The place of a chunk, and the chunk at a place.
   static __device__ __forceinline__ int place_k(int key, int chunk) {
@@ -697,7 +907,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
                                           typename Wide<T, DP>::Rows& lds_rows, int32_t& redo,
                                           const Args& a, int32_t item, int32_t kv_head) {
   using W = Wide<T, DP>;
-  constexpr int KS = W::KS, CHUNKS = W::CHUNKS, LOADS = W::LOADS;
+  constexpr int KS = W::KS, CHUNKS = W::CHUNKS;
   constexpr int NQ = DP / 16, ND = DP / 32;
   const Item it = item_of(a, item);
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, h = lane / 32, c = lane % 32;
@@ -734,45 +944,77 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
   };
   // The thread's chunks of a tile. Chunks past the head's dimensions hold its first ones: Q is
   // zero there, and nothing of V there is written.
-  using Raw = Words<8 * kBits<C> / 32>;
-  struct Staged {
+  using Raw = Words<W::template EACH<C> * kBits<C> / 32>;
+  constexpr int EACH = W::template EACH<C>, LOADS = W::template LOADS<C>;
+  struct Held {
     Raw k[LOADS], v[LOADS];
-    uint8_t k_scale[LOADS], v_scale[LOADS];      // of microscaled caches
+    uint32_t k_scales[LOADS], v_scales[LOADS];   // of microscaled caches
   };
-  const auto load = [&](int64_t (&row)[KS], typename W::Tile& kt, typename W::Tile& vt, Staged& x) {
+  // Of microscaled caches 16 dimensions at a time: the last of a head begin sooner where they
+  // would end behind it, and past it the first ones come again. `to` is the dimension they are.
+  struct Part {
+    int32_t key, from, to;
+  };
+  const auto part = [&](int i) {
+    constexpr int all = KS * DP / EACH;
+    const int32_t n = threadIdx.x + i * kThreads, at = n < all ? n : all - 1;
+    const int32_t d0 = at % (DP / EACH) * EACH, from = d0 + EACH <= d ? d0 : d0 < d ? d - EACH : 0;
+    return Part{at / (DP / EACH), from, d0 < d ? from : d0};
+  };
+  const auto load = [&](int64_t (&row)[KS], typename W::Tile& kt, typename W::Tile& vt, Held& x) {
+    if constexpr (kScaled<C>) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const Part p = part(i);
+        const int64_t from = row[p.key];
+        x.k[i] = load_bytes<code_bytes<C>(EACH)>(kc + from + code_bytes<C>(p.from));
+        x.v[i] = load_bytes<code_bytes<C>(EACH)>(vc + from + code_bytes<C>(p.from));
+        x.k_scales[i] = load_bytes<kScaleBytes>(kc + from + code_bytes<C>(d)).w[0];
+        x.v_scales[i] = load_bytes<kScaleBytes>(vc + from + code_bytes<C>(d)).w[0];
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int32_t at = threadIdx.x + i * kThreads, key = at / CHUNKS, to = at % CHUNKS;
       const int32_t dk = W::place_k(key, to) * 8, dv = W::place_v(key, to) * 8;
       const int64_t from = row[key];
-      const char* ks = kc + from + code_bytes<C>(dk < d ? dk : 0);
-      const char* vs = vc + from + code_bytes<C>(dv < d ? dv : 0);
+      const char* ks = kc + from + (dk < d ? dk : 0) * sizeof(C);
+      const char* vs = vc + from + (dv < d ? dv : 0) * sizeof(C);
       if constexpr (DIRECT) {
         const int32_t first = wave * kWave + i * kThreads;       // lane l's goes l places on
         bring16(ks, &kt[first]);
         bring16(vs, &vt[first]);
-      } else {
-        x.k[i] = load_bytes<code_bytes<C>(8)>(ks);
-        x.v[i] = load_bytes<code_bytes<C>(8)>(vs);
-        if constexpr (kScaled<C>) {
-          x.k_scale[i] = kc[from + code_bytes<C>(d) + (dk < d ? dk : 0) / kGroup];
-          x.v_scale[i] = vc[from + code_bytes<C>(d) + (dv < d ? dv : 0) / kGroup];
-        }
+      } else if constexpr (!kScaled<C>) {
+        x.k[i] = load_bytes<8 * sizeof(C)>(ks);
+        x.v[i] = load_bytes<8 * sizeof(C)>(vs);
       }
     }
   };
-  const auto store = [&](const Staged& x, typename W::Tile& kt, typename W::Tile& vt) {
-    if constexpr (!DIRECT) {
+  const auto store = [&](const Held& x, typename W::Tile& kt, typename W::Tile& vt) {
+    if constexpr (kScaled<C>) {
+      using Eight = Words<kBits<C> / 4>;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const Part p = part(i);
+#pragma unroll
+        for (int e = 0; e < EACH; e += 8) {
+          Eight k8, v8;
+          __builtin_memcpy(&k8, &x.k[i].w[e * kBits<C> / 32], sizeof(Eight));
+          __builtin_memcpy(&v8, &x.v[i].w[e * kBits<C> / 32], sizeof(Eight));
+          const int32_t shift = (p.from + e) / kGroup * 8, chunk = (p.to + e) / 8;
+          kt[p.key * CHUNKS + W::place_k(p.key, chunk)] = __builtin_bit_cast(
+              u32x4, scaled<T, C, 8>(k8, scale_of(x.k_scales[i], shift)));
+          vt[p.key * CHUNKS + W::place_v(p.key, chunk)] = __builtin_bit_cast(
+              u32x4, scaled<T, C, 8>(v8, scale_of(x.v_scales[i], shift)));
+        }
+      }
+    } else if constexpr (!DIRECT) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int32_t at = threadIdx.x + i * kThreads;
-        if constexpr (kScaled<C>) {
-          kt[at] = __builtin_bit_cast(u32x4, scaled<T, C, 8>(x.k[i], scale_of(x.k_scale[i], 0)));
-          vt[at] = __builtin_bit_cast(u32x4, scaled<T, C, 8>(x.v[i], scale_of(x.v_scale[i], 0)));
-        } else {
-          kt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.k[i]));
-          vt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.v[i]));
-        }
+        kt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.k[i]));
+        vt[at] = __builtin_bit_cast(u32x4, Convert<T, C, 8>::of(x.v[i]));
       }
     }
   };
@@ -787,7 +1029,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
   if (wave < 2) lds_rows[wave][lane] = row_of(a, place(wave)) * row_bytes;
   __syncthreads();
   {
-    Staged x;
+    Held x;
     load(lds_rows[0], k0, v0, x);
     store(x, k0, v0);
   }
@@ -798,8 +1040,8 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     // No branch around these loads, or every wait after them would be one for all: past the
     // last step they read the last key.
     const Place next = place(s + 2);
-    Staged staged;
-    load(lds_rows[half ^ 1], kn, vn, staged);
+    Held held;
+    load(lds_rows[half ^ 1], kn, vn, held);
     __builtin_amdgcn_sched_barrier(0);
 
     f32x16 sc[2];
@@ -876,7 +1118,7 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
         o[t] = mma32(Words<4>{{lo.w[0], lo.w[1], hi.w[0], hi.w[1]}}, p[i], o[t], T{});
       }
     __builtin_amdgcn_sched_barrier(0);
-    store(staged, kn, vn);
+    store(held, kn, vn);
     if (wave == 0) lds_rows[half][lane] = row_of(a, next) * row_bytes;
     arrive();
   };
@@ -926,32 +1168,35 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
 
 // A block is one or more KV heads of an item. Blocks go to the XCDs in turn: the ones of a
 // narrow item, which read neighbouring rows of the cache, go to the same one.
-template <typename T, typename C, int DP>
+template <typename T, typename C, int DP, bool TOGETHER>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_narrow(
     Args a, int32_t first, int32_t n) {
-  __shared__ typename Narrow<T, C, DP>::Lds lds;
+  using N = Narrow<T, C, DP>;
+  extern __shared__ __attribute__((aligned(16))) char shared[];
+  auto& lds = *reinterpret_cast<
+      std::conditional_t<TOGETHER, typename N::LdsTogether, typename N::Lds>*>(shared);
   constexpr int kXcds = 8;
   const int32_t each = a.kv_heads / a.together, b = blockIdx.x;
   const bool whole = b < n / kXcds * kXcds * each;
   const int32_t item = whole ? b / kXcds / each * kXcds + b % kXcds : b / each;
   const int32_t part = whole ? b / kXcds % each : b % each;
-  narrow_item<T, C, DP>(lds, a, first + item, part * a.together, blockIdx.y * 16);
+  narrow_item<T, C, DP, TOGETHER>(lds, a, first + item, part * a.together, blockIdx.y * 16);
 }
 
 constexpr int kWideRows = kWaves * 32;
 
-// Wide items from `wide` on, of 16-bit caches at 16-byte addresses. Neighbouring blocks are the
+// Wide items from `wide` on, of 16-bit caches at 16-byte addresses, whose tiles come into LDS
+// directly, and of microscaled ones. Neighbouring blocks are the
 // heads of an item, and where there are eight, all blocks of an XCD are of one head, whose
 // keys the items share in its L2.
 template <typename T, typename C, int DP>
-__global__ __launch_bounds__(kThreads, 2) void attend_wide(Args a,
-                                                                                 int32_t wide) {
+__global__ __launch_bounds__(kThreads, 2) void attend_wide(Args a, int32_t wide) {
   using W = Wide<T, DP>;
   __shared__ typename W::Tile k0, k1, v0, v1;
   __shared__ typename W::Rows rows;
   __shared__ int32_t redo;
-  wide_item<T, C, DP, true>(k0, k1, v0, v1, rows, redo, a, wide + blockIdx.x / a.kv_heads,
-                                        blockIdx.x % a.kv_heads);
+  wide_item<T, C, DP, !kScaled<C>>(k0, k1, v0, v1, rows, redo, a, wide + blockIdx.x / a.kv_heads,
+                                   blockIdx.x % a.kv_heads);
 }
 
 // `n_wide` wide items from `wide` on and `n_narrow` narrow ones from `narrow` on in one launch:
@@ -974,8 +1219,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_both(
                                            wide + before / a.together,
                                            before % a.together * each + part);
   else
-    narrow_item<T, C, DP>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared), a,
-                          narrow + run - before, part * a.together, 0);
+    narrow_item<T, C, DP, false>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared), a,
+                                 narrow + run - before, part * a.together, 0);
 }
 
 // Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, W

@@ -53,7 +53,7 @@ __host__ __device__ constexpr int32_t head_bytes(int32_t d) {
 // 2^e of a record's word: `shift` is eight times the group. 255 gives infinity, which is NaN to
 // the conversions and times an integer's zero.
 __device__ __forceinline__ float scale_of(uint32_t scales, int32_t shift) {
-  return __builtin_bit_cast(float, (scales >> shift & 255u) << 23);
+  return __builtin_bit_cast(float, __builtin_amdgcn_ubfe(scales, shift, 8) << 23);
 }
 
 template <int N>
