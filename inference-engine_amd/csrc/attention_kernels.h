@@ -568,11 +568,14 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
       }
     }
   };
+  // Loads end behind 96 dimensions.
+  const auto within = [](int32_t d0) { return d0 < DP ? d0 : 0; };
   const auto k_of = [&](int t, int i) {
+    const int32_t d0 = within((4 * i + g) * EL);
     if constexpr (TOGETHER)
-      return S::template codes<code_bytes<C>(EL)>(lds.staged.k, t * 16 + c, wave, (4 * i + g) * EL);
+      return S::template codes<code_bytes<C>(EL)>(lds.staged.k, t * 16 + c, wave, d0);
     else if constexpr (kScaled<C>)
-      return lds.staged[wave].template codes<code_bytes<C>(EL)>(t * 16 + c, (4 * i + g) * EL);
+      return lds.staged[wave].template codes<code_bytes<C>(EL)>(t * 16 + c, d0);
     else
       return k[t][i];
   };
@@ -593,10 +596,6 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
 #pragma unroll
       for (int w = 0; w < KW; ++w) r.w[w] = x.w[e * EK * kBits<C> / 32 + w];
       if (EK * kBits<C> < 32) r.w[0] >>= e * EK * kBits<C> % 32;
-      // What lies behind 96 dimensions of 8 bits is no code.
-      if (4 * NL * EL > DP && (i + 1) * 4 * EL > DP)
-#pragma unroll
-        for (int w = 0; w < KW; ++w) r.w[w] &= (4 * i + g) * EL < DP ? ~0u : 0u;
       return r;
     }
     const int32_t d0 = (4 * i + g) * EL + e * EK;
@@ -659,7 +658,7 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
         for (int e = 0; e < MF; ++e) {
           const auto raw = feed(whole, i, e);
           if constexpr (kScaled<C>)
-            sc[t] = mma16(scaled<T, C, EK>(raw, k_scale(t, (4 * i + g) * EL + e * EK)),
+            sc[t] = mma16(scaled<T, C, EK>(raw, k_scale(t, within((4 * i + g) * EL) + e * EK)),
                           q[i * MF + e], sc[t], T{});
           else
             sc[t] = mma16(Convert<T, C, EK>::of(raw), q[i * MF + e], sc[t], T{});
@@ -676,15 +675,13 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
     // V of key `e` of the lane's eight of pair `p`.
     const auto v_of = [&](int p, int e) {
       if constexpr (kScaled<C>) {
-        const int32_t at = p * 32 + e / 4 * 16 + g * 4 + e % 4;
+        const int32_t at = p * 32 + e / 4 * 16 + g * 4 + e % 4, d0 = within(c * EV);
         if constexpr (TOGETHER)
-          return scaled<T, C, EV>(
-              S::template codes<EV * kBits<C> / 8>(lds.staged.v, at, wave, c * EV),
-              S::scale(lds.staged.v, at, wave, c * EV));
+          return scaled<T, C, EV>(S::template codes<EV * kBits<C> / 8>(lds.staged.v, at, wave, d0),
+                                  S::scale(lds.staged.v, at, wave, d0));
         else
-          return scaled<T, C, EV>(
-              lds.staged[wave].template codes<EV * kBits<C> / 8>(at, c * EV),
-              lds.staged[wave].scale(at, c * EV));
+          return scaled<T, C, EV>(lds.staged[wave].template codes<EV * kBits<C> / 8>(at, d0),
+                                  lds.staged[wave].scale(at, d0));
       } else {
         return Convert<T, C, EV>::of(v[p][e]);
       }
@@ -950,16 +947,19 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
     Raw k[LOADS], v[LOADS];
     uint32_t k_scales[LOADS], v_scales[LOADS];   // of microscaled caches
   };
-  // Of microscaled caches 16 dimensions at a time: the last of a head begin sooner where they
-  // would end behind it, and past it the first ones come again. `to` is the dimension they are.
+  // Of microscaled caches 16 dimensions at a time, for the places of the dimensions from `to` on.
+  // Where only eight are left, those and the eight before them: they change places, so that the
+  // place behind them holds the latter.
   struct Part {
     int32_t key, from, to;
+    bool turned;
   };
   const auto part = [&](int i) {
     constexpr int all = KS * DP / EACH;
     const int32_t n = threadIdx.x + i * kThreads, at = n < all ? n : all - 1;
-    const int32_t d0 = at % (DP / EACH) * EACH, from = d0 + EACH <= d ? d0 : d0 < d ? d - EACH : 0;
-    return Part{at / (DP / EACH), from, d0 < d ? from : d0};
+    const int32_t d0 = at % (DP / EACH) * EACH;
+    const bool turned = d0 < d && d < d0 + EACH;
+    return Part{at / (DP / EACH), turned ? d - EACH : d0 < d ? d0 : 0, d0, turned};
   };
   const auto load = [&](int64_t (&row)[KS], typename W::Tile& kt, typename W::Tile& vt, Held& x) {
     if constexpr (kScaled<C>) {
@@ -1002,7 +1002,8 @@ __device__ __forceinline__ void wide_item(typename Wide<T, DP>::Tile& k0,
           Eight k8, v8;
           __builtin_memcpy(&k8, &x.k[i].w[e * kBits<C> / 32], sizeof(Eight));
           __builtin_memcpy(&v8, &x.v[i].w[e * kBits<C> / 32], sizeof(Eight));
-          const int32_t shift = (p.from + e) / kGroup * 8, chunk = (p.to + e) / 8;
+          const int32_t shift = (p.from + e) / kGroup * 8;
+          const int32_t chunk = (p.to + (p.turned ? EACH - 8 - e : e)) / 8;
           kt[p.key * CHUNKS + W::place_k(p.key, chunk)] = __builtin_bit_cast(
               u32x4, scaled<T, C, 8>(k8, scale_of(x.k_scales[i], shift)));
           vt[p.key * CHUNKS + W::place_v(p.key, chunk)] = __builtin_bit_cast(

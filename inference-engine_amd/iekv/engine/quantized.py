@@ -105,9 +105,14 @@ class QuantizedPool(KVPool):
         self.format = format
         self.num_kv_heads = heads
         self.head_dim = head_dim
+        # What each call hands the library.
         self._shape = _ops.MxCache(FORMATS[format], heads, head_dim, block_size, self.num_blocks)
+        self._shape_ref = ctypes.byref(self._shape)
         self._addresses = (ctypes.c_uint64 * len(self._ptrs))(*self._ptrs)
         self._at = ctypes.addressof(self._addresses)
+        self._index = self._arrays[0].get_device()
+        self._write = _ops.entry("iekv_mx_write_slots")
+        self._read = _ops.entry("iekv_mx_read_rows")
 
     def same_shape(self, other: KVPool) -> bool:
         return super().same_shape(other) and self.format == getattr(other, "format", self.format)
@@ -118,7 +123,7 @@ class QuantizedPool(KVPool):
 
     def _rows(self, t: torch.Tensor, what: str) -> torch.Tensor:
         """Rows as the library reads them: as they are where their heads are contiguous."""
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{what} on {t.device}, pool on {self.device}")
         if t.dtype not in _TYPES:
             raise ValueError(f"{what} of {t.dtype}: float32, float16 or bfloat16 are quantised")
@@ -130,13 +135,14 @@ class QuantizedPool(KVPool):
     def _slots(self, slots) -> torch.Tensor:
         """Slots on the device: a device tensor as it is, host ones checked and uploaded."""
         if isinstance(slots, torch.Tensor) and slots.device.type != "cpu":
-            if slots.device != self.device:
+            if slots.get_device() != self._index:
                 raise ValueError(f"slots on {slots.device}, pool on {self.device}")
             if slots.dim() != 1 or slots.dtype.is_floating_point or slots.dtype.is_complex or \
                     slots.dtype == torch.bool:
                 raise TypeError(f"slots must be integers in one dimension, got "
                                 f"{tuple(slots.shape)} {slots.dtype}")
-            return slots.to(torch.int64).contiguous()
+            return slots if slots.dtype == torch.int64 and slots.is_contiguous() else \
+                slots.to(torch.int64).contiguous()
         host = integer_ids(slots, "slot")
         rows = self.num_blocks * self.block_size
         bad = host[(host < 0) | (host >= rows)]
@@ -156,12 +162,13 @@ class QuantizedPool(KVPool):
                              f"{len(block_table)}")
         used = block_table[:needed]
         if isinstance(used, torch.Tensor) and used.device.type != "cpu":
-            if used.device != self.device:
+            if used.get_device() != self._index:
                 raise ValueError(f"block table on {used.device}, pool on {self.device}")
             if used.dim() != 1 or used.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"a device block table must be int32 or int64 in one dimension, "
                                 f"got {tuple(used.shape)} {used.dtype}")
-            return used.to(torch.int32).contiguous()
+            return used if used.dtype == torch.int32 and used.is_contiguous() else \
+                used.to(torch.int32).contiguous()
         return self._upload(self.host_ids(used, what="context block").astype(np.int32),
                             "a block table")
 
@@ -175,17 +182,16 @@ class QuantizedPool(KVPool):
             return torch.from_numpy(np.ascontiguousarray(host)).pin_memory().to(
                 self.device, non_blocking=True)
 
-    def _call(self, function: str, *args) -> None:
+    def _call(self, f, *args) -> None:
         """Call an entry point with the pool's shape first and its stream last, on its device."""
-        f, stream = _ops.entry(function), current_stream_handle(self.device)
-        shape = ctypes.byref(self._shape)
-        if self.device.index == current_device():
-            code = f(shape, *args, stream)
+        stream = current_stream_handle(self.device)
+        if self._index == current_device():
+            code = f(self._shape_ref, *args, stream)
         else:
             with torch.cuda.device(self.device):
-                code = f(shape, *args, stream)
+                code = f(self._shape_ref, *args, stream)
         if code:
-            _ops.fail(function, code)
+            _ops.fail(f.__name__, code)
 
 
 def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tensor,
@@ -197,8 +203,8 @@ def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tenso
         raise ValueError(f"K rows of {k.dtype} and V rows of {v.dtype}")
     where = pool._slots(slots)
     n_layers, n = k.shape[:2]
-    strides = (_ints("q", k.stride()[:3]), _ints("q", v.stride()[:3]))
-    pool._call("iekv_mx_write_slots", pool._arrays_from(first_layer),
+    strides = (_ints("q", k.stride()), _ints("q", v.stride()))
+    pool._call(pool._write, pool._arrays_from(first_layer),
                pool._arrays_from(pool.num_layers + first_layer), n_layers, _TYPES[k.dtype],
                k.data_ptr(), strides[0].buffer_info()[0], v.data_ptr(),
                strides[1].buffer_info()[0], where.data_ptr(), n)
@@ -213,6 +219,6 @@ def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, cont
     table = pool._table(block_table, context_len)
     out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim), dtype=dtype,
                       device=pool.device)
-    pool._call("iekv_mx_read_rows", pool._arrays_from(first_array), n_arrays, table.data_ptr(),
+    pool._call(pool._read, pool._arrays_from(first_array), n_arrays, table.data_ptr(),
                context_len, _TYPES[dtype], out.data_ptr())
     return out

@@ -140,18 +140,23 @@ def test_shared_prefixes(gpu, query, format, shared, contexts, queries):
     check(q, k[0], v[0], pool, tables, contexts, queries, shared_blocks=shared)
 
 
-@pytest.mark.parametrize("kv_heads", [1, 2, 4, 6, 8])
+@pytest.mark.parametrize("kv_heads, dim, query", [
+    (1, 128, BF16), (2, 128, BF16), (4, 128, F16), (6, 128, BF16), (8, 128, BF16), (8, 128, F32),
+    (4, 96, BF16), (12, 64, F16), (4, 32, BF16), (4, 64, F32), (8, 80, BF16), (4, 120, F16)])
 @pytest.mark.parametrize("format", FORMATS)
-def test_long_streams(gpu, kv_heads, format):
+def test_long_streams(gpu, kv_heads, dim, query, format):
     """Steps whose workgroups take several heads, whose items are cut into parts, and both;
-    blocks that are in several tables and several times in one."""
-    contexts = [9000 // kv_heads + 131 * i for i in range(48)]
-    bs, dim, blocks = 16, 128, 150
-    pool, k, v = make_pool(blocks, bs, kv_heads, dim, format, BF16, 19)
+    blocks that are in several tables and several times in one; a window that starts anywhere
+    in a block."""
+    contexts = [20000 // kv_heads + 131 * i for i in range(64)]
+    bs, blocks = 16, 150
+    assert sum(contexts) * kv_heads > 4 * 256 * 4 * 256      # long: of four heads together
+    pool, k, v = make_pool(blocks, bs, kv_heads, dim, format, query, 19)
     gen = torch.Generator().manual_seed(20)
     tables = [torch.randint(blocks, (-(-c // bs),), generator=gen).tolist() for c in contexts]
-    q = queries_of(48, 4 * kv_heads, dim, BF16, 21)
-    check(q, k[0], v[0], pool, tables, contexts, [1] * 48)
+    q = queries_of(64, 4 * kv_heads, dim, query, 21)
+    check(q, k[0], v[0], pool, tables, contexts, [1] * 64)
+    check(q[:32], k[0], v[0], pool, tables[32:], contexts[32:], [1] * 32, window=4001, sinks=5)
 
 
 @pytest.mark.parametrize("format", FORMATS)
