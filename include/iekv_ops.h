@@ -121,14 +121,30 @@ int iekv_mx_write_slots(const iekv_mx_cache* cache, const uint64_t* k_arrays,
                         const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
                         hipStream_t stream);
 
+/* The same with the slots in HOST memory: checked (IEKV_ERR_RANGE for one outside the pool), then
+ * carried in the launches' own arguments, IEKV_MX_INLINE_SLOTS tokens per launch. */
+#define IEKV_MX_INLINE_SLOTS 128
+int iekv_mx_write_slots_ids(const iekv_mx_cache* cache, const uint64_t* k_arrays,
+                            const uint64_t* v_arrays, int32_t n_layers, int32_t row_type,
+                            const void* k, const int64_t* k_strides, const void* v,
+                            const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
+                            hipStream_t stream);
+
 /* Read a context back as values: out [n_arrays][context_len][num_kv_heads][head_dim] of out_type
  * (F32, F16 or BF16; rounded to nearest even), row j of array i from the array at arrays[i]
  * (HOST array of device addresses), row table[j / block_size] * block_size + j % block_size
- * (int32, device memory). Rows of blocks outside the pool are left untouched. A context of
- * 2^32 / (num_kv_heads * head_dim / 8) rows or more is refused. */
+ * (int32, device memory). Rows of blocks outside the pool are left untouched. Runs on the
+ * current device, which has to be the arrays'. */
 int iekv_mx_read_rows(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
                       const int32_t* table, int64_t context_len, int32_t out_type, void* out,
                       hipStream_t stream);
+
+/* The same with the table in HOST memory: checked (IEKV_ERR_RANGE for a used block outside the
+ * pool), then carried in the launches' own arguments, IEKV_MX_INLINE_BLOCKS blocks per launch. */
+#define IEKV_MX_INLINE_BLOCKS 256
+int iekv_mx_read_rows_ids(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
+                          const int32_t* table, int64_t context_len, int32_t out_type, void* out,
+                          hipStream_t stream);
 
 #define IEKV_LOGPROBS_MAX_TOP 64
 

@@ -90,13 +90,25 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, const Divisor& by) {
 // what finds a lane's place is paid once.
 constexpr int kAtOnce = 2;
 
+// Slots or block ids: in device memory, or in a launch's own arguments, where no upload has to
+// come before it (a call with a list of 37 slots 12.6 us of the host against 24.9).
+template <typename I, int N>
+struct Ids {
+  I id[N];
+  __device__ __forceinline__ I operator[](uint32_t i) const { return id[i]; }
+};
+template <typename I>
+struct Ids<I, 0> {
+  const I* id;
+  __device__ __forceinline__ I operator[](uint32_t i) const { return id[i]; }
+};
+
 struct WriteArgs {
   uint64_t k_cache, v_cache;                   // of the first layer
   int64_t k_cache_stride, v_cache_stride;      // bytes from one layer's to the next
   const void* k;
   const void* v;
   int64_t k_layer, k_token, k_head, v_layer, v_token, v_head;   // strides in elements
-  const int64_t* slots;
   int64_t n_slots;
   uint32_t n;                                  // tokens
   int32_t layers, heads, head_dim;
@@ -108,8 +120,8 @@ struct WriteArgs {
 // caches, which leaves room there for the codes' lines to be filled: 32 layers of 2,001 tokens
 // of eight bf16 heads of 128 to mxfp8 63 us (6.3 TB/s), 74 with ordinary loads; one layer at a
 // time 86, four at a time 75 (of those).
-template <typename T, typename C>
-__global__ __launch_bounds__(kThreads) void write_rows(WriteArgs a) {
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kThreads) void write_rows(WriteArgs a, Ids<int64_t, N> slots) {
   constexpr int EACH = kEach<T>, LANES = kLanes<T>;
   const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t t = quotient(at, a.row_lanes), in_row = at - t * a.row_lanes.d;
@@ -128,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void write_rows(WriteArgs a) {
                       head * (o ? a.v_head : a.k_head);
       raw[l][o] = stream_bytes<16>(from + (in ? d0 : 0));
     }
-  const int64_t slot = a.slots[t];
+  const int64_t slot = slots[t];
   const int32_t codes = code_bytes<C>(a.head_dim), record = head_bytes<C>(a.head_dim);
 #pragma unroll
   for (int l = 0; l < kAtOnce; ++l)
@@ -167,7 +179,7 @@ struct ReadArgs {
   uint64_t cache;                              // the first array
   int64_t cache_stride;
   void* out;                                   // [arrays][n][heads][head_dim]
-  const int32_t* table;
+  int64_t out_stride;                          // elements from one array's values to the next
   uint32_t n;                                  // rows
   int32_t arrays, heads, head_dim;
   int64_t num_blocks;
@@ -179,15 +191,15 @@ struct ReadArgs {
 // rows of eight heads of 128 from mxfp8 to bf16 190 us (6.3 TB/s), 204 with ordinary stores and
 // 230 with loads past the caches; one array at a time 234, four 204. (Stores past the caches pay
 // only where a wave's are on end: with 32 bytes a lane 285.)
-template <typename T, typename C>
-__global__ __launch_bounds__(kThreads) void read_rows(ReadArgs a) {
+template <typename T, typename C, int N>
+__global__ __launch_bounds__(kThreads) void read_rows(ReadArgs a, Ids<int32_t, N> table) {
   constexpr int EACH = kEach<T>;
   const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t j = quotient(at, a.row_lanes), in_row = at - j * a.row_lanes.d;
   if (j >= a.n) return;
   const uint32_t head = quotient(in_row, a.lanes), b = quotient(j, a.block_size);
   const int32_t d0 = (in_row - head * a.lanes.d) * EACH, array0 = blockIdx.y * kAtOnce;
-  const int32_t block = a.table[b];
+  const int32_t block = table[b];
   if (block < 0 || block >= a.num_blocks) return;
   const int64_t row = static_cast<int64_t>(block) * a.block_size.d + (j - b * a.block_size.d);
   const char* from = reinterpret_cast<const char*>(a.cache) +
@@ -205,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void read_rows(ReadArgs a) {
   for (int i = 0; i < kAtOnce; ++i) {
     if (array0 + i >= a.arrays) break;
     T* to = static_cast<T*>(a.out) +
-            static_cast<int64_t>(array0 + i) * a.n * a.heads * a.head_dim + in_array;
+            static_cast<int64_t>(array0 + i) * a.out_stride + in_array;
     stream_out<16>(to, scaled<T, C, EACH>(code[i], scale_of(scales[i], d0 / kGroup * 8)));
   }
 }
@@ -263,6 +275,126 @@ void with_types(int32_t row, int32_t cache, F f) {
 }
 
 constexpr int32_t kMostLayers = 65535;         // of a launch: its grid's second dimension
+constexpr int32_t kSlots = IEKV_MX_INLINE_SLOTS, kBlocks = IEKV_MX_INLINE_BLOCKS;
+
+// N: slots on the host that a launch carries, 0 for those on the device.
+template <int N>
+int write(const iekv_mx_cache* cache, const uint64_t* k_arrays, const uint64_t* v_arrays,
+          int32_t n_layers, int32_t row_type, const void* k, const int64_t* k_strides,
+          const void* v, const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
+          hipStream_t stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (!is_float(row_type)) return set_error(IEKV_ERR_INVALID, "rows of type %d", row_type);
+  if (n_layers < 0 || n_tokens < 0)
+    return set_error(IEKV_ERR_INVALID, "%d layers of %lld tokens", n_layers,
+                     static_cast<long long>(n_tokens));
+  if (!n_layers || !n_tokens) return IEKV_OK;
+  if (!k_arrays || !v_arrays || !k || !k_strides || !v || !v_strides || !slots)
+    return set_error(IEKV_ERR_INVALID, "null argument");
+  const int64_t size = row_type == IEKV_TYPE_F32 ? 4 : 2;
+  const int64_t n_slots = cache->num_blocks * cache->block_size;
+  for (int64_t t = 0; N && t < n_tokens; ++t)
+    if (slots[t] < 0 || slots[t] >= n_slots)
+      return set_error(IEKV_ERR_RANGE, "slot %lld out of range for a pool of %lld slots",
+                       static_cast<long long>(slots[t]), static_cast<long long>(n_slots));
+  const int32_t lanes = (cache->head_dim + kGroup - 1) / kGroup *
+                        (row_type == IEKV_TYPE_F32 ? kLanes<float> : kLanes<Bf16>);
+  // Tokens of a launch.
+  const int64_t most = N ? N : kMaxGrid * kThreads / (cache->num_kv_heads * lanes);
+  for (int32_t l = 0; l < n_layers;) {
+    WriteArgs a{};
+    const int32_t run = std::min(std::min(run_of(k_arrays, l, n_layers, &a.k_cache_stride),
+                                          run_of(v_arrays, l, n_layers, &a.v_cache_stride)),
+                                 kMostLayers);
+    a.k_cache = k_arrays[l];
+    a.v_cache = v_arrays[l];
+    a.k_layer = k_strides[0], a.k_token = k_strides[1], a.k_head = k_strides[2];
+    a.v_layer = v_strides[0], a.v_token = v_strides[1], a.v_head = v_strides[2];
+    a.n_slots = n_slots;
+    a.layers = run;
+    a.heads = cache->num_kv_heads;
+    a.head_dim = cache->head_dim;
+    a.lanes = divisor(lanes);
+    a.row_lanes = divisor(a.heads * lanes);
+    for (int64_t t = 0; t < n_tokens; t += most) {
+      a.k = static_cast<const char*>(k) + (l * a.k_layer + t * a.k_token) * size;
+      a.v = static_cast<const char*>(v) + (l * a.v_layer + t * a.v_token) * size;
+      a.n = static_cast<uint32_t>(std::min(most, n_tokens - t));
+      Ids<int64_t, N> ids;
+      if constexpr (N)
+        std::copy_n(slots + t, a.n, ids.id);
+      else
+        ids.id = slots + t;
+      const int64_t threads = static_cast<int64_t>(a.n) * a.heads * lanes;
+      const dim3 grid((threads + kThreads - 1) / kThreads, (run + kAtOnce - 1) / kAtOnce);
+      with_types(row_type, cache->cache_type, [&](auto row, auto code) {
+        hipLaunchKernelGGL((write_rows<decltype(row), decltype(code), N>), grid, dim3(kThreads), 0,
+                           stream, a, ids);
+      });
+      IEKV_OPS_HIP(hipGetLastError());
+    }
+    l += run;
+  }
+  return IEKV_OK;
+}
+
+template <int N>
+int read(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
+         const int32_t* table, int64_t context_len, int32_t out_type, void* out,
+         hipStream_t stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (!is_float(out_type)) return set_error(IEKV_ERR_INVALID, "values of type %d", out_type);
+  if (n_arrays < 0 || context_len < 0 || context_len > IEKV_ATTENTION_MAX_CONTEXT)
+    return set_error(IEKV_ERR_INVALID, "%d arrays of a context of %lld", n_arrays,
+                     static_cast<long long>(context_len));
+  if (!n_arrays || !context_len) return IEKV_OK;
+  if (!arrays || !table || !out) return set_error(IEKV_ERR_INVALID, "null argument");
+  const int64_t size = out_type == IEKV_TYPE_F32 ? 4 : 2, bs = cache->block_size;
+  const int64_t used = (context_len + bs - 1) / bs;
+  for (int64_t b = 0; N && b < used; ++b)
+    if (table[b] < 0 || table[b] >= cache->num_blocks)
+      return set_error(IEKV_ERR_RANGE, "block id %d out of range for a pool of %lld blocks",
+                       table[b], static_cast<long long>(cache->num_blocks));
+  const int32_t lanes = cache->head_dim * static_cast<int32_t>(size) / 16;
+  const int64_t row = static_cast<int64_t>(cache->num_kv_heads) * cache->head_dim;
+  // Blocks of a launch.
+  const int64_t fit = kMaxGrid * kThreads / (cache->num_kv_heads * lanes) / bs;
+  const int64_t most = N ? std::min<int64_t>(N, fit) : fit;
+  if (!most)
+    return set_error(IEKV_ERR_INVALID, "blocks of %lld rows of %d heads are too large",
+                     static_cast<long long>(bs), cache->num_kv_heads);
+  for (int32_t i = 0; i < n_arrays;) {
+    ReadArgs a{};
+    const int32_t run = std::min(run_of(arrays, i, n_arrays, &a.cache_stride), kMostLayers);
+    a.cache = arrays[i];
+    a.out_stride = context_len * row;
+    a.arrays = run;
+    a.heads = cache->num_kv_heads;
+    a.head_dim = cache->head_dim;
+    a.lanes = divisor(lanes);
+    a.row_lanes = divisor(a.heads * lanes);
+    a.block_size = divisor(cache->block_size);
+    a.num_blocks = cache->num_blocks;
+    for (int64_t b = 0; b < used; b += most) {
+      a.n = static_cast<uint32_t>(std::min(most * bs, context_len - b * bs));
+      a.out = static_cast<char*>(out) + (i * context_len + b * bs) * row * size;
+      Ids<int32_t, N> ids;
+      if constexpr (N)
+        std::copy_n(table + b, std::min(most, used - b), ids.id);
+      else
+        ids.id = table + b;
+      const int64_t threads = a.n * static_cast<int64_t>(a.heads) * lanes;
+      const dim3 grid((threads + kThreads - 1) / kThreads, (run + kAtOnce - 1) / kAtOnce);
+      with_types(out_type, cache->cache_type, [&](auto value, auto code) {
+        hipLaunchKernelGGL((read_rows<decltype(value), decltype(code), N>), grid, dim3(kThreads),
+                           0, stream, a, ids);
+      });
+      IEKV_OPS_HIP(hipGetLastError());
+    }
+    i += run;
+  }
+  return IEKV_OK;
+}
 
 }  // namespace
 }  // namespace iekv_ops
@@ -283,91 +415,29 @@ int iekv_mx_write_slots(const iekv_mx_cache* cache, const uint64_t* k_arrays,
                         const void* k, const int64_t* k_strides, const void* v,
                         const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
                         hipStream_t stream) {
-  if (const int rc = check_cache(cache)) return rc;
-  if (!is_float(row_type)) return set_error(IEKV_ERR_INVALID, "rows of type %d", row_type);
-  if (n_layers < 0 || n_tokens < 0)
-    return set_error(IEKV_ERR_INVALID, "%d layers of %lld tokens", n_layers,
-                     static_cast<long long>(n_tokens));
-  if (!n_layers || !n_tokens) return IEKV_OK;
-  if (!k_arrays || !v_arrays || !k || !k_strides || !v || !v_strides || !slots)
-    return set_error(IEKV_ERR_INVALID, "null argument");
-  const int64_t size = row_type == IEKV_TYPE_F32 ? 4 : 2;
-  const int32_t lanes = (cache->head_dim + kGroup - 1) / kGroup *
-                        (row_type == IEKV_TYPE_F32 ? kLanes<float> : kLanes<Bf16>);
-  const int64_t most = kMaxGrid * kThreads / (cache->num_kv_heads * lanes);  // tokens of a launch
-  for (int32_t l = 0; l < n_layers;) {
-    WriteArgs a{};
-    const int32_t run = std::min(std::min(run_of(k_arrays, l, n_layers, &a.k_cache_stride),
-                                          run_of(v_arrays, l, n_layers, &a.v_cache_stride)),
-                                 kMostLayers);
-    for (int64_t t = 0; t < n_tokens; t += most) {
-      a.k_cache = k_arrays[l];
-      a.v_cache = v_arrays[l];
-      a.k_layer = k_strides[0], a.k_token = k_strides[1], a.k_head = k_strides[2];
-      a.v_layer = v_strides[0], a.v_token = v_strides[1], a.v_head = v_strides[2];
-      a.k = static_cast<const char*>(k) + (l * a.k_layer + t * a.k_token) * size;
-      a.v = static_cast<const char*>(v) + (l * a.v_layer + t * a.v_token) * size;
-      a.slots = slots + t;
-      a.n_slots = cache->num_blocks * cache->block_size;
-      a.n = static_cast<uint32_t>(std::min(most, n_tokens - t));
-      a.layers = run;
-      a.heads = cache->num_kv_heads;
-      a.head_dim = cache->head_dim;
-      a.lanes = divisor(lanes);
-      a.row_lanes = divisor(a.heads * lanes);
-      const int64_t threads = static_cast<int64_t>(a.n) * a.heads * lanes;
-      const dim3 grid((threads + kThreads - 1) / kThreads, (run + kAtOnce - 1) / kAtOnce);
-      with_types(row_type, cache->cache_type, [&](auto row, auto code) {
-        hipLaunchKernelGGL((write_rows<decltype(row), decltype(code)>), grid, dim3(kThreads), 0,
-                           stream, a);
-      });
-      IEKV_OPS_HIP(hipGetLastError());
-    }
-    l += run;
-  }
-  return IEKV_OK;
+  return write<0>(cache, k_arrays, v_arrays, n_layers, row_type, k, k_strides, v, v_strides, slots,
+                  n_tokens, stream);
+}
+
+int iekv_mx_write_slots_ids(const iekv_mx_cache* cache, const uint64_t* k_arrays,
+                            const uint64_t* v_arrays, int32_t n_layers, int32_t row_type,
+                            const void* k, const int64_t* k_strides, const void* v,
+                            const int64_t* v_strides, const int64_t* slots, int64_t n_tokens,
+                            hipStream_t stream) {
+  return write<kSlots>(cache, k_arrays, v_arrays, n_layers, row_type, k, k_strides, v, v_strides,
+                       slots, n_tokens, stream);
 }
 
 int iekv_mx_read_rows(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
                       const int32_t* table, int64_t context_len, int32_t out_type, void* out,
                       hipStream_t stream) {
-  if (const int rc = check_cache(cache)) return rc;
-  if (!is_float(out_type)) return set_error(IEKV_ERR_INVALID, "values of type %d", out_type);
-  if (n_arrays < 0 || context_len < 0 || context_len > IEKV_ATTENTION_MAX_CONTEXT)
-    return set_error(IEKV_ERR_INVALID, "%d arrays of a context of %lld", n_arrays,
-                     static_cast<long long>(context_len));
-  if (!n_arrays || !context_len) return IEKV_OK;
-  if (!arrays || !table || !out) return set_error(IEKV_ERR_INVALID, "null argument");
-  const int64_t size = out_type == IEKV_TYPE_F32 ? 4 : 2;
-  const int32_t lanes = cache->head_dim * static_cast<int32_t>(size) / 16;
-  for (int32_t i = 0; i < n_arrays;) {
-    ReadArgs a{};
-    const int32_t run = std::min(run_of(arrays, i, n_arrays, &a.cache_stride), kMostLayers);
-    a.cache = arrays[i];
-    a.out = static_cast<char*>(out) +
-            i * context_len * cache->num_kv_heads * cache->head_dim * size;
-    a.table = table;
-    a.n = static_cast<uint32_t>(context_len);
-    a.heads = cache->num_kv_heads;
-    a.head_dim = cache->head_dim;
-    a.arrays = run;
-    a.lanes = divisor(lanes);
-    a.row_lanes = divisor(a.heads * lanes);
-    a.block_size = divisor(cache->block_size);
-    a.num_blocks = cache->num_blocks;
-    const int64_t threads = context_len * a.heads * lanes;
-    if ((threads + kThreads - 1) / kThreads > kMaxGrid)
-      return set_error(IEKV_ERR_INVALID, "a context of %lld rows of %d heads is too long",
-                       static_cast<long long>(context_len), a.heads);
-    const dim3 grid((threads + kThreads - 1) / kThreads, (run + kAtOnce - 1) / kAtOnce);
-    with_types(out_type, cache->cache_type, [&](auto value, auto code) {
-      hipLaunchKernelGGL((read_rows<decltype(value), decltype(code)>), grid, dim3(kThreads), 0,
-                         stream, a);
-    });
-    IEKV_OPS_HIP(hipGetLastError());
-    i += run;
-  }
-  return IEKV_OK;
+  return read<0>(cache, arrays, n_arrays, table, context_len, out_type, out, stream);
+}
+
+int iekv_mx_read_rows_ids(const iekv_mx_cache* cache, const uint64_t* arrays, int32_t n_arrays,
+                          const int32_t* table, int64_t context_len, int32_t out_type, void* out,
+                          hipStream_t stream) {
+  return read<kBlocks>(cache, arrays, n_arrays, table, context_len, out_type, out, stream);
 }
 
 }  // extern "C"

@@ -22,6 +22,8 @@ IEKV_TYPE_MXFP8, IEKV_TYPE_MXINT8, IEKV_TYPE_MXFP4 = 5, 6, 7
 ATTENTION_MAX_DIM = 128              # IEKV_ATTENTION_MAX_DIM
 ATTENTION_MAX_GROUP = 128            # IEKV_ATTENTION_MAX_GROUP
 ATTENTION_MAX_CONTEXT = 1 << 30      # IEKV_ATTENTION_MAX_CONTEXT
+MX_INLINE_SLOTS = 128                # IEKV_MX_INLINE_SLOTS
+MX_INLINE_BLOCKS = 256               # IEKV_MX_INLINE_BLOCKS
 LOGPROBS_MAX_TOP = 64                # IEKV_LOGPROBS_MAX_TOP
 
 
@@ -53,11 +55,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "iekv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                             c_float, c_void_p, c_void_p, c_int64, c_void_p]),
     "iekv_mx_head_bytes": (c_int64, [c_int32, c_int32]),
-    "iekv_mx_write_slots": (c_int, [POINTER(MxCache), c_void_p, c_void_p, c_int32, c_int32,
-                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
-                                    c_void_p]),
-    "iekv_mx_read_rows": (c_int, [POINTER(MxCache), c_void_p, c_int32, c_void_p, c_int64, c_int32,
-                                  c_void_p, c_void_p]),
+    **{name: (c_int, [POINTER(MxCache), c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                      c_void_p, c_void_p, c_void_p, c_int64, c_void_p])
+       for name in ("iekv_mx_write_slots", "iekv_mx_write_slots_ids")},
+    **{name: (c_int, [POINTER(MxCache), c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p,
+                      c_void_p])
+       for name in ("iekv_mx_read_rows", "iekv_mx_read_rows_ids")},
     "iekv_logprobs_workspace": (c_int64, [c_int32, c_int64, c_int64, c_int32]),
     "iekv_logprobs": (c_int, [c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,

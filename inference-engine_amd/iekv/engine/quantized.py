@@ -42,6 +42,11 @@ FORMATS = {"mxfp8": _ops.IEKV_TYPE_MXFP8, "mxint8": _ops.IEKV_TYPE_MXINT8,
 _CODE_BITS = {"mxfp8": 8, "mxint8": 8, "mxfp4": 4}
 _SCALE_BYTES = 4
 
+# Longest host lists of slots and host block tables that the library carries in its launches'
+# arguments, in two launches; longer ones are uploaded.
+HOST_SLOTS_MAX = 2 * _ops.MX_INLINE_SLOTS
+HOST_TABLE_MAX = 2 * _ops.MX_INLINE_BLOCKS
+
 _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE_F16,
           torch.bfloat16: _native.IEKV_TYPE_BF16}
 
@@ -112,7 +117,9 @@ class QuantizedPool(KVPool):
         self._at = ctypes.addressof(self._addresses)
         self._index = self._arrays[0].get_device()
         self._write = _ops.entry("iekv_mx_write_slots")
+        self._write_ids = _ops.entry("iekv_mx_write_slots_ids")
         self._read = _ops.entry("iekv_mx_read_rows")
+        self._read_ids = _ops.entry("iekv_mx_read_rows_ids")
 
     def same_shape(self, other: KVPool) -> bool:
         return super().same_shape(other) and self.format == getattr(other, "format", self.format)
@@ -132,8 +139,9 @@ class QuantizedPool(KVPool):
             t = t.resolve_neg()
         return t if t.stride(-1) == 1 else t.contiguous()
 
-    def _slots(self, slots) -> torch.Tensor:
-        """Slots on the device: a device tensor as it is, host ones checked and uploaded."""
+    def _slots(self, slots):
+        """The slots of a call and the entry point that takes them: a device tensor as it is,
+        host ones checked, and long lists uploaded."""
         if isinstance(slots, torch.Tensor) and slots.device.type != "cpu":
             if slots.get_device() != self._index:
                 raise ValueError(f"slots on {slots.device}, pool on {self.device}")
@@ -142,7 +150,7 @@ class QuantizedPool(KVPool):
                 raise TypeError(f"slots must be integers in one dimension, got "
                                 f"{tuple(slots.shape)} {slots.dtype}")
             return slots if slots.dtype == torch.int64 and slots.is_contiguous() else \
-                slots.to(torch.int64).contiguous()
+                slots.to(torch.int64).contiguous(), self._write
         host = integer_ids(slots, "slot")
         rows = self.num_blocks * self.block_size
         bad = host[(host < 0) | (host >= rows)]
@@ -150,10 +158,13 @@ class QuantizedPool(KVPool):
             raise IndexError(f"slot {bad[0]} out of range for a pool of {rows} slots")
         if np.unique(host).size != host.size:
             raise ValueError("slots must be distinct")
-        return self._upload(host, "slots")
+        if host.size <= HOST_SLOTS_MAX:
+            return np.ascontiguousarray(host), self._write_ids
+        return self._upload(host, f"a list of {host.size} slots"), self._write
 
-    def _table(self, block_table, context_len: int) -> torch.Tensor:
-        """The entries of a block table that a context uses, on the device."""
+    def _table(self, block_table, context_len: int):
+        """The entries of a block table that a context uses, and the entry point that takes
+        them."""
         if context_len < 0:
             raise ValueError(f"context of {context_len}")
         needed = -(-context_len // self.block_size)
@@ -168,17 +179,17 @@ class QuantizedPool(KVPool):
                 raise TypeError(f"a device block table must be int32 or int64 in one dimension, "
                                 f"got {tuple(used.shape)} {used.dtype}")
             return used if used.dtype == torch.int32 and used.is_contiguous() else \
-                used.to(torch.int32).contiguous()
-        return self._upload(self.host_ids(used, what="context block").astype(np.int32),
-                            "a block table")
+                used.to(torch.int32).contiguous(), self._read
+        host = self.host_ids(used, what="context block").astype(np.int32)
+        if host.size <= HOST_TABLE_MAX:
+            return host, self._read_ids
+        return self._upload(host, f"a table of {host.size} blocks"), self._read
 
     def _upload(self, host: np.ndarray, what: str) -> torch.Tensor:
         with torch.cuda.device(self.device):
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{what} on the host are uploaded, which a stream under "
-                                   "capture cannot do: pass a device tensor")
-            if not host.size:
-                return torch.empty(0, dtype=torch.int64, device=self.device)
+                raise RuntimeError(f"{what} is uploaded, which a stream under capture cannot do: "
+                                   "pass a device tensor")
             return torch.from_numpy(np.ascontiguousarray(host)).pin_memory().to(
                 self.device, non_blocking=True)
 
@@ -194,6 +205,10 @@ class QuantizedPool(KVPool):
             _ops.fail(f.__name__, code)
 
 
+def _address(ids) -> int:
+    return ids.data_ptr() if isinstance(ids, torch.Tensor) else ids.ctypes.data
+
+
 def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tensor,
           slots) -> None:
     """``[n_layers, n, H, D]`` rows into the slots of layers ``first_layer`` and on (the calls
@@ -201,13 +216,13 @@ def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tenso
     k, v = pool._rows(k, "K rows"), pool._rows(v, "V rows")
     if k.dtype != v.dtype:
         raise ValueError(f"K rows of {k.dtype} and V rows of {v.dtype}")
-    where = pool._slots(slots)
+    where, entry = pool._slots(slots)
     n_layers, n = k.shape[:2]
     strides = (_ints("q", k.stride()), _ints("q", v.stride()))
-    pool._call(pool._write, pool._arrays_from(first_layer),
+    pool._call(entry, pool._arrays_from(first_layer),
                pool._arrays_from(pool.num_layers + first_layer), n_layers, _TYPES[k.dtype],
                k.data_ptr(), strides[0].buffer_info()[0], v.data_ptr(),
-               strides[1].buffer_info()[0], where.data_ptr(), n)
+               strides[1].buffer_info()[0], _address(where), n)
 
 
 def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, context_len: int,
@@ -216,9 +231,9 @@ def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, cont
     dtype = torch.bfloat16 if dtype is None else dtype
     if dtype not in _TYPES:
         raise ValueError(f"values of {dtype}: float32, float16 or bfloat16 are read back")
-    table = pool._table(block_table, context_len)
+    table, entry = pool._table(block_table, context_len)
     out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim), dtype=dtype,
                       device=pool.device)
-    pool._call(pool._read, pool._arrays_from(first_array), n_arrays, table.data_ptr(),
-               context_len, _TYPES[dtype], out.data_ptr())
+    pool._call(entry, pool._arrays_from(first_array), n_arrays, _address(table), context_len,
+               _TYPES[dtype], out.data_ptr())
     return out

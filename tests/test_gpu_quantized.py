@@ -248,6 +248,33 @@ def test_nothing_to_do(gpu, format):
     assert all((t == 9).all() for t in k + v)
 
 
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 256, 257, 600, 1500])
+def test_lists_of_any_length(gpu, n):
+    """Slots and tables on the host, carried in one launch, in two, and uploaded."""
+    from iekv.engine.slots import gather_rows, gather_rows_arrays, write_slots, write_slots_layers
+
+    format, bs = "mxint8", 1
+    pool, k, v = make_pool(n + 40, bs, 2, 24, format, layers=2)
+    gen = torch.Generator().manual_seed(n)
+    slots = torch.randperm(n + 40, generator=gen)[:n]
+    rows = rows_of((2, 2, n, 2, 24), F16, n)
+    write_slots_layers(pool, rows[0], rows[1], slots.tolist())
+    want = encode(rows, format)
+    for given in (slots.tolist(), slots, slots.numpy(), slots.to(gpu), slots.to(gpu).int()):
+        got = gather_rows_arrays(pool, given, n, dtype=F32)
+        assert same(got.cpu(), decode(want, format).to(F32).flatten(0, 1))
+    for given in (slots, slots.numpy().astype("int32"), tuple(slots.tolist()), slots.to(gpu).int()):
+        k[1].zero_()
+        write_slots(pool, 1, rows[0, 1], rows[1, 1], given)
+        assert same_records(k[1][slots], want[0, 1], format)
+    # Of blocks of several rows, of which the context's last holds some.
+    wide, *_ = make_pool(n, 3, 2, 24, format)
+    write_slots(wide, 0, rows[0, 0], rows[1, 0], list(range(3, 3 + n)) if n > 1 else [0])
+    blocks = list(range(1, -(-n // 3) + 1)) if n > 1 else [0]
+    got = gather_rows(wide, 1, blocks, n, dtype=F32)
+    assert same(got.cpu(), decode(want, format).to(F32)[1, 0])
+
+
 def test_offsets_past_32_bits(gpu):
     """Rows, caches and values behind the first 4 GiB."""
     from iekv.engine.slots import gather_rows, write_slots
@@ -279,6 +306,8 @@ def test_streams_and_graphs(gpu, format):
     rows = rows_of((10, 2, 64), BF16, 1)
     slots = torch.arange(10, device=gpu)
     table = torch.tensor([0, 1], dtype=torch.int32, device=gpu)
+    long, *_ = make_pool(600, 1, 2, 64, format)
+    many = rows_of((300, 2, 64), BF16, 2)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -289,10 +318,11 @@ def test_streams_and_graphs(gpu, format):
     with torch.cuda.graph(graph):
         write_slots(pool, 0, rows, rows, slots)
         out = gather_rows(pool, 0, table, 20)
+        listed = gather_rows(pool, 0, [3, 1], 20)     # a short list travels with its launch
         with pytest.raises(RuntimeError, match="capture"):
-            write_slots(pool, 0, rows, rows, list(range(10)))
+            write_slots(long, 0, many, many, list(range(300)))
         with pytest.raises(RuntimeError, match="capture"):
-            gather_rows(pool, 0, [0, 1], 20)
+            gather_rows(long, 0, list(range(600)), 600)
     for seed in range(4):
         rows.copy_(rows_of((10, 2, 64), BF16, seed + 9))
         slots.copy_(torch.randperm(128, generator=torch.Generator().manual_seed(seed))[:10])
@@ -301,7 +331,7 @@ def test_streams_and_graphs(gpu, format):
         eager = gather_rows(pool, 0, table, 20)
         torch.cuda.synchronize()
         assert same_records(k[0][slots], encode(rows, format), format)
-        assert same(out, eager)
+        assert same(out, eager) and same(listed, gather_rows(pool, 0, [3, 1], 20))
 
 
 def test_refusals(gpu):

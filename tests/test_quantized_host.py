@@ -12,7 +12,7 @@ from quantized_reference import CODES, FORMATS, decode, encode
 from test_attention_plan import make, ops  # noqa: F401  (the library, and a plan of two sequences)
 from test_ops_host import on_stub  # noqa: F401  (the library over a HIP that runs nothing)
 
-INVALID = -1
+INVALID, RANGE = -1, -4
 MOST = (2 ** 32 - 1) // 256          # workgroups of a launch
 
 
@@ -23,6 +23,9 @@ def test_types_and_structure_agree_with_the_header():
     for name in ("MXFP8", "MXINT8", "MXFP4"):
         value = re.search(rf"IEKV_TYPE_{name} = (\d+)", text).group(1)
         assert int(value) == getattr(_ops, f"IEKV_TYPE_{name}")
+    for name in ("INLINE_SLOTS", "INLINE_BLOCKS"):
+        value = re.search(rf"#define IEKV_MX_{name} (\d+)", text).group(1)
+        assert int(value) == getattr(_ops, f"MX_{name}")
     assert ctypes.sizeof(_ops.MxCache) == 24
 
 
@@ -136,18 +139,28 @@ def test_refusals_come_before_anything_is_enqueued(on_stub):  # noqa: F811
               ("read(out_type=5)", "values of type 5"), ("read(n=-2)", "-2 arrays"),
               ("read(context=-1)", "context of -1"),
               ("read(context=(1 << 30) + 1)", "context of 1073741825"),
-              ("read(context=1 << 26)", "too long"),
+              ("read(block_size=1 << 20, num_kv_heads=4096)", "too large"),
               *[(f"read({a}=None)", "null") for a in ("arrays", "table", "out")]]
     got = on_stub(CALLS + f"""
 bad = [said(eval(call)) for call in {[c for c, _ in cases]!r}]
+for f, x in ((ops.iekv_mx_write_slots_ids, i64(0, 1600)), (ops.iekv_mx_write_slots_ids, i64(-1))):
+    bad.append(said(f(cache(), u64(1 << 20), u64(1 << 21), 1, 3, 1 << 22, i64(1, 1, 1), 1 << 22,
+                      i64(1, 1, 1), x, len(x), 77)))
+for x in ((0, 100), (7, -5)):
+    bad.append(said(ops.iekv_mx_read_rows_ids(cache(), u64(1 << 20), 1,
+                                              (ctypes.c_int32 * 2)(*x), 20, 3, 1 << 22, 77)))
 bad.append(said(ops.iekv_mx_write_slots(None, *[None] * 2, 0, 3, *[None] * 5, 0, None)))
 bad.append(said(ops.iekv_mx_read_rows(None, None, 0, None, 0, 3, None, None)))
 none = [write(n=0, k=None, rows=None), write(layers=0, v=None), read(context=0, out=None),
         read(n=0, arrays=None)]
 print(json.dumps([bad, none, launches()]))
 """)
-    for (rc, message), (call, want) in zip(got[0], cases + [("", "cache is null")] * 2):
-        assert rc == INVALID and want in message, (call, rc, message)
+    ids = [("", "slot 1600 out of range"), ("", "slot -1 out"), ("", "block id 100 out of range"),
+           ("", "block id -5 out")]
+    last = [("", "cache is null")] * 2
+    assert len(got[0]) == len(cases + ids + last)
+    for (rc, message), (call, want) in zip(got[0], cases + ids + last):
+        assert rc == (RANGE if (call, want) in ids else INVALID) and want in message, (call, rc)
     assert got[1] == [0, 0, 0, 0] and got[2] == []
 
 
@@ -177,3 +190,20 @@ print(json.dumps([said(rc), launches()]))
     lanes = 16 * 16                                  # of a token
     assert len(got[1]) > 1 and all(x[1] <= MOST for x in got[1])
     assert sum(x[1] for x in got[1]) == ((1 << 28) + 5) * lanes // 256
+    got = on_stub(CALLS + """
+rcs = [read(context=(1 << 30) - 5), read(context=(1 << 29) + 1, block_size=1000, out_type=1)]
+slots = list(range(300)) + [7]
+rcs.append(ops.iekv_mx_write_slots_ids(cache(), u64(1 << 20), u64(1 << 21), 1, 3, 1 << 22,
+                                       i64(1, 1, 1), 1 << 22, i64(1, 1, 1), i64(*slots), 301, 77))
+ids = (ctypes.c_int32 * 600)(*([5] * 600))
+rcs.append(ops.iekv_mx_read_rows_ids(cache(), u64(1 << 20), 1, ids, 9591, 3, 1 << 22, 77))
+print(json.dumps([rcs, launches()]))
+""")
+    assert got[0] == [0] * 4
+    grids = [x[1] for x in got[1]]
+    assert max(grids) <= MOST
+    rows = [grids.pop() for _ in range(6)][::-1]     # the lists' launches: 128 slots, 256 blocks
+    assert rows[:3] == [128 // 2, 128 // 2, -(-45 // 2)]
+    assert rows[3:] == [4096 // 2, 4096 // 2, -(-(9591 - 8192) // 2)]
+    first = 1 + (((1 << 30) - 5) * 128 - 1) // 256   # of bf16: 16 lanes a head, 8 heads
+    assert abs(sum(grids) - first - ((1 << 29) + 1)) <= len(grids)
