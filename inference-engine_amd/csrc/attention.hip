@@ -97,10 +97,12 @@ bool together_fits(const iekv_attention_shape& s) {
          s.head_dim % kGroup == 0;
 }
 
-// Workgroups of a long stream that a compute unit runs at once. Those that take four heads
-// together have the records of 64 keys in LDS.
+// Workgroups that a long stream is cut into for each compute unit. Of four heads' long records two
+// keep the memory busy, and more drive each other's lines out of L2: 48 sequences of 6,000 tokens
+// of eight mxfp8 heads of 128 104 us with two, 129 with three. Short records take more work for
+// their bytes: 128 sequences of 4,200 tokens in mxfp4 122 us with three, 140 with two.
 int32_t streams_at_once(const iekv_attention_shape& s) {
-  return !together_fits(s) ? 3 : head_bytes_of(s) * kWaves * 64 * 2 < (36 << 10) ? 4 : 2;
+  return together_fits(s) && head_bytes_of(s) * kWaves >= 400 ? 2 : 3;
 }
 
 template <typename T, typename C, int DP>
