@@ -154,8 +154,7 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
   }
   if (narrow && !both) {
     // Only 32-bit queries have narrow items of more than 16 heads.
-    const auto run = [&](auto kernel, size_t bytes, std::atomic<uint64_t>* asked) {
-      IEKV_OPS_HIP(allow_lds(kernel, static_cast<int>(bytes), plan.device, asked));
+    const auto run = [&](auto kernel, size_t bytes) {
       return in_launches(narrow, each, [&](int64_t first, int64_t n) {
         hipLaunchKernelGGL(kernel, dim3(n * each, (a.group + 15) / 16), dim3(kThreads), bytes,
                            stream, a, static_cast<int32_t>(plan.narrow.first + first),
@@ -163,17 +162,20 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
       });
     };
     using N = Narrow<T, C, DP>;
-    static std::atomic<uint64_t> asked{0}, asked_together{0};
-    int rc = IEKV_OK;
+    constexpr size_t kUnasked = 64 << 10;           // of LDS for a workgroup
+    static_assert(sizeof(typename N::Lds) <= kUnasked);
+    bool done = false;
     if constexpr (kScaled<C>) {
-      if (a.together == kWaves && together_fits(plan.shape))
-        rc = run(attend_narrow<T, C, DP, true>, sizeof(typename N::LdsTogether), &asked_together);
-      else
-        rc = run(attend_narrow<T, C, DP, false>, sizeof(typename N::Lds), &asked);
-    } else {
-      rc = run(attend_narrow<T, C, DP, false>, sizeof(typename N::Lds), &asked);
+      static_assert(sizeof(typename N::LdsTogether) <= kUnasked);
+      if (a.together == kWaves && together_fits(plan.shape)) {
+        if (const int rc = run(attend_narrow<T, C, DP, true>, sizeof(typename N::LdsTogether)))
+          return rc;
+        done = true;
+      }
     }
-    if (rc) return rc;
+    if (!done) {
+      if (const int rc = run(attend_narrow<T, C, DP, false>, sizeof(typename N::Lds))) return rc;
+    }
   }
   if (plan.joined) {
     // Few rows have many parts each: their loads are spread over four waves.

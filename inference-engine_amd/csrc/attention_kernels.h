@@ -294,7 +294,9 @@ __device__ __forceinline__ void store_out(T* out, const float* x) {
 // operands. Records begin at any multiple of 4, and as operands sixteen lanes would take from
 // sixteen of them: what bounds such loads is the first cache, a line at a time. So a wave brings
 // the 64 records in chunks of 16 bytes laid end to end (of 32 dimensions 4), the last of each the
-// one that ends with the scales, and every lane's load is full.
+// one that ends with the scales, and every lane's load is full. 48 sequences of 6,000 tokens of
+// eight mxfp8 heads of 128 120 us, against 137 where lanes load their operands' records (and 183
+// past the caches: neighbouring records share their lines, which are then brought twice).
 template <typename C, int DP>
 struct Staged {
   static constexpr int KEYS = 64;
@@ -306,8 +308,8 @@ struct Staged {
   alignas(16) char bytes[kScaled<C> ? KEYS * PITCH : 16];
 
   using Chunk = Words<W / 4>;
-  // Load n of a wave brings chunk (n + lane) % CHUNKS of key n * 64 / CHUNKS + ...: 64 n + lane in
-  // all.
+  // What a lane brings with each of its loads: chunk 64 n + lane of all. The key, the bytes into
+  // its record, and its place here.
   struct Lane {
     int32_t key[CHUNKS], from[CHUNKS], to[CHUNKS];
   };
@@ -445,7 +447,7 @@ struct Together {
 
 // What bounds it is the cache's stream: each wave has a step's K or V (64 keys; 32 of 32-bit
 // caches) in flight at any time, straight into the registers the products read, and nothing
-// but block ids passes through LDS. A workgroup takes 1, 2 or 4 neighbouring KV heads: its
+// but block ids passes through LDS (of microscaled caches the records do, see above). A workgroup takes 1, 2 or 4 neighbouring KV heads: its
 // waves go through the same keys, whose rows are neighbours in memory, and waves of the same
 // head take steps in turn and join at the end. 64 sequences of 16,000 tokens of eight bf16
 // heads of 128: 5.45 TB/s with four waves on one head, 5.95 with one on each of four, 6.3 with

@@ -27,6 +27,7 @@ another.
 from __future__ import annotations
 
 import ctypes
+import operator
 from array import array as _ints
 from typing import Sequence as Seq
 
@@ -166,7 +167,7 @@ class QuantizedPool(KVPool):
         """The entries of a block table that a context uses, and the entry point that takes
         them."""
         if context_len < 0:
-            raise ValueError(f"context of {context_len}")
+            raise ValueError(f"context of {context_len} rows")
         needed = -(-context_len // self.block_size)
         if len(block_table) < needed:
             raise IndexError(f"context of {context_len} needs {needed} blocks, table has "
@@ -231,6 +232,7 @@ def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, cont
     dtype = torch.bfloat16 if dtype is None else dtype
     if dtype not in _TYPES:
         raise ValueError(f"values of {dtype}: float32, float16 or bfloat16 are read back")
+    context_len = operator.index(context_len)
     table, entry = pool._table(block_table, context_len)
     out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim), dtype=dtype,
                       device=pool.device)

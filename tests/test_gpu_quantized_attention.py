@@ -195,6 +195,46 @@ def test_what_masked_places_hold_stays_out(gpu, query, format):
         assert torch.isnan(got[-1]).all()
 
 
+@pytest.mark.parametrize("kv_heads, dim", [(8, 128), (4, 96), (4, 64), (3, 72)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_long_streams_beside_rows_that_are_no_numbers(gpu, kv_heads, dim, format):
+    """Every row that no query sees holds such groups: before the windows, behind the contexts
+    in their last blocks, in blocks of nobody. One visible V has one: it shows in its group of
+    its own sequence's outputs and nowhere else."""
+    from iekv.engine.attention import AttentionPlan, attend
+
+    contexts, bs, blocks, window, sinks = [5003 + 37 * i for i in range(64)], 16, 400, 4000, 3
+    pool, k, v = make_pool(blocks, bs, kv_heads, dim, format, BF16, 41)
+    gen = torch.Generator().manual_seed(42)
+    half = blocks // 2
+    tables, seen = [], torch.zeros(blocks * bs, dtype=torch.bool)
+    for c in contexts:                        # blocks of the window from one half of the pool,
+        first, n = (c - window) // bs, -(-c // bs)      # hidden ones from the other
+        table = torch.randint(half, (n,), generator=gen)
+        table[1:first] += half
+        table[0], table[-1] = 2 * half - 1, 2 * half - 2
+        tables.append(table.tolist())
+        for j in list(range(sinks)) + list(range(max(first, 1) * bs, c)):
+            if j >= c - window or j < sinks:
+                seen[int(table[j // bs]) * bs + j % bs] = True
+    hidden = ~seen
+    assert hidden.sum() > half * bs // 2
+    for t in pool._arrays:
+        t[hidden.cuda(), :, -4:] = 255
+    q = queries_of(64, 4 * kv_heads, dim, BF16, 43)
+    got, _ = check(q, k[0], v[0], pool, tables, contexts, [1] * 64, window=window, sinks=sinks)
+    assert torch.isfinite(got).all()
+    slot, shown = tables[9][0] * bs + 1, 1    # a sink of all sequences
+    codes = 16 if format == "mxfp4" else 32
+    pool._arrays[1][slot, kv_heads - 1, shown * codes:shown * codes + codes] = 0
+    pool._arrays[1][slot, kv_heads - 1, -4 + shown] = 255
+    plan = AttentionPlan(pool, tables, contexts, [1] * 64, 4 * kv_heads, window=window, sinks=sinks)
+    bad = torch.isnan(attend(plan, 0, q))
+    want = torch.zeros_like(bad)
+    want[:, 4 * (kv_heads - 1):, 32 * shown:32 * shown + 32] = True
+    assert torch.equal(bad, want)
+
+
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("query", TYPES, ids=str)
 def test_magnitudes(gpu, query, format):

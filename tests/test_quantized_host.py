@@ -100,6 +100,26 @@ def test_plans_take_microscaled_caches(ops, cache_type, query_type, taken):  # n
         assert rc == INVALID and f"cache of type {cache_type}" in message
 
 
+def test_wide_items_that_all_run_at_once_pair_long_with_short(ops):  # noqa: F811
+    """512 workgroups, two to a compute unit: item i runs beside item i + 32."""
+    n, context = 2048, 7777
+    blocks = -(-context // 16)
+    rc, plan, _ = make(ops, contexts=(context,), queries=(n,), tables=(tuple(range(blocks)),),
+                       num_blocks=blocks, num_heads=32, num_kv_heads=8, head_dim=128)
+    assert rc == 0
+    words, count = ctypes.POINTER(ctypes.c_int32)(), ctypes.c_int64()
+    tokens, workspace = ctypes.c_int64(), ctypes.c_int64()
+    ops.iekv_attention_plan_info(plan, ctypes.byref(words), ctypes.byref(count),
+                                 ctypes.byref(tokens), ctypes.byref(workspace))
+    items = [words[12 * i:12 * i + 12] for i in range(64)]
+    keys = [it[4] - it[3] + it[6] - it[5] for it in items]
+    assert sorted(keys) == [context - n + 32 * (i + 1) for i in range(64)]
+    assert keys[:32] == sorted(keys, reverse=True)[:32]
+    pairs = [a + b for a, b in zip(keys[:32], keys[32:])]
+    assert max(pairs) - min(pairs) <= 32
+    ops.iekv_attention_plan_destroy(plan)
+
+
 CALLS = """
 def cache(**over):
     fields = dict(dict(cache_type=5, num_kv_heads=8, head_dim=128, block_size=16, num_blocks=100),
