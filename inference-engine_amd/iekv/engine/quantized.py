@@ -115,7 +115,7 @@ class QuantizedPool(KVPool):
         self._shape = _ops.MxCache(FORMATS[format], heads, head_dim, block_size, self.num_blocks)
         self._shape_ref = ctypes.byref(self._shape)
         self._addresses = (ctypes.c_uint64 * len(self._ptrs))(*self._ptrs)
-        self._at = ctypes.addressof(self._addresses)
+        self._at = ctypes.addressof(self._addresses)       # K of each layer, then V
         self._index = self._arrays[0].get_device()
         self._write = _ops.entry("iekv_mx_write_slots")
         self._write_ids = _ops.entry("iekv_mx_write_slots_ids")
@@ -124,10 +124,6 @@ class QuantizedPool(KVPool):
 
     def same_shape(self, other: KVPool) -> bool:
         return super().same_shape(other) and self.format == getattr(other, "format", self.format)
-
-    def _arrays_from(self, array: int) -> int:
-        """Where the addresses of the arrays from ``array`` on begin."""
-        return self._at + 8 * array
 
     def _rows(self, t: torch.Tensor, what: str) -> torch.Tensor:
         """Rows as the library reads them: as they are where their heads are contiguous."""
@@ -140,28 +136,32 @@ class QuantizedPool(KVPool):
             t = t.resolve_neg()
         return t if t.stride(-1) == 1 else t.contiguous()
 
-    def _slots(self, slots):
-        """The slots of a call and the entry point that takes them: a device tensor as it is,
+    def _slots(self, slots, n: int):
+        """The slots of n rows and the entry point that takes them: a device tensor as it is,
         host ones checked, and long lists uploaded."""
-        if isinstance(slots, torch.Tensor) and slots.device.type != "cpu":
+        if isinstance(slots, torch.Tensor) and slots.get_device() >= 0:
             if slots.get_device() != self._index:
                 raise ValueError(f"slots on {slots.device}, pool on {self.device}")
-            if slots.dim() != 1 or slots.dtype.is_floating_point or slots.dtype.is_complex or \
-                    slots.dtype == torch.bool:
-                raise TypeError(f"slots must be integers in one dimension, got "
-                                f"{tuple(slots.shape)} {slots.dtype}")
-            return slots if slots.dtype == torch.int64 and slots.is_contiguous() else \
-                slots.to(torch.int64).contiguous(), self._write
+            if slots.dtype != torch.int64:
+                if slots.dtype.is_floating_point or slots.dtype.is_complex or \
+                        slots.dtype == torch.bool:
+                    raise TypeError(f"slots must be integers, not {slots.dtype}")
+                slots = slots.to(torch.int64)
+            if slots.dim() != 1 or slots.shape[0] != n:
+                raise ValueError(f"slots of shape {tuple(slots.shape)} for {n} rows")
+            return slots if slots.is_contiguous() else slots.contiguous(), self._write
         host = integer_ids(slots, "slot")
+        if host.size != n:
+            raise ValueError(f"{host.size} slots for {n} rows")
         rows = self.num_blocks * self.block_size
         bad = host[(host < 0) | (host >= rows)]
         if bad.size:
             raise IndexError(f"slot {bad[0]} out of range for a pool of {rows} slots")
         if np.unique(host).size != host.size:
             raise ValueError("slots must be distinct")
-        if host.size <= HOST_SLOTS_MAX:
+        if n <= HOST_SLOTS_MAX:
             return np.ascontiguousarray(host), self._write_ids
-        return self._upload(host, f"a list of {host.size} slots"), self._write
+        return self._upload(host, f"a list of {n} slots"), self._write
 
     def _table(self, block_table, context_len: int):
         """The entries of a block table that a context uses, and the entry point that takes
@@ -169,22 +169,26 @@ class QuantizedPool(KVPool):
         if context_len < 0:
             raise ValueError(f"context of {context_len} rows")
         needed = -(-context_len // self.block_size)
-        if len(block_table) < needed:
-            raise IndexError(f"context of {context_len} needs {needed} blocks, table has "
-                             f"{len(block_table)}")
-        used = block_table[:needed]
-        if isinstance(used, torch.Tensor) and used.device.type != "cpu":
-            if used.get_device() != self._index:
-                raise ValueError(f"block table on {used.device}, pool on {self.device}")
-            if used.dim() != 1 or used.dtype not in (torch.int32, torch.int64):
+        on_device = isinstance(block_table, torch.Tensor) and block_table.get_device() >= 0
+        held = block_table.shape[0] if on_device else len(block_table)
+        if held < needed:
+            raise IndexError(f"context of {context_len} needs {needed} blocks, table has {held}")
+        if on_device:
+            if block_table.get_device() != self._index:
+                raise ValueError(f"block table on {block_table.device}, pool on {self.device}")
+            if block_table.dim() != 1 or block_table.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"a device block table must be int32 or int64 in one dimension, "
-                                f"got {tuple(used.shape)} {used.dtype}")
-            return used if used.dtype == torch.int32 and used.is_contiguous() else \
-                used.to(torch.int32).contiguous(), self._read
-        host = self.host_ids(used, what="context block").astype(np.int32)
-        if host.size <= HOST_TABLE_MAX:
+                                f"got {tuple(block_table.shape)} {block_table.dtype}")
+            if block_table.dtype == torch.int32 and block_table.is_contiguous():
+                return block_table, self._read         # entries past the context are not read
+            return block_table[:needed].to(torch.int32).contiguous(), self._read
+        host = self.host_ids(block_table[:needed], what="context block")
+        if host.size != needed:
+            raise ValueError(f"a block table of {host.size} entries for {needed} blocks")
+        host = host.astype(np.int32)
+        if needed <= HOST_TABLE_MAX:
             return host, self._read_ids
-        return self._upload(host, f"a table of {host.size} blocks"), self._read
+        return self._upload(host, f"a table of {needed} blocks"), self._read
 
     def _upload(self, host: np.ndarray, what: str) -> torch.Tensor:
         with torch.cuda.device(self.device):
@@ -212,30 +216,35 @@ def _address(ids) -> int:
 
 def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tensor,
           slots) -> None:
-    """``[n_layers, n, H, D]`` rows into the slots of layers ``first_layer`` and on (the calls
-    of :mod:`iekv.engine.slots` have checked their shapes)."""
+    """``[n_layers, n, H, D]`` rows into the slots of layers ``first_layer`` and on."""
+    n_layers, n, heads, dim = k.shape
+    if heads != pool.num_kv_heads or dim != pool.head_dim:
+        raise ValueError(f"rows of shape {(heads, dim)} do not fit a pool of "
+                         f"{(pool.num_kv_heads, pool.head_dim)}")
     k, v = pool._rows(k, "K rows"), pool._rows(v, "V rows")
     if k.dtype != v.dtype:
         raise ValueError(f"K rows of {k.dtype} and V rows of {v.dtype}")
-    where, entry = pool._slots(slots)
-    n_layers, n = k.shape[:2]
-    strides = (_ints("q", k.stride()), _ints("q", v.stride()))
-    pool._call(entry, pool._arrays_from(first_layer),
-               pool._arrays_from(pool.num_layers + first_layer), n_layers, _TYPES[k.dtype],
-               k.data_ptr(), strides[0].buffer_info()[0], v.data_ptr(),
-               strides[1].buffer_info()[0], _address(where), n)
+    where, entry = pool._slots(slots, n)
+    if first_layer < 0 or first_layer + n_layers > pool.num_layers:
+        raise IndexError(f"layers {first_layer}..{first_layer + n_layers - 1} out of range for "
+                         f"{pool.num_layers} layers")
+    strides = _ints("q", (*k.stride(), *v.stride()))
+    at = strides.buffer_info()[0]
+    arrays = pool._at + 8 * first_layer            # K's; V's follow them
+    pool._call(entry, arrays, arrays + 8 * pool.num_layers, n_layers, _TYPES[k.dtype],
+               k.data_ptr(), at, v.data_ptr(), at + 32, _address(where), n)
 
 
 def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, context_len: int,
          dtype: torch.dtype | None) -> torch.Tensor:
     """``[n_arrays, context_len, H, D]`` values of a context (default: bfloat16)."""
-    dtype = torch.bfloat16 if dtype is None else dtype
-    if dtype not in _TYPES:
+    kind = _TYPES.get(torch.bfloat16 if dtype is None else dtype)
+    if kind is None:
         raise ValueError(f"values of {dtype}: float32, float16 or bfloat16 are read back")
     context_len = operator.index(context_len)
     table, entry = pool._table(block_table, context_len)
-    out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim), dtype=dtype,
-                      device=pool.device)
-    pool._call(entry, pool._arrays_from(first_array), n_arrays, _address(table), context_len,
-               _TYPES[dtype], out.data_ptr())
+    out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim),
+                      dtype=torch.bfloat16 if dtype is None else dtype, device=pool.device)
+    pool._call(entry, pool._at + 8 * first_array, n_arrays, _address(table), context_len, kind,
+               out.data_ptr())
     return out

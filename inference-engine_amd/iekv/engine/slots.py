@@ -121,13 +121,6 @@ def _write(pool: KVPool, first_layer: int, n_layers: int, n: int, k: torch.Tenso
                  current_stream_handle(pool.device))
 
 
-def _row_shape(pool: KVPool) -> tuple[int, ...]:
-    """What a row of the pool holds: its values' shape, where the cache holds records."""
-    if isinstance(pool, QuantizedPool):
-        return pool.num_kv_heads, pool.head_dim
-    return pool.tile_shape[1:]
-
-
 def _cache_dtype_only(pool: KVPool, dtype: torch.dtype | None) -> None:
     if dtype is not None and dtype != pool.dtype:
         raise ValueError(f"rows of a {pool.dtype} cache are read as they are, not as {dtype}")
@@ -144,17 +137,20 @@ def write_slots(pool: KVPool, layer: int, k: torch.Tensor, v: torch.Tensor, slot
     host slots given twice raise ValueError there (on the device, any of the rows may be held,
     or parts of several), and device slots outside the pool are skipped.
     """
+    if isinstance(pool, QuantizedPool):
+        if k.dim() != 3 or k.shape != v.shape:
+            raise ValueError(f"K rows {tuple(k.shape)} and V rows {tuple(v.shape)} must both be "
+                             "[n, H, D]")
+        quantized.write(pool, layer, k[None], v[None], slots)
+        return
     n = k.shape[0]
     if v.shape[0] != n or len(slots) != n:
         raise ValueError(f"{len(slots)} slots for {n} K rows and {v.shape[0]} V rows")
-    row = _row_shape(pool)
-    if tuple(k.shape[1:]) != row or tuple(v.shape[1:]) != row:
-        raise ValueError(f"rows of shape {tuple(k.shape[1:])} do not fit a pool of {row}")
+    if tuple(k.shape[1:]) != pool.tile_shape[1:] or tuple(v.shape[1:]) != pool.tile_shape[1:]:
+        raise ValueError(f"rows of shape {tuple(k.shape[1:])} do not fit a pool of "
+                         f"{pool.tile_shape[1:]}")
     if not 0 <= layer < pool.num_layers:
         raise IndexError(f"layer {layer} out of range for {pool.num_layers} layers")
-    if isinstance(pool, QuantizedPool):
-        quantized.write(pool, layer, k[None], v[None], slots)
-        return
     _write(pool, layer, 1, n, k, v, slots)
 
 
@@ -219,18 +215,18 @@ def write_slots_layers(pool: KVPool, k: torch.Tensor, v: torch.Tensor, slots,
     if k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"K rows {tuple(k.shape)} and V rows {tuple(v.shape)} must both be "
                          "[n_layers, n, H, D]")
-    n_layers, n = k.shape[0], k.shape[1]
-    if len(slots) != n:
-        raise ValueError(f"{len(slots)} slots for {n} rows per layer")
-    if tuple(k.shape[2:]) != _row_shape(pool):
-        raise ValueError(f"rows of shape {tuple(k.shape[2:])} do not fit a pool of "
-                         f"{_row_shape(pool)}")
-    if first_layer < 0 or first_layer + n_layers > pool.num_layers:
-        raise IndexError(f"layers {first_layer}..{first_layer + n_layers - 1} out of range for "
-                         f"{pool.num_layers} layers")
     if isinstance(pool, QuantizedPool):
         quantized.write(pool, first_layer, k, v, slots)
         return
+    n_layers, n = k.shape[0], k.shape[1]
+    if len(slots) != n:
+        raise ValueError(f"{len(slots)} slots for {n} rows per layer")
+    if tuple(k.shape[2:]) != pool.tile_shape[1:]:
+        raise ValueError(f"rows of shape {tuple(k.shape[2:])} do not fit a pool of "
+                         f"{pool.tile_shape[1:]}")
+    if first_layer < 0 or first_layer + n_layers > pool.num_layers:
+        raise IndexError(f"layers {first_layer}..{first_layer + n_layers - 1} out of range for "
+                         f"{pool.num_layers} layers")
     _write(pool, first_layer, n_layers, n, k, v, slots)
 
 

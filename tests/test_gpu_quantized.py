@@ -344,9 +344,21 @@ def test_refusals(gpu):
     slots = torch.arange(3, device=gpu)
     bad = [
         (ValueError, "slots for", lambda: write_slots(pool, 0, rows, rows, [1, 2])),
-        (ValueError, "do not fit", lambda: write_slots(pool, 0, rows[..., :24], rows, slots)),
-        (ValueError, "do not fit", lambda: write_slots(pool, 0, rows, rows[:, :1], slots)),
-        (IndexError, "layer 2", lambda: write_slots(pool, 2, rows, rows, slots)),
+        (ValueError, "do not fit", lambda: write_slots(pool, 0, rows[..., :24], rows[..., :24], slots)),
+        (ValueError, "must both be", lambda: write_slots(pool, 0, rows, rows[:, :1], slots)),
+        (ValueError, "do not fit", lambda: write_slots(pool, 0, rows[:, :1], rows[:, :1], slots)),
+        (ValueError, "must both be", lambda: write_slots(pool, 0, rows, rows[:2], slots)),
+        (ValueError, "must both be", lambda: write_slots_layers(pool, rows, rows, slots)),
+        (ValueError, "slots of shape", lambda: write_slots(pool, 0, rows, rows, slots[:2])),
+        (ValueError, "slots of shape",
+         lambda: write_slots(pool, 0, rows, rows, slots[:, None].repeat(1, 2))),
+        (ValueError, "6 slots",
+         lambda: write_slots(pool, 0, rows, rows, torch.arange(6).view(3, 2))),
+        (ValueError, "table of 4", lambda: gather_rows(pool, 0, [[1, 2], [3, 0]], 16)),
+        (TypeError, "one dimension", lambda: gather_rows(pool, 0, slots[:, None], 16)),
+        (TypeError, "integer", lambda: gather_rows(pool, 0, [1], 8.0)),
+        (IndexError, "layers 2..2", lambda: write_slots(pool, 2, rows, rows, slots)),
+        (IndexError, "layers -1..-1", lambda: write_slots(pool, -1, rows, rows, slots)),
         (IndexError, "layers 1..2",
          lambda: write_slots_layers(pool, rows[None].repeat(2, 1, 1, 1),
                                     rows[None].repeat(2, 1, 1, 1), slots, first_layer=1)),
