@@ -447,14 +447,15 @@ struct Together {
 
 // What bounds it is the cache's stream: each wave has a step's K or V (64 keys; 32 of 32-bit
 // caches) in flight at any time, straight into the registers the products read, and nothing
-// but block ids passes through LDS (of microscaled caches the records do, see above). A workgroup takes 1, 2 or 4 neighbouring KV heads: its
-// waves go through the same keys, whose rows are neighbours in memory, and waves of the same
-// head take steps in turn and join at the end. 64 sequences of 16,000 tokens of eight bf16
-// heads of 128: 5.45 TB/s with four waves on one head, 5.95 with one on each of four, 6.3 with
-// loads that pass the caches by besides (an 8-bit cache 4.7, 5.0 and 5.7). Of a pair of key
-// tiles (32 keys), lane group g = lane / 16 holds the weights of keys 8 g .. 8 g + 7: a lane
-// loads those keys' V, EV dimensions each, and turns them in its own registers into the EV
-// operands of V^T (dimension c EV + t at place c of tile t).
+// but block ids passes through LDS (of microscaled caches the records do, see above). A
+// workgroup takes 1, 2 or 4 neighbouring KV heads: its waves go through the same keys, whose
+// rows are neighbours in memory, and waves of the same head take steps in turn and join at the
+// end. 64 sequences of 16,000 tokens of eight bf16 heads of 128: 5.45 TB/s with four waves on
+// one head, 5.95 with one on each of four, 6.3 with loads that pass the caches by besides (an
+// 8-bit cache 4.7, 5.0 and 5.7). Of a pair of key tiles (32 keys), lane group g = lane / 16
+// holds the weights of keys 8 g .. 8 g + 7: a lane loads those keys' V, EV dimensions each,
+// and turns them in its own registers into the EV operands of V^T (dimension c EV + t at place
+// c of tile t).
 //
 // 16-bit operands hold a weight as two, its value rounded to the type and what that leaves:
 // together off by 2^-16 (bf16) of it, as good as 32 bits beside V's own. The second product is

@@ -209,8 +209,8 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // Two workgroups fit a compute unit. Long streams are cut for half as many again: 128
   // sequences of unlike lengths 182 us against 191 with two, of one length 175 against 173.
   if (!whole)
-    narrow = split(narrow, sh.kv_heads / plan.together, (plan.streams ? sh.at_once : 2) * compute_units, 256,
-                   64);
+    narrow = split(narrow, sh.kv_heads / plan.together,
+                   (plan.streams ? sh.at_once : 2) * compute_units, 256, 64);
   const int64_t narrow_blocks = int64_t(narrow.size()) * sh.kv_heads / plan.together;
   // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
   // are: they are cut only where more than half of the compute units would have none, and so

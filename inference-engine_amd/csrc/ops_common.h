@@ -95,7 +95,6 @@ __device__ __forceinline__ uint32_t lane_move(uint32_t x) {
 }
 constexpr int kQuad1 = 0xb1, kQuad2 = 0x4e, kQuad3 = 0x1b;   // lane ^ 1, ^ 2, ^ 3
 constexpr int kMirror8 = 0x141, kMirror16 = 0x140;           // lane ^ 7, ^ 15
-constexpr int kLast16 = 0x15f;                               // lane 15 of the row of 16
 
 // The word of lane ^ M.
 template <int M>
