@@ -98,9 +98,10 @@ bool together_fits(const iekv_attention_shape& s) {
 }
 
 // Workgroups that a long stream is cut into for each compute unit. Of four heads' long records two
-// keep the memory busy, and more drive each other's lines out of L2: 48 sequences of 6,000 tokens
-// of eight mxfp8 heads of 128 104 us with two, 129 with three. Short records take more work for
-// their bytes: 128 sequences of 4,200 tokens in mxfp4 122 us with three, 140 with two.
+// keep the memory busy (and have LDS for two), and more drive each other's lines out of L2: 48
+// sequences of 6,000 tokens of eight mxfp8 heads of 128 107 us with two, 127 with three. Short
+// records take more work for their bytes: 128 sequences of 4,200 tokens in mxfp4 115 us with
+// three, 126 with two, 143 with four.
 int32_t streams_at_once(const iekv_attention_shape& s) {
   return together_fits(s) && head_bytes_of(s) * kWaves >= 400 ? 2 : 3;
 }
@@ -166,10 +167,10 @@ int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t strea
     static_assert(sizeof(typename N::Lds) <= kUnasked);
     bool done = false;
     if constexpr (kScaled<C>) {
-      static_assert(sizeof(typename N::LdsTogether) <= kUnasked);
-      if (a.together == kWaves && together_fits(plan.shape)) {
-        if (const int rc = run(attend_narrow<T, C, DP, true>, sizeof(typename N::LdsTogether)))
-          return rc;
+      // Chunks of 16 bytes come into LDS directly.
+      const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+      if (a.together == kWaves && together_fits(plan.shape) && aligned(a.k) && aligned(a.v)) {
+        if (const int rc = run(attend_narrow<T, C, DP, true>, 0)) return rc;
         done = true;
       }
     }

@@ -290,6 +290,20 @@ __device__ __forceinline__ void store_out(T* out, const float* x) {
   }
 }
 
+// 16 bytes of each lane into LDS, the wave's in a row from `to` on; past the caches if STREAM.
+template <bool STREAM = false>
+__device__ __forceinline__ void bring16(const char* from, u32x4* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) uint32_t*)reinterpret_cast<uintptr_t>(from),
+      (__attribute__((address_space(3))) uint32_t*)to, 16, 0, STREAM ? 2 : 0);
+}
+
+// A barrier that the wave's loads into LDS have ended at, too.
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_s_waitcnt(0xf70);      // vmcnt 0; the other counters are not waited for
+  __syncthreads();
+}
+
 // The records of a step of a microscaled cache, on their way through LDS into the products'
 // operands. Records begin at any multiple of 4, and as operands sixteen lanes would take from
 // sixteen of them: what bounds such loads is the first cache, a line at a time. So a wave brings
@@ -378,55 +392,51 @@ struct Staged {
 
 // The same of the four neighbouring heads that a workgroup takes: their records lie on end, and
 // of whole groups of 32 dimensions four are a multiple of 16 bytes. The workgroup brings them as
-// they lie, each line once; a wave reads its own head's out of them. 32 keys at a time and two
-// workgroups to a compute unit: what is on its way then stays in L2 until the workgroup of the
-// next four heads has taken its part of the lines that they share. 48 sequences of 6,000 tokens
-// of eight mxfp8 heads of 128: 104 us (6.3 TB/s with such lines twice), with 64 keys 115, with
-// three workgroups 129, each wave with its own head's records (Staged) 120.
+// they lie, straight into LDS and each line once; a wave reads its own head's out of them. Two
+// tiles in turn, so that a step's loads are on their way while the one before is worked on and a
+// step has one barrier: 48 sequences of 6,000 tokens of eight mxfp8 heads of 128 107 us a call
+// with its joins, 128 of 4,200 in mxfp4 115; through registers and one tile 112 and 127, each
+// wave with its own head's records (Staged) 128 and 145. 32 keys at a time and two workgroups to a
+// compute unit (short records three): what is on its way then stays in L2 until the workgroup of
+// the next four heads has taken its part of the lines that they share. Through the caches mxfp4
+// takes 117.
 template <typename C, int DP>
 struct Together {
   static constexpr int KEYS = 32, HEADS = 4;
   static constexpr int CODES = DP * kBits<C> / 8, RECORD = head_bytes<C>(DP);
-  static constexpr int OF_KEY = HEADS * RECORD / 16;         // chunks
-  static constexpr int CHUNKS = (KEYS * OF_KEY + kThreads - 1) / kThreads;   // of a thread
   static constexpr int PITCH = HEADS * RECORD;
+  // Chunks of 16 bytes of a key, as many loads as K's and V's of a step are (of 64 chunks each),
+  // and what a wave has of these.
+  static constexpr int OF_KEY = PITCH / 16, LOADS = (OF_KEY + kWaves - 1) / kWaves;
   static_assert(!kScaled<C> || PITCH % 16 == 0);
-  alignas(16) char k[kScaled<C> ? KEYS * PITCH : 16], v[kScaled<C> ? KEYS * PITCH : 16];
-
-  using Chunk = Words<4>;
-  struct Lane {
-    int32_t key[CHUNKS], from[CHUNKS], to[CHUNKS];
+  struct Tile {
+    alignas(16) char k[KEYS * PITCH], v[KEYS * PITCH];
   };
-  static __device__ __forceinline__ Lane lane_of() {
+  struct Lane {
+    const char* from[LOADS];
+    int32_t key[LOADS];
+  };
+  // Chunks lie in LDS in the order of the lanes that bring them, so a lane finds its key from
+  // the place: the inverse of Staged's.
+  static __device__ __forceinline__ Lane lane_of(const char* k, const char* v, int wave, int lane) {
     Lane r;
 #pragma unroll
-    for (int n = 0; n < CHUNKS; ++n) {
-      // The last threads bring the last chunk once more.
-      const int32_t all = KEYS * OF_KEY, i = n * kThreads + threadIdx.x, at = i < all ? i : all - 1;
-      r.key[n] = at / OF_KEY;
-      r.from[n] = at % OF_KEY * 16;
-      r.to[n] = Staged<C, DP>::placed(r.key[n]) * PITCH + r.from[n];
+    for (int i = 0; i < LOADS; ++i) {
+      const int32_t at = (wave + i * kWaves) * kWave + lane, place = at / OF_KEY % KEYS;
+      r.key[i] = (place & 16) >> 2 | (place & 12) << 1 | (place & 3);
+      r.from[i] = (at < KEYS * OF_KEY ? k : v) + at % OF_KEY * 16;
     }
     return r;
   }
-  static __device__ __forceinline__ void load(Chunk (&x)[CHUNKS], const Lane& lane,
-                                              const char* heads, const int64_t* rows) {
+  static __device__ __forceinline__ void bring(Tile& tile, const Lane& lane, int wave,
+                                               const int64_t* rows) {
 #pragma unroll
-    for (int n = 0; n < CHUNKS; ++n) {
-      const char* at = heads + rows[lane.key[n]] + lane.from[n];
-      // Past the caches where the heads' bytes are long beside the lines at their ends, which
-      // another workgroup's heads have a part of.
-      if constexpr (PITCH >= 512)
-        x[n] = stream_bytes<16>(at);
-      else
-        x[n] = load_bytes<16>(at);
+    for (int i = 0; i < LOADS; ++i) {
+      const int n = wave + i * kWaves;
+      if ((i + 1) * kWaves > OF_KEY && n >= OF_KEY) break;   // the same for a whole wave
+      bring16<true>(lane.from[i] + rows[lane.key[i]],
+                    reinterpret_cast<u32x4*>(tile.k) + n * kWave);
     }
-  }
-  static __device__ __forceinline__ void put(char* tile, const Chunk (&x)[CHUNKS],
-                                             const Lane& lane) {
-#pragma unroll
-    for (int n = 0; n < CHUNKS; ++n)
-      __builtin_memcpy(__builtin_assume_aligned(tile + lane.to[n], 16), &x[n], 16);
   }
   // As Staged's, of a head.
   template <int BYTES>
@@ -483,22 +493,59 @@ struct Narrow {
     };
     int32_t redo[kWaves];
   };
-  struct LdsTogether {
-    alignas(16) int64_t rows[kWaves][2][KS];
-    float2 ml[kWaves][16];
-    union {
-      alignas(16) float o[kWaves][16][LDO];
-      Together<C, DP> staged;
-    };
-    int32_t redo[kWaves];
+  struct Rows {                                           // of heads taken together
+    int64_t rows[kWaves][2][Together<C, DP>::KEYS];
   };
 };
 
+// The rows of a head that a wave has to itself: a lane holds EV dimensions on end of row c at a
+// time (of `o`: dimension (4 g + r) EV + t at o[t][r]).
+template <typename T, typename C, int DP>
+__device__ __forceinline__ void write_head(const Args& a, const Item& it, int32_t kv_head,
+                                           int32_t head0, int32_t heads, int32_t rows,
+                                           const f32x4 (&o)[Narrow<T, C, DP>::EV], float m, float l,
+                                           int lane) {
+  constexpr int EV = Narrow<T, C, DP>::EV;
+  const int32_t g = lane / 16, c = lane % 16;
+  bool odd = l != l || is_far(m);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int t = 0; t < EV; ++t) odd = odd || ((g * 4 + r) * EV < DP && o[t][r] != o[t][r]);
+  // Nothing is written where rows are done again: the output may lie where their queries do.
+  if (__any(odd && c < rows)) {
+    for (int32_t r = 0; r < rows; ++r)
+      attend_row<T, C>(a, it, kv_head, r / heads * a.group + head0 + r % heads, lane);
+    return;
+  }
+  if (c >= rows) return;
+  const int32_t token = c / heads, in_group = head0 + c % heads;
+  const int64_t slot =
+      static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv_head;
+  const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
+                     static_cast<int64_t>(kv_head) * a.group + in_group;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int32_t d0 = (g * 4 + r) * EV;
+    if (d0 >= DP) break;
+    float x[EV];
+#pragma unroll
+    for (int t = 0; t < EV; ++t) x[t] = it.slot >= 0 ? o[t][r] : o[t][r] / l;
+    if (it.slot >= 0)
+      __builtin_memcpy(a.part_o + slot * DP + d0, x, EV * 4);
+    else
+      store_out<T, EV>(static_cast<T*>(a.out) + at * DP + d0, x);
+  }
+  if (it.slot >= 0 && g == 0) a.part_ml[slot] = {m, l};
+}
+
 // A group of more than 16 heads takes several workgroups for each of its tokens, `head0` on.
-// TOGETHER: four KV heads of a microscaled cache, of DP dimensions each.
+// TOGETHER: four KV heads of a microscaled cache, of DP dimensions each; their records come into
+// two `tiles`.
 template <typename T, typename C, int DP, bool TOGETHER, typename Lds>
-__device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t item,
-                                            int32_t kv_head0, int32_t head0) {
+__device__ __forceinline__ void narrow_item(Lds& lds, typename Together<C, DP>::Tile* tiles,
+                                            const Args& a, int32_t item, int32_t kv_head0,
+                                            int32_t head0) {
   using N = Narrow<T, C, DP>;
   constexpr int EK = N::EK, EL = N::EL, NL = N::NL, MF = N::MF, NK = N::NK;
   constexpr int EV = N::EV, KS = TOGETHER ? Together<C, DP>::KEYS : N::KS, KT = KS / 16;
@@ -511,7 +558,9 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
   const int32_t n = (it.a1 - it.a0) + (it.b1 - it.b0), steps = (n + KS - 1) / KS;
   const int32_t size = head_bytes<C>(d);
   const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * size;
-  if (threadIdx.x < kWaves) lds.redo[threadIdx.x] = 0;
+  if constexpr (!TOGETHER) {
+    if (threadIdx.x < kWaves) lds.redo[threadIdx.x] = 0;
+  }
 
   // Q^T: row c, zeros past the rows and past the dimensions.
   Words<4> q[NK];
@@ -545,21 +594,21 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
   };
   typename N::RawK k[kScaled<C> ? 1 : KT][NL];
   // Of microscaled caches: what a lane brings of a step's records, K's and V's.
-  using S = std::conditional_t<TOGETHER, Together<C, DP>, Staged<C, DP>>;
-  static_assert(!kScaled<C> || KS == S::KEYS);
+  using G = Together<C, DP>;
+  using S = Staged<C, DP>;
+  static_assert(!kScaled<C> || KS == (TOGETHER ? G::KEYS : S::KEYS));
+  typename G::Lane brings_all;
   typename S::Lane brings;
   typename S::Chunk k_chunks[kScaled<C> ? S::CHUNKS : 1], v_chunks[kScaled<C> ? S::CHUNKS : 1];
   if constexpr (TOGETHER) {
-    brings = S::lane_of();
+    brings_all = G::lane_of(kc - wave * size, vh - wave * size, wave, lane);
   } else if constexpr (kScaled<C>) {
     brings = S::lane_of(lane, d);
     if (d < DP) lds.staged[wave].clear(lane);
   }
-  const char* const k_heads = TOGETHER ? kc - wave * size : kc;
-  const char* const v_heads = TOGETHER ? vh - wave * size : vh;
   const auto load_k = [&](int half) {
     if constexpr (kScaled<C>) {
-      S::load(k_chunks, brings, k_heads, lds.rows[wave][half]);
+      S::load(k_chunks, brings, kc, lds.rows[wave][half]);
     } else {
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
@@ -577,19 +626,19 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
   };
   // Loads end behind 96 dimensions.
   const auto within = [](int32_t d0) { return d0 < DP ? d0 : 0; };
-  const auto k_of = [&](int t, int i) {
+  using Tile = typename G::Tile;
+  const auto k_of = [&](const Tile* tile, int t, int i) {
     const int32_t d0 = within((4 * i + g) * EL);
     if constexpr (TOGETHER)
-      return S::template codes<code_bytes<C>(EL)>(lds.staged.k, t * 16 + c, wave, d0);
+      return G::template codes<code_bytes<C>(EL)>(tile->k, t * 16 + c, wave, d0);
     else if constexpr (kScaled<C>)
       return lds.staged[wave].template codes<code_bytes<C>(EL)>(t * 16 + c, d0);
     else
       return k[t][i];
   };
-
-  const auto k_scale = [&](int t, int32_t d0) {
+  const auto k_scale = [&](const Tile* tile, int t, int32_t d0) {
     if constexpr (TOGETHER)
-      return S::scale(lds.staged.k, t * 16 + c, wave, d0);
+      return G::scale(tile->k, t * 16 + c, wave, d0);
     else
       return lds.staged[wave].scale(t * 16 + c, d0);
   };
@@ -622,28 +671,29 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
   for (int t = 0; t < EV; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;                 // l: of the lane's own keys
 
-  int half = 0;
   Place next{0, 0};
   if (turn < steps) {
     const Place now = place(turn);
     next = place(turn + turns);                 // before K's loads: see below
     keep(0, now);
-    load_k(0);
-    if constexpr (TOGETHER) S::load(v_chunks, brings, v_heads, lds.rows[wave][0]);
+    if constexpr (TOGETHER) {
+      G::bring(tiles[0], brings_all, wave, lds.rows[wave][0]);
+      arrive();
+    } else {
+      load_k(0);
+    }
   }
-  for (int32_t s = turn; s < steps; s += turns, half ^= 1) {
+  // Step s, whose rows are in `half`. Of heads taken together its records are in `tile`, and the
+  // next one's go to `after`, which the compiler has to know to be another: it would wait for
+  // loads into LDS before it reads there.
+  const auto step = [&](int32_t s, int half, const Tile* __restrict tile, Tile* __restrict after) {
     keep(half ^ 1, next);
     typename N::RawV v[KT / 2][kScaled<C> ? 1 : 8];
     if constexpr (TOGETHER) {
-      __syncthreads();                          // the step before has been read
-      S::put(lds.staged.k, k_chunks, brings);
-      S::put(lds.staged.v, v_chunks, brings);
-      __syncthreads();
       next = place(s + 2);
-      load_k(half ^ 1);
-      S::load(v_chunks, brings, v_heads, lds.rows[wave][half ^ 1]);
+      if (s + 1 < steps) G::bring(*after, brings_all, wave, lds.rows[wave][half ^ 1]);
     } else if constexpr (kScaled<C>) {
-      S::load(v_chunks, brings, v_heads, lds.rows[wave][half]);
+      S::load(v_chunks, brings, vh, lds.rows[wave][half]);
       __builtin_amdgcn_sched_barrier(0);
       lds.staged[wave].put(k_chunks, brings, d);
     } else {
@@ -660,13 +710,14 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
       sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const typename N::RawK whole = k_of(t, i);
+        const typename N::RawK whole = k_of(tile, t, i);
 #pragma unroll
         for (int e = 0; e < MF; ++e) {
           const auto raw = feed(whole, i, e);
           if constexpr (kScaled<C>)
-            sc[t] = mma16(scaled<T, C, EK>(raw, k_scale(t, within((4 * i + g) * EL) + e * EK)),
-                          q[i * MF + e], sc[t], T{});
+            sc[t] = mma16(
+                scaled<T, C, EK>(raw, k_scale(tile, t, within((4 * i + g) * EL) + e * EK)),
+                q[i * MF + e], sc[t], T{});
           else
             sc[t] = mma16(Convert<T, C, EK>::of(raw), q[i * MF + e], sc[t], T{});
         }
@@ -684,8 +735,8 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
       if constexpr (kScaled<C>) {
         const int32_t at = p * 32 + e / 4 * 16 + g * 4 + e % 4, d0 = within(c * EV);
         if constexpr (TOGETHER)
-          return scaled<T, C, EV>(S::template codes<EV * kBits<C> / 8>(lds.staged.v, at, wave, d0),
-                                  S::scale(lds.staged.v, at, wave, d0));
+          return scaled<T, C, EV>(G::template codes<EV * kBits<C> / 8>(tile->v, at, wave, d0),
+                                  G::scale(tile->v, at, wave, d0));
         else
           return scaled<T, C, EV>(lds.staged[wave].template codes<EV * kBits<C> / 8>(at, d0),
                                   lds.staged[wave].scale(at, d0));
@@ -768,72 +819,79 @@ __device__ __forceinline__ void narrow_item(Lds& lds, const Args& a, int32_t ite
         }
       }
     }
-  }
+    if constexpr (TOGETHER) arrive();
+  };
+  int half = 0;
+  for (int32_t s = turn; s < steps; s += turns, half ^= 1)
+    step(s, half, TOGETHER ? tiles + half : nullptr, TOGETHER ? tiles + (half ^ 1) : nullptr);
 
-  // The parts of each head's waves.
   l += lane_xor<16>(l);
   l += lane_xor<32>(l);
-  if (lane < 16) lds.ml[wave][lane] = {m, l};
-  __syncthreads();
-  float all = -INFINITY;
-  for (int w = wave % together; w < kWaves; w += together) all = fmaxf(all, lds.ml[w][c].x);
-  const float fade = power2(m - (all == -INFINITY ? 0.f : all));
+  if constexpr (TOGETHER) {
+    write_head<T, C, DP>(a, it, kv_head, head0, heads, rows, o, m, l, lane);
+  } else {
+    if (lane < 16) lds.ml[wave][lane] = {m, l};
+    __syncthreads();
+    float all = -INFINITY;
+    for (int w = wave % together; w < kWaves; w += together) all = fmaxf(all, lds.ml[w][c].x);
+    const float fade = power2(m - (all == -INFINITY ? 0.f : all));
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int t = 0; t < EV; ++t)
-      if ((g * 4 + r) * EV + t < DP) lds.o[wave][c][(g * 4 + r) * EV + t] = o[t][r] * fade;
-  __syncthreads();
-  // Eight dimensions of a row a thread, of each head.
-  const int32_t row = threadIdx.x / 16, d0 = threadIdx.x % 16 * 8;
-  const int32_t in_group = head0 + row % heads, token = row / heads;
-  const bool mine = row < rows && d0 < d;
-  float x[kWaves][8];
-  float2 ml[kWaves];
+      for (int t = 0; t < EV; ++t)
+        if ((g * 4 + r) * EV + t < DP) lds.o[wave][c][(g * 4 + r) * EV + t] = o[t][r] * fade;
+    __syncthreads();
+    // Eight dimensions of a row a thread, of each head.
+    const int32_t row = threadIdx.x / 16, d0 = threadIdx.x % 16 * 8;
+    const int32_t in_group = head0 + row % heads, token = row / heads;
+    const bool mine = row < rows && d0 < d;
+    float x[kWaves][8];
+    float2 ml[kWaves];
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) {
-    if (!mine || k >= together) break;
-    float total = 0.f, most = -INFINITY;
-    for (int w = k; w < kWaves; w += together) most = fmaxf(most, lds.ml[w][row].x);
-    const float from = most == -INFINITY ? 0.f : most;
-    for (int w = k; w < kWaves; w += together)
-      total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
-    ml[k] = {most, total};
-    bool odd = total != total || is_far(most);
+    for (int k = 0; k < kWaves; ++k) {
+      if (!mine || k >= together) break;
+      float total = 0.f, most = -INFINITY;
+      for (int w = k; w < kWaves; w += together) most = fmaxf(most, lds.ml[w][row].x);
+      const float from = most == -INFINITY ? 0.f : most;
+      for (int w = k; w < kWaves; w += together)
+        total = fmaf(lds.ml[w][row].y, power2(lds.ml[w][row].x - from), total);
+      ml[k] = {most, total};
+      bool odd = total != total || is_far(most);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[k][i] = lds.o[k][row][d0 + i];
-    for (int w = k + together; w < kWaves; w += together)
+      for (int i = 0; i < 8; ++i) x[k][i] = lds.o[k][row][d0 + i];
+      for (int w = k + together; w < kWaves; w += together)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[k][i] += lds.o[w][row][d0 + i];
+        for (int i = 0; i < 8; ++i) x[k][i] += lds.o[w][row][d0 + i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) odd = odd || x[k][i] != x[k][i];
-    if (odd) lds.redo[k] = 1;
-  }
-  __syncthreads();
-  // Nothing is written of a head whose rows are done again: the output may lie where their
-  // queries do.
-#pragma unroll
-  for (int k = 0; k < kWaves; ++k) {
-    if (!mine || k >= together) break;
-    if (lds.redo[k]) continue;
-    const int64_t kv = kv_head0 + k;
-    if (it.slot >= 0) {
-      const int64_t slot =
-          static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv;
-      __builtin_memcpy(a.part_o + slot * d + d0, x[k], 32);
-      if (d0 == 0) a.part_ml[slot] = ml[k];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[k][i] /= ml[k].y;
-      const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
-                         kv * a.group + in_group;
-      store_out<T, 8>(static_cast<T*>(a.out) + at * d + d0, x[k]);
+      for (int i = 0; i < 8; ++i) odd = odd || x[k][i] != x[k][i];
+      if (odd) lds.redo[k] = 1;
     }
-  }
-  for (int k = 0; k < together; ++k) {
-    if (!lds.redo[k]) continue;
-    for (int32_t r = wave; r < rows; r += kWaves)
-      attend_row<T, C>(a, it, kv_head0 + k, r / heads * a.group + head0 + r % heads, lane);
+    __syncthreads();
+    // Nothing is written of a head whose rows are done again: the output may lie where their
+    // queries do.
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      if (!mine || k >= together) break;
+      if (lds.redo[k]) continue;
+      const int64_t kv = kv_head0 + k;
+      if (it.slot >= 0) {
+        const int64_t slot =
+            static_cast<int64_t>(it.slot + token * a.group + in_group) * a.kv_heads + kv;
+        __builtin_memcpy(a.part_o + slot * d + d0, x[k], 32);
+        if (d0 == 0) a.part_ml[slot] = ml[k];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[k][i] /= ml[k].y;
+        const int64_t at = (it.token0 + token) * static_cast<int64_t>(a.kv_heads) * a.group +
+                           kv * a.group + in_group;
+        store_out<T, 8>(static_cast<T*>(a.out) + at * d + d0, x[k]);
+      }
+    }
+    for (int k = 0; k < together; ++k) {
+      if (!lds.redo[k]) continue;
+      for (int32_t r = wave; r < rows; r += kWaves)
+        attend_row<T, C>(a, it, kv_head0 + k, r / heads * a.group + head0 + r % heads, lane);
+    }
   }
 }
 
@@ -886,19 +944,6 @@ __device__ __forceinline__ Words<2> transposed(const char* lds) {
   return __builtin_bit_cast(
       Words<2>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (__attribute__((address_space(3))) s16x4*)const_cast<char*>(lds)));
-}
-
-// 16 bytes of each lane into LDS, the wave's in a row from `to` on.
-__device__ __forceinline__ void bring16(const char* from, u32x4* to) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) uint32_t*)reinterpret_cast<uintptr_t>(from),
-      (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
-}
-
-// A barrier that the wave's loads into LDS have ended at, too.
-__device__ __forceinline__ void arrive() {
-  __builtin_amdgcn_s_waitcnt(0xf70);      // vmcnt 0; the other counters are not waited for
-  __syncthreads();
 }
 
 // K's and V's buffers are arguments of their own: the compiler then knows that a load into one
@@ -1180,15 +1225,21 @@ template <typename T, typename C, int DP, bool TOGETHER>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 4 && DP > 64 ? 1 : 2) void attend_narrow(
     Args a, int32_t first, int32_t n) {
   using N = Narrow<T, C, DP>;
-  extern __shared__ __attribute__((aligned(16))) char shared[];
-  auto& lds = *reinterpret_cast<
-      std::conditional_t<TOGETHER, typename N::LdsTogether, typename N::Lds>*>(shared);
   constexpr int kXcds = 8;
   const int32_t each = a.kv_heads / a.together, b = blockIdx.x;
   const bool whole = b < n / kXcds * kXcds * each;
   const int32_t item = whole ? b / kXcds / each * kXcds + b % kXcds : b / each;
   const int32_t part = whole ? b / kXcds % each : b % each;
-  narrow_item<T, C, DP, TOGETHER>(lds, a, first + item, part * a.together, blockIdx.y * 16);
+  const int32_t kv_head0 = part * a.together, head0 = blockIdx.y * 16;
+  if constexpr (TOGETHER) {
+    __shared__ typename Together<C, DP>::Tile tiles[2];
+    __shared__ typename N::Rows rows;
+    narrow_item<T, C, DP, true>(rows, tiles, a, first + item, kv_head0, head0);
+  } else {
+    extern __shared__ __attribute__((aligned(16))) char shared[];
+    narrow_item<T, C, DP, false>(*reinterpret_cast<typename N::Lds*>(shared), nullptr, a,
+                                 first + item, kv_head0, head0);
+  }
 }
 
 constexpr int kWideRows = kWaves * 32;
@@ -1227,8 +1278,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_both(
                                            wide + before / a.together,
                                            before % a.together * each + part);
   else
-    narrow_item<T, C, DP, false>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared), a,
-                                 narrow + run - before, part * a.together, 0);
+    narrow_item<T, C, DP, false>(*reinterpret_cast<typename Narrow<T, C, DP>::Lds*>(shared),
+                                 nullptr, a, narrow + run - before, part * a.together, 0);
 }
 
 // Joins the parts of a (token, head): o = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, W

@@ -161,6 +161,32 @@ def test_long_streams(gpu, kv_heads, dim, query, format):
 
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("query", TYPES, ids=str)
+def test_long_streams_at_any_address(gpu, query, format):
+    """Caches that begin at a multiple of 16 bytes, of 4, and at an odd byte; the output in the
+    queries' place."""
+    from iekv.engine.attention import AttentionPlan, attend
+    from iekv.engine.quantized import QuantizedPool
+
+    contexts = [5000 + 131 * i for i in range(64)]
+    pool, k, v = make_pool(150, 16, 4, 64, format, query, 51)
+    gen = torch.Generator().manual_seed(52)
+    tables = [torch.randint(150, (-(-c // 16),), generator=gen).tolist() for c in contexts]
+    q = queries_of(64, 12, 64, query, 53)
+    check(q, k[0], v[0], pool, tables, contexts, [1] * 64)
+    for first, second in ((16, 16), (4, 0), (0, 4), (1, 3)):
+        arrays = []
+        for t, skip in zip(pool._arrays, (first, second)):
+            o = torch.zeros(t.numel() + skip, dtype=torch.uint8, device="cuda")[skip:].view(t.shape)
+            o.copy_(t)
+            arrays.append(o)
+        moved = QuantizedPool(arrays[:1], arrays[1:], 16, format)
+        want, plan = check(q, k[0], v[0], moved, tables, contexts, [1] * 64)
+        again = q.clone()
+        assert attend(plan, 0, again, out=again) is again and torch.equal(again, want)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("query", TYPES, ids=str)
 def test_what_masked_places_hold_stays_out(gpu, query, format):
     """Rows that no query may see hold groups that are no numbers; so, in a prompt, does the
     last token's V or K, which only its own row may show."""
