@@ -226,8 +226,8 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // shortest: the second ones come in the other order. (A chunk of 2,048 tokens at the end of
   // 7,777, eight heads, 512 workgroups of 90 to 122 steps: 8% less.)
   const int64_t first_ones = compute_units / sh.kv_heads;
-  if (int64_t(wide.size()) > first_ones && int64_t(wide.size()) <= 2 * first_ones)
-    std::reverse(wide.begin() + first_ones, wide.end());
+  const bool paired = int64_t(wide.size()) > first_ones && int64_t(wide.size()) <= 2 * first_ones;
+  if (paired) std::reverse(wide.begin() + first_ones, wide.end());
   plan.narrow = {0, static_cast<int32_t>(narrow.size())};
   plan.wide = {plan.narrow.n, static_cast<int32_t>(wide.size())};
   plan.items = std::move(narrow);
@@ -257,9 +257,14 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   for (Item& it : plan.items) {
     if (it.slot < 0) continue;
     it.slot = static_cast<int32_t>(plan.slots);
-    for (int32_t t = 0; t < it.tokens; ++t)
-      plan.join_parts[at[it.token0 + t]++] = it.slot + t * sh.group;
     plan.slots += int64_t(it.tokens) * sh.group;
+  }
+  // Parts are joined with the longest first, in whatever order they are made.
+  const int64_t n = plan.items.size(), turned = paired ? plan.wide.first + first_ones : n;
+  for (int64_t i = 0; i < n; ++i) {
+    const Item& it = plan.items[i < turned ? i : n - 1 - (i - turned)];
+    for (int32_t t = 0; t < it.tokens && it.slot >= 0; ++t)
+      plan.join_parts[at[it.token0 + t]++] = it.slot + t * sh.group;
   }
   return plan;
 }

@@ -3,11 +3,12 @@ from __future__ import annotations
 
 import ctypes
 import re
+import subprocess
 
 import pytest
 import torch
 
-from conftest import ROOT
+from conftest import PACKAGE_ROOT, ROOT
 from quantized_reference import CODES, FORMATS, decode, encode
 from test_attention_plan import make, ops  # noqa: F401  (the library, and a plan of two sequences)
 from test_ops_host import on_stub  # noqa: F401  (the library over a HIP that runs nothing)
@@ -118,6 +119,53 @@ def test_wide_items_that_all_run_at_once_pair_long_with_short(ops):  # noqa: F81
     pairs = [a + b for a, b in zip(keys[:32], keys[32:])]
     assert max(pairs) - min(pairs) <= 32
     ops.iekv_attention_plan_destroy(plan)
+
+
+PARTS = r"""
+#include <cstdio>
+#include <map>
+#include "attention_plan.h"
+using namespace iekv_attention;
+
+int main() {
+  int turned = 0;
+  for (int units = 16; units <= 256; units += 16)
+    for (int heads = 1; heads <= 4; ++heads)
+      for (int many = 8; many <= 56; many += 8) {
+        const int context = 2400 + 8 * many;
+        std::vector<Sequence> seqs{{context, 0, 0, 0}, {context - 900, 0, 0, 200}};
+        int tokens = 0;
+        for (Sequence& s : seqs) s.token0 = tokens, s.queries = many, tokens += many;
+        const Plan p = make_plan(Shape{4, heads, 16, 0, 0, 0, 128}, seqs, units);
+        std::map<int, const Item*> of;               // by slot
+        bool in_order = true;
+        for (int i = 0; i < p.wide.n; ++i) {
+          const Item& it = p.items[p.wide.first + i];
+          in_order = in_order && (!i || keys_of(it) <= keys_of((&it)[-1]));
+          for (int t = 0; t < it.tokens && it.slot >= 0; ++t) of[it.slot + 4 * t] = &it;
+        }
+        turned += !in_order && !p.join_parts.empty();
+        for (size_t e = 0; e < p.join_tokens.size(); ++e)
+          for (int i = p.join_starts[e] + 1; i < p.join_starts[e + 1]; ++i) {
+            const Item &x = *of.at(p.join_parts[i - 1]), &y = *of.at(p.join_parts[i]);
+            if (keys_of(x) < keys_of(y) || (keys_of(x) == keys_of(y) && x.a0 + x.b0 >= y.a0 + y.b0))
+              return std::printf("%d units, %d heads, %d tokens\n", units, heads, many), 1;
+          }
+      }
+  std::printf("%d\n", turned);
+}
+"""
+
+
+def test_parts_are_joined_in_one_order(tmp_path):
+    """The longest first, then by their keys, however the items that make them are ordered."""
+    (tmp_path / "parts.cpp").write_text(PARTS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I",
+                    str(PACKAGE_ROOT / "csrc"), str(tmp_path / "parts.cpp"), "-o",
+                    str(tmp_path / "parts")], check=True)
+    run = subprocess.run([str(tmp_path / "parts")], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout
+    assert int(run.stdout) > 0                       # of steps whose items are in another order
 
 
 CALLS = """
