@@ -730,16 +730,18 @@ __device__ __forceinline__ void narrow_item(Lds& lds, typename Together<C, DP>::
       load_k(half ^ 1);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // V of key `e` of the lane's eight of pair `p`.
-    const auto v_of = [&](int p, int e) {
+    // V of key `e` of the lane's eight of pair `p`, as the type of `as`.
+    const auto v_of = [&](auto as, int p, int e) {
       if constexpr (kScaled<C>) {
         const int32_t at = p * 32 + e / 4 * 16 + g * 4 + e % 4, d0 = within(c * EV);
         if constexpr (TOGETHER)
-          return scaled<T, C, EV>(G::template codes<EV * kBits<C> / 8>(tile->v, at, wave, d0),
-                                  G::scale(tile->v, at, wave, d0));
+          return scaled<decltype(as), C, EV>(
+              G::template codes<EV * kBits<C> / 8>(tile->v, at, wave, d0),
+              G::scale(tile->v, at, wave, d0));
         else
-          return scaled<T, C, EV>(lds.staged[wave].template codes<EV * kBits<C> / 8>(at, d0),
-                                  lds.staged[wave].scale(at, d0));
+          return scaled<decltype(as), C, EV>(
+              lds.staged[wave].template codes<EV * kBits<C> / 8>(at, d0),
+              lds.staged[wave].scale(at, d0));
       } else {
         return Convert<T, C, EV>::of(v[p][e]);
       }
@@ -788,7 +790,7 @@ __device__ __forceinline__ void narrow_item(Lds& lds, typename Together<C, DP>::
       if constexpr (sizeof(T) == 4) {
         Words<EV> x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = v_of(pr, e);
+        for (int e = 0; e < 8; ++e) x[e] = v_of(T{}, pr, e);
 #pragma unroll
         for (int t = 0; t < EV; ++t)
 #pragma unroll
@@ -796,9 +798,24 @@ __device__ __forceinline__ void narrow_item(Lds& lds, typename Together<C, DP>::
             o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x[e].w[t]),
                                                         p[2 * pr + e / 4][e % 4], o[t], 0, 0, 0);
       } else {
-        Words<EV / 2> x[8];
+        // Integers become floats first, which two keys at a time are rounded to where V^T has them;
+        // the others come as words of two dimensions, which change places with another key's.
+        constexpr bool BY_KEY = std::is_same_v<C, Mxint8>;
+        Words<4> by_key[BY_KEY ? EV : 1];
+        Words<EV / 2> x[BY_KEY ? 1 : 8];
+        if constexpr (BY_KEY) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = v_of(pr, e);
+          for (int i = 0; i < 4; ++i) {
+            const Words<EV> v0 = v_of(0.f, pr, 2 * i), v1 = v_of(0.f, pr, 2 * i + 1);
+#pragma unroll
+            for (int t = 0; t < EV; ++t)
+              by_key[t].w[i] = pack2<T>(__builtin_bit_cast(float, v0.w[t]),
+                                        __builtin_bit_cast(float, v1.w[t]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = v_of(T{}, pr, e);
+        }
         Words<4> w, rest;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -813,8 +830,11 @@ __device__ __forceinline__ void narrow_item(Lds& lds, typename Together<C, DP>::
           Words<4> vt;                          // dimension c EV + t of keys 8 g ..
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            vt.w[i] = __builtin_amdgcn_perm(x[2 * i + 1].w[t / 2], x[2 * i].w[t / 2],
-                                            t % 2 ? 0x07060302u : 0x05040100u);
+            if constexpr (BY_KEY)
+              vt.w[i] = by_key[t].w[i];
+            else
+              vt.w[i] = __builtin_amdgcn_perm(x[2 * i + 1].w[t / 2], x[2 * i].w[t / 2],
+                                              t % 2 ? 0x07060302u : 0x05040100u);
           o[t] = mma16(vt, rest, mma16(vt, w, o[t], T{}), T{});
         }
       }
