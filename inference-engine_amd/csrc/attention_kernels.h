@@ -396,10 +396,10 @@ struct Staged {
 // tiles in turn, so that a step's loads are on their way while the one before is worked on and a
 // step has one barrier: 48 sequences of 6,000 tokens of eight mxfp8 heads of 128 107 us a call
 // with its joins, 128 of 4,200 in mxfp4 115; through registers and one tile 112 and 127, each
-// wave with its own head's records (Staged) 128 and 145. 32 keys at a time and two workgroups to a
+// wave with its own head's records (Staged) 131 and 144. 32 keys at a time and two workgroups to a
 // compute unit (short records three): what is on its way then stays in L2 until the workgroup of
-// the next four heads has taken its part of the lines that they share. Through the caches mxfp4
-// takes 117.
+// the next four heads has taken its part of the lines that they share. Past the caches, or 117
+// and 116.
 template <typename C, int DP>
 struct Together {
   static constexpr int KEYS = 32, HEADS = 4;
