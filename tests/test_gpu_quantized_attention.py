@@ -159,6 +159,38 @@ def test_long_streams(gpu, kv_heads, dim, query, format):
     check(q[:32], k[0], v[0], pool, tables[32:], contexts[32:], [1] * 32, window=4001, sinks=5)
 
 
+@pytest.mark.parametrize("group, queries, query, window", [
+    (4, 3, BF16, None), (4, 4, BF16, 3000), (7, 2, F16, None), (1, 5, F32, 77), (20, 1, F32, None)])
+@pytest.mark.parametrize("format", FORMATS)
+def test_long_streams_of_several_rows(gpu, group, queries, query, window, format):
+    """Rows of several tokens, whose masks end a stream differently; more heads in a group than a
+    workgroup holds; a captured call that is replayed among eager ones."""
+    from iekv.engine.attention import attend
+
+    contexts = [5000 + 131 * i for i in range(64)]
+    pool, k, v = make_pool(150, 16, 4, 64, format, query, 54)
+    gen = torch.Generator().manual_seed(55)
+    tables = [torch.randint(150, (-(-c // 16),), generator=gen).tolist() for c in contexts]
+    q = queries_of(64 * queries, 4 * group, 64, query, 56)
+    want, plan = check(q, k[0], v[0], pool, tables, contexts, [queries] * 64,
+                       **({} if window is None else dict(window=window, sinks=3)))
+    side, now, out = torch.cuda.Stream(), torch.zeros_like(q), torch.empty_like(q)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attend(plan, 0, now, out=out)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(plan, 0, now, out=out)
+    for x in (q, -q, q):
+        now.copy_(x)
+        graph.replay()
+        replayed = out.clone()
+        assert torch.equal(replayed, attend(plan, 0, x))
+        torch.cuda.synchronize()
+    assert torch.equal(replayed, want)
+
+
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("query", TYPES, ids=str)
 def test_long_streams_at_any_address(gpu, query, format):
