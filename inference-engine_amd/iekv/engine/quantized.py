@@ -181,6 +181,8 @@ class QuantizedPool(KVPool):
                                 f"got {tuple(block_table.shape)} {block_table.dtype}")
             if block_table.dtype == torch.int32 and block_table.is_contiguous():
                 return block_table, self._read         # entries past the context are not read
+            if block_table.dtype == torch.int64:       # outside the pool in 32 bits too
+                block_table = block_table.clamp(-1, self.num_blocks)
             return block_table[:needed].to(torch.int32).contiguous(), self._read
         host = self.host_ids(block_table[:needed], what="context block")
         if host.size != needed:

@@ -234,6 +234,15 @@ def test_device_slots_and_blocks_outside_the_pool(gpu, format):
     assert same(out[:8].cpu(), decode(k[0][16:], format).to(F32))
 
 
+def test_blocks_past_32_bits_are_outside_the_pool(gpu):
+    """As entries of a table of 64 bits, of which a kernel takes 32."""
+    pool, _, _ = make_pool(3, 8, 2, 48, "mxfp8")
+    for wide in (1 << 32, (1 << 32) + 1, -(1 << 32), (1 << 62) + 2, 3, -1):
+        table, _ = pool._table(torch.tensor([2, wide, 0], device=gpu), 24)
+        first, bad, last = table.tolist()
+        assert (first, last) == (2, 0) and not 0 <= bad < 3
+
+
 @pytest.mark.parametrize("format", FORMATS)
 def test_nothing_to_do(gpu, format):
     from iekv.engine.slots import gather_rows, gather_rows_arrays, write_slots, write_slots_layers
