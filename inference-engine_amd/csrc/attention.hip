@@ -106,6 +106,12 @@ int32_t streams_at_once(const iekv_attention_shape& s) {
   return together_fits(s) && head_bytes_of(s) * kWaves >= 400 ? 2 : 3;
 }
 
+// And few items: twice the steps for a wave of microscaled caches take less than twice the parts do,
+// the joins' reads included. One sequence of 16,384 tokens of eight heads of 128 in mxint8 17.0 us
+// with one, 18.6 with two; two of them in mxfp8 22.2 and 23.8. (Of eight sequences of unlike
+// lengths and more, two are better balanced: 16 of 6,000 50 us, with one 55.)
+int32_t few_at_once(const iekv_attention_shape& s) { return s.cache_type >= IEKV_TYPE_MXFP8 ? 1 : 2; }
+
 template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
@@ -322,7 +328,7 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
                            few_keys(shape), 2 * head_bytes_of(shape),
-                           streams_at_once(shape)};
+                           streams_at_once(shape), few_at_once(shape)};
   const int device = current_device();
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||

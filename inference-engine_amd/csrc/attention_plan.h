@@ -33,7 +33,8 @@ struct Shape {
   int32_t wide_rows;      // rows an item of the wide kernel holds at most (0: there is none)
   int32_t few_keys = 1024;  // that a narrow workgroup takes whole rather than leave parts
   int32_t key_bytes = 512;  // K and V of a key in one KV head
-  int32_t at_once = 3;      // narrow workgroups that a long stream is cut into for a compute unit
+  int32_t at_once = 3;      // narrow workgroups that a long stream is cut into for a compute unit,
+  int32_t few_at_once = 2;  // and few items that each have eight compute units or more
 };
 
 struct Sequence {
@@ -208,9 +209,10 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   const bool whole = longest_item <= sh.few_keys && !worth;
   // Two workgroups fit a compute unit. Long streams are cut for half as many again: 128
   // sequences of unlike lengths 182 us against 191 with two, of one length 175 against 173.
+  const bool few = int64_t(narrow.size()) * sh.kv_heads * 8 <= compute_units;
   if (!whole)
     narrow = split(narrow, sh.kv_heads / plan.together,
-                   (plan.streams ? sh.at_once : 2) * compute_units, 256, 64);
+                   (plan.streams ? sh.at_once : few ? sh.few_at_once : 2) * compute_units, 256, 64);
   const int64_t narrow_blocks = int64_t(narrow.size()) * sh.kv_heads / plan.together;
   // Parts of wide items are 64 times as many rows to write and join as those of narrow ones
   // are: they are cut only where more than half of the compute units would have none, and so

@@ -121,6 +121,24 @@ def test_wide_items_that_all_run_at_once_pair_long_with_short(ops):  # noqa: F81
     ops.iekv_attention_plan_destroy(plan)
 
 
+@pytest.mark.parametrize("cache_type, parts", [(3, 64), (4, 64), (5, 32), (6, 32), (7, 32)])
+def test_few_sequences_are_cut_into_a_workgroup_for_each_compute_unit(ops, cache_type, parts):  # noqa: F811
+    """Of microscaled caches; of the others two."""
+    context, blocks = 16384, 1024
+    rc, plan, _ = make(ops, contexts=(context,), queries=(1,), tables=(tuple(range(blocks)),),
+                       num_blocks=blocks, num_heads=64, num_kv_heads=8, head_dim=128,
+                       cache_type=cache_type)
+    assert rc == 0
+    words, count = ctypes.POINTER(ctypes.c_int32)(), ctypes.c_int64()
+    tokens, workspace = ctypes.c_int64(), ctypes.c_int64()
+    ops.iekv_attention_plan_info(plan, ctypes.byref(words), ctypes.byref(count),
+                                 ctypes.byref(tokens), ctypes.byref(workspace))
+    items = [words[12 * i:12 * i + 12] for i in range(parts)]
+    assert all(it[:2] == [0, 1] and it[8:10] == [context - 1] * 2 for it in items)
+    assert sum(it[4] - it[3] + it[6] - it[5] for it in items) == context
+    ops.iekv_attention_plan_destroy(plan)
+
+
 PARTS = r"""
 #include <cstdio>
 #include <map>
