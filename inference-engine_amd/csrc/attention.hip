@@ -112,6 +112,12 @@ int32_t streams_at_once(const iekv_attention_shape& s) {
 // lengths and more, two are better balanced: 16 of 6,000 50 us, with one 55.)
 int32_t few_at_once(const iekv_attention_shape& s) { return s.cache_type >= IEKV_TYPE_MXFP8 ? 1 : 2; }
 
+// And what a long stream is: four heads' records come together sooner than other caches' rows pay
+// for their parts. 16 sequences of 6,000 tokens of eight mxfp8 heads of 128 42 us together, 50 each
+// head by itself, 8 of 8,000 31.5 and 36 (in mxfp4 32 and 35, both 25); 8 of 6,000 beside a chunk
+// of 2,048 tokens, then in a launch of its own, 370 and 498.
+int32_t stream_steps(const iekv_attention_shape& s) { return together_fits(s) ? 1 : 4; }
+
 template <typename T, typename C, int DP>
 int launch_dim(const iekv_attention_plan& plan, const Args& a, hipStream_t stream) {
   const int32_t wide = plan.wide.n, narrow = plan.narrow.n;
@@ -328,7 +334,8 @@ int make(const iekv_attention_shape& shape, int32_t n_seqs, const int32_t* conte
                            static_cast<int32_t>(shape.shared_blocks * bs),
                            shape.query_type == IEKV_TYPE_F32 ? 0 : kWideRows,
                            few_keys(shape), 2 * head_bytes_of(shape),
-                           streams_at_once(shape), few_at_once(shape)};
+                           streams_at_once(shape), few_at_once(shape),
+                           stream_steps(shape)};
   const int device = current_device();
   iekv_attention::Plan made = iekv_attention::make_plan(sh, seqs, compute_units(device));
   if (static_cast<int64_t>(made.items.size()) * shape.num_kv_heads > INT32_MAX ||

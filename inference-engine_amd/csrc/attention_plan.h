@@ -35,6 +35,7 @@ struct Shape {
   int32_t key_bytes = 512;  // K and V of a key in one KV head
   int32_t at_once = 3;      // narrow workgroups that a long stream is cut into for a compute unit,
   int32_t few_at_once = 2;  // and few items that each have eight compute units or more
+  int32_t stream_steps = 4; // of 256 keys that each of a compute unit's waves has in a long stream
 };
 
 struct Sequence {
@@ -200,7 +201,8 @@ inline Plan make_plan(const Shape& sh, const std::vector<Sequence>& seqs, int32_
   // a part of its own: worth it where a wave has steps enough to outweigh the part.
   int64_t narrow_keys = 0;
   for (const Item& it : narrow) narrow_keys += keys_of(it);
-  plan.streams = narrow_keys * sh.kv_heads >= int64_t(4) * compute_units * kNarrowWaves * 256;
+  plan.streams =
+      narrow_keys * sh.kv_heads >= int64_t(sh.stream_steps) * compute_units * kNarrowWaves * 256;
   if (plan.streams)
     plan.together = sh.kv_heads % 4 == 0 ? 4 : sh.kv_heads % 2 == 0 ? 2 : 1;
   // Few keys take less time in turn than a join does, if there is none yet.

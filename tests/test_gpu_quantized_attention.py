@@ -159,6 +159,20 @@ def test_long_streams(gpu, kv_heads, dim, query, format):
     check(q[:32], k[0], v[0], pool, tables[32:], contexts[32:], [1] * 32, window=4001, sinks=5)
 
 
+@pytest.mark.parametrize("query", [BF16, F32], ids=str)
+@pytest.mark.parametrize("format", FORMATS)
+def test_streams_of_middle_length_and_a_chunk(gpu, query, format):
+    """Long enough for heads to be taken together, alone and beside a prompt's chunk."""
+    contexts = [4000 + 131 * i for i in range(16)]
+    assert 4 * 256 * 256 < sum(contexts) * 4 < 4 * 4 * 256 * 256
+    pool, k, v = make_pool(150, 16, 4, 128, format, query, 57)
+    gen = torch.Generator().manual_seed(58)
+    tables = [torch.randint(150, (-(-c // 16),), generator=gen).tolist() for c in contexts]
+    q = queries_of(16 + 299, 16, 128, query, 59)
+    check(q[:16], k[0], v[0], pool, tables, contexts, [1] * 16)
+    check(q, k[0], v[0], pool, tables, contexts, [1] * 15 + [300])
+
+
 @pytest.mark.parametrize("group, queries, query, window", [
     (4, 3, BF16, None), (4, 4, BF16, 3000), (7, 2, F16, None), (1, 5, F32, 77), (20, 1, F32, None)])
 @pytest.mark.parametrize("format", FORMATS)
