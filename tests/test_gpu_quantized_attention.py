@@ -475,3 +475,46 @@ def test_refusals(gpu):
         AttentionPlan(pool, *args, query_dtype=torch.float8_e4m3fn)
     with pytest.raises(IndexError, match="out of range"):
         AttentionPlan(pool, [[1, 8], [3]], *args[1:])
+
+
+# contexts, queries, shared blocks, options: chunks alone, beside single tokens in one launch and
+# behind long streams, in parts, and sequences that share their first blocks.
+WEIGHTED = {
+    "prompt": ([129], [129], 0, {}),
+    "chunks": ([300, 200, 77, 640], [1, 131, 3, 333], 0, {}),
+    "window": ([900], [500], 0, dict(window=170, sinks=9)),
+    "parts": ([6000], [33], 0, {}),
+    "shared": ([1300 + i for i in range(40)], [1] * 40, 80, {}),
+}
+
+
+@pytest.mark.parametrize("step", list(WEIGHTED))
+@pytest.mark.parametrize("dim", [128, 72])
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("query", [BF16, F16], ids=str)
+def test_weights_are_held_as_two_numbers(gpu, query, format, dim, step):
+    """A weight is its value rounded to the queries' type and what that leaves, rounded: off by
+    u^2 of it (u: half a step) where one number would be off by u. V of mixed signs, so that an
+    output, whose own rounding is allowed u of it, is small beside A = sum p |v|; short queries,
+    so that scores are nearly exact. Twice as many terms are summed in 32 bits."""
+    from iekv.engine.attention import AttentionPlan, attend
+
+    contexts, queries, shared, options = WEIGHTED[step]
+    bs, kv_heads, group = 16, 2, 4
+    blocks = sum(-(-c // bs) for c in contexts) + 3
+    pool, k, v = make_pool(blocks, bs, kv_heads, dim, format, query, 71)
+    tables = make_tables(contexts, bs, blocks, 72, shared)
+    q = queries_of(sum(queries), kv_heads * group, dim, query, 73, scale=0.05)
+    plan = AttentionPlan(pool, tables, contexts, queries, kv_heads * group, query_dtype=query,
+                         shared_blocks=shared, **options)
+    got = attend(plan, 0, q)
+    want, tol = reference(q, k[0], v[0], bs, tables, contexts, queries, **options)
+    a, _ = reference(q, k[0], v[0].abs(), bs, tables, contexts, queries, **options)
+    u, n = torch.finfo(query).eps / 2, max(contexts)
+    tol = tol + (u * u - u + n * 2.0 ** -24) * a
+    if query == F16:                     # the end of float16 below weights held 2^7 above: check
+        tol = tol + 2.0 ** -32 * n * v[0].double().abs().amax()
+    off = (got.double() - want).abs()
+    assert not torch.isnan(off).any()
+    worst = (off / tol.clamp_min(1e-300)).max().item()   # a key of zeros alone: both are 0
+    assert worst <= 1.0, f"{worst} times the tolerance"
