@@ -71,13 +71,14 @@ class PackedBlocks:
     """
 
     def __init__(self, data: torch.Tensor, num_layers: int, tile_shape: tuple[int, ...],
-                 dtype: torch.dtype) -> None:
+                 dtype: torch.dtype, format: str | None = None) -> None:
         if data.dtype != torch.uint8 or data.dim() != 3 or data.shape[1] != 2 * num_layers:
             raise ValueError(f"packed data must be uint8 [n, {2 * num_layers}, T]")
         self.data = data
         self.num_layers = num_layers
         self.tile_shape = tuple(tile_shape)
         self.dtype = dtype
+        self.format = format           # of records (KVPool.format)
         self._event: torch.cuda.Event | None = None  # last async copy touching host data
         self._parent: PackedBlocks | None = None  # the buffer a slice views (kept alive)
         self._offset: int | None = 0   # first row in the root buffer (None: a strided view)
@@ -86,13 +87,14 @@ class PackedBlocks:
 
     @classmethod
     def _new(cls, data: torch.Tensor, num_layers: int, tile_shape: tuple[int, ...],
-             dtype: torch.dtype, pinned: bool) -> "PackedBlocks":
+             dtype: torch.dtype, format: str | None, pinned: bool) -> "PackedBlocks":
         """A buffer a copier has just allocated in its pool's layout (no re-validation)."""
         self = cls.__new__(cls)
         self.data = data
         self.num_layers = num_layers
         self.tile_shape = tile_shape
         self.dtype = dtype
+        self.format = format
         self._event = None
         self._parent = None
         self._offset = 0
@@ -129,7 +131,8 @@ class PackedBlocks:
 
     def __getitem__(self, index):
         if isinstance(index, slice):
-            view = PackedBlocks(self.data[index], self.num_layers, self.tile_shape, self.dtype)
+            view = PackedBlocks(self.data[index], self.num_layers, self.tile_shape, self.dtype,
+                                self.format)
             view._parent = self._root
             start, _, step = index.indices(len(self))
             view._offset = self._offset + start if step == 1 and self._offset is not None \
@@ -444,11 +447,15 @@ class HipSlotCopier:
     for its answer, so it is for callers that prefer the error to the speed.
     Without it, device ids are taken as they are (the kernels skip ids outside
     the pool).
+    ``format`` says that the caches hold records of a microscaled format
+    (:mod:`iekv.engine.quantized`): payloads carry it, and blocks of another format, or
+    of values, are refused.
     """
 
     def __init__(self, k_caches: Seq[torch.Tensor], v_caches: Seq[torch.Tensor],
                  block_size: int, *, payload_location: str = "device",
-                 defer_reads: bool | None = None, check_device_ids: bool = False) -> None:
+                 defer_reads: bool | None = None, check_device_ids: bool = False,
+                 format: str | None = None) -> None:
         if payload_location not in ("device", "host"):
             raise ValueError("payload_location must be 'device' or 'host'")
         self.k_caches = k_caches
@@ -474,8 +481,25 @@ class HipSlotCopier:
         # again (a tier entry restored in a batch) is not validated again.
         self._layout_key = (self.pool.n_arrays, self.pool.tile_bytes, self.pool.device)
         self._tile_shape = tuple(self.pool.tile_shape)
+        if format is not None:
+            self.format = format
 
     # -- helpers -------------------------------------------------------------
+    @property
+    def format(self) -> str | None:
+        """The microscaled format of the caches' records (None: they hold values)."""
+        return self.pool.format
+
+    @format.setter
+    def format(self, format: str | None) -> None:
+        if format is not None:
+            from .quantized import head_dim_of
+
+            head_dim_of(self.pool, format)       # ValueError where they cannot be its records
+        self.pool.format = format
+        # Payloads accepted so far are judged again.
+        self._layout_key = (self.pool.n_arrays, self.pool.tile_bytes, self.pool.device)
+
     @property
     def device(self) -> torch.device:
         return self.pool.device
@@ -494,7 +518,7 @@ class HipSlotCopier:
         else:
             data = torch.empty(shape, dtype=torch.uint8, device=self.device)
         out = PackedBlocks._new(data, self.pool.num_layers, self._tile_shape, self.pool.dtype,
-                                pinned=on_host)
+                                self.pool.format, pinned=on_host)
         out._checked = self._layout_key        # made in this pool's layout
         return out
 
@@ -545,6 +569,9 @@ class HipSlotCopier:
             raise ValueError(
                 f"payload of {packed.data.shape[1]} tiles x {packed.data.shape[2]} B does not "
                 f"fit a pool of {self.pool.n_arrays} tiles x {self.pool.tile_bytes} B")
+        if packed.format != self.pool.format:
+            raise ValueError(f"payload of {_holds(packed.format)} for a pool of "
+                             f"{_holds(self.pool.format)}")
         if not packed.data.is_contiguous():
             raise ValueError("payload data must be contiguous")
         if not packed.on_host and packed.data.device != self.device:
@@ -833,8 +860,7 @@ class HipSlotCopier:
 
     def _copy_blocks(self, source: "HipSlotCopier", src_ids, dst_ids,
                      on: torch.cuda.Stream | None) -> None:
-        if not self.pool.same_shape(source.pool):
-            raise ValueError("source and destination pools differ in layout")
+        _refuse_other_layout(source.pool, self.pool)
         if source.device != self.device:
             raise ValueError(f"pools on {source.device} and {self.device}")
         on_device = (isinstance(src_ids, torch.Tensor) and src_ids.device.type == "cuda") or \
@@ -926,8 +952,7 @@ class HipSlotCopier:
         carry up to INLINE_IDS pairs each (up to MERGED_IDS_MAX pairs on one stream),
         else in one launch per stream.
         """
-        if not self.pool.same_shape(source.pool):
-            raise ValueError("source and destination pools differ in layout")
+        _refuse_other_layout(source.pool, self.pool)
         if source.device != self.device:
             raise ValueError(f"pools on {source.device} and {self.device}")
         streams = list(streams) if streams else [torch.cuda.current_stream(self.device)]
@@ -1074,6 +1099,19 @@ def _merged_tables(tables) -> tuple[array, array] | None:
     return src, dst
 
 
+def _holds(format: str | None) -> str:
+    return "values" if format is None else f"{format} records"
+
+
+def _refuse_other_layout(source: KVPool, destination: KVPool) -> None:
+    if destination.same_shape(source):
+        return
+    if source.format != destination.format:
+        raise ValueError(f"a source of {_holds(source.format)} and a destination of "
+                         f"{_holds(destination.format)}")
+    raise ValueError("source and destination pools differ in layout")
+
+
 def copier_for(k_caches, v_caches, block_size: int, role: str = "transfer") -> HipSlotCopier:
     """Default copier factory of the engine.
 
@@ -1094,8 +1132,11 @@ def stack_payloads(payloads: Iterable[BlockPayload]) -> PackedBlocks:
     if not items:
         raise ValueError("no payloads")
     first = items[0].packed
+    for p in items:
+        if p.packed.format != first.format:
+            raise ValueError(f"payloads of {_holds(first.format)} and of {_holds(p.packed.format)}")
     data = torch.stack([p.packed.data[p.index] for p in items])
-    return PackedBlocks(data, first.num_layers, first.tile_shape, first.dtype)
+    return PackedBlocks(data, first.num_layers, first.tile_shape, first.dtype, first.format)
 
 
 __all__ = ["BlockPayload", "DeferredBlockPayload", "HipSlotCopier", "PackedBlocks", "copier_for",

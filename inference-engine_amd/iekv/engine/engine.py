@@ -119,16 +119,14 @@ class Engine:
             if bind is not None else None
         self.swapper = None
         if self.config.preemption == "swap":
-            self.swapper = self.copier_factory(self.k_caches, self.v_caches,
-                                               self.config.block_size, "swap")
+            self.swapper = self.make_copier("swap")
         self.scheduler = Scheduler(self.blocks,
                                    max_batch_sequences=self.config.max_batch_sequences,
                                    max_batch_tokens=self.config.max_batch_tokens,
                                    swapper=self.swapper)
         self.copier = None
         if self.config.offload_blocks > 0:
-            self.copier = self.copier_factory(self.k_caches, self.v_caches,
-                                              self.config.block_size, "offload")
+            self.copier = self.make_copier("offload")
             self.blocks.tier = KVTier(self.config.offload_blocks)
             self.blocks.copier = self.copier
 
@@ -149,7 +147,12 @@ class Engine:
                              f"{device}")
 
     def make_copier(self, role: str = "transfer"):
-        return self.copier_factory(self.k_caches, self.v_caches, self.config.block_size, role)
+        copier = self.copier_factory(self.k_caches, self.v_caches, self.config.block_size, role)
+        # A model's caches may hold records, which a copier's payloads say if they can.
+        format = getattr(self.model, "cache_format", None)
+        if format is not None and hasattr(copier, "format"):
+            copier.format = format
+        return copier
 
     def submit(self, prompt_ids: list[int], max_new_tokens: int = 32,
                temperature: float = 1.0, eos_id: int | None = None) -> Sequence:

@@ -189,6 +189,9 @@ class KVPool:
         self.tile_shape = (block_size, *first.shape[1:])
         self.tile_bytes = math.prod(self.tile_shape) * first.element_size()
         self.dtype = first.dtype
+        # What the bytes are where their type does not say it: the microscaled format of a
+        # pool of records (iekv.engine.quantized), None of values.
+        self.format: str | None = None
         self.device = first.device
         self._arrays = arrays  # keeps the memory alive while the handle exists
         # Array addresses and the byte range they span, for comparing pools by memory
@@ -253,7 +256,8 @@ class KVPool:
 
     def same_shape(self, other: "KVPool") -> bool:
         return (self.n_arrays == other.n_arrays and self.tile_bytes == other.tile_bytes
-                and self.tile_shape == other.tile_shape and self.dtype == other.dtype)
+                and self.tile_shape == other.tile_shape and self.dtype == other.dtype
+                and self.format == other.format)
 
     def block_ids(self, ids, *, unique: bool = False, what: str = "block") -> torch.Tensor:
         """Block ids as a contiguous int32 tensor on this pool's device.

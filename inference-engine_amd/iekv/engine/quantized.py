@@ -21,8 +21,9 @@ tier and the wire move its blocks as they move any other's.
     out = attend(plan, layer, q)                             # iekv.engine.attention
     rows = gather_rows(pool, layer, table, context_len, dtype=torch.bfloat16)
 
-Both pools of a handoff have to be of one format: their records may be of the same size in
-another.
+Records of two formats may be of the same size, so what moves them carries the format: copiers
+(``HipSlotCopier(..., format=...)``, or an engine's of a model with a ``cache_format``), their
+payloads and the wire's header. Blocks go only where the format is the same.
 """
 from __future__ import annotations
 
@@ -52,14 +53,37 @@ _TYPES = {torch.float32: _native.IEKV_TYPE_F32, torch.float16: _native.IEKV_TYPE
           torch.bfloat16: _native.IEKV_TYPE_BF16}
 
 
-def record_bytes(format: str, head_dim: int) -> int:
-    """Bytes of one head of one token: its elements and the groups' exponents."""
+def _known(format: str) -> None:
     if format not in FORMATS:
         raise ValueError(f"no format {format!r}: one of {', '.join(FORMATS)}")
+
+
+def record_bytes(format: str, head_dim: int) -> int:
+    """Bytes of one head of one token: its elements and the groups' exponents."""
+    _known(format)
     if not 8 <= head_dim <= _ops.ATTENTION_MAX_DIM or head_dim % 8:
         raise ValueError(f"head_dim {head_dim} is not a multiple of 8 up to "
                          f"{_ops.ATTENTION_MAX_DIM}")
     return head_dim * _CODE_BITS[format] // 8 + _SCALE_BYTES
+
+
+def head_dim_of(pool: KVPool, format: str) -> int:
+    """The head dimension of the records that ``pool``'s caches hold; ValueError where they
+    can hold none of ``format``."""
+    _known(format)
+    if pool.dtype != torch.uint8 or len(pool.tile_shape) != 3:
+        raise ValueError(f"caches of records are [rows, KV heads, record] uint8, got tiles of "
+                         f"{pool.tile_shape} {pool.dtype}")
+    record = pool.tile_shape[2]
+    head_dim = (record - _SCALE_BYTES) * 8 // _CODE_BITS[format]
+    try:
+        fits = record_bytes(format, head_dim) == record
+    except ValueError:
+        fits = False
+    if not fits:
+        raise ValueError(f"records of {record} bytes are none of {format}: head_dim is a "
+                         f"multiple of 8 up to {_ops.ATTENTION_MAX_DIM}")
+    return head_dim
 
 
 def allocate_quantized_pool(num_blocks: int, block_size: int, num_layers: int,
@@ -93,21 +117,9 @@ class QuantizedPool(KVPool):
 
     def __init__(self, k_caches: Seq[torch.Tensor], v_caches: Seq[torch.Tensor],
                  block_size: int, format: str) -> None:
-        if format not in FORMATS:
-            raise ValueError(f"no format {format!r}: one of {', '.join(FORMATS)}")
+        _known(format)
         super().__init__(k_caches, v_caches, block_size)
-        if self.dtype != torch.uint8 or len(self.tile_shape) != 3:
-            raise ValueError(f"caches of records are [rows, KV heads, record] uint8, got tiles of "
-                             f"{self.tile_shape} {self.dtype}")
-        _, heads, record = self.tile_shape
-        head_dim = (record - _SCALE_BYTES) * 8 // _CODE_BITS[format]
-        try:
-            fits = record_bytes(format, head_dim) == record
-        except ValueError:
-            fits = False
-        if not fits:
-            raise ValueError(f"records of {record} bytes are none of {format}: head_dim is a "
-                             f"multiple of 8 up to {_ops.ATTENTION_MAX_DIM}")
+        head_dim, heads = head_dim_of(self, format), self.tile_shape[1]
         self.format = format
         self.num_kv_heads = heads
         self.head_dim = head_dim
@@ -121,9 +133,6 @@ class QuantizedPool(KVPool):
         self._write_ids = _ops.entry("iekv_mx_write_slots_ids")
         self._read = _ops.entry("iekv_mx_read_rows")
         self._read_ids = _ops.entry("iekv_mx_read_rows_ids")
-
-    def same_shape(self, other: KVPool) -> bool:
-        return super().same_shape(other) and self.format == getattr(other, "format", self.format)
 
     def _rows(self, t: torch.Tensor, what: str) -> torch.Tensor:
         """Rows as the library reads them: as they are where their heads are contiguous."""

@@ -62,7 +62,7 @@ class HandoffQueue:
     def __init__(self, src: KVPool, dst: KVPool, *, workers: int = 0, claim_bytes: int = 0,
                  idle_ms: float = 0.0, life_ms: float = 0.0) -> None:
         if not src.same_shape(dst):
-            raise ValueError("the pools differ in shape")
+            raise ValueError("the pools differ in shape or in what they hold")
         handle = c_void_p()
         _native.call("iekv_queue_create", src.native.handle, dst.native.handle, workers,
                      claim_bytes, int(idle_ms * 1000), int(life_ms * 1000),

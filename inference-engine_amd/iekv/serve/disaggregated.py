@@ -254,6 +254,7 @@ class DecodeWorker:
         all (its blocks are freed at once and never read).
         """
         engine = self.engine
+        self._refuse_other_format(transfer)
         seq = engine.submit(transfer.token_ids[:-1], max_new_tokens=max_new_tokens,
                             temperature=temperature)
         if transfer.first_block:
@@ -294,6 +295,16 @@ class DecodeWorker:
         seq.status = Status.RUNNING
         engine.scheduler.running.append(seq)
         return seq
+
+    def _refuse_other_format(self, transfer: KVTransfer) -> None:
+        """ValueError, before anything is reserved, for blocks of another format than this
+        pool's (payloads and copiers without one are left to the move)."""
+        source = transfer.source.copier if transfer.source is not None else \
+            transfer.block_payloads
+        mine = getattr(self.copier, "format", None)
+        if getattr(source, "format", mine) != mine:
+            raise ValueError(f"a transfer of {source.format or 'values'}, this worker's caches "
+                             f"hold {mine or 'values'}")
 
     def _claim_with_prefix(self, seq: Sequence, transfer: KVTransfer) -> list[int]:
         blocks = self.engine.blocks

@@ -8,7 +8,8 @@ messages:
 1. a self-describing header: magic ``b"IEKV"``, a little-endian u32 format
    version, a u32 length, then UTF-8 JSON with the sequence state
    (``token_ids``, ``num_computed``, ``first_block``, ``bytes_moved``) and the
-   payload layout (blocks, layers, tile shape, dtype, tile bytes); where the prefill
+   payload layout (blocks, layers, tile shape, dtype, tile bytes, and for records of a
+   microscaled cache ``cache_format``, without which a payload holds values); where the prefill
    worker scored its tokens also ``scores``, a ``[token, log probability, entropy,
    [[token, log probability], ...]]`` or null each (infinities and NaN, which JSON has no
    numbers for, as "-inf", "inf" and "nan");
@@ -100,6 +101,8 @@ def encode_header(transfer: KVTransfer, packed) -> bytes:
         "dtype": dtype,
         "tile_bytes": packed.tile_bytes,
     }
+    if packed.format is not None:
+        meta["cache_format"] = packed.format
     if transfer.scores:
         meta["scores"] = [_encode_score(s) for s in transfer.scores]
     body = json.dumps(meta, separators=(",", ":"), allow_nan=False).encode()
@@ -120,6 +123,11 @@ def decode_header(buf: bytes) -> dict[str, Any]:
     meta = json.loads(body)
     if meta["dtype"] not in _DTYPES:
         raise ValueError(f"unknown cache dtype {meta['dtype']!r}")
+    if meta.get("cache_format") is not None:
+        from ..engine.quantized import FORMATS
+
+        if meta["cache_format"] not in FORMATS:
+            raise ValueError(f"unknown cache format {meta['cache_format']!r}")
     return meta
 
 
@@ -141,7 +149,7 @@ def from_wire(header: bytes, payload: torch.Tensor) -> KVTransfer:
         raise ValueError(f"payload of shape {tuple(payload.shape)} / {payload.dtype} does not "
                          f"match the header's {shape} uint8")
     packed = PackedBlocks(payload, meta["num_layers"], tuple(meta["tile_shape"]),
-                          _DTYPES[meta["dtype"]])
+                          _DTYPES[meta["dtype"]], meta.get("cache_format"))
     return KVTransfer(token_ids=list(meta["token_ids"]), num_computed=meta["num_computed"],
                       block_payloads=packed, bytes_moved=meta["bytes_moved"],
                       first_block=meta["first_block"],

@@ -96,3 +96,81 @@ def test_models_without_the_slot_kernels_are_refused(gpu):
         model(gpu, cache_format="mxfp8")
     with pytest.raises(ValueError, match="no format"):
         model(gpu, hip_kv=True, cache_format="fp8")
+
+
+def pools_of(format, other, dim=32):
+    """Two registered pools of the same bytes in records of `format` and of `other` (None: bytes)."""
+    from iekv.engine.copier import HipSlotCopier
+    from iekv.engine.quantized import allocate_quantized_pool
+
+    made = []
+    for f in (format, other):
+        k, v = allocate_quantized_pool(6, 4, 2, 2, dim, format="mxfp8")
+        made.append(HipSlotCopier(k, v, 4, format=f))
+    return made
+
+
+@pytest.mark.parametrize("format, other", [("mxfp8", "mxint8"), ("mxint8", "mxfp8"),
+                                           ("mxfp8", None), (None, "mxint8")])
+def test_blocks_do_not_go_where_another_format_is(gpu, format, other):
+    """The records of both are of one size: nothing but the format tells them apart."""
+    from iekv.engine.quantized import QuantizedPool
+    from iekv.engine.queue import HandoffQueue
+
+    source, destination = pools_of(format, other)
+    for t in source.k_caches + source.v_caches:
+        t.fill_(7)
+    refused = pytest.raises(ValueError, match="records")
+    with refused:
+        destination.copy_blocks(source, [0, 1], [2, 3])
+    with refused:
+        destination.copy_requests(source, [([0, 1], [2, 3])])
+    with pytest.raises(ValueError, match="what they hold"):
+        HandoffQueue(source.pool, destination.pool)
+    for location in ("device", "host"):
+        packed = source.read_blocks([0, 1, 4], location=location)
+        for payloads in (packed, [packed[2], packed[0]], packed[::2]):
+            with refused:
+                destination.write_blocks([1, 2, 3][:len(payloads)], payloads)
+        with refused:
+            destination.read_blocks([1, 2, 3], into=source.empty_payloads(3))
+    torch.cuda.synchronize()
+    assert not any(t.any() for t in destination.k_caches + destination.v_caches)
+    for f, copier in ((format, source), (other, destination)):
+        if f is not None:
+            pool = QuantizedPool(copier.k_caches, copier.v_caches, 4, f)
+            assert pool.same_shape(copier.pool) and copier.pool.same_shape(pool)
+    # Of one format, as ever.
+    destination.format = format
+    destination.copy_blocks(source, [0], [2])
+    destination.write_blocks([3], source.read_blocks([1]))
+    torch.cuda.synchronize()
+    for t in destination.k_caches + destination.v_caches:
+        assert t.view(6, -1)[2:4].eq(7).all() and not t.view(6, -1)[[0, 1, 4, 5]].any()
+
+
+def test_a_copiers_format_is_one_that_its_caches_can_hold(gpu):
+    source, _ = pools_of("mxfp8", None)
+    with pytest.raises(ValueError, match="no format"):
+        source.format = "mxfp6"
+    with pytest.raises(ValueError, match="none of mxfp4"):       # that would be heads of 144
+        pools_of("mxfp8", None, dim=72)[0].format = "mxfp4"
+    assert source.format == "mxfp8"
+
+
+@pytest.mark.parametrize("mode", ["pack", "direct", "queue"])
+def test_a_worker_refuses_transfers_of_another_format(gpu, mode):
+    from iekv.serve.disaggregated import DecodeWorker, PrefillWorker
+    from iekv.serve.wire import from_wire, to_wire
+
+    prefill = PrefillWorker(model(gpu, hip_attention=True, cache_format="mxfp8"), engine_config(),
+                            mode=mode)
+    worker = DecodeWorker(model(gpu, hip_attention=True, cache_format="mxint8"), engine_config())
+    worker.use_queue = mode == "queue"
+    free = worker.engine.blocks.num_free
+    transfer = prefill.prefill(G["prompts"][1], 0.0)
+    with pytest.raises(ValueError, match="transfer of mxfp8, .* hold mxint8"):
+        worker.admit(transfer, max_new_tokens=4)
+    with pytest.raises(ValueError, match="transfer of mxfp8, .* hold mxint8"):
+        worker.admit(from_wire(*to_wire(transfer)), max_new_tokens=4)
+    assert worker.engine.blocks.num_free == free and not worker.engine.scheduler.waiting
