@@ -174,3 +174,67 @@ def test_a_worker_refuses_transfers_of_another_format(gpu, mode):
     with pytest.raises(ValueError, match="transfer of mxfp8, .* hold mxint8"):
         worker.admit(from_wire(*to_wire(transfer)), max_new_tokens=4)
     assert worker.engine.blocks.num_free == free and not worker.engine.scheduler.waiting
+
+
+def watched_copier():
+    """A copier that compares what it moves to and from host memory with the pool's bytes."""
+    from iekv.engine.copier import HipSlotCopier
+
+    class Watched(HipSlotCopier):
+        out = back = 0
+
+        def same(self, block_ids, images):
+            torch.cuda.synchronize()
+            for block, image in zip(block_ids, images, strict=True):
+                rows = slice(block * self.block_size, (block + 1) * self.block_size)
+                for a, cache in enumerate((*self.k_caches, *self.v_caches)):
+                    assert torch.equal(cache[rows].cpu().view(-1), image[a])
+
+        def read_blocks(self, block_ids, **kw):
+            packed = super().read_blocks(block_ids, **kw)
+            assert packed.on_host and packed.format == self.format is not None
+            self.same(block_ids, packed.host_data())
+            self.out += len(packed)
+            return packed
+
+        def _offload_each(self, block_ids, payloads):
+            super()._offload_each(block_ids, payloads)
+            self.same(block_ids, [p.packed.host_data()[p.index] for p in payloads])
+            self.out += len(payloads)
+
+        def write_blocks(self, block_ids, payloads, **kw):
+            images = [p.packed.host_data()[p.index].clone() for p in payloads]
+            super().write_blocks(block_ids, payloads, **kw)
+            self.same(block_ids, images)
+            self.back += len(images)
+
+    return lambda k, v, block_size, role: Watched(k, v, block_size, payload_location="host",
+                                                  defer_reads=role == "offload")
+
+
+# Pools that hold two of four prompts: the second time behind offloaded blocks, and requests that
+# grow past the pool while they decode.
+PRESSED = {"tier": (dict(offload_blocks=64, num_blocks=8), 48, 8),
+           "swap": (dict(block_size=8, num_blocks=8, preemption="swap"), 12, 10)}
+
+
+@pytest.mark.parametrize("where", list(PRESSED))
+@pytest.mark.parametrize("format", FORMATS)
+def test_records_go_to_host_memory_and_come_back(gpu, format, where):
+    from iekv.engine.engine import Engine
+
+    over, length, n = PRESSED[where]
+    prompts = [p[:length] for p in G["prompts"]]
+    want = decided(gpu, prompts, n, hip_kv=True, cache_format=format)
+    assert sum(map(len, want)) > 4 * len(want)
+    m = model(gpu, hip_kv=True, hip_attention=True, cache_format=format)
+    engine = Engine(m, engine_config(**over), copier_factory=watched_copier())
+    for _ in range(2):
+        agree(engine.generate(prompts, max_new_tokens=n, temperature=0.0), want)
+    if where == "tier":
+        assert engine.blocks.tier.stats.restored == engine.copier.back > 0
+        assert engine.copier.out >= engine.copier.back
+    else:
+        stats = engine.scheduler.stats
+        assert stats.swapped_in == stats.swapped_out > 0
+        assert engine.swapper.out == engine.swapper.back > 0
