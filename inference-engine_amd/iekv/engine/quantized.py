@@ -5,10 +5,14 @@ ie/model/torch_transformer.py:82-86). A :class:`QuantizedPool` holds half of a 1
 bytes, or a quarter: 32 dimensions of a head share a power of two, and an element is what is
 left in 8 or 4 bits, rounded to nearest even.
 
-    ``mxfp8``    e4m3: 3 bits after the leading one, off by 2^-4 of a value at most
-    ``mxint8``   integers up to 127: off by 2^-7 of the group's largest value at most
+    ``mxfp8``    e4m3: 3 bits after the leading one, off by 2^-4 of a value or, of small ones
+                 beside a large one, by 2^-17 of the group's largest at most
+    ``mxint8``   integers up to 127: off by 1/127 of the group's largest at most
     ``mxfp4``    e2m1: 1 bit after the leading one, off by 2^-2 of a value, or a twelfth of the
                  group's largest
+
+The power is 2^-100 at least. Of a group too small for it elements are off by half a step there,
+whatever they are of the largest: by 2^-110, 2^-101 and 2^-102.
 
 A head's record is its elements and four bytes of exponents, so that a cache is an ordinary
 array ``[num_blocks * block_size, num_kv_heads, record]`` of bytes: the handoff, the offload

@@ -78,6 +78,41 @@ def test_the_definition():
             assert torch.equal((part - got[..., g * 32:g * 32 + 32]).abs(), off)
 
 
+@pytest.mark.parametrize("format, of_value, of_largest, smallest", [
+    ("mxfp8", 2.0 ** -4, 2.0 ** -17, 2.0 ** -110), ("mxint8", 0.0, 1 / 127, 2.0 ** -101),
+    ("mxfp4", 2.0 ** -2, 1 / 12, 2.0 ** -102)])
+def test_how_far_an_element_is_off(format, of_value, of_largest, smallest):
+    """As the module says: a part of the value, or of its group's largest where that is more, or
+    half a step of the least power. Groups whose largest is just past what the power before would
+    hold, and elements between two codes there, are where the bounds are met."""
+    top = {"mxfp8": 448.0, "mxint8": 127.0, "mxfp4": 6.0}[format]
+    gen = torch.Generator().manual_seed(5)
+    groups = torch.randn((4000, 32), generator=gen, dtype=torch.float64)
+    groups *= torch.exp2(torch.randn((4000, 32), generator=gen, dtype=torch.float64) * 6)
+    values = CODES[format][torch.isfinite(CODES[format])].unique()
+    halves = (values[1:] + values[:-1]) / 2
+    edges = torch.zeros((len(halves), 32), dtype=torch.float64)
+    edges[:, 0] = top / 2 * (1 + 2.0 ** -30)                  # of steps of 1: not held in halves
+    edges[:, 1] = halves * (1 - 2.0 ** -40)
+    edges[:, 2] = -halves * (1 + 2.0 ** -40)
+    edges = edges[edges.abs().amax(-1) == edges[:, 0]]
+    tiny = torch.cat((groups, edges)) * 2.0 ** -105
+    held = torch.cat((groups, edges, edges * 2.0 ** -60, edges * 2.0 ** 60))
+    for x, least in ((held, 0.0), (tiny, smallest)):
+        off = (x - decode(encode(x, format), format)).abs()
+        bound = torch.maximum(of_value * x.abs(), of_largest * x.abs().amax(-1, keepdim=True))
+        assert (off <= bound.clamp(min=least)).all()
+    # And no smaller ones hold: mxint8's is past 2^-7, e4m3's small ones are lost altogether.
+    off = (edges - decode(encode(edges, format), format)).abs()
+    relative = off / edges.abs().amax(-1, keepdim=True)
+    if of_value:
+        assert (off[:, 1] / edges[:, 1].abs()).nan_to_num(0.0).max() > of_value
+        assert relative[:, 1:].max() > of_largest
+        assert ((off == edges.abs()) & (edges != 0)).any()
+    else:
+        assert relative.max() > 0.999 * of_largest > 2.0 ** -7
+
+
 def test_pools_of_host_tensors_are_refused():
     from iekv.engine.quantized import QuantizedPool, allocate_quantized_pool
 
