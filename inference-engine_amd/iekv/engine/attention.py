@@ -85,7 +85,7 @@ class AttentionPlan:
     float16 or bfloat16 on a cache of the same type, float8_e4m3fn or a quantised pool
     (default: the cache's type, bfloat16 on an fp8 cache and a quantised pool). A quantised
     pool's values are taken as :func:`~iekv.engine.slots.gather_rows` reads them back in the
-    queries' type. IndexError for a block outside the pool or a table
+    queries' type (of float16 queries infinities from 57,344 on). IndexError for a block outside the pool or a table
     too short for its context, ValueError for tables that do not begin with the shared
     blocks and for arguments out of range.
 

@@ -12,7 +12,11 @@ left in 8 or 4 bits, rounded to nearest even.
                  group's largest
 
 The power is 2^-100 at least. Of a group too small for it elements are off by half a step there,
-whatever they are of the largest: by 2^-110, 2^-101 and 2^-102.
+whatever they are of the largest: by 2^-110, 2^-101 and 2^-102. At the other end an element is
+rounded past what a type of 16 or 32 bits holds, where reading it back in that type gives an
+infinity, as its own rounding does: in float16 from 63,488 on (``mxfp8``), past 65,024
+(``mxint8``) and from 57,344 on (``mxfp4``), though a float16 row goes up to 65,504; in bfloat16
+and float32 2^112 times that.
 
 A head's record is its elements and four bytes of exponents, so that a cache is an ordinary
 array ``[num_blocks * block_size, num_kv_heads, record]`` of bytes: the handoff, the offload

@@ -518,3 +518,45 @@ def test_weights_are_held_as_two_numbers(gpu, query, format, dim, step):
     assert not torch.isnan(off).any()
     worst = (off / tol.clamp_min(1e-300)).max().item()   # a key of zeros alone: both are 0
     assert worst <= 1.0, f"{worst} times the tolerance"
+
+
+# float16 numbers that a format rounds to float16's infinity, and the next below, which it does not.
+ENDS = {"mxfp8": [(63488.0, 63456.0), (65504.0, 61440.0)],
+        "mxint8": [(65056.0, 65024.0), (65504.0, 64992.0)],
+        "mxfp4": [(57344.0, 57312.0), (65504.0, 49152.0)]}
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("format", FORMATS)
+def test_the_end_of_float16(gpu, format, rows):
+    """Rows of float16 near its largest, as the documents have it: read back in float16 they are
+    infinite from there on, finite below and in wider types; attention takes them as read."""
+    from iekv.engine.attention import AttentionPlan, attend
+    from iekv.engine.quantized import QuantizedPool, allocate_quantized_pool
+    from iekv.engine.slots import gather_rows, write_slots
+
+    context, dim = 80, 64
+    for past, below in ENDS[format]:
+        k, v = allocate_quantized_pool(5, 16, 1, 1, dim, format=format)
+        pool = QuantizedPool(k, v, 16, format)
+        gen = torch.Generator(device="cuda").manual_seed(81)
+        key = torch.randn((context, 1, dim), generator=gen, device="cuda").half()
+        value = torch.randn((context, 1, dim), generator=gen, device="cuda").half()
+        value[3, 0, 5], value[3, 0, 40] = past, -below          # of a group of their own each
+        table = list(range(5))
+        write_slots(pool, 0, key, value, list(range(context)))
+        read = gather_rows(pool, 1, table, context, dtype=F16)
+        assert read[3, 0, 5] == float("inf")
+        assert torch.isinf(read).sum() == 1 and not torch.isnan(read).any()
+        wide = gather_rows(pool, 1, table, context, dtype=F32)
+        assert torch.isfinite(wide).all() and wide[3, 0, 5] == 65536.0
+        assert torch.equal(wide.half(), read)
+        q = torch.randn((rows, 2, dim), generator=gen, device="cuda").half() * 0.1
+        plan = AttentionPlan(pool, [table], [context], [rows], 2, query_dtype=F16)
+        got = attend(plan, 0, q)
+        if rows == 1 or context - rows >= 3:                    # every row sees the third key
+            assert (got[..., 5] == float("inf")).all()
+        assert torch.isfinite(got[..., :5]).all() and torch.isfinite(got[..., 6:]).all()
+        wider = attend(AttentionPlan(pool, [table], [context], [rows], 2, query_dtype=F32), 0,
+                       q.float())
+        assert torch.isfinite(wider).all()
