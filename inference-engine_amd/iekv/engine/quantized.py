@@ -244,6 +244,7 @@ def write(pool: QuantizedPool, first_layer: int, k: torch.Tensor, v: torch.Tenso
     if k.dtype != v.dtype:
         raise ValueError(f"K rows of {k.dtype} and V rows of {v.dtype}")
     where, entry = pool._slots(slots, n)
+    first_layer = operator.index(first_layer)      # NumPy's too: an address is made of it
     if first_layer < 0 or first_layer + n_layers > pool.num_layers:
         raise IndexError(f"layers {first_layer}..{first_layer + n_layers - 1} out of range for "
                          f"{pool.num_layers} layers")
@@ -261,6 +262,10 @@ def read(pool: QuantizedPool, first_array: int, n_arrays: int, block_table, cont
     if kind is None:
         raise ValueError(f"values of {dtype}: float32, float16 or bfloat16 are read back")
     context_len = operator.index(context_len)
+    first_array, n_arrays = operator.index(first_array), operator.index(n_arrays)
+    if first_array < 0 or n_arrays <= 0 or first_array + n_arrays > pool.n_arrays:
+        raise IndexError(f"arrays {first_array}..{first_array + n_arrays - 1} out of range for "
+                         f"{pool.n_arrays} arrays")
     table, entry = pool._table(block_table, context_len)
     out = torch.empty((n_arrays, context_len, pool.num_kv_heads, pool.head_dim),
                       dtype=torch.bfloat16 if dtype is None else dtype, device=pool.device)

@@ -198,7 +198,6 @@ def gather_rows(pool: KVPool, array: int, block_table, context_len: int, *,
     the memory was.
     """
     if isinstance(pool, QuantizedPool):
-        _check_arrays(pool, array, 1)
         return quantized.read(pool, array, 1, block_table, context_len, dtype)[0]
     _cache_dtype_only(pool, dtype)
     table, fn = _context_table(pool, block_table, context_len)
@@ -231,12 +230,6 @@ def write_slots_layers(pool: KVPool, k: torch.Tensor, v: torch.Tensor, slots,
     _write(pool, first_layer, n_layers, n, k, v, slots)
 
 
-def _check_arrays(pool: KVPool, first_array: int, n_arrays: int) -> None:
-    if first_array < 0 or n_arrays <= 0 or first_array + n_arrays > pool.n_arrays:
-        raise IndexError(f"arrays {first_array}..{first_array + n_arrays - 1} out of range for "
-                         f"{pool.n_arrays} arrays")
-
-
 def gather_rows_arrays(pool: KVPool, block_table, context_len: int, first_array: int = 0,
                        n_arrays: int | None = None, *,
                        dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -245,9 +238,11 @@ def gather_rows_arrays(pool: KVPool, block_table, context_len: int, first_array:
     ``[n_arrays, context_len, H, D]`` tensor of the cache dtype, of a quantised pool's values
     in ``dtype`` as :func:`gather_rows` has them."""
     n_arrays = pool.n_arrays - first_array if n_arrays is None else n_arrays
-    _check_arrays(pool, first_array, n_arrays)
     if isinstance(pool, QuantizedPool):
         return quantized.read(pool, first_array, n_arrays, block_table, context_len, dtype)
+    if first_array < 0 or n_arrays <= 0 or first_array + n_arrays > pool.n_arrays:
+        raise IndexError(f"arrays {first_array}..{first_array + n_arrays - 1} out of range for "
+                         f"{pool.n_arrays} arrays")
     _cache_dtype_only(pool, dtype)
     table, fn = _context_table(pool, block_table, context_len)
     out = torch.empty((n_arrays, context_len, *pool.tile_shape[1:]), dtype=pool.dtype,

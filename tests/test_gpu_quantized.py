@@ -407,3 +407,31 @@ def test_refusals(gpu):
     # The records themselves, as bytes.
     raw = gather_rows(KVPool(k, v, 8), 0, [1], 8)
     assert raw.dtype == torch.uint8 and raw.shape == (8, 2, 36)
+
+
+@pytest.mark.parametrize("kind", ["int64", "int32", "uint8", "int8"])
+def test_layers_are_whole_numbers_of_any_kind(gpu, kind):
+    """NumPy's among them, as of other pools: 40 of 8 bits times 8 would be past their end."""
+    import numpy as np
+
+    from iekv.engine.slots import gather_rows, gather_rows_arrays, write_slots, write_slots_layers
+
+    kind = np.dtype(kind).type
+    pool, _, _ = make_pool(2, 4, 1, 32, "mxint8", layers=41)
+    k, v = (rows_of((2, 3, 1, 32), F32, seed) for seed in (91, 92))
+    write_slots(pool, kind(40), k[0], v[0], [1, 2, 3])
+    write_slots_layers(pool, k, v, [4, 5, 6], first_layer=kind(38))
+    for layer, slots, x in ((40, [1, 2, 3], k[0]), (38, [4, 5, 6], k[0]), (39, [4, 5, 6], k[1])):
+        got = gather_rows_arrays(pool, [0, 1], kind(8), first_array=kind(layer), n_arrays=kind(2),
+                                 dtype=F32)
+        assert torch.equal(got[0, slots], decode(encode(x, "mxint8"), "mxint8").float().cuda())
+        assert torch.equal(gather_rows(pool, kind(layer), [0, 1], 8, dtype=F32), got[0])
+    got = gather_rows(pool, kind(81), [0, 1], 8, dtype=F32)           # V of the last layer
+    assert torch.equal(got[1:4], decode(encode(v[0], "mxint8"), "mxint8").float().cuda())
+    for first, n in ((81, 100), (82, 1), (40, 0)):                   # 181 of 8 bits is below 0
+        with pytest.raises(IndexError, match="out of range for 82 arrays"):
+            gather_rows_arrays(pool, [0, 1], 8, first_array=kind(first), n_arrays=kind(n))
+    with pytest.raises(IndexError, match="out of range for 41 layers"):
+        write_slots_layers(pool, k, v, [4, 5, 6], first_layer=kind(40))
+    with pytest.raises(TypeError):
+        write_slots(pool, 1.0, k[0], v[0], [1, 2, 3])
