@@ -99,11 +99,13 @@ bool together_fits(const iekv_attention_shape& s) {
 
 // Workgroups that a long stream is cut into for each compute unit. Of four heads' long records two
 // keep the memory busy (and have LDS for two), and more drive each other's lines out of L2: 48
-// sequences of 6,000 tokens of eight mxfp8 heads of 128 107 us with two, 127 with three. Short
-// records take more work for their bytes: 128 sequences of 4,200 tokens in mxfp4 115 us with
-// three, 126 with two, 143 with four.
+// sequences of 6,000 tokens of eight mxfp8 heads of 128 107 us with two, 127 with three, of 96 86
+// and 94. Short records take more work for their bytes: 128 sequences of 4,200 tokens in mxfp4 115
+// us with three, 126 with two, 143 with four, in mxfp8 heads of 64 107 and 116. So do integers: in
+// mxint8 heads of 96 182 us with three and 201 with two, of 128 252 and 225.
 int32_t streams_at_once(const iekv_attention_shape& s) {
-  return together_fits(s) && head_bytes_of(s) * kWaves >= 400 ? 2 : 3;
+  const int32_t is_long = s.cache_type == IEKV_TYPE_MXINT8 ? 500 : 400;
+  return together_fits(s) && head_bytes_of(s) * kWaves >= is_long ? 2 : 3;
 }
 
 // And few items: twice the steps for a wave of microscaled caches take less than twice the parts do,
@@ -114,8 +116,10 @@ int32_t few_at_once(const iekv_attention_shape& s) { return s.cache_type >= IEKV
 
 // And what a long stream is: four heads' records come together sooner than other caches' rows pay
 // for their parts. 16 sequences of 6,000 tokens of eight mxfp8 heads of 128 42 us together, 50 each
-// head by itself, 8 of 8,000 31.5 and 36 (in mxfp4 32 and 35, both 25); 8 of 6,000 beside a chunk
-// of 2,048 tokens, then in a launch of its own, 370 and 498.
+// head by itself, 8 of 8,000 31.5 and 36 (in mxfp4 32 and 35, 24 and 27; in mxint8 51 and 52, 36
+// and 39, though 8 of 6,000 34 and 32). A chunk beside them is then in a launch of its own: with
+// the last 2,048 of 7,777 tokens 8 of 6,000 360 us, in one launch 450, but with a prompt of 2,048
+// 100 and 85 (in the caches of a card that holds many layers, as all of these).
 int32_t stream_steps(const iekv_attention_shape& s) { return together_fits(s) ? 1 : 4; }
 
 template <typename T, typename C, int DP>

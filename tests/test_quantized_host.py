@@ -328,3 +328,26 @@ print(json.dumps([rcs, launches()]))
     assert rows[3:] == [4096 // 2, 4096 // 2, -(-(9591 - 8192) // 2)]
     first = 1 + (((1 << 30) - 5) * 128 - 1) // 256   # of bf16: 16 lanes a head, 8 heads
     assert abs(sum(grids) - first - ((1 << 29) + 1)) <= len(grids)
+
+
+@pytest.mark.parametrize("cache_type, dim, at_once", [
+    (5, 128, 2), (5, 96, 2), (5, 64, 3), (6, 128, 2), (6, 96, 3), (6, 64, 3), (7, 128, 3),
+    (7, 96, 3)])
+def test_long_streams_are_cut_by_the_work_of_their_records(ops, cache_type, dim, at_once):  # noqa: F811
+    """Into two or three workgroups of four heads for each of 256 compute units."""
+    n, context = 48, 6000
+    blocks = context // 16
+    rc, plan, _ = make(ops, contexts=(context,) * n, queries=(1,) * n,
+                       tables=(tuple(range(blocks)),) * n, num_blocks=blocks, num_heads=32,
+                       num_kv_heads=8, head_dim=dim, cache_type=cache_type)
+    assert rc == 0
+    words, count = ctypes.POINTER(ctypes.c_int32)(), ctypes.c_int64()
+    tokens, workspace = ctypes.c_int64(), ctypes.c_int64()
+    ops.iekv_attention_plan_info(plan, ctypes.byref(words), ctypes.byref(count),
+                                 ctypes.byref(tokens), ctypes.byref(workspace))
+    items, keys = 0, 0
+    while keys < n * context:
+        it = words[12 * items:12 * items + 12]
+        items, keys = items + 1, keys + it[4] - it[3] + it[6] - it[5]
+    assert (at_once - 1) * 256 < items * 2 <= at_once * 256
+    ops.iekv_attention_plan_destroy(plan)
