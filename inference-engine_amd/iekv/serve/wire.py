@@ -126,7 +126,7 @@ def decode_header(buf: bytes) -> dict[str, Any]:
     if meta.get("cache_format") is not None:
         from ..engine.quantized import FORMATS
 
-        if meta["cache_format"] not in FORMATS:
+        if meta["cache_format"] not in list(FORMATS):        # whatever JSON holds there
             raise ValueError(f"unknown cache format {meta['cache_format']!r}")
     return meta
 

@@ -37,15 +37,16 @@ def test_the_format_is_in_the_header(format):
     assert from_wire(*to_wire(transfer)).block_payloads.format == format
 
 
-def test_formats_that_are_not_known_are_refused():
+@pytest.mark.parametrize("said", ["mxfp6", 5, ["mxfp8"], False])
+def test_formats_that_are_not_known_are_refused(said):
     from iekv.serve.wire import _PREFIX, decode_header, encode_header
 
     header = encode_header(make_transfer(packed_of("mxfp8")), packed_of("mxfp8"))
     magic, version, _ = _PREFIX.unpack_from(header)
     meta = json.loads(header[_PREFIX.size:])
-    meta["cache_format"] = "mxfp6"
+    meta["cache_format"] = said
     body = json.dumps(meta).encode()
-    with pytest.raises(ValueError, match="mxfp6"):
+    with pytest.raises(ValueError, match="unknown cache format"):
         decode_header(_PREFIX.pack(magic, version, len(body)) + body)
 
 
