@@ -85,9 +85,9 @@ class AttentionPlan:
     float16 or bfloat16 on a cache of the same type, float8_e4m3fn or a quantised pool
     (default: the cache's type, bfloat16 on an fp8 cache and a quantised pool). A quantised
     pool's values are taken as :func:`~iekv.engine.slots.gather_rows` reads them back in the
-    queries' type (of float16 queries infinities from 57,344 on). IndexError for a block outside the pool or a table
-    too short for its context, ValueError for tables that do not begin with the shared
-    blocks and for arguments out of range.
+    queries' type (of float16 queries infinities from 57,344 on). IndexError for a block
+    outside the pool or a table too short for its context, ValueError for tables that do not
+    begin with the shared blocks and for arguments out of range.
 
     Making one costs the host 20-45 us for a few sequences, 220 us for 48 of 6,000 tokens in
     blocks of 16 and 400 us for 128 of 4,200, most of it to flatten the tables.

@@ -194,8 +194,8 @@ def gather_rows(pool: KVPool, array: int, block_table, context_len: int, *,
 
     A quantised pool's values come in ``dtype`` (float32, float16, bfloat16; default bfloat16),
     rounded to nearest even: to an infinity past the type's largest, where the format may have
-    rounded a row of that type, too (float16 from 57,344 on, :mod:`iekv.engine.quantized`). Rows of blocks of a device table outside the pool are left as
-    the memory was.
+    rounded a row of that type, too (float16 from 57,344 on, :mod:`iekv.engine.quantized`).
+    Rows of blocks of a device table outside the pool are left as the memory was.
     """
     if isinstance(pool, QuantizedPool):
         return quantized.read(pool, array, 1, block_table, context_len, dtype)[0]

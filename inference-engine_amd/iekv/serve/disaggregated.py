@@ -301,10 +301,11 @@ class DecodeWorker:
         pool's (payloads and copiers without one are left to the move)."""
         source = transfer.source.copier if transfer.source is not None else \
             transfer.block_payloads
-        mine = getattr(self.copier, "format", None)
-        if getattr(source, "format", mine) != mine:
+        if not (hasattr(source, "format") and hasattr(self.copier, "format")):
+            return
+        if source.format != self.copier.format:
             raise ValueError(f"a transfer of {source.format or 'values'}, this worker's caches "
-                             f"hold {mine or 'values'}")
+                             f"hold {self.copier.format or 'values'}")
 
     def _claim_with_prefix(self, seq: Sequence, transfer: KVTransfer) -> list[int]:
         blocks = self.engine.blocks

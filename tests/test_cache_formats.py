@@ -98,3 +98,14 @@ def test_an_engine_tells_its_copiers_what_its_model_keeps():
     assert {engine.make_copier().format, engine.copier.format, engine.swapper.format} == {"mxfp4"}
     plain = Engine(toy, engine_config(), copier_factory=oracle_factory)   # of no such knowledge
     assert not hasattr(plain.make_copier(), "format")
+
+
+def test_what_a_copier_without_formats_moves_is_its_own_matter():
+    from iekv.serve.disaggregated import DecodeWorker
+
+    worker = DecodeWorker(model(), engine_config(), copier_factory=oracle_factory)
+    worker._refuse_other_format(make_transfer(packed_of("mxfp8")))
+    transfer = make_transfer(packed_of("mxfp8"))
+    transfer.block_payloads = list(packed_of("mxfp8"))      # of a list each payload says, if it can
+    DecodeWorker(model(), engine_config(),
+                 copier_factory=tagged("mxint8"))._refuse_other_format(transfer)
